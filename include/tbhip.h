@@ -379,6 +379,105 @@ TB_API int tb_fused_transformer_layer_step_w4a32(
     void *stream);
 
 /* ------------------------------------------------------------------------ */
+/*
+ * Speculative decoding over a drafted tree (the reference verifies chains only,
+ * src/llm/decoder.rs:565-727).  A tree has n nodes in topological order (n up to
+ * 1024): parents[i] is -1 (a root, a child of the prefix's last token) or the
+ * index of an earlier node; any other value marks node i as padding, and its
+ * descendants with it.  The K / V row of node i is in the cache at position
+ * kv_len + i, behind the prefix of kv_len positions.  Nothing here waits for the
+ * device, so all of it can be captured into a graph.
+ *
+ * tb_tree_masks: parents i32 [batch, n] -> mask i32 [batch, n, ceil(n / 32)], bit
+ * j % 32 of word j / 32 of row i set when node j is node i or an ancestor of it,
+ * and depth i32 [batch, n], the number of proper ancestors (node i's token has
+ * position kv_len + depth[i]).  A padding node has no bits and depth 0.
+ */
+TB_API int tb_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, int64_t batch,
+                         int64_t n, void *stream);
+
+/*
+ * GQA attention of the tree's nodes: node i of sequence b sees the positions
+ * below kv_len and kv_len + j for every bit j of its mask row (any mask may be
+ * given, not only a tree's).  A row without bits is padding: zeros.  Positions
+ * that a row does not see take no part, whatever the cache holds there.
+ * q and out f32 [batch, n, num_heads, head_dim] (query head h reads KV head
+ * h / (num_heads / num_kv_heads)); caches f32 with strides in elements for
+ * sequence (sb), KV head (sh) and position (ss), all multiples of 4, head_dim
+ * contiguous; mask_sb words between the sequences' masks (0: one mask for all).
+ * kv_lens: device i32 [batch], clamped to [0, max_seq] (nodes past the cache's
+ * end do not exist), or NULL: kv_len for every sequence, and TB_ERR_VALUE when
+ * kv_len + n > max_seq.  head_dim a multiple of 32 up to 256; q, out and the
+ * caches 16-byte aligned.
+ */
+TB_API int tb_tree_attention(const float *q, const float *k_cache, const float *v_cache,
+                             const int32_t *mask, const int32_t *kv_lens, float *out,
+                             int64_t batch, int64_t n, int64_t num_heads, int64_t num_kv_heads,
+                             int64_t head_dim, int64_t max_seq, int64_t kv_len, int64_t k_sb,
+                             int64_t k_sh, int64_t k_ss, int64_t v_sb, int64_t v_sh, int64_t v_ss,
+                             int64_t mask_sb, float scale, void *stream);
+
+/*
+ * Acceptance: the path starts at node 0 (which must be a root) and goes from a
+ * node to its lowest child whose draft token is the node's next token, the one
+ * that the model chose there (a negative token matches none).  path i32
+ * [batch, n] receives the path's nodes, then -1; n_path i32 [batch] its length (0
+ * when node 0 is padding); token i64 [batch] the next token of its last node
+ * (-1 without a path).  draft_tokens and next_tokens i64 [batch, n].
+ * In each of the `layers` caches (host arrays of device pointers; layers may be
+ * 0) K / V row kv_len + path[j] moves to kv_len + j, so that the accepted rows
+ * follow the prefix; rows past the path keep what they held, and rows past
+ * max_seq do not exist.  Strides, kv_lens and kv_len as above.
+ */
+TB_API int tb_tree_accept(const int32_t *parents, const int64_t *draft_tokens,
+                          const int64_t *next_tokens, const int32_t *kv_lens, int64_t kv_len,
+                          int32_t *path, int32_t *n_path, int64_t *token, float *const *k_caches,
+                          float *const *v_caches, int64_t layers, int64_t batch, int64_t n,
+                          int64_t num_kv_heads, int64_t head_dim, int64_t max_seq, int64_t k_sb,
+                          int64_t k_sh, int64_t k_ss, int64_t v_sb, int64_t v_sh, int64_t v_ss,
+                          void *stream);
+
+/*
+ * Penalties, biases and masks on `rows` rows of logits [rows, vocab] before a
+ * token is taken from each (the reference has the repetition penalty only,
+ * src/llm/decoder.rs:878-899).  For token t of a row, with count its occurrences
+ * in the generated part of the row's history and on its tree path, and seen when
+ * it occurs anywhere in them:
+ *   y = seen ? (x > 0 ? x / repetition : x * repetition) : x
+ *   y = count > 0 ? (y - frequency * count) - presence : y
+ *   y = y + bias[t];  -inf where the mask's bit t is not set.
+ * out f32 [rows, vocab] (may be logits itself) receives y; tokens i64 [rows]
+ * the best token of each row: the largest y, the lowest index on ties, never NaN
+ * or -inf (-1 where nothing else is left).  One of the two may be NULL.
+ *
+ * history i64 [groups, hist]: row r has list r / (rows / groups); history_len
+ * i32 [groups] the length of each (NULL: hist), prompt_len i32 [groups] how many
+ * of its first tokens are prompt (NULL: prompt): seen, not counted.  Tokens
+ * outside the vocabulary are skipped.  A penalty is one value, or f32 [rows] on
+ * the device (repetition_rows, ... not NULL).  bias_ids i64 / bias f32
+ * [bias_groups, n_bias], likewise; a token named twice gets the sum.
+ * allowed i32 [rows, ceil(vocab / 32)], allowed_stride words between rows (0: one
+ * mask for all); NULL: every token.  draft_tokens i64 [rows / nodes, nodes] and
+ * tree_mask [rows / nodes, nodes, ceil(nodes / 32)]: row r is node r % nodes of
+ * tree r / nodes, and the draft tokens of its mask bits are part of its generated
+ * history.  nodes 0: no trees.
+ * scratch: tb_process_logits_scratch bytes of device memory, needed with tokens
+ * only; NULL: the stream's workspace (TB_ERR_UNSUPPORTED while capturing, since
+ * graphs that are replayed side by side would share it).
+ */
+TB_API int64_t tb_process_logits_scratch(int64_t rows, int64_t vocab);
+TB_API int tb_process_logits(const float *logits, float *out, int64_t *tokens, int64_t rows,
+                             int64_t vocab, const int64_t *history, const int32_t *history_len,
+                             const int32_t *prompt_len, int64_t groups, int64_t hist,
+                             int64_t prompt, float repetition_penalty, float presence_penalty,
+                             float frequency_penalty, const float *repetition_rows,
+                             const float *presence_rows, const float *frequency_rows,
+                             const int64_t *bias_ids, const float *bias, int64_t bias_groups,
+                             int64_t n_bias, const int32_t *allowed, int64_t allowed_stride,
+                             const int64_t *draft_tokens, const int32_t *tree_mask, int64_t nodes,
+                             void *scratch, int64_t scratch_bytes, void *stream);
+
+/* ------------------------------------------------------------------------ */
 
 typedef struct tb_decoder tb_decoder;
 

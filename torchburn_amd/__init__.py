@@ -7,7 +7,8 @@ meaning and error behaviour.
 """
 from ._lib import UnsupportedOpError
 from .decoder import RustQwenDecoder, create_rust_qwen_decoder
-from .sampling import sample_logits, sample_uniform
+from .sampling import greedy_tokens, process_logits, sample_logits, sample_uniform
+from .tree import tree_accept, tree_attention, tree_masks
 from .quantization import (
     QuantizedLinear,
     fused_attention_step,
@@ -71,4 +72,9 @@ __all__ = [
     "unpack_rows_w4a32_group64_v2_to_v1",
     "sample_logits",
     "sample_uniform",
+    "process_logits",
+    "greedy_tokens",
+    "tree_masks",
+    "tree_attention",
+    "tree_accept",
 ]

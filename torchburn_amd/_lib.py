@@ -67,13 +67,18 @@ _SIGS = {
     "tb_fused_attention_step_w8a32": [_p] * 3 + [_i64] + [_p] * 3 + [_i64] + [_p] * 6 +
                                      [_i64] * 6 + [_p],
     "tb_fused_transformer_layer_step_w4a32": [_p] * 22 + [_i64] * 8 + [C.c_double, _p],
+    "tb_tree_masks": [_p, _p, _p, _i64, _i64, _p],
+    "tb_tree_attention": [_p] * 6 + [_i64] * 14 + [C.c_float, _p],
+    "tb_tree_accept": [_p] * 4 + [_i64] + [_p] * 5 + [_i64] * 12 + [_p],
+    "tb_process_logits": [_p] * 3 + [_i64] * 2 + [_p] * 3 + [_i64] * 3 + [C.c_float] * 3 +
+                         [_p] * 5 + [_i64] * 2 + [_p, _i64, _p, _p, _i64, _p, _i64, _p],
 }
 
 
 def declared_symbols() -> list:
     """Every entry point the Python layer binds (all are declared in include/tbhip.h)."""
     return ["tb_last_error", "tb_version", "tb_x_records_bytes", "tb_sample_uniform",
-            "tb_w4_kernel",
+            "tb_w4_kernel", "tb_process_logits_scratch",
             *_SIGS.keys()]
 
 
@@ -94,6 +99,8 @@ def lib():
             L.tb_x_records_bytes.argtypes = [C.c_int64, C.c_int64]
             L.tb_w4_kernel.restype = C.c_char_p
             L.tb_w4_kernel.argtypes = [C.c_int64] * 5
+            L.tb_process_logits_scratch.restype = C.c_int64
+            L.tb_process_logits_scratch.argtypes = [C.c_int64] * 2
             L.tb_sample_uniform.restype = C.c_float
             L.tb_sample_uniform.argtypes = [C.c_uint64, C.c_uint64]
             for name, args in _SIGS.items():
@@ -115,6 +122,15 @@ def check(rc: int) -> None:
     if rc == TB_ERR_MEMORY:
         raise MemoryError(msg)
     raise RuntimeError(f"HIP error: {msg}")
+
+
+def call_on(dev, name: str, *args) -> None:
+    """call() with ``dev`` as the current device, for kernels launched on one of its streams."""
+    import torch
+    if dev.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(dev):
+        return call(name, *args)
 
 
 def call(name: str, *args) -> None:

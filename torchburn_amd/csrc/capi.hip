@@ -26,6 +26,8 @@
 #include "../../include/tbhip_bench.h"
 #include "quantize.hpp"
 #include "sample.hpp"
+#include "logits.hpp"
+#include "tree.hpp"
 
 namespace tb {
 
@@ -1175,6 +1177,205 @@ int tb_fused_swiglu_mlp_w8a32(const float *x, const int8_t *gate_w, const float 
     d.x = h;
     if ((rc = w8_rows(p, pp, m, scratch, st))) return rc;
     return w8_rows(d, pd, m, scratch, st);
+}
+
+// ---- draft trees and logits -------------------------------------------------
+
+// The shape of a batch of draft trees.
+static int check_tree(const char *what, int64_t batch, int64_t n) {
+    const std::string op(what);
+    TB_REQUIRE(batch >= 0 && batch <= 65535, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: " + op + ": batch of " + std::to_string(batch) + " outside 0..65535");
+    TB_REQUIRE(n >= 0 && n <= kMaxTreeNodes, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: " + op + ": " + std::to_string(n) + " tree nodes outside 0.." +
+                   std::to_string(kMaxTreeNodes));
+    return TB_OK;
+}
+
+// The geometry of KV caches whose rows are read and moved 16 bytes at a time.
+static int check_cache(const char *what, int64_t hkv, int64_t hd, int64_t max_seq,
+                       const int64_t (&k)[3], const int64_t (&v)[3]) {
+    const std::string op(what);
+    TB_REQUIRE(hkv > 0 && hkv <= 65535, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: " + op + ": num_kv_heads outside 1..65535");
+    TB_REQUIRE(hd >= 32 && hd <= 256 && hd % 32 == 0, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: " + op + ": head_dim must be a multiple of 32 in 32..256, got " +
+                   std::to_string(hd));
+    TB_REQUIRE(max_seq >= 0 && max_seq <= (1 << 30), TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: " + op + ": max_seq outside 0..2^30");
+    for (int i = 0; i < 3; ++i)
+        TB_REQUIRE(k[i] >= 0 && v[i] >= 0 && k[i] % 4 == 0 && v[i] % 4 == 0, TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: " + op + ": cache strides must be multiples of 4 elements");
+    return TB_OK;
+}
+
+// Whether no two elements of a cache of this geometry share memory.
+static bool disjoint(const int64_t (&st)[3], const int64_t (&size)[3], int64_t hd) {
+    std::pair<int64_t, int64_t> d[3];
+    for (int i = 0; i < 3; ++i) d[i] = {st[i], size[i]};
+    std::sort(d, d + 3);
+    int64_t extent = hd;
+    for (const auto &[stride, n] : d) {
+        if (n <= 1) continue;
+        if (stride < extent) return false;
+        extent = stride * (n - 1) + extent;
+    }
+    return true;
+}
+
+int tb_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, int64_t batch, int64_t n,
+                  void *stream) {
+    int rc = check_tree("tree_masks", batch, n);
+    if (rc) return rc;
+    if (batch == 0 || n == 0) return TB_OK;
+    TB_REQUIRE(parents && mask && depth, TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: tree_masks: null pointer");
+    return launch_tree_masks(parents, mask, depth, (int)batch, (int)n, (hipStream_t)stream);
+}
+
+int tb_tree_attention(const float *q, const float *k_cache, const float *v_cache,
+                      const int32_t *mask, const int32_t *kv_lens, float *out, int64_t batch,
+                      int64_t n, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                      int64_t max_seq, int64_t kv_len, int64_t k_sb, int64_t k_sh, int64_t k_ss,
+                      int64_t v_sb, int64_t v_sh, int64_t v_ss, int64_t mask_sb, float scale,
+                      void *stream) {
+    int rc = check_tree("tree_attention", batch, n);
+    if (!rc) rc = check_cache("tree_attention", num_kv_heads, head_dim, max_seq, {k_sb, k_sh, k_ss},
+                              {v_sb, v_sh, v_ss});
+    if (rc) return rc;
+    TB_REQUIRE(num_heads > 0 && num_heads <= 65535 && num_heads % num_kv_heads == 0,
+               TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: tree_attention: num_heads must be a multiple of num_kv_heads");
+    TB_REQUIRE(kv_lens || (kv_len >= 0 && kv_len + n <= max_seq), TB_ERR_VALUE,
+               "tree_attention: " + std::to_string(n) + " nodes at position " +
+                   std::to_string(kv_len) + " exceed the cache's " + std::to_string(max_seq));
+    if (batch == 0 || n == 0) return TB_OK;
+    TB_REQUIRE(q && k_cache && v_cache && mask && out, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: tree_attention: null pointer");
+    TB_REQUIRE(aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16),
+               TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: tree_attention: q, out and the caches must be 16-byte aligned");
+    TreeAttn a{};
+    a.q = q;
+    a.k = {k_cache, k_sb, k_sh, k_ss};
+    a.v = {v_cache, v_sb, v_sh, v_ss};
+    a.mask = mask; a.mask_sb = mask_sb; a.kv_lens = kv_lens; a.kv_len = kv_lens ? 0 : (int)kv_len;
+    a.out = out;
+    a.batch = (int)batch; a.n = (int)n; a.hq = (int)num_heads; a.hkv = (int)num_kv_heads;
+    a.hd = (int)head_dim; a.max_seq = (int)max_seq; a.scale = scale;
+    return launch_tree_attention(a, (hipStream_t)stream);
+}
+
+int tb_tree_accept(const int32_t *parents, const int64_t *draft_tokens, const int64_t *next_tokens,
+                   const int32_t *kv_lens, int64_t kv_len, int32_t *path, int32_t *n_path,
+                   int64_t *token, float *const *k_caches, float *const *v_caches, int64_t layers,
+                   int64_t batch, int64_t n, int64_t num_kv_heads, int64_t head_dim,
+                   int64_t max_seq, int64_t k_sb, int64_t k_sh, int64_t k_ss, int64_t v_sb,
+                   int64_t v_sh, int64_t v_ss, void *stream) {
+    int rc = check_tree("tree_accept", batch, n);
+    if (rc) return rc;
+    TB_REQUIRE(layers >= 0 && layers <= 65535, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: tree_accept: layers outside 0..65535");
+    TB_REQUIRE(n > 0 || batch == 0, TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: tree_accept: empty trees");
+    if (batch == 0) return TB_OK;
+    TB_REQUIRE(parents && draft_tokens && next_tokens && path && n_path && token,
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: tree_accept: null pointer");
+    TreeAccept a{};
+    if (layers > 0) {
+        if ((rc = check_cache("tree_accept", num_kv_heads, head_dim, max_seq, {k_sb, k_sh, k_ss},
+                              {v_sb, v_sh, v_ss})))
+            return rc;
+        TB_REQUIRE(kv_lens || (kv_len >= 0 && kv_len + n <= max_seq), TB_ERR_VALUE,
+                   "tree_accept: " + std::to_string(n) + " nodes at position " +
+                       std::to_string(kv_len) + " exceed the cache's " + std::to_string(max_seq));
+        TB_REQUIRE(k_caches && v_caches, TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: tree_accept: null pointer");
+        for (int64_t l = 0; l < layers; ++l)
+            TB_REQUIRE(k_caches[l] && v_caches[l] && aligned(k_caches[l], 16) &&
+                           aligned(v_caches[l], 16),
+                       TB_ERR_UNSUPPORTED,
+                       "TB_UNSUPPORTED: tree_accept: the caches must be 16-byte aligned");
+        // rows move in place: two blocks must not move the same ones
+        const int64_t size[3] = {batch, num_kv_heads, max_seq};
+        TB_REQUIRE(disjoint({k_sb, k_sh, k_ss}, size, head_dim) &&
+                       disjoint({v_sb, v_sh, v_ss}, size, head_dim),
+                   TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: tree_accept: a cache overlaps itself");
+        std::vector<const float *> all(k_caches, k_caches + layers);
+        all.insert(all.end(), v_caches, v_caches + layers);
+        std::sort(all.begin(), all.end());
+        TB_REQUIRE(std::adjacent_find(all.begin(), all.end()) == all.end(), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: tree_accept: a cache is given twice");
+        a.hkv = (int)num_kv_heads; a.hd = (int)head_dim; a.max_seq = (int)max_seq;
+        a.k = {nullptr, k_sb, k_sh, k_ss};
+        a.v = {nullptr, v_sb, v_sh, v_ss};
+    }
+    a.parents = parents; a.draft = draft_tokens; a.next = next_tokens;
+    a.kv_lens = kv_lens; a.kv_len = kv_lens || !layers ? 0 : (int)kv_len;
+    a.path = path; a.n_path = n_path; a.token = token;
+    a.batch = (int)batch; a.n = (int)n; a.layers = (int)layers;
+    return launch_tree_accept(a, k_caches, v_caches, (hipStream_t)stream);
+}
+
+int64_t tb_process_logits_scratch(int64_t rows, int64_t vocab) {
+    if (rows <= 0 || vocab <= 0 || rows > 65535 || vocab > (1 << 30)) return 0;
+    return (int64_t)logits_scratch((int)rows, (int)vocab, true);
+}
+
+int tb_process_logits(const float *logits, float *out, int64_t *tokens, int64_t rows,
+                      int64_t vocab, const int64_t *history, const int32_t *history_len,
+                      const int32_t *prompt_len, int64_t groups, int64_t hist, int64_t prompt,
+                      float repetition_penalty, float presence_penalty, float frequency_penalty,
+                      const float *repetition_rows, const float *presence_rows,
+                      const float *frequency_rows, const int64_t *bias_ids, const float *bias,
+                      int64_t bias_groups, int64_t n_bias, const int32_t *allowed,
+                      int64_t allowed_stride, const int64_t *draft_tokens,
+                      const int32_t *tree_mask, int64_t nodes, void *scratch,
+                      int64_t scratch_bytes, void *stream) {
+    TB_REQUIRE(rows >= 0 && rows <= 65535 && vocab > 0 && vocab <= (1 << 30), TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: process_logits: rows outside 0..65535 or vocabulary outside 1..2^30");
+    TB_REQUIRE(hist >= 0 && hist <= (1 << 30) && n_bias >= 0 && n_bias <= (1 << 30),
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: process_logits: bad history or bias length");
+    TB_REQUIRE(hist == 0 || (groups > 0 && rows % groups == 0), TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: process_logits: " + std::to_string(groups) +
+                   " histories do not divide " + std::to_string(rows) + " rows");
+    TB_REQUIRE(n_bias == 0 || (bias_groups > 0 && rows % bias_groups == 0), TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: process_logits: " + std::to_string(bias_groups) +
+                   " bias lists do not divide " + std::to_string(rows) + " rows");
+    TB_REQUIRE(nodes >= 0 && nodes <= kMaxTreeNodes && (nodes == 0 || rows % nodes == 0),
+               TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: process_logits: trees of " + std::to_string(nodes) +
+                   " nodes do not divide " + std::to_string(rows) + " rows");
+    TB_REQUIRE(repetition_rows || repetition_penalty > 0.f, TB_ERR_VALUE,
+               "process_logits: repetition_penalty must be positive");
+    if (rows == 0) return TB_OK;
+    TB_REQUIRE(logits && (out || tokens) && (hist == 0 || history) &&
+                   (n_bias == 0 || (bias_ids && bias)) && (nodes == 0 || (draft_tokens && tree_mask)),
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: process_logits: null pointer");
+    TB_REQUIRE(allowed_stride == 0 || allowed_stride >= (vocab + 31) / 32, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: process_logits: mask rows shorter than the vocabulary");
+    LogitsParams p{};
+    p.x = logits; p.y = out; p.tokens = tokens;
+    p.rows = (int)rows; p.vocab = (int)vocab;
+    p.history = history; p.history_len = history_len; p.prompt_len = prompt_len;
+    p.groups = (int)groups; p.hist = (int)hist; p.prompt = (int)std::min<int64_t>(prompt, hist);
+    p.rep = repetition_penalty; p.pres = presence_penalty; p.freq = frequency_penalty;
+    p.rep_rows = repetition_rows; p.pres_rows = presence_rows; p.freq_rows = frequency_rows;
+    p.bias_ids = bias_ids; p.bias = bias; p.bias_groups = (int)bias_groups; p.n_bias = (int)n_bias;
+    p.allowed = allowed; p.allowed_stride = allowed_stride;
+    p.draft = draft_tokens; p.tree_mask = tree_mask; p.nodes = (int)nodes;
+    hipStream_t st = (hipStream_t)stream;
+    const size_t need = logits_scratch(p.rows, p.vocab, tokens != nullptr);
+    WsLease lease;
+    if (need && !scratch) {
+        TB_REQUIRE(!capturing(st), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: process_logits: a captured call needs scratch of its own");
+        int rc = workspace(need, st, lease);
+        if (rc) return rc;
+        scratch = lease.ptr;
+    } else if (need) {
+        TB_REQUIRE(scratch_bytes >= (int64_t)need && aligned(scratch, 16), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: process_logits: scratch too short or not 16-byte aligned");
+    }
+    return launch_logits(p, scratch, st);
 }
 
 }  // extern "C"

@@ -1,0 +1,209 @@
+// Speculative decoding over a drafted tree, the device side: ancestor masks from
+// the parent list, attention of the tree's nodes over the cached prefix and their
+// own ancestors, and acceptance, which keeps one path of the tree in the cache.
+//
+// A tree's n nodes are in topological order: parents[i] is -1 (a root: a child
+// of the prefix's last token) or an earlier node.  Anything else marks node i
+// as padding, and its descendants with it.  Node i's K / V row sits in the cache
+// at position len + i, behind the prefix of len positions.
+#include <math.h>
+
+#include <algorithm>
+#include <string>
+
+#include "tb_common.hpp"
+#include "tree.hpp"
+
+namespace tb {
+
+namespace {
+
+// ---- ancestor masks -------------------------------------------------------
+//
+// mask(i) = {i} u mask(parent(i)), depth(i) = depth(parent(i)) + 1; a padding
+// node has no bits and depth 0.  One block per tree, a thread per node walks up
+// its chain, whose indices fall, so that each word of the row is written once.
+__global__ void k_tree_masks(const int32_t *__restrict__ parents, int32_t *__restrict__ mask,
+                             int32_t *__restrict__ depth, int n) {
+    __shared__ int par[kMaxTreeNodes];
+    const size_t b = blockIdx.x;
+    const int words = (n + 31) / 32;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) par[i] = parents[b * n + i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        int d = 0, at = i;
+        while (par[at] >= 0 && par[at] < at) {
+            at = par[at];
+            ++d;
+        }
+        const bool live = par[at] == -1;
+        int32_t *row = mask + (b * n + i) * words;
+        at = live ? i : -1;
+        for (int w = words - 1; w >= 0; --w) {
+            uint32_t bits = 0;
+            while (at >= 32 * w) {   // at < 32 * (w + 1) here, and -1 past the root
+                bits |= 1u << (at & 31);
+                at = par[at];
+            }
+            row[w] = (int32_t)bits;
+        }
+        depth[b * n + i] = live ? d : 0;
+    }
+}
+
+// ---- attention --------------------------------------------------------------
+
+__device__ __forceinline__ int prefix_len(const int32_t *lens, int len, int b, int max_seq) {
+    const int l = lens ? lens[b] : len;
+    return min(max(l, 0), max_seq);
+}
+
+// One block per query row (sequence, node, head): tiles of 256 keys, a key per
+// thread for the scores, an output column per thread for P V.  A row without
+// mask bits is padding and gives zeros; keys that a row does not see take no
+// part, whatever their K / V rows hold.
+__global__ __launch_bounds__(256) void k_tree_attn(TreeAttn a) {
+    __shared__ float qs[256], ps[256], red[8];
+    __shared__ int any_bits;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int node = blockIdx.x / a.hq, h = blockIdx.x % a.hq, b = blockIdx.y;
+    const int kvh = h / (a.hq / a.hkv), words = (a.n + 31) / 32;
+    const size_t row = ((size_t)b * a.n + node) * a.hq + h;
+    const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq);
+    const int end = min(len + a.n, a.max_seq);
+    const int32_t *mrow = a.mask + b * a.mask_sb + (int64_t)node * words;
+    const float *kb = a.k.p + b * a.k.sb + kvh * a.k.sh, *vb = a.v.p + b * a.v.sb + kvh * a.v.sh;
+    if (t == 0) any_bits = 0;
+    if (t < a.hd) qs[t] = a.q[row * a.hd + t] * a.scale;
+    __syncthreads();
+    for (int w = t; w < words; w += 256)
+        if (mrow[w]) any_bits = 1;
+    __syncthreads();
+    const bool live = any_bits != 0;
+    float m = -INFINITY, l = 0.f, o = 0.f;
+    for (int p0 = 0; live && p0 < end; p0 += 256) {
+        const int p = p0 + t;
+        float s = -INFINITY;
+        const bool see = p < len || (p < end && ((uint32_t)mrow[(p - len) >> 5] >> ((p - len) & 31) & 1));
+        if (see) {
+            const float4 *kr = reinterpret_cast<const float4 *>(kb + p * a.k.ss);
+            s = 0.f;
+            for (int c = 0; c < a.hd / 4; ++c) {
+                const float4 x = kr[c];
+                s += qs[4 * c] * x.x + qs[4 * c + 1] * x.y + qs[4 * c + 2] * x.z + qs[4 * c + 3] * x.w;
+            }
+        }
+        float top = s;
+        for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+        if (lane == 0) red[wave] = top;
+        __syncthreads();
+        const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+        const float pj = see ? expf(s - (mn == -INFINITY ? 0.f : mn)) : 0.f;
+        ps[t] = pj;
+        float sum = pj;
+        for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off);
+        if (lane == 0) red[4 + wave] = sum;
+        __syncthreads();
+        const float alpha = m == mn ? 1.f : expf(m - mn);
+        l = l * alpha + (red[4] + red[5]) + (red[6] + red[7]);
+        o *= alpha;
+        m = mn;
+        if (t < a.hd)
+            for (int j = 0; j < min(256, end - p0); ++j)
+                if (ps[j] != 0.f) o += ps[j] * vb[(p0 + j) * a.v.ss + t];
+        __syncthreads();
+    }
+    if (t < a.hd) a.out[row * a.hd + t] = l > 0.f || l != l ? o / l : 0.f;
+}
+
+// ---- acceptance -------------------------------------------------------------
+
+struct LayerCaches {
+    float *k[kTreeLayersPerLaunch], *v[kTreeLayersPerLaunch];
+};
+
+// The walk: node 0 is the root; from a node the path goes on to its lowest child
+// whose drafted token (a negative one is none) is the node's next token.  Whether a node is such a child
+// does not depend on the walk, so every node is tested at once (child[p] = the
+// lowest one of node p), and one thread then follows child[].
+//
+// The move: K / V row len + path[j] to len + j.  path[j] >= j and path rises, so
+// row j's source is past every row written for j' < j: each thread copies its
+// columns in path order, and blocks share no columns.  Every block does the walk
+// for itself (a few LDS steps against a second launch); block (0, 0) writes it.
+// Grid (max(1, 2 * layers), column blocks, batch).
+__global__ __launch_bounds__(256) void k_tree_accept(TreeAccept a, LayerCaches lc, bool report) {
+    __shared__ int child[kMaxTreeNodes], path[kMaxTreeNodes];
+    __shared__ int count;
+    const int t = threadIdx.x, b = blockIdx.z, n = a.n;
+    const int32_t *par = a.parents + (size_t)b * n;
+    const int64_t *draft = a.draft + (size_t)b * n, *next = a.next + (size_t)b * n;
+    for (int i = t; i < n; i += 256) child[i] = n;
+    __syncthreads();
+    for (int i = t; i < n; i += 256) {
+        const int p = par[i];
+        if (p >= 0 && p < i && draft[i] >= 0 && draft[i] == next[p]) atomicMin(&child[p], i);
+    }
+    __syncthreads();
+    if (t == 0) {
+        int c = 0;
+        for (int at = par[0] == -1 ? 0 : n; at < n; at = child[at]) path[c++] = at;
+        count = c;
+    }
+    __syncthreads();
+    const int c = count;
+    if (report && blockIdx.x == 0 && blockIdx.y == 0) {
+        for (int i = t; i < n; i += 256) a.path[(size_t)b * n + i] = i < c ? path[i] : -1;
+        if (t == 0) {
+            a.n_path[b] = c;
+            a.token[b] = c ? next[path[c - 1]] : -1;
+        }
+    }
+    const int layer = blockIdx.x >> 1, col = blockIdx.y * 256 + t, per = a.hd / 4;
+    if (layer >= a.layers || col >= a.hkv * per) return;
+    const bool is_v = blockIdx.x & 1;
+    const TreeCache &ca = is_v ? a.v : a.k;
+    const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq);
+    float *base = (is_v ? lc.v[layer] : lc.k[layer]) + b * ca.sb + (col / per) * ca.sh + 4 * (col % per);
+    for (int j = 0; j < c; ++j) {
+        const int from = path[j];
+        if (from == j || len + from >= a.max_seq) continue;
+        *reinterpret_cast<float4 *>(base + (len + j) * ca.ss) =
+            *reinterpret_cast<const float4 *>(base + (len + from) * ca.ss);
+    }
+}
+
+}  // namespace
+
+int launch_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, int batch, int n,
+                      hipStream_t s) {
+    const int threads = std::min(1024, (n + 63) / 64 * 64);
+    hipLaunchKernelGGL(k_tree_masks, dim3(batch), dim3(threads), 0, s, parents, mask, depth, n);
+    TB_LAUNCHED();
+    return TB_OK;
+}
+
+int launch_tree_attention(const TreeAttn &a, hipStream_t s) {
+    hipLaunchKernelGGL(k_tree_attn, dim3(a.n * a.hq, a.batch), dim3(256), 0, s, a);
+    TB_LAUNCHED();
+    return TB_OK;
+}
+
+int launch_tree_accept(const TreeAccept &a, float *const *kc, float *const *vc, hipStream_t s) {
+    for (int l0 = 0; l0 == 0 || l0 < a.layers; l0 += kTreeLayersPerLaunch) {
+        TreeAccept p = a;
+        LayerCaches lc{};
+        p.layers = std::min(kTreeLayersPerLaunch, a.layers - l0);
+        for (int l = 0; l < p.layers; ++l) {
+            lc.k[l] = kc[l0 + l];
+            lc.v[l] = vc[l0 + l];
+        }
+        const dim3 grid(std::max(1, 2 * p.layers),
+                        p.layers ? (p.hkv * (p.hd / 4) + 255) / 256 : 1, p.batch);
+        hipLaunchKernelGGL(k_tree_accept, grid, dim3(256), 0, s, p, lc, l0 == 0);
+        TB_LAUNCHED();
+    }
+    return TB_OK;
+}
+
+}  // namespace tb
