@@ -409,13 +409,21 @@ TB_API int tb_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, 
  * end do not exist), or NULL: kv_len for every sequence, and TB_ERR_VALUE when
  * kv_len + n > max_seq.  head_dim a multiple of 32 up to 256; q, out and the
  * caches 16-byte aligned.
+ * scratch: tb_tree_attention_scratch bytes of device memory, 16-byte aligned
+ * (max_len: kv_len + n, or max_seq with kv_lens); NULL: the stream's workspace
+ * (TB_ERR_UNSUPPORTED while capturing, since graphs that are replayed side by
+ * side would share it).
  */
+TB_API int64_t tb_tree_attention_scratch(int64_t batch, int64_t n, int64_t num_heads,
+                                         int64_t num_kv_heads, int64_t head_dim,
+                                         int64_t max_len);
 TB_API int tb_tree_attention(const float *q, const float *k_cache, const float *v_cache,
                              const int32_t *mask, const int32_t *kv_lens, float *out,
                              int64_t batch, int64_t n, int64_t num_heads, int64_t num_kv_heads,
                              int64_t head_dim, int64_t max_seq, int64_t kv_len, int64_t k_sb,
                              int64_t k_sh, int64_t k_ss, int64_t v_sb, int64_t v_sh, int64_t v_ss,
-                             int64_t mask_sb, float scale, void *stream);
+                             int64_t mask_sb, float scale, void *scratch,
+                             int64_t scratch_bytes, void *stream);
 
 /*
  * Acceptance: the path starts at node 0 (which must be a root) and goes from a

@@ -20,7 +20,7 @@ def masks(**kw):
 def attention(**kw):
     a = dict(q=A, k=A, v=A, mask=A, kv_lens=None, out=A, batch=1, n=4, heads=4, kv_heads=2, hd=64,
              max_seq=32, kv_len=8, k_sb=4096, k_sh=2048, k_ss=64, v_sb=4096, v_sh=2048, v_ss=64,
-             mask_sb=0, scale=1.0)
+             mask_sb=0, scale=1.0, scratch=None, size=0)
     a.update(kw)
     return _lib.lib().tb_tree_attention(*a.values(), None)
 
@@ -59,6 +59,8 @@ U, V = _lib.TB_ERR_UNSUPPORTED, _lib.TB_ERR_VALUE
     (attention, dict(n=1025), U, b"1024"), (attention, dict(k_ss=66), U, b"strides"),
     (attention, dict(v_sh=-64), U, b"strides"), (attention, dict(kv_len=29), V, b"exceed"),
     (attention, dict(kv_len=-1), V, b"exceed"), (attention, dict(max_seq=(1 << 30) + 1), U, b"max_seq"),
+    (attention, dict(scratch=A, size=8, max_seq=4096, kv_len=2000), U, b"scratch"),
+    (attention, dict(scratch=A + 8, size=1 << 40, max_seq=4096, kv_len=2000), U, b"scratch"),
     (accept, dict(parents=None), U, b"null"), (accept, dict(token=None), U, b"null"),
     (accept, dict(n=0), U, b"empty"), (accept, dict(n=1025), U, b"1024"),
     (accept, dict(kv_len=30), V, b"exceed"), (accept, dict(layers=-1), U, b"layers"),

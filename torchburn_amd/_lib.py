@@ -68,7 +68,7 @@ _SIGS = {
                                      [_i64] * 6 + [_p],
     "tb_fused_transformer_layer_step_w4a32": [_p] * 22 + [_i64] * 8 + [C.c_double, _p],
     "tb_tree_masks": [_p, _p, _p, _i64, _i64, _p],
-    "tb_tree_attention": [_p] * 6 + [_i64] * 14 + [C.c_float, _p],
+    "tb_tree_attention": [_p] * 6 + [_i64] * 14 + [C.c_float, _p, _i64, _p],
     "tb_tree_accept": [_p] * 4 + [_i64] + [_p] * 5 + [_i64] * 12 + [_p],
     "tb_process_logits": [_p] * 3 + [_i64] * 2 + [_p] * 3 + [_i64] * 3 + [C.c_float] * 3 +
                          [_p] * 5 + [_i64] * 2 + [_p, _i64, _p, _p, _i64, _p, _i64, _p],
@@ -78,7 +78,7 @@ _SIGS = {
 def declared_symbols() -> list:
     """Every entry point the Python layer binds (all are declared in include/tbhip.h)."""
     return ["tb_last_error", "tb_version", "tb_x_records_bytes", "tb_sample_uniform",
-            "tb_w4_kernel", "tb_process_logits_scratch",
+            "tb_w4_kernel", "tb_process_logits_scratch", "tb_tree_attention_scratch",
             *_SIGS.keys()]
 
 
@@ -101,6 +101,8 @@ def lib():
             L.tb_w4_kernel.argtypes = [C.c_int64] * 5
             L.tb_process_logits_scratch.restype = C.c_int64
             L.tb_process_logits_scratch.argtypes = [C.c_int64] * 2
+            L.tb_tree_attention_scratch.restype = C.c_int64
+            L.tb_tree_attention_scratch.argtypes = [C.c_int64] * 6
             L.tb_sample_uniform.restype = C.c_float
             L.tb_sample_uniform.argtypes = [C.c_uint64, C.c_uint64]
             for name, args in _SIGS.items():

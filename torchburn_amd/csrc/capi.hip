@@ -1232,12 +1232,22 @@ int tb_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, int64_t
     return launch_tree_masks(parents, mask, depth, (int)batch, (int)n, (hipStream_t)stream);
 }
 
+int64_t tb_tree_attention_scratch(int64_t batch, int64_t n, int64_t num_heads,
+                                  int64_t num_kv_heads, int64_t head_dim, int64_t max_len) {
+    if (batch <= 0 || batch > 65535 || n <= 0 || n > kMaxTreeNodes || num_kv_heads <= 0 ||
+        num_heads <= 0 || num_heads > 65535 || num_heads % num_kv_heads || head_dim <= 0 ||
+        head_dim > 256 || max_len < 0 || max_len > (1 << 30))
+        return 0;
+    return (int64_t)tree_attention_scratch((int)batch, (int)n, (int)num_heads, (int)num_kv_heads,
+                                           (int)head_dim, (int)max_len);
+}
+
 int tb_tree_attention(const float *q, const float *k_cache, const float *v_cache,
                       const int32_t *mask, const int32_t *kv_lens, float *out, int64_t batch,
                       int64_t n, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
                       int64_t max_seq, int64_t kv_len, int64_t k_sb, int64_t k_sh, int64_t k_ss,
                       int64_t v_sb, int64_t v_sh, int64_t v_ss, int64_t mask_sb, float scale,
-                      void *stream) {
+                      void *scratch, int64_t scratch_bytes, void *stream) {
     int rc = check_tree("tree_attention", batch, n);
     if (!rc) rc = check_cache("tree_attention", num_kv_heads, head_dim, max_seq, {k_sb, k_sh, k_ss},
                               {v_sb, v_sh, v_ss});
@@ -1262,7 +1272,20 @@ int tb_tree_attention(const float *q, const float *k_cache, const float *v_cache
     a.out = out;
     a.batch = (int)batch; a.n = (int)n; a.hq = (int)num_heads; a.hkv = (int)num_kv_heads;
     a.hd = (int)head_dim; a.max_seq = (int)max_seq; a.scale = scale;
-    return launch_tree_attention(a, (hipStream_t)stream);
+    const int max_len = kv_lens ? a.max_seq : (int)(kv_len + n);
+    const size_t need = tree_attention_scratch(a.batch, a.n, a.hq, a.hkv, a.hd, max_len);
+    hipStream_t st = (hipStream_t)stream;
+    WsLease lease;
+    if (need && !scratch) {
+        TB_REQUIRE(!capturing(st), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: tree_attention: a captured call needs scratch of its own");
+        if ((rc = workspace(need, st, lease))) return rc;
+        scratch = lease.ptr;
+    } else if (need) {
+        TB_REQUIRE(scratch_bytes >= (int64_t)need && aligned(scratch, 16), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: tree_attention: scratch too short or not 16-byte aligned");
+    }
+    return launch_tree_attention(a, max_len, static_cast<float *>(scratch), st);
 }
 
 int tb_tree_accept(const int32_t *parents, const int64_t *draft_tokens, const int64_t *next_tokens,

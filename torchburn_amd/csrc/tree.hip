@@ -1,6 +1,6 @@
-// Speculative decoding over a drafted tree, the device side: ancestor masks from
-// the parent list, attention of the tree's nodes over the cached prefix and their
-// own ancestors, and acceptance, which keeps one path of the tree in the cache.
+// Speculative decoding over a drafted tree: ancestor masks from the parent list,
+// and acceptance, which keeps one path of the tree in the cache (the attention
+// between them is tree_attn.hip).
 //
 // A tree's n nodes are in topological order: parents[i] is -1 (a root: a child
 // of the prefix's last token) or an earlier node.  Anything else marks node i
@@ -49,71 +49,6 @@ __global__ void k_tree_masks(const int32_t *__restrict__ parents, int32_t *__res
         }
         depth[b * n + i] = live ? d : 0;
     }
-}
-
-// ---- attention --------------------------------------------------------------
-
-__device__ __forceinline__ int prefix_len(const int32_t *lens, int len, int b, int max_seq) {
-    const int l = lens ? lens[b] : len;
-    return min(max(l, 0), max_seq);
-}
-
-// One block per query row (sequence, node, head): tiles of 256 keys, a key per
-// thread for the scores, an output column per thread for P V.  A row without
-// mask bits is padding and gives zeros; keys that a row does not see take no
-// part, whatever their K / V rows hold.
-__global__ __launch_bounds__(256) void k_tree_attn(TreeAttn a) {
-    __shared__ float qs[256], ps[256], red[8];
-    __shared__ int any_bits;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int node = blockIdx.x / a.hq, h = blockIdx.x % a.hq, b = blockIdx.y;
-    const int kvh = h / (a.hq / a.hkv), words = (a.n + 31) / 32;
-    const size_t row = ((size_t)b * a.n + node) * a.hq + h;
-    const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq);
-    const int end = min(len + a.n, a.max_seq);
-    const int32_t *mrow = a.mask + b * a.mask_sb + (int64_t)node * words;
-    const float *kb = a.k.p + b * a.k.sb + kvh * a.k.sh, *vb = a.v.p + b * a.v.sb + kvh * a.v.sh;
-    if (t == 0) any_bits = 0;
-    if (t < a.hd) qs[t] = a.q[row * a.hd + t] * a.scale;
-    __syncthreads();
-    for (int w = t; w < words; w += 256)
-        if (mrow[w]) any_bits = 1;
-    __syncthreads();
-    const bool live = any_bits != 0;
-    float m = -INFINITY, l = 0.f, o = 0.f;
-    for (int p0 = 0; live && p0 < end; p0 += 256) {
-        const int p = p0 + t;
-        float s = -INFINITY;
-        const bool see = p < len || (p < end && ((uint32_t)mrow[(p - len) >> 5] >> ((p - len) & 31) & 1));
-        if (see) {
-            const float4 *kr = reinterpret_cast<const float4 *>(kb + p * a.k.ss);
-            s = 0.f;
-            for (int c = 0; c < a.hd / 4; ++c) {
-                const float4 x = kr[c];
-                s += qs[4 * c] * x.x + qs[4 * c + 1] * x.y + qs[4 * c + 2] * x.z + qs[4 * c + 3] * x.w;
-            }
-        }
-        float top = s;
-        for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-        if (lane == 0) red[wave] = top;
-        __syncthreads();
-        const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        const float pj = see ? expf(s - (mn == -INFINITY ? 0.f : mn)) : 0.f;
-        ps[t] = pj;
-        float sum = pj;
-        for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off);
-        if (lane == 0) red[4 + wave] = sum;
-        __syncthreads();
-        const float alpha = m == mn ? 1.f : expf(m - mn);
-        l = l * alpha + (red[4] + red[5]) + (red[6] + red[7]);
-        o *= alpha;
-        m = mn;
-        if (t < a.hd)
-            for (int j = 0; j < min(256, end - p0); ++j)
-                if (ps[j] != 0.f) o += ps[j] * vb[(p0 + j) * a.v.ss + t];
-        __syncthreads();
-    }
-    if (t < a.hd) a.out[row * a.hd + t] = l > 0.f || l != l ? o / l : 0.f;
 }
 
 // ---- acceptance -------------------------------------------------------------
@@ -179,12 +114,6 @@ int launch_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, int
                       hipStream_t s) {
     const int threads = std::min(1024, (n + 63) / 64 * 64);
     hipLaunchKernelGGL(k_tree_masks, dim3(batch), dim3(threads), 0, s, parents, mask, depth, n);
-    TB_LAUNCHED();
-    return TB_OK;
-}
-
-int launch_tree_attention(const TreeAttn &a, hipStream_t s) {
-    hipLaunchKernelGGL(k_tree_attn, dim3(a.n * a.hq, a.batch), dim3(256), 0, s, a);
     TB_LAUNCHED();
     return TB_OK;
 }

@@ -33,7 +33,16 @@ struct TreeAttn {
     float scale;
 };
 
-int launch_tree_attention(const TreeAttn &a, hipStream_t s);
+// Scratch for keys up to position max_len (kv_len + n, or max_seq where the
+// lengths are on the device); 0 where one block walks all of them.
+size_t tree_attention_scratch(int batch, int n, int hq, int hkv, int hd, int max_len);
+int launch_tree_attention(const TreeAttn &a, int max_len, float *scratch, hipStream_t s);
+
+// The length of sequence b's prefix, inside the cache whatever the device holds.
+__device__ __forceinline__ int prefix_len(const int32_t *lens, int len, int b, int max_seq) {
+    const int l = lens ? lens[b] : len;
+    return min(max(l, 0), max_seq);
+}
 
 struct TreeAccept {
     const int32_t *parents;          // [batch][n]

@@ -107,10 +107,14 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     lens, ln = _kv_len(op, kv_len, batch, dev)
     out = torch.empty(x.shape, dtype=torch.float32, device=dev)
     ks, vs = kc.stride(), vc.stride()
+    # scratch of this call's own, so that graphs captured on one stream share none
+    size = _lib.lib().tb_tree_attention_scratch(batch, n, heads, kc.shape[1], hd,
+                                                kc.shape[2] if lens is not None else ln + n)
+    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
     _lib.call_on(dev, "tb_tree_attention", _ptr(x), _ptr(kc), _ptr(vc), _ptr(mk), _ptr(lens),
                  _ptr(out), batch, n, heads, kc.shape[1], hd, kc.shape[2], ln, ks[0], ks[1], ks[2],
                  vs[0], vs[1], vs[2], n * words if mk.ndim == 3 else 0,
-                 hd ** -0.5 if scale is None else float(scale), _stream(dev))
+                 hd ** -0.5 if scale is None else float(scale), _ptr(scratch), size, _stream(dev))
     return out if q.is_cuda else out.to(q.device)
 
 
