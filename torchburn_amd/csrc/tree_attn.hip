@@ -27,9 +27,9 @@ namespace tb {
 namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 32;        // positions per tile of one wave
 constexpr int kMaxSplits = 128;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kTop = 14;         // factors are scaled to below 2^(kTop + 1)
@@ -73,97 +73,193 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
     return __builtin_amdgcn_readfirstlane(v);
 }
 
-// Tiles of one split: whole rounds of the block's four waves.
-__host__ __device__ inline int tiles_per_split(int tiles, int nsplit) {
-    return ((tiles + nsplit - 1) / nsplit + 3) / 4 * 4;
+// Position j of lane group g's scores among a tile's.
+__device__ __forceinline__ int position(int j, int g) {
+    return 32 * (j >> 3) + 16 * (j >> 2 & 1) + 4 * g + (j & 3);
 }
 
-// A block takes 16 * RB query rows of one KV head, a row being a (node, head of
-// the group) pair i = node * G + head, and a range of the positions.  Its four
-// waves take tiles of 32 positions in turn, each with its own running maximum,
-// sum and output; they meet in LDS once at the end.  So nothing in the loop
-// waits for another wave, and K and V go from memory to MFMA operands in
-// registers:
-//   lane (g, c) = (lane / 16, lane % 16) has A[c][8g ..] and B[8g ..][c] of a
-//   product of depth 32, and gets D[4g + r][c] in register r;
+// Which of the positions p0 .. p0 + 31 a row sees, as bits.
+__device__ __forceinline__ uint32_t seen(const int32_t *mrow, int words, int p0, int len, int end) {
+    const int at = p0 - len;   // the tree's bit of the first one
+    uint32_t see = 0;
+    if (at <= -32) {
+        see = ~0u;
+    } else if (at < 0) {
+        see = ((1u << -at) - 1) | (uint32_t)mrow[0] << -at;
+    } else if (at >> 5 < words) {
+        const int w = at >> 5, sh = at & 31;
+        see = (uint32_t)mrow[w] >> sh;
+        if (sh && w + 1 < words) see |= (uint32_t)mrow[w + 1] << (32 - sh);
+    }
+    if (end - p0 < 32) see = end > p0 ? see & ((1u << (end - p0)) - 1) : 0;
+    return see;
+}
+
+// Positions per tile: the same bytes for every head_dim up to 128.
+__host__ __device__ constexpr int tile_of(int dp) { return dp == 64 ? 64 : 32; }
+// Tiles per split where at most `cap` splits are wanted.  Only the sequence's own
+// length counts, so a result is the same whatever the cache's size.
+constexpr int kMinTiles = 4;
+__host__ __device__ inline int tiles_per_split(int tiles, int cap) {
+    const int t = (tiles + cap - 1) / cap;
+    return t < kMinTiles ? kMinTiles : t;
+}
+
+// A block takes 64 * RB query rows of one KV head, a row being a (node, head of
+// the group) pair i = node * G + head, 16 * RB of them a wave, and a range of
+// the positions in tiles of TK.  Per tile the four waves build the limbs of a
+// quarter of K and of V each, in LDS and in MFMA operand order, and then every
+// wave multiplies all of them with its rows: so each f32 of the cache is read
+// and split once a block.  Two buffers, one barrier a tile: while tile i is
+// multiplied, tile i + 1 goes from registers to the other buffer and tile i + 2
+// is requested.
+//   Lane (g, c) = (lane / 16, lane % 16) has A[c][8g ..] and B[8g ..][c] of a
+//   product of depth 32, and gets D[4g + r][c] in register r:
 //   S^T = K Q^T: A = 16 positions, position c with the 8 dimensions 4g.. and
-//     16 + 4g.. of each 32 (a K row is read in whole 64-byte pieces); B = the
-//     query rows, from LDS in operand order;
-//   O^T = V^T P^T: A's row c of block (b, j) is dimension 64 b + 4 c + j and its
-//     depth 8g + i is position 4g + i (i < 4) or 16 + 4g + i - 4, the positions
-//     whose scores the lane holds for row c, so P^T needs no exchange and a V
-//     row is read in 256-byte pieces.
-// The next tile's K is requested when this one's limbs are built, V likewise.
+//     16 + 4g.. of each 32 (K rows are read in whole 64-byte pieces); B = the
+//     wave's query rows, in registers;
+//   O^T = V^T P^T: A's row c of block (q, j) is dimension 64 q + 4 c + j and its
+//     depth 8g + i is position 4g + i (i < 4) or 16 + 4g + i - 4 of 32: the
+//     positions whose scores the lane holds for row c, so P^T needs no exchange
+//     and V rows are read in whole 256-byte pieces.
+// Each wave's quarter has a scale of its own: a quarter of K is 8 positions
+// 16 (w / 2) + 8 (w % 2) .. of every 32, one of V the positions of lane group
+// g = w, so a lane needs two scales for its scores and one for its weights.
 //
 // A tile with infinities (or NaN, behind the prefix) takes its sums one by one
 // in f32, so that positions that a row does not see stay out of its result.
 template <int DP, int RB>
-__global__ __launch_bounds__(256, RB * DP <= 64 ? 2 : 1) void k_tree_attn(TreeAttn a, int nsplit,
-                                                                         float *__restrict__ part,
-                                                                         float *__restrict__ pml) {
-    constexpr int NS = DP / 32, NB = DP / 64, ROWS = 16 * RB;
-    __shared__ __attribute__((aligned(16))) float lds[ROWS * DP];   // Q limbs; then the outputs
-    __shared__ float sm[4][ROWS], sl[4][ROWS];
+__global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
+    TreeAttn a, int cap, float *__restrict__ part, float *__restrict__ pml) {
+    constexpr int NS = DP / 32, NB = DP / 64, TK = tile_of(DP), KT = TK / 32;
+    constexpr int KU = KT * NS / 2, VU = KT * NB / 2;   // operands of 8 K values, 16 V values a lane
+    __shared__ f16x8 sk[2][KT * 2 * NS * 2 * 64];       // [32 positions][16][32 dims][limb][lane]
+    __shared__ f16x8 sv[2][KT * NB * 4 * 2 * 64];       // [32 positions][64 dims][j][limb][lane]
+    __shared__ int se[2][2][4], bad[2][2][4];           // K's, V's quarters: exponent, not finite
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, g = lane >> 4;
     const int G = a.hq / a.hkv, R = a.n * G, D = a.hd, words = (a.n + 31) / 32;
-    const int split = blockIdx.x, kvh = blockIdx.y % a.hkv, i0 = blockIdx.y / a.hkv * ROWS;
-    const int b = blockIdx.z;
+    const int split = blockIdx.x, kvh = blockIdx.y % a.hkv, b = blockIdx.z;
+    const int w0 = (blockIdx.y / a.hkv * 4 + wave) * 16 * RB;   // the wave's first row
     const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
-    const int tiles = (end + kTile - 1) / kTile, tps = tiles_per_split(tiles, nsplit);
+    const int tiles = (end + TK - 1) / TK, tps = tiles_per_split(tiles, cap);
     const int t0 = split * tps, t1 = min(tiles, t0 + tps);
     if (split > 0 && t0 >= t1) return;   // the merge skips this split
-    const float *kb = a.k.p + b * a.k.sb + kvh * a.k.sh + 4 * g;
-    const float *vb = a.v.p + b * a.v.sb + kvh * a.v.sh + 4 * c;
+    const float *kb = a.k.p + b * a.k.sb + kvh * a.k.sh, *vb = a.v.p + b * a.v.sb + kvh * a.v.sh;
 
-    float kr[2][NS][8], vr[8][NB][4];
+    // ---- this thread's part of a tile
+    const int kkey = 16 * (wave >> 1) + 8 * (wave & 1) + (lane & 7), kg = lane >> 3 & 3;
+    const int kx = lane >> 5;             // K: dimension block's parity
+    const int half = lane & 1, vc = lane >> 1 & 15, vx = lane >> 5;
+    float kr[KU][8], vr[VU][4][4];
+    auto load = [&](int tile) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
+        for (int u = 0; u < KU; ++u) {
+            const int sub = KT == 2 ? u : 0, s = KT == 2 ? kx : kx + 2 * u;
+            const float *r = kb + min(tile * TK + 32 * sub + kkey, end - 1) * a.k.ss + 4 * kg;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+            if (32 * s < D) {
+                x = *reinterpret_cast<const float4 *>(r + 32 * s);
+                y = *reinterpret_cast<const float4 *>(r + 32 * s + 16);
+            }
+            kr[u][0] = x.x; kr[u][1] = x.y; kr[u][2] = x.z; kr[u][3] = x.w;
+            kr[u][4] = y.x; kr[u][5] = y.y; kr[u][6] = y.z; kr[u][7] = y.w;
+        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) kr[0][s][j] = kr[1][s][j] = 0.f;
+        for (int u = 0; u < VU; ++u) {
+            const int sub = KT == 2 ? vx : 0, q = KT == 2 ? 0 : vx + 2 * u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int q = 0; q < NB; ++q)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) vr[i][q][j] = 0.f;
-    auto load_k = [&](int tile) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float *r = kb + min(tile * kTile + 16 * h + c, end - 1) * a.k.ss;
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                if (32 * s < D) {
-                    const float4 x = *reinterpret_cast<const float4 *>(r + 32 * s);
-                    const float4 y = *reinterpret_cast<const float4 *>(r + 32 * s + 16);
-                    float *k = kr[h][s];
-                    k[0] = x.x; k[1] = x.y; k[2] = x.z; k[3] = x.w;
-                    k[4] = y.x; k[5] = y.y; k[6] = y.z; k[7] = y.w;
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int p = min(tile * TK + 32 * sub + 16 * half + 4 * wave + i, end - 1);
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (64 * q + 4 * vc < D)
+                    x = *reinterpret_cast<const float4 *>(vb + p * a.v.ss + 64 * q + 4 * vc);
+                vr[u][i][0] = x.x; vr[u][i][1] = x.y; vr[u][i][2] = x.z; vr[u][i][3] = x.w;
+            }
         }
     };
-    auto load_v = [&](int tile) {
+    auto store = [&](int tile, int buf) {
+        const bool open = (tile + 1) * TK <= len;
+        float km = 0.f, vm = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int p = min(tile * kTile + (i < 4 ? 4 * g + i : 12 + 4 * g + i), end - 1);
-            const float *r = vb + p * a.v.ss;
+        for (int u = 0; u < KU; ++u)
 #pragma unroll
-            for (int q = 0; q < NB; ++q)
-                if (64 * q + 4 * c < D) {
-                    const float4 x = *reinterpret_cast<const float4 *>(r + 64 * q);
-                    vr[i][q][0] = x.x; vr[i][q][1] = x.y; vr[i][q][2] = x.z; vr[i][q][3] = x.w;
+            for (int j = 0; j < 8; j += 2) max3_abs(km, kr[u][j], kr[u][j + 1]);
+#pragma unroll
+        for (int u = 0; u < VU; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                max3_abs(vm, vr[u][i][0], vr[u][i][1]);
+                max3_abs(vm, vr[u][i][2], vr[u][i][3]);
+            }
+        uint32_t kt = wave_max_bits(abs_bits(km)), vt = abs_bits(vm);
+        if (!open) {   // NaN in V too: a row that does not see its position must not get it
+#pragma unroll
+            for (int u = 0; u < VU; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) vt = max(vt, abs_bits(vr[u][i >> 2][i & 3]));
+        }
+        vt = wave_max_bits(vt);
+        const bool bad_k = kt >= kInf, bad_v = vt >= kInf;
+        if (bad_v) {   // the finite values' scale
+            vt = 0;
+#pragma unroll
+            for (int u = 0; u < VU; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t x = abs_bits(vr[u][i >> 2][i & 3]);
+                    vt = max(vt, x < kInf ? x : 0u);
                 }
+            vt = wave_max_bits(vt);
+        }
+        const int ke = exponent(kt), ve = exponent(vt);
+        if (lane == 0) {
+            se[buf][0][wave] = ke;
+            se[buf][1][wave] = ve;
+            bad[buf][0][wave] = bad_k;
+            bad[buf][1][wave] = bad_v;
+        }
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int sub = KT == 2 ? u : 0, s = KT == 2 ? kx : kx + 2 * u;
+            f16x8 hi, lo;
+            split8(kr[u], pow2(kTop - ke), hi, lo);
+            f16x8 *d = sk[buf] + (((sub * 2 + (wave >> 1)) * NS + s) * 2) * 64 + 16 * kg +
+                       8 * (wave & 1) + (lane & 7);
+            d[0] = hi;
+            d[64] = lo;
+        }
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+            const int sub = KT == 2 ? vx : 0, q = KT == 2 ? 0 : vx + 2 * u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f16x4 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    hi[i] = (_Float16)__builtin_fmaf(vr[u][i][j], pow2(kTop - ve), 0.f);
+                    lo[i] = (_Float16)__builtin_fmaf(vr[u][i][j], pow2(kTop - ve), -(float)hi[i]);
+                }
+                f16x4 *d = reinterpret_cast<f16x4 *>(
+                               sv[buf] + (((sub * NB + q) * 4 + j) * 2) * 64 + 16 * wave + vc) + half;
+                d[0] = hi;
+                d[128] = lo;
+            }
         }
     };
-    const int first = t0 + wave;
-    if (first < t1) {
-        load_k(first);
-        load_v(first);
-    }
+    if (t0 < t1) load(t0);
 
-    // The query rows' limbs, in B-operand order: [row block][32 dimensions][limb][lane].
-    f16x8 *qs = reinterpret_cast<f16x8 *>(lds);
-    for (int rb = wave; rb < RB; rb += 4) {
-        const int i = i0 + 16 * rb + c, iq = i < R ? i : 0;
+    // ---- the wave's query rows, row c of each block in this lane
+    f16x8 qh[RB][NS], ql[RB][NS];
+    const int32_t *mrow[RB];
+    bool live[RB];
+    float m[RB], l[RB];
+    int qe[RB];
+    f32x4 o[RB][NB][4];
+    const uint32_t last_bits = a.n % 32 ? (1u << (a.n % 32)) - 1 : ~0u;
+    const bool busy = w0 < R;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int i = w0 + 16 * rb + c, iq = i < R ? i : 0;
         const float *q = a.q + (((size_t)b * a.n + iq / G) * a.hq + kvh * G + iq % G) * D + 4 * g;
         float x[NS][8];
         float top = 0.f;
@@ -179,27 +275,10 @@ __global__ __launch_bounds__(256, RB * DP <= 64 ? 2 : 1) void k_tree_attn(TreeAt
 #pragma unroll
             for (int j = 0; j < 8; j += 2) max3_abs(top, x[s][j], x[s][j + 1]);
         }
-        const int e = exponent(__float_as_uint(max_over_groups(top)));
-        if (g == 0) sm[0][16 * rb + c] = __int_as_float(e);
+        qe[rb] = exponent(abs_bits(max_over_groups(top)));
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            f16x8 hi, lo;
-            split8(x[s], pow2(kTop - e), hi, lo);
-            qs[((rb * NS + s) * 2 + 0) * 64 + lane] = hi;
-            qs[((rb * NS + s) * 2 + 1) * 64 + lane] = lo;
-        }
-    }
-    // Per row block: the lane's row c.
-    const int32_t *mrow[RB];
-    bool live[RB];
-    float m[RB], l[RB];
-    int qe[RB];
-    f32x4 o[RB][NB][4];
-    const uint32_t last_bits = a.n % 32 ? (1u << (a.n % 32)) - 1 : ~0u;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const int i = i0 + 16 * rb + c;
-        mrow[rb] = a.mask + b * a.mask_sb + (int64_t)((i < R ? i : 0) / G) * words;
+        for (int s = 0; s < NS; ++s) split8(x[s], pow2(kTop - qe[rb]), qh[rb][s], ql[rb][s]);
+        mrow[rb] = a.mask + b * a.mask_sb + (int64_t)(iq / G) * words;
         uint32_t any = 0;
         for (int w = g; w < words; w += 4)
             any |= (uint32_t)mrow[rb][w] & (w == words - 1 ? last_bits : ~0u);
@@ -211,277 +290,219 @@ __global__ __launch_bounds__(256, RB * DP <= 64 ? 2 : 1) void k_tree_attn(TreeAt
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[rb][q][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    __syncthreads();
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) qe[rb] = __float_as_int(sm[0][16 * rb + c]);
-    int ve = 0, ve_top = -1000;   // exponent of the outputs' scale; the largest one so far
+    int oe = 0, oe_top = -1000;   // exponent of the outputs' scale; the largest V's so far
     const float f = a.scale * kLog2e;
 
-    for (int tile = first; tile < t1; tile += 4) {
-        const int p0 = tile * kTile;
-        const bool open = p0 + kTile <= len;   // every live row sees every position
-        // ---- K: the tile's scale, its limbs, the next tile's request
-        uint32_t top;
-        {
-            float mx = 0.f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int s = 0; s < NS; ++s)
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) max3_abs(mx, kr[h][s][j], kr[h][s][j + 1]);
-            top = wave_max_bits(__float_as_uint(mx) & 0x7FFFFFFFu);
-        }
-        const bool slow_k = top >= kInf;
-        const int ke = exponent(top);
-        f16x8 kh[2][NS], kl[2][NS];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int s = 0; s < NS; ++s) split8(kr[h][s], pow2(kTop - ke), kh[h][s], kl[h][s]);
-        if (tile + 4 < t1) load_k(tile + 4);
-        // ---- scores, running maxima, weights
-        f16x8 ph[RB], pl[RB];
-        float alpha[RB];
-        bool moved = false;
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-            float s8[8];
+    if (t0 < t1) {
+        store(t0, 0);
+        if (t0 + 1 < t1) load(t0 + 1);
+        __syncthreads();
+    }
+    for (int tile = t0; tile < t1; ++tile) {
+        const int buf = (tile - t0) & 1, p0 = tile * TK;
+        if (busy) {
+            const bool open = p0 + TK <= len;   // every live row sees every position
+            const int ke[2] = {se[buf][0][g >> 1], se[buf][0][2 + (g >> 1)]};
+            const int ve = se[buf][1][g];
+            const bool slow_k = bad[buf][0][0] | bad[buf][0][1] | bad[buf][0][2] | bad[buf][0][3];
+            const bool slow_v = bad[buf][1][0] | bad[buf][1][1] | bad[buf][1][2] | bad[buf][1][3];
+            // ---- scores
+            float s8[RB][8 * KT];
             if (!slow_k) {
 #pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    const f16x8 qh = qs[((rb * NS + s) * 2 + 0) * 64 + lane];
-                    const f16x8 ql = qs[((rb * NS + s) * 2 + 1) * 64 + lane];
+                for (int sub = 0; sub < KT; ++sub) {
+                    f32x4 acc[RB][2];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[h][s], qh, acc[h], 0, 0, 0);
-                        acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[h][s], ql, acc[h], 0, 0, 0);
-                        acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[h][s], qh, acc[h], 0, 0, 0);
+                    for (int rb = 0; rb < RB; ++rb)
+                        acc[rb][0] = acc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) {
+                        f16x8 kh[2], kl[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            kh[h] = sk[buf][(((sub * 2 + h) * NS + s) * 2 + 0) * 64 + lane];
+                            kl[h] = sk[buf][(((sub * 2 + h) * NS + s) * 2 + 1) * 64 + lane];
+                        }
+#pragma unroll
+                        for (int x = 0; x < 3; ++x)
+#pragma unroll
+                            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    acc[rb][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                        x == 0 ? kl[h] : kh[h], x == 1 ? ql[rb][s] : qh[rb][s],
+                                        acc[rb][h], 0, 0, 0);
                     }
-                }
-                const float fx = ldexpf(f, qe[rb] + ke - 2 * kTop);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) s8[j] = acc[j >> 2][j & 3] * fx;
+                    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float x = ldexpf(f, qe[rb] + ke[h] - 2 * kTop);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                s8[rb][8 * sub + 4 * h + r] = acc[rb][h][r] * x;
+                        }
+                }
             } else {
-                const int i = min(i0 + 16 * rb + c, R - 1);
-                const float *q = a.q + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int p = min(p0 + (j < 4 ? 4 * g + j : 12 + 4 * g + j), end - 1);
-                    const float *k = a.k.p + b * a.k.sb + kvh * a.k.sh + p * a.k.ss;
-                    float s = 0.f;
-                    for (int d = 0; d < D; ++d) s = fmaf(q[d], k[d], s);
-                    s8[j] = s * f;
-                }
-            }
-            if (!open) {
-                // 32 bits: which of the tile's positions row c sees
-                uint32_t see = 0;
-                const int at = p0 - len;   // the tree's bit of the tile's first position
-                if (live[rb]) {
-                    if (at < 0) {
-                        see = (1u << -at) - 1;
-                        see |= (uint32_t)mrow[rb][0] << -at;
-                    } else {
-                        const int w = at >> 5, sh = at & 31;
-                        see = (uint32_t)mrow[rb][w] >> sh;
-                        if (sh && w + 1 < words) see |= (uint32_t)mrow[rb][w + 1] << (32 - sh);
-                    }
-                    if (end - p0 < 32) see &= (1u << (end - p0)) - 1;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (!(see >> (j < 4 ? 4 * g + j : 12 + 4 * g + j) & 1)) s8[j] = -INFINITY;
-            }
-            float mt = s8[0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) mt = fmaxf(mt, s8[j]);
-            const float mn = fmaxf(m[rb], max_over_groups(mt));
-            const float base = mn == -INFINITY ? 0.f : mn;   // nothing seen so far: every weight 0
-            alpha[rb] = __builtin_amdgcn_exp2f(m[rb] - base);
-            moved |= m[rb] != mn;
-            m[rb] = mn;
-            float sum = 0.f;
-            float p8[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                p8[j] = __builtin_amdgcn_exp2f(s8[j] - base);
-                sum += p8[j];
-            }
-            l[rb] = fmaf(l[rb], alpha[rb], sum);
-            split8(p8, pow2(kTop), ph[rb], pl[rb]);
-        }
-        // ---- V: the tile's scale, the outputs' rescale, the limbs, the next request
-        if (open) {
-            float mx = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int q = 0; q < NB; ++q) {
-                    max3_abs(mx, vr[i][q][0], vr[i][q][1]);
-                    max3_abs(mx, vr[i][q][2], vr[i][q][3]);
-                }
-            top = __float_as_uint(mx) & 0x7FFFFFFFu;
-        } else {   // NaN too: a row that does not see its position must not get it
-            top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int q = 0; q < NB; ++q)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) top = max(top, abs_bits(vr[i][q][j]));
-        }
-        top = wave_max_bits(top);
-        const bool slow_v = top >= kInf;
-        if (slow_v) {   // the finite values' scale
-            top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int q = 0; q < NB; ++q)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t x = abs_bits(vr[i][q][j]);
-                        top = max(top, x < kInf ? x : 0u);
-                    }
-            top = wave_max_bits(top);
-        }
-        // The outputs keep their scale while the tile fits it and loses at most 6
-        // bits of range to it; 64 bits below the largest scale it stays (their f32
-        // must not overflow).
-        const int e = exponent(top);
-        ve_top = max(ve_top, e);
-        int down = 0;
-        if (e > ve || e < ve - 6) {
-            const int to = max(e, ve_top - 64);
-            down = ve - to;
-            ve = to;
-        }
-        if (__any(moved) || down != 0) {
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                const float x = ldexpf(alpha[rb], min(down, 120));
-#pragma unroll
-                for (int q = 0; q < NB; ++q)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[rb][q][j] *= x;
-            }
-        }
-        if (!slow_v) {
-#pragma unroll
-            for (int q = 0; q < NB; ++q) {
-                f16x8 vh[4], vl[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float x[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = vr[i][q][j];
-                    split8(x, pow2(kTop - ve), vh[j], vl[j]);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) {
-                        f32x4 &x = o[rb][q][j];
-                        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[j], ph[rb], x, 0, 0, 0);
-                        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[j], pl[rb], x, 0, 0, 0);
-                        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh[j], ph[rb], x, 0, 0, 0);
-                    }
-            }
-        } else {
-            const float *v = a.v.p + b * a.v.sb + kvh * a.v.sh + 16 * g;
-            for (int i = 0; i < 32; ++i) {
-                const int from = i >> 3, j = i & 7;
-                const int p = min(p0 + (j < 4 ? 4 * from + j : 12 + 4 * from + j), end - 1);
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    float w = 0.f;
+                    const int i = min(w0 + 16 * rb + c, R - 1);
+                    const float *q = a.q + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (k == j) w = (float)ph[rb][k] + (float)pl[rb][k];
-                    w = __shfl(w, c + 16 * from);
-                    if (w == 0.f) continue;
+                    for (int j = 0; j < 8 * KT; ++j) {
+                        const float *k = kb + min(p0 + position(j, g), end - 1) * a.k.ss;
+                        float s = 0.f;
+                        for (int d = 0; d < D; ++d) s = fmaf(q[d], k[d], s);
+                        s8[rb][j] = s * f;
+                    }
+                }
+            }
+            // ---- running maxima
+            float alpha[RB];
+            bool moved = false;
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                if (!open) {
+#pragma unroll
+                    for (int sub = 0; sub < KT; ++sub) {
+                        const uint32_t see =
+                            live[rb] ? seen(mrow[rb], words, p0 + 32 * sub, len, end) : 0;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (!(see >> position(j, g) & 1)) s8[rb][8 * sub + j] = -INFINITY;
+                    }
+                }
+                float mt = s8[rb][0];
+#pragma unroll
+                for (int j = 1; j < 8 * KT; ++j) mt = fmaxf(mt, s8[rb][j]);
+                const float mn = fmaxf(m[rb], max_over_groups(mt));
+                alpha[rb] = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rb] - mn);
+                moved |= m[rb] != mn;
+                m[rb] = mn;
+            }
+            // ---- the outputs' scale.  It stays while the tile fits it and loses at most 6
+            // bits of range to it, and stays 64 bits below the largest one so far (the
+            // outputs' f32 must not overflow).
+            const int vtop = max(max(se[buf][1][0], se[buf][1][1]), max(se[buf][1][2], se[buf][1][3]));
+            int down = 0;
+            oe_top = max(oe_top, vtop);
+            if (vtop > oe || vtop < oe - 6) {
+                const int to = max(vtop, oe_top - 64);
+                down = oe - to;
+                oe = to;
+            }
+            if (__any(moved) || down != 0) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    l[rb] *= alpha[rb];
+                    const float x = ldexpf(alpha[rb], min(down, 120));
 #pragma unroll
                     for (int q = 0; q < NB; ++q)
 #pragma unroll
-                        for (int y = 0; y < 16; ++y)
-                            if (64 * q + 16 * g < D)
-                                o[rb][q][y & 3][y >> 2] =
-                                    fmaf(w, ldexpf(v[p * a.v.ss + 64 * q + y], kTop - ve),
-                                         o[rb][q][y & 3][y >> 2]);
+                        for (int j = 0; j < 4; ++j) o[rb][q][j] *= x;
+                }
+            }
+            // ---- weights, in the scale of the positions' V
+            f16x8 ph[RB][KT], pl[RB][KT];
+            const float px = pow2(max(kTop + ve - oe, -126));
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const float base = m[rb] == -INFINITY ? 0.f : m[rb];   // nothing seen: weights 0
+#pragma unroll
+                for (int sub = 0; sub < KT; ++sub) {
+                    float p8[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        p8[j] = __builtin_amdgcn_exp2f(s8[rb][8 * sub + j] - base);
+                        l[rb] += p8[j];
+                    }
+                    split8(p8, px, ph[rb][sub], pl[rb][sub]);
+                }
+            }
+            // ---- outputs
+            if (!slow_v) {
+#pragma unroll
+                for (int sub = 0; sub < KT; ++sub)
+#pragma unroll
+                    for (int q = 0; q < NB; ++q)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const f16x8 *v = sv[buf] + ((sub * NB + q) * 4 + j) * 128 + lane;
+                            const f16x8 vh = v[0], vl = v[64];
+#pragma unroll
+                            for (int x = 0; x < 3; ++x)
+#pragma unroll
+                                for (int rb = 0; rb < RB; ++rb)
+                                    o[rb][q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                        x == 0 ? vl : vh, x == 1 ? pl[rb][sub] : ph[rb][sub],
+                                        o[rb][q][j], 0, 0, 0);
+                        }
+            } else {
+                for (int i = 0; i < TK; ++i) {
+                    const int sub = i >> 5, from = i >> 3 & 3, j = i & 7;
+                    const float *v = vb + min(p0 + 32 * sub + position(j, from), end - 1) * a.v.ss;
+                    const int x = kTop - se[buf][1][from];
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        float w = 0.f;
+#pragma unroll
+                        for (int k = 0; k < 8 * KT; ++k)
+                            if (k == (i & 7) + 8 * sub)
+                                w = (float)ph[rb][k >> 3][k & 7] + (float)pl[rb][k >> 3][k & 7];
+                        w = __shfl(w, c + 16 * from);
+                        if (w == 0.f) continue;
+#pragma unroll
+                        for (int q = 0; q < NB; ++q)
+#pragma unroll
+                            for (int y = 0; y < 16; ++y)
+                                if (64 * q + 16 * g < D)
+                                    o[rb][q][y & 3][y >> 2] =
+                                        fmaf(w, ldexpf(v[64 * q + 16 * g + y], x),
+                                             o[rb][q][y & 3][y >> 2]);
+                    }
                 }
             }
         }
-        if (tile + 4 < t1) load_v(tile + 4);
-    }
-
-    // ---- the four waves' outputs, brought to one maximum and summed in wave order
-    __syncthreads();   // every wave is done with the query rows and sm
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        if (!live[rb]) m[rb] = -INFINITY;
-        l[rb] = live[rb] ? sum_over_groups(l[rb]) : 0.f;
-        if (g == 0) {
-            sm[wave][16 * rb + c] = m[rb];
-            sl[wave][16 * rb + c] = l[rb];
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (wave == w) {
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                const int r = 16 * rb + c;
-                const float top = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
-                const float x = m[rb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rb] - top);
-#pragma unroll
-                for (int q = 0; q < NB; ++q)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float4 *d = reinterpret_cast<float4 *>(lds + r * DP + 64 * q + 16 * g) + i;
-                        float4 y = w ? *d : make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (x != 0.f) {
-                            y.x = fmaf(ldexpf(o[rb][q][0][i], ve - 2 * kTop), x, y.x);
-                            y.y = fmaf(ldexpf(o[rb][q][1][i], ve - 2 * kTop), x, y.y);
-                            y.z = fmaf(ldexpf(o[rb][q][2][i], ve - 2 * kTop), x, y.z);
-                            y.w = fmaf(ldexpf(o[rb][q][3][i], ve - 2 * kTop), x, y.w);
-                        }
-                        *d = y;
-                    }
-            }
+        if (tile + 1 < t1) {
+            store(tile + 1, buf ^ 1);
+            if (tile + 2 < t1) load(tile + 2);
         }
         __syncthreads();
     }
-    const int cols = D / 4;
-    for (int x = t; x < ROWS * cols; x += 256) {
-        const int r = x / cols, d = x % cols, i = i0 + r;
-        if (i >= R) break;
-        const float top = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
-        float sum = 0.f;
+    if (!busy) return;
+
+    // ---- results: lane (g, c) holds dimensions 64 q + 16 g .. + 15 of row c
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-            if (sm[w][r] != -INFINITY) sum = fmaf(sl[w][r], __builtin_amdgcn_exp2f(sm[w][r] - top), sum);
-        float4 y = *reinterpret_cast<const float4 *>(lds + r * DP + 4 * d);
-        if (part) {
-            const size_t at = (((size_t)b * a.hkv + kvh) * nsplit + split) * R + i;
-            reinterpret_cast<float4 *>(part + at * D)[d] = y;
-            if (d == 0) {
-                pml[2 * at] = top;
-                pml[2 * at + 1] = sum;
-            }
-        } else {
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-            float *out = a.out + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D;
-            reinterpret_cast<float4 *>(out)[d] =
-                make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+    for (int rb = 0; rb < RB; ++rb) {
+        const int i = w0 + 16 * rb + c;
+        const float sum = live[rb] ? sum_over_groups(l[rb]) : 0.f;
+        if (i >= R) continue;
+        const size_t at = (((size_t)b * a.hkv + kvh) * gridDim.x + split) * R + i;
+        float *to = part ? part + at * D
+                         : a.out + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D;
+        const float x = part ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;
+        if (part && g == 0) {
+            pml[2 * at] = live[rb] ? m[rb] : -INFINITY;
+            pml[2 * at + 1] = sum;
         }
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+            if (64 * q + 16 * g < D)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float4 y;
+                    y.x = ldexpf(o[rb][q][0][r], oe - 2 * kTop) * x;
+                    y.y = ldexpf(o[rb][q][1][r], oe - 2 * kTop) * x;
+                    y.z = ldexpf(o[rb][q][2][r], oe - 2 * kTop) * x;
+                    y.w = ldexpf(o[rb][q][3][r], oe - 2 * kTop) * x;
+                    if (!live[rb]) y = make_float4(0.f, 0.f, 0.f, 0.f);
+                    reinterpret_cast<float4 *>(to + 64 * q + 16 * g)[r] = y;
+                }
     }
 }
 
 // The splits' outputs brought to one maximum: a thread per four columns of a row.
-__global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int nsplit,
+__global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int tk, int cap, int nsplit,
                                                     const float *__restrict__ part,
                                                     const float *__restrict__ pml) {
     const int G = a.hq / a.hkv, R = a.n * G, cols = a.hd / 4, per = 256 / cols;
@@ -489,8 +510,8 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int nsplit,
     const int i = blockIdx.x * per + r, kvh = blockIdx.y, b = blockIdx.z;
     if (r >= per || i >= R) return;
     const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
-    const int tiles = (end + kTile - 1) / kTile, tps = tiles_per_split(tiles, nsplit);
-    const int used = tps ? (tiles + tps - 1) / tps : 0;
+    const int tiles = (end + tk - 1) / tk, tps = tiles_per_split(tiles, cap);
+    const int used = (tiles + tps - 1) / tps;
     const size_t at = ((size_t)b * a.hkv + kvh) * nsplit * R + i;
     float top = -INFINITY;
     for (int s = 0; s < used; ++s) top = fmaxf(top, pml[2 * (at + (size_t)s * R)]);
@@ -514,18 +535,18 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int nsplit,
 }
 
 struct Plan {
-    int dp, rb, nsplit;
+    int dp, rb, rtiles, cap, nsplit;
 };
 
 Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len) {
     Plan p;
     p.dp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-    const int R = n * (hq / hkv);
-    p.rb = R <= 16 ? 1 : R <= 32 || p.dp == 256 ? 2 : 4;
-    const int rtiles = (R + 16 * p.rb - 1) / (16 * p.rb), tiles = (max_len + kTile - 1) / kTile;
-    const int64_t blocks = (int64_t)rtiles * hkv * batch;
-    const int64_t want = std::max<int64_t>(1, 512 / blocks);
-    p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({want, (tiles + 3) / 4, kMaxSplits}));
+    const int R = n * (hq / hkv), tk = tile_of(p.dp), tiles = (max_len + tk - 1) / tk;
+    p.rb = R <= 64 || p.dp == 256 ? 1 : 2;
+    p.rtiles = (R + 64 * p.rb - 1) / (64 * p.rb);
+    const int64_t want = 512 / ((int64_t)p.rtiles * hkv * batch);
+    p.cap = (int)std::max<int64_t>(1, std::min<int64_t>(want, kMaxSplits));
+    p.nsplit = std::max(1, std::min(p.cap, (tiles + kMinTiles - 1) / kMinTiles));
     return p;
 }
 
@@ -538,27 +559,23 @@ size_t tree_attention_scratch(int batch, int n, int hq, int hkv, int hd, int max
 
 int launch_tree_attention(const TreeAttn &a, int max_len, float *scratch, hipStream_t s) {
     const Plan p = plan(a.batch, a.n, a.hq, a.hkv, a.hd, max_len);
-    const int R = a.n * (a.hq / a.hkv), rtiles = (R + 16 * p.rb - 1) / (16 * p.rb);
     float *part = p.nsplit > 1 ? scratch : nullptr;
     float *pml = part ? part + (size_t)a.batch * a.hq * a.n * p.nsplit * a.hd : nullptr;
-    const dim3 grid(p.nsplit, a.hkv * rtiles, a.batch);
+    const dim3 grid(p.nsplit, a.hkv * p.rtiles, a.batch);
 #define TB_TA(DP, RB)                                                                        \
     if (p.dp == DP && p.rb == RB)                                                            \
-    hipLaunchKernelGGL((k_tree_attn<DP, RB>), grid, dim3(256), 0, s, a, p.nsplit, part, pml)
+    hipLaunchKernelGGL((k_tree_attn<DP, RB>), grid, dim3(256), 0, s, a, p.cap, part, pml)
     TB_TA(64, 1);
     TB_TA(64, 2);
-    TB_TA(64, 4);
     TB_TA(128, 1);
     TB_TA(128, 2);
-    TB_TA(128, 4);
     TB_TA(256, 1);
-    TB_TA(256, 2);
 #undef TB_TA
     TB_LAUNCHED();
     if (part) {
-        const int per = 256 / (a.hd / 4);
+        const int per = 256 / (a.hd / 4), R = a.n * (a.hq / a.hkv);
         hipLaunchKernelGGL(k_tree_merge, dim3((R + per - 1) / per, a.hkv, a.batch), dim3(256), 0, s,
-                           a, p.nsplit, part, pml);
+                           a, tile_of(p.dp), p.cap, p.nsplit, part, pml);
         TB_LAUNCHED();
     }
     return TB_OK;
