@@ -151,31 +151,30 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
     const int kx = lane >> 5;             // K: dimension block's parity
     const int half = lane & 1, vc = lane >> 1 & 15, vx = lane >> 5;
     float kr[KU][8], vr[VU][4][4];
+    // Dimensions past head_dim repeat its last ones: the query limbs are zero there, and
+    // those outputs are not kept.
+    int kd[KU], vd[VU];
+#pragma unroll
+    for (int u = 0; u < KU; ++u) kd[u] = min(32 * (KT == 2 ? kx : kx + 2 * u), D - 32) + 4 * kg;
+#pragma unroll
+    for (int u = 0; u < VU; ++u) vd[u] = min(64 * (KT == 2 ? 0 : vx + 2 * u) + 4 * vc, D - 4);
     auto load = [&](int tile) {
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
-            const int sub = KT == 2 ? u : 0, s = KT == 2 ? kx : kx + 2 * u;
-            const float *r = kb + min(tile * TK + 32 * sub + kkey, end - 1) * a.k.ss + 4 * kg;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-            if (32 * s < D) {
-                x = *reinterpret_cast<const float4 *>(r + 32 * s);
-                y = *reinterpret_cast<const float4 *>(r + 32 * s + 16);
-            }
+            const int p = min(tile * TK + 32 * (KT == 2 ? u : 0) + kkey, end - 1);
+            const float4 *r = reinterpret_cast<const float4 *>(kb + p * a.k.ss + kd[u]);
+            const float4 x = r[0], y = r[4];
             kr[u][0] = x.x; kr[u][1] = x.y; kr[u][2] = x.z; kr[u][3] = x.w;
             kr[u][4] = y.x; kr[u][5] = y.y; kr[u][6] = y.z; kr[u][7] = y.w;
         }
 #pragma unroll
-        for (int u = 0; u < VU; ++u) {
-            const int sub = KT == 2 ? vx : 0, q = KT == 2 ? 0 : vx + 2 * u;
+        for (int u = 0; u < VU; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int p = min(tile * TK + 32 * sub + 16 * half + 4 * wave + i, end - 1);
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (64 * q + 4 * vc < D)
-                    x = *reinterpret_cast<const float4 *>(vb + p * a.v.ss + 64 * q + 4 * vc);
+                const int p = min(tile * TK + 32 * (KT == 2 ? vx : 0) + 16 * half + 4 * wave + i, end - 1);
+                const float4 x = *reinterpret_cast<const float4 *>(vb + p * a.v.ss + vd[u]);
                 vr[u][i][0] = x.x; vr[u][i][1] = x.y; vr[u][i][2] = x.z; vr[u][i][3] = x.w;
             }
-        }
     };
     auto store = [&](int tile, int buf) {
         const bool open = (tile + 1) * TK <= len;
@@ -265,11 +264,9 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
         float top = 0.f;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
-            if (32 * s < D) {
-                u = *reinterpret_cast<const float4 *>(q + 32 * s);
-                v = *reinterpret_cast<const float4 *>(q + 32 * s + 16);
-            }
+            float4 u = *reinterpret_cast<const float4 *>(q + min(32 * s, D - 32));
+            float4 v = *reinterpret_cast<const float4 *>(q + min(32 * s, D - 32) + 16);
+            if (32 * s >= D) u = v = make_float4(0.f, 0.f, 0.f, 0.f);
             x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w;
             x[s][4] = v.x; x[s][5] = v.y; x[s][6] = v.z; x[s][7] = v.w;
 #pragma unroll
@@ -501,34 +498,66 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
     }
 }
 
-// The splits' outputs brought to one maximum: a thread per four columns of a row.
+// The splits' outputs brought to one maximum, a wave per row: lane s takes the
+// maxima and sums of splits s and s + 64, whose weights then pass through LDS to
+// the lanes of the columns.  Those are 64 / LC groups of LC lanes, each group
+// with every (64 / LC)-th split, so that a lane's loads are independent.
+template <int LC>
 __global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int tk, int cap, int nsplit,
                                                     const float *__restrict__ part,
                                                     const float *__restrict__ pml) {
-    const int G = a.hq / a.hkv, R = a.n * G, cols = a.hd / 4, per = 256 / cols;
-    const int r = threadIdx.x / cols, d = threadIdx.x % cols;
-    const int i = blockIdx.x * per + r, kvh = blockIdx.y, b = blockIdx.z;
-    if (r >= per || i >= R) return;
+    __shared__ float w[4][kMaxSplits];
+    const int G = a.hq / a.hkv, R = a.n * G, cols = a.hd / 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int i = blockIdx.x * 4 + wave, kvh = blockIdx.y, b = blockIdx.z;
+    if (i >= R) return;
     const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
     const int tiles = (end + tk - 1) / tk, tps = tiles_per_split(tiles, cap);
     const int used = (tiles + tps - 1) / tps;
     const size_t at = ((size_t)b * a.hkv + kvh) * nsplit * R + i;
-    float top = -INFINITY;
-    for (int s = 0; s < used; ++s) top = fmaxf(top, pml[2 * (at + (size_t)s * R)]);
-    float sum = 0.f;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < used; ++s) {
-        const size_t p = at + (size_t)s * R;
-        const float m = pml[2 * p];
-        if (m == -INFINITY) continue;
-        const float x = __builtin_amdgcn_exp2f(m - top);
-        const float4 z = reinterpret_cast<const float4 *>(part + p * a.hd)[d];
-        sum = fmaf(pml[2 * p + 1], x, sum);
-        y.x = fmaf(z.x, x, y.x);
-        y.y = fmaf(z.y, x, y.y);
-        y.z = fmaf(z.z, x, y.z);
-        y.w = fmaf(z.w, x, y.w);
+    float m[2], l[2], top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int s = lane + 64 * x;
+        m[x] = s < used ? pml[2 * (at + (size_t)s * R)] : -INFINITY;
+        l[x] = s < used ? pml[2 * (at + (size_t)s * R) + 1] : 0.f;
+        top = fmaxf(top, m[x]);
     }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, gemv::shfl_xor_u(top, o));
+    float sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const float y = m[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[x] - top);
+        w[wave][lane + 64 * x] = y;
+        sum = fmaf(l[x], y, sum);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += gemv::shfl_xor_u(sum, o);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // w: written and read by this wave
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int d = min(lane % LC, cols - 1);
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = lane / LC; s < used; s += 64 / LC) {
+        const float x = w[wave][s];
+        const float4 z = reinterpret_cast<const float4 *>(part + (at + (size_t)s * R) * a.hd)[d];
+        if (x != 0.f) {   // a split that sees nothing of the row counts for nothing
+            y.x = fmaf(z.x, x, y.x);
+            y.y = fmaf(z.y, x, y.y);
+            y.z = fmaf(z.z, x, y.z);
+            y.w = fmaf(z.w, x, y.w);
+        }
+    }
+#pragma unroll
+    for (int o = LC; o < 64; o <<= 1) {
+        y.x += gemv::shfl_xor_u(y.x, o);
+        y.y += gemv::shfl_xor_u(y.y, o);
+        y.z += gemv::shfl_xor_u(y.z, o);
+        y.w += gemv::shfl_xor_u(y.w, o);
+    }
+    if (lane >= cols) return;
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     float *out = a.out + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * a.hd;
     reinterpret_cast<float4 *>(out)[d] = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
@@ -573,9 +602,20 @@ int launch_tree_attention(const TreeAttn &a, int max_len, float *scratch, hipStr
 #undef TB_TA
     TB_LAUNCHED();
     if (part) {
-        const int per = 256 / (a.hd / 4), R = a.n * (a.hq / a.hkv);
-        hipLaunchKernelGGL(k_tree_merge, dim3((R + per - 1) / per, a.hkv, a.batch), dim3(256), 0, s,
-                           a, tile_of(p.dp), p.cap, p.nsplit, part, pml);
+        const int R = a.n * (a.hq / a.hkv);
+        const dim3 rows((R + 3) / 4, a.hkv, a.batch);
+        if (a.hd <= 32)
+            hipLaunchKernelGGL(k_tree_merge<8>, rows, dim3(256), 0, s, a, tile_of(p.dp), p.cap,
+                               p.nsplit, part, pml);
+        else if (a.hd <= 64)
+            hipLaunchKernelGGL(k_tree_merge<16>, rows, dim3(256), 0, s, a, tile_of(p.dp), p.cap,
+                               p.nsplit, part, pml);
+        else if (a.hd <= 128)
+            hipLaunchKernelGGL(k_tree_merge<32>, rows, dim3(256), 0, s, a, tile_of(p.dp), p.cap,
+                               p.nsplit, part, pml);
+        else
+            hipLaunchKernelGGL(k_tree_merge<64>, rows, dim3(256), 0, s, a, tile_of(p.dp), p.cap,
+                               p.nsplit, part, pml);
         TB_LAUNCHED();
     }
     return TB_OK;
