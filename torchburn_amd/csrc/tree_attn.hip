@@ -27,7 +27,9 @@ namespace tb {
 namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxSplits = 128;
@@ -41,36 +43,103 @@ __device__ __forceinline__ int exponent(uint32_t bits) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-// The two f16 limbs of 8 values times sc, as MFMA operands.  x * sc is exact, so
-// lo is the rounded rest of hi.
+// The two f16 limbs of 8 values times sc, x sc being exact: hi the rounded
+// product, lo its rounded rest.  (`one` keeps a v_fma_mix of the f16 and f32
+// factors where a constant would make it a conversion and a difference.)
 __device__ __forceinline__ void split8(const float (&x)[8], float sc, f16x8 &hi, f16x8 &lo) {
+    float one = 1.f;
+    asm("" : "+s"(one));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        hi[j] = (_Float16)__builtin_fmaf(x[j], sc, 0.f);
-        lo[j] = (_Float16)__builtin_fmaf(x[j], sc, -(float)hi[j]);
+    for (int j = 0; j < 8; j += 2) {
+        const f32x2 y = {x[j] * sc, x[j + 1] * sc};
+        const f16x2 h = __builtin_convertvector(y, f16x2);
+        const f32x2 r = {__builtin_fmaf(y.x, one, -(float)h.x), __builtin_fmaf(y.y, one, -(float)h.y)};
+        const f16x2 e = __builtin_convertvector(r, f16x2);
+        hi[j] = h.x; hi[j + 1] = h.y;
+        lo[j] = e.x; lo[j + 1] = e.y;
     }
 }
 
-// max(m, |a|, |b|) without the canonicalising moves of fmaxf.
+// The same of N loaded values on their way to LDS, an instruction per limb:
+// v_fma_mix takes f32 and f16 factors side by side and writes either half of a
+// register.  Only for results that no MFMA reads: the compiler does not count the
+// wait states from inline assembly to one.
+template <int N>
+using f16v = _Float16 __attribute__((ext_vector_type(N)));
+template <int N>
+__device__ __forceinline__ void split_to_lds(const float (&x)[N], float sc, f16v<N> &hi,
+                                             f16v<N> &lo) {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        f16x2 h, r;
+        asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(h) : "v"(x[j]), "v"(sc));
+        asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(h) : "v"(x[j + 1]), "v"(sc));
+        asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]"
+            : "=v"(r)
+            : "v"(x[j]), "v"(sc), "v"(h));
+        asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]"
+            : "+v"(r)
+            : "v"(x[j + 1]), "v"(sc), "v"(h));
+        hi[j] = h.x; hi[j + 1] = h.y;
+        lo[j] = r.x; lo[j + 1] = r.y;
+    }
+}
+
+// max(m, |a|, |b|) of loaded values without the canonicalising moves of fmaxf.
 __device__ __forceinline__ void max3_abs(float &m, float a, float b) {
     asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(a), "v"(b));
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 constexpr uint32_t kInf = 0x7F800000u;
 
-__device__ __forceinline__ float max_over_groups(float v) {   // lanes c, c + 16, c + 32, c + 48
-    v = fmaxf(v, gemv::shfl_xor_u(v, 16));
-    return fmaxf(v, gemv::shfl_xor_u(v, 32));
+// Over the lanes c, c + 16, c + 32, c + 48: a swap of 16- or 32-lane halves of a
+// register with itself leaves both halves' values in every lane.
+template <class F>
+__device__ __forceinline__ float over_groups(float v, F f) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_over_groups(float v) {
+    return over_groups(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float sum_over_groups(float v) {
-    v += gemv::shfl_xor_u(v, 16);
-    return v + gemv::shfl_xor_u(v, 32);
+    return over_groups(v, [](float a, float b) { return a + b; });
 }
-__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1)
-        v = max(v, __float_as_uint(gemv::shfl_xor_u(__uint_as_float(v), m)));
-    return __builtin_amdgcn_readfirstlane(v);
+// Two maxima over the wave side by side: rotations within 16 lanes, then as above.
+__device__ __forceinline__ void wave_max_bits(uint32_t &a, uint32_t &b) {
+#define TB_ROR(n)                                                                       \
+    {                                                                                   \
+        const uint32_t x = (uint32_t)__builtin_amdgcn_mov_dpp((int)a, 0x120 + n, 0xF, 0xF, true); \
+        const uint32_t y = (uint32_t)__builtin_amdgcn_mov_dpp((int)b, 0x120 + n, 0xF, 0xF, true); \
+        a = max(a, x);                                                                  \
+        b = max(b, y);                                                                  \
+    }
+    TB_ROR(8) TB_ROR(4) TB_ROR(2) TB_ROR(1)
+#undef TB_ROR
+    auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    auto s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    a = max(r[0], r[1]);
+    b = max(s[0], s[1]);
+    r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+    s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    a = __builtin_amdgcn_readfirstlane(max(r[0], r[1]));
+    b = __builtin_amdgcn_readfirstlane(max(s[0], s[1]));
+}
+
+// x, which the compiler must take as new: what follows from it is worked out where
+// it is used instead of waiting in registers across the loop.
+__device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// The lane, counted anew.
+__device__ __forceinline__ int fresh_lane() {
+    int x;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+    return x;
 }
 
 // Position j of lane group g's scores among a tile's.
@@ -115,9 +184,9 @@ __host__ __device__ inline int tiles_per_split(int tiles, int cap) {
 // is requested.
 //   Lane (g, c) = (lane / 16, lane % 16) has A[c][8g ..] and B[8g ..][c] of a
 //   product of depth 32, and gets D[4g + r][c] in register r:
-//   S^T = K Q^T: A = 16 positions, position c with the 8 dimensions 4g.. and
-//     16 + 4g.. of each 32 (K rows are read in whole 64-byte pieces); B = the
-//     wave's query rows, in registers;
+//   S^T = K Q^T: A = 16 positions, position c with the 8 dimensions 16 x + 4g ..
+//     and 32 + 16 x + 4g .. of each 64, x = 0, 1 (so that the lanes read K rows in
+//     whole 128-byte pieces); B = the wave's query rows, in registers;
 //   O^T = V^T P^T: A's row c of block (q, j) is dimension 64 q + 4 c + j and its
 //     depth 8g + i is position 4g + i (i < 4) or 16 + 4g + i - 4 of 32: the
 //     positions whose scores the lane holds for row c, so P^T needs no exchange
@@ -133,6 +202,7 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
     TreeAttn a, int cap, float *__restrict__ part, float *__restrict__ pml) {
     constexpr int NS = DP / 32, NB = DP / 64, TK = tile_of(DP), KT = TK / 32;
     constexpr int KU = KT * NS / 2, VU = KT * NB / 2;   // operands of 8 K values, 16 V values a lane
+    constexpr int KG = RB == 1 ? 2 : 1, VG = RB == 1 ? 4 : 2;   // operands read at a time
     __shared__ f16x8 sk[2][KT * 2 * NS * 2 * 64];       // [32 positions][16][32 dims][limb][lane]
     __shared__ f16x8 sv[2][KT * NB * 4 * 2 * 64];       // [32 positions][64 dims][j][limb][lane]
     __shared__ int se[2][2][4], bad[2][2][4];           // K's, V's quarters: exponent, not finite
@@ -151,67 +221,100 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
     const int kx = lane >> 5;             // K: dimension block's parity
     const int half = lane & 1, vc = lane >> 1 & 15, vx = lane >> 5;
     float kr[KU][8], vr[VU][4][4];
-    // Dimensions past head_dim repeat its last ones: the query limbs are zero there, and
-    // those outputs are not kept.
-    int kd[KU], vd[VU];
+    // Its addresses, in 16-byte units from the tile's first row.  Dimensions past head_dim
+    // repeat its last ones: the query limbs are zero there, and those outputs are not kept.
+    const uint32_t ks4 = (uint32_t)(a.k.ss / 4), vs4 = (uint32_t)(a.v.ss / 4);
+    const uint32_t koff = kkey * ks4 + 4 * kx + kg;
+    uint32_t voff[VU];
 #pragma unroll
-    for (int u = 0; u < KU; ++u) kd[u] = min(32 * (KT == 2 ? kx : kx + 2 * u), D - 32) + 4 * kg;
-#pragma unroll
-    for (int u = 0; u < VU; ++u) vd[u] = min(64 * (KT == 2 ? 0 : vx + 2 * u) + 4 * vc, D - 4);
-    auto load = [&](int tile) {
+    for (int u = 0; u < VU; ++u)
+        voff[u] = (32 * (KT == 2 ? vx : 0) + 16 * half + 4 * wave) * vs4 +
+                  min(16 * (KT == 2 ? 0 : vx + 2 * u) + vc, D / 4 - 1);
+    auto load_k = [&](int tile) {
+        const float4 *kt = reinterpret_cast<const float4 *>(kb + (int64_t)tile * TK * a.k.ss);
+        const int last = end - 1 - tile * TK;   // the last tile repeats the last position
+        const bool whole = last >= TK - 1;
+        const int ln = fresh_lane();
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
-            const int p = min(tile * TK + 32 * (KT == 2 ? u : 0) + kkey, end - 1);
-            const float4 *r = reinterpret_cast<const float4 *>(kb + p * a.k.ss + kd[u]);
-            const float4 x = r[0], y = r[4];
+            const int sub = KT == 2 ? u : 0, d = KT == 2 ? 0 : 64 * u;   // 64 dimensions from d
+            uint32_t at = (uint32_t)fresh((int)koff) + sub * 32 * ks4;
+            if (!whole)
+                at -= max(32 * sub + 16 * (wave >> 1) + 8 * (wave & 1) + (ln & 7) - last, 0) * ks4;
+            const float4 x = kt[at + (d < D ? d / 4 : 0)];
+            const float4 y = kt[at + (d + 32 < D ? d / 4 + 8 : 0)];
             kr[u][0] = x.x; kr[u][1] = x.y; kr[u][2] = x.z; kr[u][3] = x.w;
             kr[u][4] = y.x; kr[u][5] = y.y; kr[u][6] = y.z; kr[u][7] = y.w;
         }
+    };
+    auto load_v = [&](int tile) {
+        const float4 *vt = reinterpret_cast<const float4 *>(vb + (int64_t)tile * TK * a.v.ss);
+        const int last = end - 1 - tile * TK;
+        const bool whole = last >= TK - 1;
+        const int ln = fresh_lane();
 #pragma unroll
         for (int u = 0; u < VU; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int p = min(tile * TK + 32 * (KT == 2 ? vx : 0) + 16 * half + 4 * wave + i, end - 1);
-                const float4 x = *reinterpret_cast<const float4 *>(vb + p * a.v.ss + vd[u]);
+                uint32_t at = (uint32_t)fresh((int)voff[u]) + i * vs4;
+                if (!whole)
+                    at -= max(32 * (KT == 2 ? ln >> 5 : 0) + 16 * (ln & 1) + 4 * wave + i - last,
+                              0) * vs4;
+                const float4 x = vt[at];
                 vr[u][i][0] = x.x; vr[u][i][1] = x.y; vr[u][i][2] = x.z; vr[u][i][3] = x.w;
             }
     };
+    // The tile's limbs to a buffer; the registers then take the next tile's values.
     auto store = [&](int tile, int buf) {
+        const int ln = fresh_lane(), kx = ln >> 5, kg = ln >> 3 & 3, vx = ln >> 5, vc = ln >> 1 & 15,
+                  half = ln & 1;
         const bool open = (tile + 1) * TK <= len;
-        float km = 0.f, vm = 0.f;
+        float km = 0.f, vm = 0.f, kn = 0.f, vn = 0.f;
 #pragma unroll
         for (int u = 0; u < KU; ++u)
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) max3_abs(km, kr[u][j], kr[u][j + 1]);
+            for (int j = 0; j < 8; j += 4) {
+                max3_abs(km, kr[u][j], kr[u][j + 1]);
+                max3_abs(kn, kr[u][j + 2], kr[u][j + 3]);
+            }
 #pragma unroll
         for (int u = 0; u < VU; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 max3_abs(vm, vr[u][i][0], vr[u][i][1]);
-                max3_abs(vm, vr[u][i][2], vr[u][i][3]);
+                max3_abs(vn, vr[u][i][2], vr[u][i][3]);
             }
-        uint32_t kt = wave_max_bits(abs_bits(km)), vt = abs_bits(vm);
+        uint32_t kt = max(abs_bits(km), abs_bits(kn)), vt = max(abs_bits(vm), abs_bits(vn));
         if (!open) {   // NaN in V too: a row that does not see its position must not get it
 #pragma unroll
             for (int u = 0; u < VU; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) vt = max(vt, abs_bits(vr[u][i >> 2][i & 3]));
         }
-        vt = wave_max_bits(vt);
+        wave_max_bits(kt, vt);
         const bool bad_k = kt >= kInf, bad_v = vt >= kInf;
-        if (bad_v) {   // the finite values' scale
+        if (__builtin_expect(bad_k | bad_v, 0)) {
+            // Out of the limbs: the tile's scores are summed in f32, and what of V has weight
+            // is added in f32.
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) kr[u][j] = bad_k ? 0.f : kr[u][j];
+            kt = bad_k ? 0 : kt;
             vt = 0;
 #pragma unroll
             for (int u = 0; u < VU; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const uint32_t x = abs_bits(vr[u][i >> 2][i & 3]);
-                    vt = max(vt, x < kInf ? x : 0u);
+                    float &x = vr[u][i >> 2][i & 3];
+                    x = abs_bits(x) < kInf ? x : 0.f;
+                    vt = max(vt, abs_bits(x));
                 }
-            vt = wave_max_bits(vt);
+            uint32_t k2 = kt;
+            wave_max_bits(k2, vt);
         }
         const int ke = exponent(kt), ve = exponent(vt);
-        if (lane == 0) {
+        if (ln == 0) {
             se[buf][0][wave] = ke;
             se[buf][1][wave] = ve;
             bad[buf][0][wave] = bad_k;
@@ -221,35 +324,38 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
         for (int u = 0; u < KU; ++u) {
             const int sub = KT == 2 ? u : 0, s = KT == 2 ? kx : kx + 2 * u;
             f16x8 hi, lo;
-            split8(kr[u], pow2(kTop - ke), hi, lo);
+            split_to_lds<8>(kr[u], pow2(kTop - ke), hi, lo);
             f16x8 *d = sk[buf] + (((sub * 2 + (wave >> 1)) * NS + s) * 2) * 64 + 16 * kg +
-                       8 * (wave & 1) + (lane & 7);
+                       8 * (wave & 1) + (ln & 7);
             d[0] = hi;
             d[64] = lo;
         }
+        if (tile + 1 < t1) load_k(tile + 1);
 #pragma unroll
         for (int u = 0; u < VU; ++u) {
             const int sub = KT == 2 ? vx : 0, q = KT == 2 ? 0 : vx + 2 * u;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
+                const float x[4] = {vr[u][0][j], vr[u][1][j], vr[u][2][j], vr[u][3][j]};
                 f16x4 hi, lo;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    hi[i] = (_Float16)__builtin_fmaf(vr[u][i][j], pow2(kTop - ve), 0.f);
-                    lo[i] = (_Float16)__builtin_fmaf(vr[u][i][j], pow2(kTop - ve), -(float)hi[i]);
-                }
+                split_to_lds<4>(x, pow2(kTop - ve), hi, lo);
                 f16x4 *d = reinterpret_cast<f16x4 *>(
                                sv[buf] + (((sub * NB + q) * 4 + j) * 2) * 64 + 16 * wave + vc) + half;
                 d[0] = hi;
                 d[128] = lo;
             }
         }
+        if (tile + 1 < t1) load_v(tile + 1);
     };
-    if (t0 < t1) load(t0);
+    if (t0 < t1) {
+        load_k(t0);
+        load_v(t0);
+    }
 
+    const int32_t *mask = a.mask + b * a.mask_sb;
     // ---- the wave's query rows, row c of each block in this lane
     f16x8 qh[RB][NS], ql[RB][NS];
-    const int32_t *mrow[RB];
+    int mrow[RB];   // its mask row's first word
     bool live[RB];
     float m[RB], l[RB];
     int qe[RB];
@@ -264,9 +370,11 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
         float top = 0.f;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            float4 u = *reinterpret_cast<const float4 *>(q + min(32 * s, D - 32));
-            float4 v = *reinterpret_cast<const float4 *>(q + min(32 * s, D - 32) + 16);
-            if (32 * s >= D) u = v = make_float4(0.f, 0.f, 0.f, 0.f);
+            const int d = 64 * (s >> 1);
+            float4 u = *reinterpret_cast<const float4 *>(q + 16 * (s & 1) + (d < D ? d : 0));
+            float4 v = *reinterpret_cast<const float4 *>(q + 16 * (s & 1) + (d + 32 < D ? d + 32 : 0));
+            if (d >= D) u = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (d + 32 >= D) v = make_float4(0.f, 0.f, 0.f, 0.f);
             x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w;
             x[s][4] = v.x; x[s][5] = v.y; x[s][6] = v.z; x[s][7] = v.w;
 #pragma unroll
@@ -274,11 +382,13 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
         }
         qe[rb] = exponent(abs_bits(max_over_groups(top)));
 #pragma unroll
-        for (int s = 0; s < NS; ++s) split8(x[s], pow2(kTop - qe[rb]), qh[rb][s], ql[rb][s]);
-        mrow[rb] = a.mask + b * a.mask_sb + (int64_t)(iq / G) * words;
+        for (int s = 0; s < NS; ++s)   // with the sign of the score's factor, which is then positive
+            split8(x[s], a.scale < 0.f ? -pow2(kTop - qe[rb]) : pow2(kTop - qe[rb]), qh[rb][s],
+                   ql[rb][s]);
+        mrow[rb] = iq / G * words;
         uint32_t any = 0;
         for (int w = g; w < words; w += 4)
-            any |= (uint32_t)mrow[rb][w] & (w == words - 1 ? last_bits : ~0u);
+            any |= (uint32_t)mask[mrow[rb] + w] & (w == words - 1 ? last_bits : ~0u);
         live[rb] = i < R && max_over_groups(any ? 1.f : 0.f) > 0.f;
         m[rb] = -INFINITY;
         l[rb] = 0.f;
@@ -288,74 +398,100 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
             for (int j = 0; j < 4; ++j) o[rb][q][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     int oe = 0, oe_top = -1000;   // exponent of the outputs' scale; the largest V's so far
-    const float f = a.scale * kLog2e;
+    const float f = fabsf(a.scale) * kLog2e;
 
     if (t0 < t1) {
         store(t0, 0);
-        if (t0 + 1 < t1) load(t0 + 1);
         __syncthreads();
     }
     for (int tile = t0; tile < t1; ++tile) {
         const int buf = (tile - t0) & 1, p0 = tile * TK;
         if (busy) {
             const bool open = p0 + TK <= len;   // every live row sees every position
+            const int ln = fresh_lane(), g = ln >> 4;
+            // ---- scores, in powers of two.  A group's operands are read while the
+            // MFMAs of the one before run.
+            float s8[RB][8 * KT];
+            f32x4 acc[RB][KT][2];
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                for (int sub = 0; sub < KT; ++sub)
+                    acc[rb][sub][0] = acc[rb][sub][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+            f16x8 kf[2][KG][2][2];   // [group parity][32 dimensions][16 positions][limb]
+            auto read_k = [&](int grp) {
+#pragma unroll
+                for (int x = 0; x < KG; ++x)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const int sub = grp / (NS / KG), s = grp % (NS / KG) * KG + x;
+                            kf[grp & 1][x][h][y] =
+                                sk[buf][(((sub * 2 + h) * NS + s) * 2 + y) * 64 + ln];
+                        }
+            };
+            read_k(0);
+#pragma unroll
+            for (int grp = 0; grp < KT * NS / KG; ++grp) {
+                if (grp + 1 < KT * NS / KG) read_k(grp + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 0; x < KG; ++x)
+#pragma unroll
+                    for (int y = 0; y < 3; ++y)
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const int sub = grp / (NS / KG), s = grp % (NS / KG) * KG + x;
+                                f32x4 &d = acc[rb][sub][h];
+                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    kf[grp & 1][x][h][y == 0], y == 1 ? ql[rb][s] : qh[rb][s], d,
+                                    0, 0, 0);
+                            }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // The first operands of the outputs, read during the softmax.
+            f16x8 vf[2][VG][2];   // [group parity][block of 16 dimensions][limb]
+            auto read_v = [&](int grp) {
+#pragma unroll
+                for (int j = 0; j < VG; ++j)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+                        vf[grp & 1][j][y] = sv[buf][((grp * VG + j) * 2 + y) * 64 + ln];
+            };
+            read_v(0);
             const int ke[2] = {se[buf][0][g >> 1], se[buf][0][2 + (g >> 1)]};
             const int ve = se[buf][1][g];
+            const int vtop = __builtin_amdgcn_readfirstlane(max(
+                max(se[buf][1][0], se[buf][1][1]), max(se[buf][1][2], se[buf][1][3])));
             const bool slow_k = bad[buf][0][0] | bad[buf][0][1] | bad[buf][0][2] | bad[buf][0][3];
             const bool slow_v = bad[buf][1][0] | bad[buf][1][1] | bad[buf][1][2] | bad[buf][1][3];
-            // ---- scores
-            float s8[RB][8 * KT];
-            if (!slow_k) {
 #pragma unroll
-                for (int sub = 0; sub < KT; ++sub) {
-                    f32x4 acc[RB][2];
+            for (int rb = 0; rb < RB; ++rb) {
+                const float sx[2] = {ldexpf(f, qe[rb] + ke[0] - 2 * kTop),
+                                     ldexpf(f, qe[rb] + ke[1] - 2 * kTop)};
 #pragma unroll
-                    for (int rb = 0; rb < RB; ++rb)
-                        acc[rb][0] = acc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) {
-                        f16x8 kh[2], kl[2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            kh[h] = sk[buf][(((sub * 2 + h) * NS + s) * 2 + 0) * 64 + lane];
-                            kl[h] = sk[buf][(((sub * 2 + h) * NS + s) * 2 + 1) * 64 + lane];
-                        }
-#pragma unroll
-                        for (int x = 0; x < 3; ++x)
-#pragma unroll
-                            for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                                for (int h = 0; h < 2; ++h)
-                                    acc[rb][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                        x == 0 ? kl[h] : kh[h], x == 1 ? ql[rb][s] : qh[rb][s],
-                                        acc[rb][h], 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float x = ldexpf(f, qe[rb] + ke[h] - 2 * kTop);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                s8[rb][8 * sub + 4 * h + r] = acc[rb][h][r] * x;
-                        }
-                }
-            } else {
+                for (int j = 0; j < 8 * KT; ++j)
+                    s8[rb][j] = acc[rb][j >> 3][j >> 2 & 1][j & 3] * sx[j >> 2 & 1];
+            }
+            if (__builtin_expect(slow_k, 0)) {
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    const int i = min(w0 + 16 * rb + c, R - 1);
+                    const int i = fresh(min(w0 + 16 * rb + c, R - 1));
                     const float *q = a.q + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D;
 #pragma unroll
                     for (int j = 0; j < 8 * KT; ++j) {
                         const float *k = kb + min(p0 + position(j, g), end - 1) * a.k.ss;
                         float s = 0.f;
                         for (int d = 0; d < D; ++d) s = fmaf(q[d], k[d], s);
-                        s8[rb][j] = s * f;
+                        s8[rb][j] = s * a.scale * kLog2e;
                     }
                 }
             }
             // ---- running maxima
-            float alpha[RB];
+            float was[RB];
             bool moved = false;
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
@@ -363,24 +499,22 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
 #pragma unroll
                     for (int sub = 0; sub < KT; ++sub) {
                         const uint32_t see =
-                            live[rb] ? seen(mrow[rb], words, p0 + 32 * sub, len, end) : 0;
+                            live[rb] ? seen(mask + mrow[rb], words, p0 + 32 * sub, len, end) : 0;
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
                             if (!(see >> position(j, g) & 1)) s8[rb][8 * sub + j] = -INFINITY;
                     }
                 }
-                float mt = s8[rb][0];
+                float top = s8[rb][0];
 #pragma unroll
-                for (int j = 1; j < 8 * KT; ++j) mt = fmaxf(mt, s8[rb][j]);
-                const float mn = fmaxf(m[rb], max_over_groups(mt));
-                alpha[rb] = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rb] - mn);
-                moved |= m[rb] != mn;
-                m[rb] = mn;
+                for (int j = 1; j < 8 * KT; ++j) top = fmaxf(top, s8[rb][j]);
+                was[rb] = m[rb];
+                m[rb] = max_over_groups(fmaxf(top, m[rb]));
+                moved |= m[rb] != was[rb];
             }
             // ---- the outputs' scale.  It stays while the tile fits it and loses at most 6
             // bits of range to it, and stays 64 bits below the largest one so far (the
             // outputs' f32 must not overflow).
-            const int vtop = max(max(se[buf][1][0], se[buf][1][1]), max(se[buf][1][2], se[buf][1][3]));
             int down = 0;
             oe_top = max(oe_top, vtop);
             if (vtop > oe || vtop < oe - 6) {
@@ -391,54 +525,57 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
             if (__any(moved) || down != 0) {
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    l[rb] *= alpha[rb];
-                    const float x = ldexpf(alpha[rb], min(down, 120));
+                    const float alpha =
+                        was[rb] == m[rb] ? 1.f : __builtin_amdgcn_exp2f(was[rb] - m[rb]);
+                    l[rb] *= alpha;
+                    const float x = ldexpf(alpha, min(down, 120));
 #pragma unroll
                     for (int q = 0; q < NB; ++q)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) o[rb][q][j] *= x;
                 }
             }
-            // ---- weights, in the scale of the positions' V
+            // ---- weights, in the scale of the positions' V: 2^pe w
             f16x8 ph[RB][KT], pl[RB][KT];
-            const float px = pow2(max(kTop + ve - oe, -126));
+            const int pe = max(kTop + ve - oe, -126);
+            const float back = pow2(-pe);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                const float base = m[rb] == -INFINITY ? 0.f : m[rb];   // nothing seen: weights 0
+                const float base = (float)pe - (m[rb] == -INFINITY ? 0.f : m[rb]);
 #pragma unroll
                 for (int sub = 0; sub < KT; ++sub) {
                     float p8[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        p8[j] = __builtin_amdgcn_exp2f(s8[rb][8 * sub + j] - base);
-                        l[rb] += p8[j];
+                        p8[j] = __builtin_amdgcn_exp2f(s8[rb][8 * sub + j] + base);
+                        l[rb] = fmaf(p8[j], back, l[rb]);
                     }
-                    split8(p8, px, ph[rb][sub], pl[rb][sub]);
+                    split8(p8, 1.f, ph[rb][sub], pl[rb][sub]);
                 }
             }
             // ---- outputs
-            if (!slow_v) {
 #pragma unroll
-                for (int sub = 0; sub < KT; ++sub)
+            for (int grp = 0; grp < KT * NB * 4 / VG; ++grp) {
+                if (grp + 1 < KT * NB * 4 / VG) read_v(grp + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int q = 0; q < NB; ++q)
+                for (int y = 0; y < 3; ++y)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const f16x8 *v = sv[buf] + ((sub * NB + q) * 4 + j) * 128 + lane;
-                            const f16x8 vh = v[0], vl = v[64];
+                    for (int j = 0; j < VG; ++j)
 #pragma unroll
-                            for (int x = 0; x < 3; ++x)
-#pragma unroll
-                                for (int rb = 0; rb < RB; ++rb)
-                                    o[rb][q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                        x == 0 ? vl : vh, x == 1 ? pl[rb][sub] : ph[rb][sub],
-                                        o[rb][q][j], 0, 0, 0);
+                        for (int rb = 0; rb < RB; ++rb) {
+                            const int at = grp * VG + j;   // [32 positions][64 dims][j]
+                            f32x4 &d = o[rb][at / 4 % NB][at % 4];
+                            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                vf[grp & 1][j][y == 0],
+                                y == 1 ? pl[rb][at / (4 * NB)] : ph[rb][at / (4 * NB)], d, 0, 0, 0);
                         }
-            } else {
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (__builtin_expect(slow_v, 0)) {   // the values that are not finite
                 for (int i = 0; i < TK; ++i) {
                     const int sub = i >> 5, from = i >> 3 & 3, j = i & 7;
                     const float *v = vb + min(p0 + 32 * sub + position(j, from), end - 1) * a.v.ss;
-                    const int x = kTop - se[buf][1][from];
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb) {
                         float w = 0.f;
@@ -452,18 +589,17 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
                         for (int q = 0; q < NB; ++q)
 #pragma unroll
                             for (int y = 0; y < 16; ++y)
-                                if (64 * q + 16 * g < D)
-                                    o[rb][q][y & 3][y >> 2] =
-                                        fmaf(w, ldexpf(v[64 * q + 16 * g + y], x),
-                                             o[rb][q][y & 3][y >> 2]);
+                                if (64 * q + 16 * g < D) {
+                                    const float x = v[64 * q + 16 * g + y];
+                                    if (abs_bits(x) >= kInf)
+                                        o[rb][q][y & 3][y >> 2] =
+                                            fmaf(w, x, o[rb][q][y & 3][y >> 2]);
+                                }
                     }
                 }
             }
         }
-        if (tile + 1 < t1) {
-            store(tile + 1, buf ^ 1);
-            if (tile + 2 < t1) load(tile + 2);
-        }
+        if (tile + 1 < t1) store(tile + 1, buf ^ 1);
         __syncthreads();
     }
     if (!busy) return;
