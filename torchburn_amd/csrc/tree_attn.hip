@@ -164,6 +164,96 @@ __device__ __forceinline__ uint32_t seen(const int32_t *mrow, int words, int p0,
     return see;
 }
 
+// Query row i's limbs for lane group g, and its scale's exponent; with the sign of
+// the score's factor, which is then positive.  Rows past the last one repeat row 0.
+template <int NS>
+__device__ __forceinline__ void query_row(const TreeAttn &a, int b, int kvh, int i, int g,
+                                          f16x8 (&qh)[NS], f16x8 (&ql)[NS], int &qe) {
+    const int G = a.hq / a.hkv, D = a.hd;
+    i = i < a.n * G ? i : 0;
+    const float *q = a.q + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D + 4 * g;
+    float x[NS][8];
+    float top = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        const int d = 64 * (s >> 1);
+        float4 u = *reinterpret_cast<const float4 *>(q + 16 * (s & 1) + (d < D ? d : 0));
+        float4 v = *reinterpret_cast<const float4 *>(q + 16 * (s & 1) + (d + 32 < D ? d + 32 : 0));
+        if (d >= D) u = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (d + 32 >= D) v = make_float4(0.f, 0.f, 0.f, 0.f);
+        x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w;
+        x[s][4] = v.x; x[s][5] = v.y; x[s][6] = v.z; x[s][7] = v.w;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) max3_abs(top, x[s][j], x[s][j + 1]);
+    }
+    qe = exponent(abs_bits(max_over_groups(top)));
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+        split8(x[s], a.scale < 0.f ? -pow2(kTop - qe) : pow2(kTop - qe), qh[s], ql[s]);
+}
+
+// Whether a mask row has a bit among the tree's n, its words shared by the lane groups.
+__device__ __forceinline__ bool any_bit(const int32_t *row, int words, int n, int g) {
+    const uint32_t last = n % 32 ? (1u << (n % 32)) - 1 : ~0u;
+    uint32_t any = 0;
+    for (int w = g; w < words; w += 4) any |= (uint32_t)row[w] & (w == words - 1 ? last : ~0u);
+    return max_over_groups(any ? 1.f : 0.f) > 0.f;
+}
+
+// Row i's scores with the lane's positions of a tile whose K is not finite.
+template <int N>
+__device__ __forceinline__ void scores_in_f32(const TreeAttn &a, int b, int kvh, int i, int p0,
+                                              int end, int g, float (&s8)[N]) {
+    const int G = a.hq / a.hkv, D = a.hd;
+    i = fresh(i);
+    const float *q = a.q + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D;
+    const float *kb = a.k.p + b * a.k.sb + kvh * a.k.sh;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float *k = kb + min(p0 + position(j, g), end - 1) * a.k.ss;
+        float s = 0.f;
+        for (int d = 0; d < D; ++d) s = fmaf(q[d], k[d], s);
+        s8[j] = s * a.scale * kLog2e;
+    }
+}
+
+// Adds the values of a tile's V that are not finite, with their weights (row c's in
+// lane group `from` for its positions), to the outputs of row c.
+template <int NB, int KT>
+__device__ __forceinline__ void add_not_finite(const TreeAttn &a, const float *vb, int p0, int end,
+                                               int g, int c, const f16x8 *ph, const f16x8 *pl,
+                                               f32x4 (&o)[NB][4]) {
+    for (int i = 0; i < 32 * KT; ++i) {
+        const int sub = i >> 5, from = i >> 3 & 3, j = i & 7;
+        const float *v = vb + min(p0 + 32 * sub + position(j, from), end - 1) * a.v.ss;
+        float w = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8 * KT; ++k)
+            if (k == j + 8 * sub) w = (float)ph[k >> 3][k & 7] + (float)pl[k >> 3][k & 7];
+        w = __shfl(w, c + 16 * from);
+        if (w == 0.f) continue;
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+#pragma unroll
+            for (int y = 0; y < 16; ++y)
+                if (64 * q + 16 * g < a.hd) {
+                    const float x = v[64 * q + 16 * g + y];
+                    if (abs_bits(x) >= kInf) o[q][y & 3][y >> 2] = fmaf(w, x, o[q][y & 3][y >> 2]);
+                }
+    }
+}
+
+// The outputs' scale 2^(kTop - oe) for a tile of V's exponent ve: how far it moves
+// down.  It stays while the tile fits it and loses at most 6 bits of range to it, and
+// stays 64 bits below the largest one so far (the outputs' f32 must not overflow).
+__device__ __forceinline__ int rescale(int ve, int &oe, int &oe_top) {
+    oe_top = max(oe_top, ve);
+    if (ve <= oe && ve >= oe - 6) return 0;
+    const int to = max(ve, oe_top - 64), down = oe - to;
+    oe = to;
+    return down;
+}
+
 // Positions per tile: the same bytes for every head_dim up to 128.
 __host__ __device__ constexpr int tile_of(int dp) { return dp == 64 ? 64 : 32; }
 // Tiles per split where at most `cap` splits are wanted.  Only the sequence's own
@@ -355,41 +445,17 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
     const int32_t *mask = a.mask + b * a.mask_sb;
     // ---- the wave's query rows, row c of each block in this lane
     f16x8 qh[RB][NS], ql[RB][NS];
-    int mrow[RB];   // its mask row's first word
+    int mrow[RB], qe[RB];
     bool live[RB];
     float m[RB], l[RB];
-    int qe[RB];
     f32x4 o[RB][NB][4];
-    const uint32_t last_bits = a.n % 32 ? (1u << (a.n % 32)) - 1 : ~0u;
     const bool busy = w0 < R;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        const int i = w0 + 16 * rb + c, iq = i < R ? i : 0;
-        const float *q = a.q + (((size_t)b * a.n + iq / G) * a.hq + kvh * G + iq % G) * D + 4 * g;
-        float x[NS][8];
-        float top = 0.f;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            const int d = 64 * (s >> 1);
-            float4 u = *reinterpret_cast<const float4 *>(q + 16 * (s & 1) + (d < D ? d : 0));
-            float4 v = *reinterpret_cast<const float4 *>(q + 16 * (s & 1) + (d + 32 < D ? d + 32 : 0));
-            if (d >= D) u = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (d + 32 >= D) v = make_float4(0.f, 0.f, 0.f, 0.f);
-            x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w;
-            x[s][4] = v.x; x[s][5] = v.y; x[s][6] = v.z; x[s][7] = v.w;
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) max3_abs(top, x[s][j], x[s][j + 1]);
-        }
-        qe[rb] = exponent(abs_bits(max_over_groups(top)));
-#pragma unroll
-        for (int s = 0; s < NS; ++s)   // with the sign of the score's factor, which is then positive
-            split8(x[s], a.scale < 0.f ? -pow2(kTop - qe[rb]) : pow2(kTop - qe[rb]), qh[rb][s],
-                   ql[rb][s]);
-        mrow[rb] = iq / G * words;
-        uint32_t any = 0;
-        for (int w = g; w < words; w += 4)
-            any |= (uint32_t)mask[mrow[rb] + w] & (w == words - 1 ? last_bits : ~0u);
-        live[rb] = i < R && max_over_groups(any ? 1.f : 0.f) > 0.f;
+        const int i = w0 + 16 * rb + c;
+        query_row<NS>(a, b, kvh, i, g, qh[rb], ql[rb], qe[rb]);
+        mrow[rb] = (i < R ? i : 0) / G * words;
+        live[rb] = i < R && any_bit(mask + mrow[rb], words, a.n, g);
         m[rb] = -INFINITY;
         l[rb] = 0.f;
 #pragma unroll
@@ -478,17 +544,9 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
             }
             if (__builtin_expect(slow_k, 0)) {
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    const int i = fresh(min(w0 + 16 * rb + c, R - 1));
-                    const float *q = a.q + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D;
-#pragma unroll
-                    for (int j = 0; j < 8 * KT; ++j) {
-                        const float *k = kb + min(p0 + position(j, g), end - 1) * a.k.ss;
-                        float s = 0.f;
-                        for (int d = 0; d < D; ++d) s = fmaf(q[d], k[d], s);
-                        s8[rb][j] = s * a.scale * kLog2e;
-                    }
-                }
+                for (int rb = 0; rb < RB; ++rb)
+                    scores_in_f32<8 * KT>(a, b, kvh, min(w0 + 16 * rb + c, R - 1), p0, end, g,
+                                          s8[rb]);
             }
             // ---- running maxima
             float was[RB];
@@ -512,16 +570,7 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
                 m[rb] = max_over_groups(fmaxf(top, m[rb]));
                 moved |= m[rb] != was[rb];
             }
-            // ---- the outputs' scale.  It stays while the tile fits it and loses at most 6
-            // bits of range to it, and stays 64 bits below the largest one so far (the
-            // outputs' f32 must not overflow).
-            int down = 0;
-            oe_top = max(oe_top, vtop);
-            if (vtop > oe || vtop < oe - 6) {
-                const int to = max(vtop, oe_top - 64);
-                down = oe - to;
-                oe = to;
-            }
+            const int down = rescale(vtop, oe, oe_top);
             if (__any(moved) || down != 0) {
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
@@ -572,31 +621,10 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
                         }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (__builtin_expect(slow_v, 0)) {   // the values that are not finite
-                for (int i = 0; i < TK; ++i) {
-                    const int sub = i >> 5, from = i >> 3 & 3, j = i & 7;
-                    const float *v = vb + min(p0 + 32 * sub + position(j, from), end - 1) * a.v.ss;
+            if (__builtin_expect(slow_v, 0)) {
 #pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) {
-                        float w = 0.f;
-#pragma unroll
-                        for (int k = 0; k < 8 * KT; ++k)
-                            if (k == (i & 7) + 8 * sub)
-                                w = (float)ph[rb][k >> 3][k & 7] + (float)pl[rb][k >> 3][k & 7];
-                        w = __shfl(w, c + 16 * from);
-                        if (w == 0.f) continue;
-#pragma unroll
-                        for (int q = 0; q < NB; ++q)
-#pragma unroll
-                            for (int y = 0; y < 16; ++y)
-                                if (64 * q + 16 * g < D) {
-                                    const float x = v[64 * q + 16 * g + y];
-                                    if (abs_bits(x) >= kInf)
-                                        o[rb][q][y & 3][y >> 2] =
-                                            fmaf(w, x, o[rb][q][y & 3][y >> 2]);
-                                }
-                    }
-                }
+                for (int rb = 0; rb < RB; ++rb)
+                    add_not_finite<NB, KT>(a, vb, p0, end, g, c, ph[rb], pl[rb], o[rb]);
             }
         }
         if (tile + 1 < t1) store(tile + 1, buf ^ 1);
@@ -631,6 +659,302 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
                     if (!live[rb]) y = make_float4(0.f, 0.f, 0.f, 0.f);
                     reinterpret_cast<float4 *>(to + 64 * q + 16 * g)[r] = y;
                 }
+    }
+}
+
+// The same for few rows (up to 32 of a KV head), where K and V have to stream: a
+// block's waves take tiles of 32 positions in turn, each with the block's 16 * RB
+// rows and maxima, sums and outputs of its own, and meet in LDS once at the end.
+// K and V go from memory to MFMA operands in the wave's own registers, and nothing
+// in the loop waits for another wave.  The next tile's K is requested when this
+// one's scores are on their way, its V when this one's limbs are built.
+template <int DP, int RB>
+__global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
+                                                          float *__restrict__ part,
+                                                          float *__restrict__ pml) {
+    constexpr int NS = DP / 32, NB = DP / 64, ROWS = 16 * RB, TK = 32;
+    __shared__ __attribute__((aligned(16))) float lo[ROWS][DP + 4];
+    __shared__ float lm[4][ROWS], ls[4][ROWS];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, g = lane >> 4;
+    const int G = a.hq / a.hkv, R = a.n * G, D = a.hd, words = (a.n + 31) / 32;
+    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
+    const int tiles = (end + TK - 1) / TK, tps = tiles_per_split(tiles, cap);
+    const int t0 = split * tps, t1 = min(tiles, t0 + tps);
+    if (split > 0 && t0 >= t1) return;   // the merge skips this split
+    const float *kb = a.k.p + b * a.k.sb + kvh * a.k.sh, *vb = a.v.p + b * a.v.sb + kvh * a.v.sh;
+    const int32_t *mask = a.mask + b * a.mask_sb;
+
+    float kr[2][NS][8], vr[8][NB][4];
+    auto load_k = [&](int tile) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float *r = kb + min(tile * TK + 16 * h + c, end - 1) * a.k.ss + 4 * g;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                const int d = 64 * (s >> 1);
+                const float4 x =
+                    *reinterpret_cast<const float4 *>(r + 16 * (s & 1) + (d < D ? d : 0));
+                const float4 y =
+                    *reinterpret_cast<const float4 *>(r + 16 * (s & 1) + (d + 32 < D ? d + 32 : 0));
+                float *k = kr[h][s];
+                k[0] = x.x; k[1] = x.y; k[2] = x.z; k[3] = x.w;
+                k[4] = y.x; k[5] = y.y; k[6] = y.z; k[7] = y.w;
+            }
+        }
+    };
+    auto load_v = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float *r = vb + min(tile * TK + position(i, g), end - 1) * a.v.ss;
+#pragma unroll
+            for (int q = 0; q < NB; ++q) {
+                const float4 x = *reinterpret_cast<const float4 *>(r + min(64 * q + 4 * c, D - 4));
+                vr[i][q][0] = x.x; vr[i][q][1] = x.y; vr[i][q][2] = x.z; vr[i][q][3] = x.w;
+            }
+        }
+    };
+    const int first = t0 + wave;
+    if (first < t1) {
+        load_k(first);
+        load_v(first);
+    }
+    f16x8 qh[RB][NS], ql[RB][NS];
+    int mrow[RB], qe[RB];
+    bool live[RB];
+    float m[RB], l[RB];
+    f32x4 o[RB][NB][4];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int i = 16 * rb + c;
+        query_row<NS>(a, b, kvh, i, g, qh[rb], ql[rb], qe[rb]);
+        mrow[rb] = (i < R ? i : 0) / G * words;
+        live[rb] = i < R && any_bit(mask + mrow[rb], words, a.n, g);
+        m[rb] = -INFINITY;
+        l[rb] = 0.f;
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[rb][q][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    int oe = 0, oe_top = -1000;   // exponent of the outputs' scale; the largest V's so far
+    const float f = fabsf(a.scale) * kLog2e;
+
+    for (int tile = first; tile < t1; tile += 4) {
+        const int p0 = tile * TK;
+        const bool open = p0 + TK <= len;   // every live row sees every position
+        // ---- the tile's scales
+        float km = 0.f, kn = 0.f, vm = 0.f, vn = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                max3_abs(km, kr[0][s][j], kr[0][s][j + 1]);
+                max3_abs(kn, kr[1][s][j], kr[1][s][j + 1]);
+            }
+        uint32_t kt = max(abs_bits(km), abs_bits(kn)), zero = 0;
+        wave_max_bits(kt, zero);
+        const bool bad_k = kt >= kInf;
+        const int ke = exponent(kt);
+        // ---- scores, in powers of two
+        f32x4 acc[RB][2];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) acc[rb][0] = acc[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            f16x8 kh[2], kl[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) split8(kr[h][s], pow2(kTop - ke), kh[h], kl[h]);
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        acc[rb][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            x == 0 ? kl[h] : kh[h], x == 1 ? ql[rb][s] : qh[rb][s], acc[rb][h], 0,
+                            0, 0);
+        }
+        if (tile + 4 < t1) load_k(tile + 4);
+        float s8[RB][8];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const float sx = ldexpf(f, qe[rb] + ke - 2 * kTop);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s8[rb][j] = acc[rb][j >> 2][j & 3] * sx;
+        }
+        if (__builtin_expect(bad_k, 0)) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+                scores_in_f32<8>(a, b, kvh, min(16 * rb + c, R - 1), p0, end, g, s8[rb]);
+        }
+        // ---- running maxima
+        float was[RB];
+        bool moved = false;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            if (!open) {
+                const uint32_t see = live[rb] ? seen(mask + mrow[rb], words, p0, len, end) : 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!(see >> position(j, g) & 1)) s8[rb][j] = -INFINITY;
+            }
+            float top = s8[rb][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) top = fmaxf(top, s8[rb][j]);
+            was[rb] = m[rb];
+            m[rb] = max_over_groups(fmaxf(top, m[rb]));
+            moved |= m[rb] != was[rb];
+        }
+        // ---- V's scale and the outputs'
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int q = 0; q < NB; ++q) {
+                max3_abs(vm, vr[i][q][0], vr[i][q][1]);
+                max3_abs(vn, vr[i][q][2], vr[i][q][3]);
+            }
+        uint32_t vt = max(abs_bits(vm), abs_bits(vn));
+        if (!open) {   // NaN too: a row that does not see its position must not get it
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int q = 0; q < NB; ++q)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) vt = max(vt, abs_bits(vr[i][q][j]));
+        }
+        wave_max_bits(vt, zero);
+        const bool bad_v = vt >= kInf;
+        if (__builtin_expect(bad_v, 0)) {   // out of the limbs; what has weight is added in f32
+            vt = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int q = 0; q < NB; ++q)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        vr[i][q][j] = abs_bits(vr[i][q][j]) < kInf ? vr[i][q][j] : 0.f;
+                        vt = max(vt, abs_bits(vr[i][q][j]));
+                    }
+            wave_max_bits(vt, zero);
+        }
+        const int ve = exponent(vt), down = rescale(ve, oe, oe_top);
+        if (__any(moved) || down != 0) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const float alpha = was[rb] == m[rb] ? 1.f : __builtin_amdgcn_exp2f(was[rb] - m[rb]);
+                l[rb] *= alpha;
+                const float x = ldexpf(alpha, min(down, 120));
+#pragma unroll
+                for (int q = 0; q < NB; ++q)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[rb][q][j] *= x;
+            }
+        }
+        // ---- weights 2^kTop w
+        f16x8 ph[RB], pl[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const float base = (float)kTop - (m[rb] == -INFINITY ? 0.f : m[rb]);
+            float p8[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p8[j] = __builtin_amdgcn_exp2f(s8[rb][j] + base);
+                l[rb] += p8[j];
+            }
+            split8(p8, 1.f, ph[rb], pl[rb]);
+        }
+        // ---- outputs; V takes the outputs' scale
+#pragma unroll
+        for (int q = 0; q < NB; ++q) {
+            f16x8 vh[4], vl[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x[8] = {vr[0][q][j], vr[1][q][j], vr[2][q][j], vr[3][q][j],
+                                    vr[4][q][j], vr[5][q][j], vr[6][q][j], vr[7][q][j]};
+                split8(x, pow2(kTop - oe), vh[j], vl[j]);
+            }
+#pragma unroll
+            for (int x = 0; x < 3; ++x)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb)
+                        o[rb][q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            x == 0 ? vl[j] : vh[j], x == 1 ? pl[rb] : ph[rb], o[rb][q][j], 0, 0, 0);
+        }
+        if (tile + 4 < t1) load_v(tile + 4);
+        if (__builtin_expect(bad_v, 0)) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+                add_not_finite<NB, 1>(a, vb, p0, end, g, c, &ph[rb], &pl[rb], o[rb]);
+        }
+    }
+
+    // ---- the four waves' outputs, brought to one maximum and summed in wave order
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        if (!live[rb]) m[rb] = -INFINITY;
+        const float sum = sum_over_groups(l[rb]);
+        l[rb] = live[rb] ? sum : 0.f;
+        if (g == 0) {
+            lm[wave][16 * rb + c] = m[rb];
+            ls[wave][16 * rb + c] = l[rb];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (wave == w) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const int r = 16 * rb + c;
+                const float top = fmaxf(fmaxf(lm[0][r], lm[1][r]), fmaxf(lm[2][r], lm[3][r]));
+                const float x = m[rb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rb] - top);
+#pragma unroll
+                for (int q = 0; q < NB; ++q)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float4 *d = reinterpret_cast<float4 *>(&lo[r][64 * q + 16 * g]) + i;
+                        float4 y = w ? *d : make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (x != 0.f) {
+                            y.x = fmaf(ldexpf(o[rb][q][0][i], oe - kTop), x, y.x);
+                            y.y = fmaf(ldexpf(o[rb][q][1][i], oe - kTop), x, y.y);
+                            y.z = fmaf(ldexpf(o[rb][q][2][i], oe - kTop), x, y.z);
+                            y.w = fmaf(ldexpf(o[rb][q][3][i], oe - kTop), x, y.w);
+                        }
+                        *d = y;
+                    }
+            }
+        }
+        __syncthreads();
+    }
+    const int cols = D / 4;
+    for (int x = t; x < ROWS * cols; x += 256) {
+        const int r = x / cols, d = x % cols;
+        if (r >= R) break;
+        const float top = fmaxf(fmaxf(lm[0][r], lm[1][r]), fmaxf(lm[2][r], lm[3][r]));
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            if (lm[w][r] != -INFINITY)
+                sum = fmaf(ls[w][r], __builtin_amdgcn_exp2f(lm[w][r] - top), sum);
+        const float4 y = *reinterpret_cast<const float4 *>(&lo[r][4 * d]);
+        if (part) {
+            const size_t at = (((size_t)b * a.hkv + kvh) * gridDim.x + split) * R + r;
+            // sums and outputs as the other kernel leaves them, without 2^kTop
+            reinterpret_cast<float4 *>(part + at * D)[d] =
+                make_float4(y.x * pow2(-kTop), y.y * pow2(-kTop), y.z * pow2(-kTop), y.w * pow2(-kTop));
+            if (d == 0) {
+                pml[2 * at] = top;
+                pml[2 * at + 1] = sum * pow2(-kTop);
+            }
+        } else {
+            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            float *out = a.out + (((size_t)b * a.n + r / G) * a.hq + kvh * G + r % G) * D;
+            reinterpret_cast<float4 *>(out)[d] =
+                make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+        }
     }
 }
 
@@ -700,17 +1024,21 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int tk, int cap,
 }
 
 struct Plan {
-    int dp, rb, rtiles, cap, nsplit;
+    bool few;
+    int dp, rb, tk, rtiles, cap, nsplit;
 };
 
 Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len) {
     Plan p;
     p.dp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-    const int R = n * (hq / hkv), tk = tile_of(p.dp), tiles = (max_len + tk - 1) / tk;
-    p.rb = R <= 64 || p.dp == 256 ? 1 : 2;
-    p.rtiles = (R + 64 * p.rb - 1) / (64 * p.rb);
-    const int64_t want = 512 / ((int64_t)p.rtiles * hkv * batch);
+    const int R = n * (hq / hkv);
+    p.few = R <= 32 && p.dp <= 128;
+    p.rb = p.few ? (R <= 16 ? 1 : 2) : R <= 64 || p.dp == 256 ? 1 : 2;
+    p.tk = p.few ? 32 : tile_of(p.dp);
+    p.rtiles = p.few ? 1 : (R + 64 * p.rb - 1) / (64 * p.rb);
+    const int64_t want = (p.few ? 256 : 512) / ((int64_t)p.rtiles * hkv * batch);
     p.cap = (int)std::max<int64_t>(1, std::min<int64_t>(want, kMaxSplits));
+    const int tiles = (max_len + p.tk - 1) / p.tk;
     p.nsplit = std::max(1, std::min(p.cap, (tiles + kMinTiles - 1) / kMinTiles));
     return p;
 }
@@ -727,30 +1055,38 @@ int launch_tree_attention(const TreeAttn &a, int max_len, float *scratch, hipStr
     float *part = p.nsplit > 1 ? scratch : nullptr;
     float *pml = part ? part + (size_t)a.batch * a.hq * a.n * p.nsplit * a.hd : nullptr;
     const dim3 grid(p.nsplit, a.hkv * p.rtiles, a.batch);
+#define TB_TF(DP, RB)                                                                        \
+    if (p.few && p.dp == DP && p.rb == RB)                                                   \
+    hipLaunchKernelGGL((k_tree_attn_few<DP, RB>), grid, dim3(256), 0, s, a, p.cap, part, pml)
 #define TB_TA(DP, RB)                                                                        \
-    if (p.dp == DP && p.rb == RB)                                                            \
+    if (!p.few && p.dp == DP && p.rb == RB)                                                  \
     hipLaunchKernelGGL((k_tree_attn<DP, RB>), grid, dim3(256), 0, s, a, p.cap, part, pml)
+    TB_TF(64, 1);
+    TB_TF(64, 2);
+    TB_TF(128, 1);
+    TB_TF(128, 2);
     TB_TA(64, 1);
     TB_TA(64, 2);
     TB_TA(128, 1);
     TB_TA(128, 2);
     TB_TA(256, 1);
 #undef TB_TA
+#undef TB_TF
     TB_LAUNCHED();
     if (part) {
         const int R = a.n * (a.hq / a.hkv);
         const dim3 rows((R + 3) / 4, a.hkv, a.batch);
         if (a.hd <= 32)
-            hipLaunchKernelGGL(k_tree_merge<8>, rows, dim3(256), 0, s, a, tile_of(p.dp), p.cap,
+            hipLaunchKernelGGL(k_tree_merge<8>, rows, dim3(256), 0, s, a, p.tk, p.cap,
                                p.nsplit, part, pml);
         else if (a.hd <= 64)
-            hipLaunchKernelGGL(k_tree_merge<16>, rows, dim3(256), 0, s, a, tile_of(p.dp), p.cap,
+            hipLaunchKernelGGL(k_tree_merge<16>, rows, dim3(256), 0, s, a, p.tk, p.cap,
                                p.nsplit, part, pml);
         else if (a.hd <= 128)
-            hipLaunchKernelGGL(k_tree_merge<32>, rows, dim3(256), 0, s, a, tile_of(p.dp), p.cap,
+            hipLaunchKernelGGL(k_tree_merge<32>, rows, dim3(256), 0, s, a, p.tk, p.cap,
                                p.nsplit, part, pml);
         else
-            hipLaunchKernelGGL(k_tree_merge<64>, rows, dim3(256), 0, s, a, tile_of(p.dp), p.cap,
+            hipLaunchKernelGGL(k_tree_merge<64>, rows, dim3(256), 0, s, a, p.tk, p.cap,
                                p.nsplit, part, pml);
         TB_LAUNCHED();
     }
