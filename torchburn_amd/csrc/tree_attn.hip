@@ -12,7 +12,7 @@
 // stays that of an f32 product, at a third of the f16 rate (the f32 MFMA has a
 // sixteenth of it).  s puts the largest factor of a tile (K, V) or row (Q) at
 // 2^14, so factors down to 2^-25 of it keep both limbs whole and smaller ones an
-// error of 2^-39 of it.  Weights are taken as w 2^14 for the same reason.  Scores,
+// error of 2^-39 of it.  Weights are taken as w 2^7 for the same reason.  Scores,
 // running maxima, sums and outputs are f32.
 #include <math.h>
 
@@ -35,6 +35,12 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kMaxSplits = 128;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kTop = 14;         // factors are scaled to below 2^(kTop + 1)
+// A row's reference maximum follows its scores only when they pass it by more than
+// 2^kLag: the outputs' rescale (a third of a tile's vector work where one of 32
+// rows needs it in most tiles) then runs in few of them.  Weights reach 2^kLag and
+// are scaled by 2^kWeight, so that they stay below 2^(kTop + 2), the f16 range.
+constexpr float kLag = 8.f;
+constexpr int kWeight = 7;
 
 // Exponent of the largest magnitude given its bits, such that 2^(kTop - e) is a
 // normal f32 (values below 2^-113 keep an error below the smallest f32).
@@ -567,7 +573,8 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
 #pragma unroll
                 for (int j = 1; j < 8 * KT; ++j) top = fmaxf(top, s8[rb][j]);
                 was[rb] = m[rb];
-                m[rb] = max_over_groups(fmaxf(top, m[rb]));
+                top = max_over_groups(top);
+                m[rb] = top > m[rb] + kLag ? top : m[rb];
                 moved |= m[rb] != was[rb];
             }
             const int down = rescale(vtop, oe, oe_top);
@@ -586,7 +593,7 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
             }
             // ---- weights, in the scale of the positions' V: 2^pe w
             f16x8 ph[RB][KT], pl[RB][KT];
-            const int pe = max(kTop + ve - oe, -126);
+            const int pe = max(kWeight + ve - oe, -126);
             const float back = pow2(-pe);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
@@ -652,10 +659,10 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float4 y;
-                    y.x = ldexpf(o[rb][q][0][r], oe - 2 * kTop) * x;
-                    y.y = ldexpf(o[rb][q][1][r], oe - 2 * kTop) * x;
-                    y.z = ldexpf(o[rb][q][2][r], oe - 2 * kTop) * x;
-                    y.w = ldexpf(o[rb][q][3][r], oe - 2 * kTop) * x;
+                    y.x = ldexpf(o[rb][q][0][r], oe - kTop - kWeight) * x;
+                    y.y = ldexpf(o[rb][q][1][r], oe - kTop - kWeight) * x;
+                    y.z = ldexpf(o[rb][q][2][r], oe - kTop - kWeight) * x;
+                    y.w = ldexpf(o[rb][q][3][r], oe - kTop - kWeight) * x;
                     if (!live[rb]) y = make_float4(0.f, 0.f, 0.f, 0.f);
                     reinterpret_cast<float4 *>(to + 64 * q + 16 * g)[r] = y;
                 }
@@ -803,7 +810,8 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
 #pragma unroll
             for (int j = 1; j < 8; ++j) top = fmaxf(top, s8[rb][j]);
             was[rb] = m[rb];
-            m[rb] = max_over_groups(fmaxf(top, m[rb]));
+            top = max_over_groups(top);
+            m[rb] = top > m[rb] + kLag ? top : m[rb];
             moved |= m[rb] != was[rb];
         }
         // ---- V's scale and the outputs'
@@ -851,11 +859,11 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
                     for (int j = 0; j < 4; ++j) o[rb][q][j] *= x;
             }
         }
-        // ---- weights 2^kTop w
+        // ---- weights 2^kWeight w
         f16x8 ph[RB], pl[RB];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            const float base = (float)kTop - (m[rb] == -INFINITY ? 0.f : m[rb]);
+            const float base = (float)kWeight - (m[rb] == -INFINITY ? 0.f : m[rb]);
             float p8[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -942,12 +950,12 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
         const float4 y = *reinterpret_cast<const float4 *>(&lo[r][4 * d]);
         if (part) {
             const size_t at = (((size_t)b * a.hkv + kvh) * gridDim.x + split) * R + r;
-            // sums and outputs as the other kernel leaves them, without 2^kTop
+            // sums and outputs as the other kernel leaves them, without 2^kWeight
             reinterpret_cast<float4 *>(part + at * D)[d] =
-                make_float4(y.x * pow2(-kTop), y.y * pow2(-kTop), y.z * pow2(-kTop), y.w * pow2(-kTop));
+                make_float4(y.x * pow2(-kWeight), y.y * pow2(-kWeight), y.z * pow2(-kWeight), y.w * pow2(-kWeight));
             if (d == 0) {
                 pml[2 * at] = top;
-                pml[2 * at + 1] = sum * pow2(-kTop);
+                pml[2 * at + 1] = sum * pow2(-kWeight);
             }
         } else {
             const float inv = sum == 0.f ? 0.f : 1.0f / sum;
