@@ -199,3 +199,37 @@ def test_history_forms(cuda):
     assert torch.equal(tb.process_logits(half, h, **kw), tb.process_logits(half.float(), h, **kw))
     assert tb.process_logits(x[:0], h, **kw).shape == (0, V)
     assert tb.greedy_tokens(x[:0], h).shape == (0,)
+
+
+def test_alignment_and_many_biases(cuda):
+    """Rows at every distance from a 16-byte boundary, input and output apart or alike, and
+    more biases than one block lists, some tokens named many times."""
+    print("case process_logits alignment, many biases", flush=True)
+    V, R = 2053, 5
+    g = np.random.default_rng(3)
+    x = (g.standard_normal((R, V)) * 2).astype(np.float32)
+    hist = g.integers(0, V, (1, 200))
+    ids = g.integers(0, 300, (1, 4000))
+    bias = g.standard_normal((1, 4000)).astype(np.float32) / 16
+    ids[:, 600:] += 1000
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    kw = dict(history=T(hist), repetition_penalty=1.5, presence_penalty=0.5, frequency_penalty=0.25,
+              bias_ids=T(ids), bias_values=T(bias), allowed=T(pack(g.random((R, V)) < 0.8)))
+    want = tb.process_logits(T(x), **kw)
+    ref, bound = reference(x, np.repeat(hist, R, 0).tolist(), [200] * R, [0] * R, [1.5] * R,
+                           [0.5] * R, [0.25] * R, np.repeat(ids, R, 0).tolist(),
+                           np.repeat(bias, R, 0).tolist(), None, [[]] * R)
+    y = want.cpu().numpy()
+    fin = np.isfinite(y)
+    assert fin.any() and (np.abs(y - ref)[fin] <= bound[fin]).all()
+    buf = torch.empty(R * V + 8, device=cuda)
+    obuf = torch.empty(R * V + 8, device=cuda)
+    for a in range(4):
+        xs = buf[a:a + R * V].view(R, V)
+        for b in range(4):
+            xs.copy_(T(x))
+            out = obuf[b:b + R * V].view(R, V)
+            assert torch.equal(tb.process_logits(xs, **kw, out=out), want)
+        assert tb.greedy_tokens(xs, **kw).tolist() == best(y)
+        tb.process_logits(xs, **kw, out=xs)
+        assert torch.equal(xs, want)

@@ -75,7 +75,8 @@ U, V = _lib.TB_ERR_UNSUPPORTED, _lib.TB_ERR_VALUE
     (logits, dict(n_bias=2), U, b"null"), (logits, dict(n_bias=2, bias_groups=3), U, b"divide"),
     (logits, dict(nodes=3), U, b"divide"), (logits, dict(nodes=2), U, b"null"),
     (logits, dict(nodes=1028, rows=1028), U, b"nodes"),
-    (logits, dict(allowed=A, stride=3), U, b"mask rows"),
+    (logits, dict(allowed=A, stride=3), U, b"mask rows"), (logits, dict(x=A + 2), U, b"misaligned"),
+    (logits, dict(history=A + 4), U, b"misaligned"),
     (logits, dict(tokens=A, scratch=A, size=1), U, b"scratch"),
 ])
 def test_c_refusals(call, kw, code, msg):

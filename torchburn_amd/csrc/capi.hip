@@ -1355,7 +1355,7 @@ int tb_process_logits(const float *logits, float *out, int64_t *tokens, int64_t 
                       int64_t scratch_bytes, void *stream) {
     TB_REQUIRE(rows >= 0 && rows <= 65535 && vocab > 0 && vocab <= (1 << 30), TB_ERR_UNSUPPORTED,
                "TB_UNSUPPORTED: process_logits: rows outside 0..65535 or vocabulary outside 1..2^30");
-    TB_REQUIRE(hist >= 0 && hist <= (1 << 30) && n_bias >= 0 && n_bias <= (1 << 30),
+    TB_REQUIRE(hist >= 0 && hist <= (1 << 29) && n_bias >= 0 && n_bias <= (1 << 29),
                TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: process_logits: bad history or bias length");
     TB_REQUIRE(hist == 0 || (groups > 0 && rows % groups == 0), TB_ERR_UNSUPPORTED,
                "TB_UNSUPPORTED: process_logits: " + std::to_string(groups) +
@@ -1373,6 +1373,10 @@ int tb_process_logits(const float *logits, float *out, int64_t *tokens, int64_t 
     TB_REQUIRE(logits && (out || tokens) && (hist == 0 || history) &&
                    (n_bias == 0 || (bias_ids && bias)) && (nodes == 0 || (draft_tokens && tree_mask)),
                TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: process_logits: null pointer");
+    TB_REQUIRE(aligned(logits, 4) && aligned(out, 4) && aligned(tokens, 8) && aligned(history, 8) &&
+                   aligned(draft_tokens, 8) && aligned(bias_ids, 8) && aligned(bias, 4) &&
+                   aligned(allowed, 4) && aligned(tree_mask, 4),
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: process_logits: misaligned device pointer");
     TB_REQUIRE(allowed_stride == 0 || allowed_stride >= (vocab + 31) / 32, TB_ERR_UNSUPPORTED,
                "TB_UNSUPPORTED: process_logits: mask rows shorter than the vocabulary");
     LogitsParams p{};

@@ -21,15 +21,11 @@ namespace tb {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr uint32_t kSeen = 0x80000000u;   // counts: occurs in the prompt part
-
-// Tokens of one block: its counts (and biases) are kept in LDS.
-int chunk_tokens(int rows, int vocab) {
-    (void)rows;
-    (void)vocab;
-    return 4096;
-}
+constexpr int kThreads = 512;
+constexpr uint32_t kSeen = 1u << 31;   // of a token's LDS word: occurs in the history
+constexpr uint32_t kBias = 1u << 30;   // has a bias; the rest: its count
+constexpr uint32_t kCount = kBias - 1;
+constexpr int kBiasList = 512;         // biases of one block kept in LDS
 
 // Orders as the values do, ties to the lower index; 0: nothing to take.
 __device__ __forceinline__ uint64_t best_item(float y, int t) {
@@ -48,30 +44,76 @@ __device__ __forceinline__ uint64_t max_over_wave(uint64_t v) {
     return v;
 }
 
-// Grid (token chunks, rows).
-__global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, uint64_t *part) {
-    extern __shared__ uint32_t lds[];
-    __shared__ uint64_t red[kThreads / 64];
-    uint32_t *cnt = lds;
-    float *bias = reinterpret_cast<float *>(lds + (p.hist || p.nodes ? chunk : 0));
-    const int tid = threadIdx.x, r = blockIdx.y;
-    const int t0 = blockIdx.x * chunk, nt = min(chunk, p.vocab - t0);
-    const bool counted = p.hist || p.nodes;
-    for (int i = tid; i < nt; i += kThreads) {
-        if (counted) cnt[i] = 0;
-        if (p.n_bias) bias[i] = 0.f;
+struct Biases {
+    const int64_t *ids;
+    const float *val;
+    int n;              // entries of the row's list
+    int at[kBiasList], token[kBiasList];   // those of the block's tokens, in any order
+    int count;          // how many there are (past kBiasList: not listed)
+};
+
+// Token t's biases added to y in the order of the list.
+__device__ float add_biases(float y, int t, const Biases &b) {
+    float s = 0.f;
+    bool any = false;
+    if (b.count <= kBiasList) {
+        for (int last = -1;;) {   // the lowest entry past the last one taken
+            int next = b.n;
+            for (int j = 0; j < b.count; ++j) {
+                const int i = b.at[j];
+                if (b.token[j] == t && i > last && i < next) next = i;
+            }
+            if (next == b.n) break;
+            s = any ? __fadd_rn(s, b.val[next]) : b.val[next];
+            any = true;
+            last = next;
+        }
+    } else {
+        for (int i = 0; i < b.n; ++i)
+            if (b.ids[i] == t) {
+                s = any ? __fadd_rn(s, b.val[i]) : b.val[i];
+                any = true;
+            }
     }
-    __syncthreads();
+    return any ? __fadd_rn(y, s) : y;
+}
+
+// One block per row and chunk of the vocabulary.  Bound by the logits' bytes: they
+// pass through once, 16 bytes a lane, four loads in flight (a lane whose four
+// tokens the mask excludes reads none).  A word of LDS per token holds what the
+// history, the tree path and the biases say of it; the block reads those lists
+// whole, which is why chunks are as large as the row count lets them be.
+// Vectors start where the row's address is a multiple of 16 bytes, `lead` tokens
+// into it; LDS word 4 is the chunk's first vector, the words before it are chunk
+// 0's tokens ahead of that.  The last vector may be cut.
+template <bool VEC>
+__global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, uint64_t *part) {
+    extern __shared__ uint32_t word[];
+    __shared__ uint64_t red[kThreads / 64];
+    __shared__ Biases bias;
+    const int tid = threadIdx.x, r = blockIdx.y, V = p.vocab;
+    const bool marked = p.hist || p.nodes || p.n_bias;
+    const float *x = p.x + (size_t)r * V;
+    float *y = p.y ? p.y + (size_t)r * V : nullptr;
+    const int lead = VEC ? (int)((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / 4) : 0;
+    const int v0 = lead + blockIdx.x * chunk;                     // the first vector's token
+    const int t0 = blockIdx.x ? v0 : 0, t1 = min(V, v0 + chunk);   // the block's tokens
+    if (marked) {
+        for (int i = tid; i < chunk + 4; i += kThreads) word[i] = 0;
+        if (tid == 0) bias.count = 0;
+        __syncthreads();
+    }
+    uint32_t *at = word + 4 - v0;   // token t's word
     if (p.hist) {
         const int g = r / (p.rows / p.groups);
         const int len = p.history_len ? min(max(p.history_len[g], 0), p.hist) : p.hist;
         const int prompt = p.prompt_len ? p.prompt_len[g] : p.prompt;
         const int64_t *h = p.history + (size_t)g * p.hist;
         for (int i = tid; i < len; i += kThreads) {
-            const int64_t t = h[i] - t0;
-            if (t < 0 || t >= nt) continue;
-            if (i < prompt) atomicOr(&cnt[t], kSeen);
-            else atomicAdd(&cnt[t], 1u);
+            const int64_t t = h[i];
+            if (t < t0 || t >= t1) continue;
+            if (i < prompt) atomicOr(&at[t], kSeen);
+            else atomicAdd(&at[t], 1u);
         }
     }
     if (p.nodes) {
@@ -79,49 +121,102 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, 
         const int64_t *d = p.draft + (size_t)(r / p.nodes) * p.nodes;
         const int32_t *m = p.tree_mask + ((size_t)(r / p.nodes) * p.nodes + node) * words;
         for (int j = tid; j < p.nodes; j += kThreads) {
-            if (!((uint32_t)m[j >> 5] >> (j & 31) & 1)) continue;
-            const int64_t t = d[j] - t0;
-            if (t >= 0 && t < nt) atomicAdd(&cnt[t], 1u);
+            const int64_t t = d[j];
+            if (t >= t0 && t < t1 && ((uint32_t)m[j >> 5] >> (j & 31) & 1)) atomicAdd(&at[t], 1u);
         }
     }
     if (p.n_bias) {
-        // a token named several times gets the sum, taken in order by the thread
-        // of its first entry
         const size_t g = r / (p.rows / p.bias_groups);
         const int64_t *ids = p.bias_ids + g * p.n_bias;
-        const float *val = p.bias + g * p.n_bias;
+        if (tid == 0) {
+            bias.ids = ids;
+            bias.val = p.bias + g * p.n_bias;
+            bias.n = p.n_bias;
+        }
         for (int i = tid; i < p.n_bias; i += kThreads) {
-            const int64_t id = ids[i];
-            if (id < t0 || id >= t0 + nt) continue;
-            bool first = true;
-            for (int j = 0; j < i && first; ++j) first = ids[j] != id;
-            if (!first) continue;
-            float s = val[i];
-            for (int j = i + 1; j < p.n_bias; ++j)
-                if (ids[j] == id) s = __fadd_rn(s, val[j]);
-            bias[id - t0] = s;
+            const int64_t t = ids[i];
+            if (t < t0 || t >= t1) continue;
+            atomicOr(&at[t], kBias);
+            const int j = atomicAdd(&bias.count, 1);
+            if (j < kBiasList) {
+                bias.at[j] = i;
+                bias.token[j] = (int)t;
+            }
         }
     }
-    __syncthreads();
+    if (marked) __syncthreads();
     const float rep = p.rep_rows ? p.rep_rows[r] : p.rep;
     const float pres = p.pres_rows ? p.pres_rows[r] : p.pres;
     const float freq = p.freq_rows ? p.freq_rows[r] : p.freq;
-    const float *x = p.x + (size_t)r * p.vocab + t0;
+    const uint32_t *allow =
+        p.allowed ? reinterpret_cast<const uint32_t *>(p.allowed) + r * p.allowed_stride : nullptr;
     uint64_t best = 0;
-    for (int i = tid; i < nt; i += kThreads) {
-        float y = x[i];
-        if (counted && cnt[i]) {
-            const uint32_t c = cnt[i] & ~kSeen;
-            y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-            if (c) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, (float)c)), pres);
+    auto one = [&](float v, int t, uint32_t w, bool ok) {
+        if (w) {
+            if (w & ~kBias) v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+            const uint32_t n = w & kCount;
+            if (n) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)n)), pres);
+            if (w & kBias) v = add_biases(v, t, bias);
         }
-        if (p.n_bias) y = __fadd_rn(y, bias[i]);
-        const int t = t0 + i;
-        if (p.allowed && !((uint32_t)p.allowed[r * p.allowed_stride + (t >> 5)] >> (t & 31) & 1))
-            y = -INFINITY;
-        if (p.y) p.y[(size_t)r * p.vocab + t] = y;
-        const uint64_t it = best_item(y, t);
-        best = it > best ? it : best;
+        v = ok ? v : -INFINITY;
+        if (part) {
+            const uint64_t it = best_item(v, t);
+            best = it > best ? it : best;
+        }
+        return v;
+    };
+    auto scalar = [&](int t) {
+        const bool ok = !allow || (allow[t >> 5] >> (t & 31) & 1);
+        const float v = one(ok ? x[t] : 0.f, t, marked ? at[t] : 0u, ok);
+        if (y) y[t] = v;
+    };
+    if (VEC) {
+        const int nv = t1 > v0 ? (t1 - v0) / 4 : 0;   // whole vectors
+        constexpr int U = 4;
+        for (int v = tid; v < nv; v += U * kThreads) {
+            uint32_t ok[U];
+            float4 f[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = v + u * kThreads, t = v0 + 4 * i, sh = t & 31;
+                ok[u] = 0;
+                if (i < nv) {
+                    ok[u] = 15u;
+                    if (allow) {
+                        ok[u] = allow[t >> 5] >> sh;
+                        if (sh > 28) ok[u] |= allow[(t >> 5) + 1] << (32 - sh);
+                        ok[u] &= 15u;
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                f[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (ok[u])
+                    f[u] = *reinterpret_cast<const float4 *>(x + v0 + 4 * (v + u * kThreads));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = v + u * kThreads, t = v0 + 4 * i;
+                if (i >= nv || (!ok[u] && !y)) continue;
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (marked) w = *reinterpret_cast<const uint4 *>(word + 4 + 4 * i);
+                const float4 was = f[u];
+                float4 z;
+                z.x = one(was.x, t, w.x, ok[u] & 1);
+                z.y = one(was.y, t + 1, w.y, ok[u] & 2);
+                z.z = one(was.z, t + 2, w.z, ok[u] & 4);
+                z.w = one(was.w, t + 3, w.w, ok[u] & 8);
+                // in place, what stays is not written
+                if (y && !(y == x && ok[u] == 15u && (w.x | w.y | w.z | w.w) == 0))
+                    *reinterpret_cast<float4 *>(y + t) = z;
+            }
+        }
+        if (t0 + tid < min(v0, t1)) scalar(t0 + tid);
+        const int rest = v0 + 4 * nv;
+        if (rest + tid < t1) scalar(rest + tid);
+    } else {
+        for (int t = t0 + tid; t < t1; t += kThreads) scalar(t);
     }
     if (!part) return;
     best = max_over_wave(best);
@@ -145,6 +240,14 @@ __global__ __launch_bounds__(64) void k_best_token(const uint64_t *__restrict__ 
     if (threadIdx.x == 0) tokens[blockIdx.x] = best ? (int64_t)(uint32_t)~(uint32_t)best : -1;
 }
 
+// Tokens of one block: large enough that the lists are read few times, small
+// enough that the rows fill the GPU (four blocks a CU).
+int chunk_tokens(int rows, int vocab) {
+    int chunk = 2048;
+    while (chunk < 8192 && (int64_t)rows * ((vocab + 2 * chunk - 1) / (2 * chunk)) >= 512) chunk *= 2;
+    return chunk;
+}
+
 }  // namespace
 
 size_t logits_scratch(int rows, int vocab, bool tokens) {
@@ -156,8 +259,13 @@ size_t logits_scratch(int rows, int vocab, bool tokens) {
 int launch_logits(const LogitsParams &p, void *scratch, hipStream_t s) {
     const int chunk = chunk_tokens(p.rows, p.vocab), chunks = (p.vocab + chunk - 1) / chunk;
     uint64_t *part = p.tokens ? static_cast<uint64_t *>(scratch) : nullptr;
-    const size_t lds = ((p.hist || p.nodes ? 1 : 0) + (p.n_bias ? 1 : 0)) * (size_t)chunk * 4;
-    hipLaunchKernelGGL(k_logits, dim3(chunks, p.rows), dim3(kThreads), lds, s, p, chunk, part);
+    const size_t lds = p.hist || p.nodes || p.n_bias ? (size_t)(chunk + 4) * 4 : 0;
+    // Rows of x and y are equally far from a 16-byte boundary, or go word by word.
+    const bool vec = !p.y || (reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.y)) % 16 == 0;
+    if (vec)
+        hipLaunchKernelGGL(k_logits<true>, dim3(chunks, p.rows), dim3(kThreads), lds, s, p, chunk, part);
+    else
+        hipLaunchKernelGGL(k_logits<false>, dim3(chunks, p.rows), dim3(kThreads), lds, s, p, chunk, part);
     TB_LAUNCHED();
     if (part) {
         hipLaunchKernelGGL(k_best_token, dim3(p.rows), dim3(64), 0, s, part, chunks, p.tokens);

@@ -1061,7 +1061,12 @@ Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len) {
     p.rb = p.few ? (R <= 16 ? 1 : 2) : R <= 64 || p.dp == 256 ? 1 : 2;
     p.tk = p.few ? 32 : tile_of(p.dp);
     p.rtiles = p.few ? 1 : (R + 64 * p.rb - 1) / (64 * p.rb);
-    const int64_t want = (p.few ? 256 : 512) / ((int64_t)p.rtiles * hkv * batch);
+    // As many blocks as run at once: two per CU, or one where registers or LDS allow one
+    // (few rows, head_dim past 128).  us at half as many / this / half as many again, 8
+    // heads of 128: 4096 + 49 nodes 41.7 / 43.4 / 51.5, 32767 + 64 198 / 178 / 201, 8
+    // sequences of up to 6000 + 16 100 / 73 / 78; head_dim 256, 8192 + 16: - / 37.1 / 43.9.
+    const int64_t want =
+        (p.few || p.dp == 256 ? 256 : 512) / ((int64_t)p.rtiles * hkv * batch);
     p.cap = (int)std::max<int64_t>(1, std::min<int64_t>(want, kMaxSplits));
     const int tiles = (max_len + p.tk - 1) / p.tk;
     p.nsplit = std::max(1, std::min(p.cap, (tiles + kMinTiles - 1) / kMinTiles));
