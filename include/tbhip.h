@@ -584,6 +584,40 @@ TB_API int tb_speculative_accept_rows(const float *target_rows, const int64_t *d
 /* The f64 uniform in [0, 1) (53 bits) of draw `counter` under `seed`. */
 TB_API double tb_spec_uniform(uint64_t seed, uint64_t counter);
 
+/* A drafted tree verified as one batched forward, as tb_decoder_verify runs a chain
+ * (no reference counterpart: the reference verifies chains only).  parents as for
+ * tb_tree_masks, every node real and node 0 a root; node 0 is usually the last
+ * token chosen, whose K / V row is not in the cache yet.  Node i has position
+ * start_offset + its depth and sees the positions below start_offset and its own
+ * ancestors.  logits_out (host [n, vocab]) receives every node's logits; cache rows
+ * start_offset + i hold the nodes until tb_decoder_accept_tree keeps a path of
+ * them.  TB_ERR_VALUE for a bad tree, a token outside the vocabulary or positions
+ * past max_seq_len; TB_ERR_UNSUPPORTED past the attention cap and with W4A8
+ * semantics; TB_ERR_MEMORY where the device has no room for the nodes in one batch. */
+TB_API int tb_decoder_verify_tree(tb_decoder *d, int64_t start_offset, const int64_t *tokens,
+                                  const int32_t *parents, int64_t n, float *logits_out);
+
+/* The path of that tree along next_tokens (host [n], the token chosen at each node),
+ * as tb_tree_accept walks it: its rows move to start_offset .. in every layer's cache
+ * and kv_len becomes start_offset + *n_path_out.  path_out host [n] (-1 behind the
+ * path), *token_out the next token of its last node. */
+TB_API int tb_decoder_accept_tree(tb_decoder *d, int64_t start_offset, const int64_t *tokens,
+                                  const int32_t *parents, const int64_t *next_tokens, int64_t n,
+                                  int32_t *path_out, int64_t *n_path_out, int64_t *token_out);
+
+/* Both with greedy next tokens, without reading the logits back: the forward, each
+ * node's best token after the penalties over `history` (host [n_history], the first
+ * prompt_len tokens prompt) and the node's own path, and the grammar mask `allowed`
+ * (host i32 [n, ceil(vocab / 32)] or NULL; tb_process_logits), then the acceptance.
+ * tb_decoder_get_logits then gives the row of the path's last node (after
+ * tb_decoder_verify_tree: of the tree's last one). */
+TB_API int tb_decoder_tree_step(tb_decoder *d, int64_t start_offset, const int64_t *tokens,
+                                const int32_t *parents, int64_t n, const int64_t *history,
+                                int64_t n_history, int64_t prompt_len, float repetition_penalty,
+                                float presence_penalty, float frequency_penalty,
+                                const int32_t *allowed, int32_t *path_out, int64_t *n_path_out,
+                                int64_t *token_out);
+
 /* prefill_tokens (decoder.rs:431-447): TB_ERR_VALUE when start_offset + n >
  * max_seq_len. */
 TB_API int tb_decoder_prefill(tb_decoder *d, const int64_t *tokens, int64_t n,

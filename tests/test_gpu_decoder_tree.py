@@ -1,0 +1,195 @@
+"""verify_tree, accept_tree and tree_step of the GPU decoder against the oracle's
+step-by-step decoder: every node's logits equal the oracle's after stepping the
+node's own path behind the prefix (within 2e-4, as verify_tokens is held), and the
+cache that acceptance leaves drives the following steps like the oracle's."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import oracle as O
+from torchburn_amd import synth
+from torchburn_amd.decoder import decoder_from_weights
+import torchburn_amd as tb
+
+pytestmark = pytest.mark.gpu
+
+V = 1000
+
+
+def rel(a, b):
+    a, b = np.asarray(a, np.float64), np.asarray(b, np.float64)
+    return float(np.abs(a - b).max() / max(np.abs(b).max(), 1e-30))
+
+
+def make(wk, lk, max_seq=160, seed=71, **kw):
+    cfg = dict(num_layers=2, hidden=256, intermediate=512, num_heads=4, num_kv_heads=2,
+               head_dim=64, vocab=V, eps=1e-6, rope_theta=1e6, qkv_bias=True)
+    cfg.update(kw)
+    w = synth.decoder_weights(cfg, seed, wk, lk, 32)
+    ocfg = dict(num_layers=cfg["num_layers"], hidden=cfg["hidden"],
+                intermediate=cfg["intermediate"], num_heads=cfg["num_heads"],
+                num_kv_heads=cfg["num_kv_heads"], head_dim=cfg["head_dim"], vocab=V,
+                group_size=32, max_seq=max_seq, rope_theta=cfg["rope_theta"], eps=cfg["eps"],
+                wkind=wk, lmkind=lk)
+    return O.Decoder(w, ocfg), decoder_from_weights(w, cfg, group_size=32, max_seq_len=max_seq), cfg
+
+
+def prefix(ref, dec, g, n):
+    toks = [int(t) for t in g.integers(0, V, n)]
+    for i, t in enumerate(toks):
+        lo = ref.step(t, i)
+    dec.prefill_tokens(toks, 0)
+    return toks, lo
+
+
+def branch(par, i):
+    p = []
+    while i >= 0:
+        p.append(i)
+        i = par[i]
+    return p[::-1]
+
+
+@pytest.mark.parametrize("wk,lk,n,kw", [
+    (4, 4, 1, {}), (4, 4, 7, {}), (4, 32, 12, {}), (8, 8, 9, {}), (4, 4, 40, {}),
+    (4, 4, 21, dict(num_heads=8, num_kv_heads=2, head_dim=128, hidden=1024, qkv_bias=False))])
+def test_verify_tree(cuda, wk, lk, n, kw):
+    print(f"case verify_tree wk={wk} lk={lk} n={n} {kw}", flush=True)
+    ref, dec, _ = make(wk, lk, **kw)
+    g = np.random.default_rng(n + wk)
+    prefix(ref, dec, g, 30)
+    par = [-1] + [int(g.integers(0, i)) for i in range(1, n)]
+    toks = [int(t) for t in g.integers(0, V, n)]
+    rows = dec.verify_tree(30, toks, par).numpy()
+    assert rows.shape == (n, V) and dec.kv_len() == 30 + n
+    worst = 0.0
+    for i in range(n):
+        for depth, j in enumerate(branch(par, i)):
+            lo = ref.step(toks[j], 30 + depth)
+        worst = max(worst, rel(rows[i], lo))
+    print(f"verify_tree rel err {worst:.3g}", flush=True)
+    assert worst < 2e-4
+    # any accepted path continues as the oracle's steps along it
+    want = branch(par, n - 1)
+    nxt = [V - 1] * n
+    for a, b in zip(want, want[1:]):
+        nxt[a] = toks[b]
+    lowest = [0]      # siblings with the same token: the walk takes the lowest
+    while True:
+        kids = [j for j in range(lowest[-1] + 1, n)
+                if par[j] == lowest[-1] and toks[j] == nxt[lowest[-1]]]
+        if not kids:
+            break
+        lowest.append(kids[0])
+    path, tok = dec.accept_tree(30, toks, par, nxt)
+    assert path == lowest and tok == nxt[lowest[-1]] and dec.kv_len() == 30 + len(path)
+    for depth, j in enumerate(path):
+        ref.step(toks[j], 30 + depth)
+    pos = 30 + len(path)
+    for t in (tok, 5, 17):
+        lg, am = dec._step(t, pos, True)
+        lo = ref.step(t, pos)
+        assert rel(lg, lo) < 2e-4 and am == O.argmax(lo)
+        pos += 1
+    ref.close()
+    dec.close()
+
+
+def best(lo, hist, path, rep, pres, freq, allowed):
+    y = lo.astype(np.float64).copy()
+    for t in set(hist) | set(path):
+        y[t] = y[t] / rep if y[t] > 0 else y[t] * rep
+    c = np.bincount(np.array(list(hist) + list(path), dtype=np.int64), minlength=V)
+    y -= freq * c + pres * (c > 0)
+    if allowed is not None:
+        y[~allowed] = -np.inf
+    return int(np.argmax(y))
+
+
+@pytest.mark.parametrize("wk,rep,freq,mask", [(4, 1.0, 0.0, False), (4, 1.25, 0.0, False),
+                                             (8, 1.25, 0.0, True), (4, 1.0, 0.001, True)])
+def test_tree_steps_generate_the_oracles_tokens(cuda, wk, rep, freq, mask):
+    """Greedy speculative decoding with trees: whatever is drafted, the tokens are those of
+    greedy decoding token by token with the same penalties.  Drafts: the right token on a
+    random one of a node's children, wrong ones elsewhere."""
+    print(f"case tree_step generation wk={wk} rep={rep} freq={freq} mask={mask}", flush=True)
+    ref, dec, _ = make(wk, 4, seed=80 + wk)
+    g = np.random.default_rng(7)
+    hist, lo = prefix(ref, dec, g, 12)
+    allowed = g.random(V) < 0.5 if mask else None
+    words = None
+    if mask:
+        bits = np.zeros(((V + 31) // 32) * 32, bool)
+        bits[:V] = allowed
+        words = np.packbits(bits.reshape(-1, 32), axis=-1, bitorder="little").view(np.uint32) \
+            .reshape(-1).astype(np.int32, casting="unsafe")
+    # the oracle's tokens
+    want, h = [], list(hist)
+    for i in range(24):
+        t = best(lo, h, [], rep, 0.0, freq, allowed)
+        want.append(t)
+        h.append(t)
+        lo = ref.step(t, 12 + i)
+    got, pos, tok, counts = [want[0]], 12, want[0], []
+    while len(got) < 20:
+        par, toks = [-1], [tok]
+        at = 0
+        for depth in range(int(g.integers(0, 4))):      # a right chain among wrong siblings
+            kids = [int(t) for t in g.integers(0, V, 3)]
+            kids[int(g.integers(0, 3))] = want[len(got) + depth]
+            nxt = len(par) + kids.index(want[len(got) + depth])
+            par += [at] * 3
+            toks += kids
+            at = nxt
+        kw = dict(history=hist + got[:-1], repetition_penalty=rep, frequency_penalty=freq)
+        if mask:
+            kw["allowed"] = np.tile(words, (len(par), 1))
+        path, tok = dec.tree_step(pos, toks, par, **kw)
+        counts.append(len(path))
+        got += [toks[i] for i in path[1:]] + [tok]
+        pos += len(path)
+        assert dec.kv_len() == pos
+        at = dec.get_logits()      # the row that tok came from
+        assert best(np.array(at, np.float32), hist + got[:-1], [], rep, 0.0, freq, allowed) == tok
+    print(f"tokens kept a step: {counts}", flush=True)
+    assert got[:20] == want[:20] and max(counts) > 1
+    ref.close()
+    dec.close()
+
+
+def test_tree_refusals(cuda):
+    print("case tree refusals", flush=True)
+    ref, dec, _ = make(4, 4, max_seq=20)
+    for toks, par in (([1, 2], [-1, 1]), ([1, 2], [0, 0]), ([1, 2], [-1, -2]), ([1, V], [-1, 0]),
+                      ([1, -1], [-1, 0]), ([], []), ([1, 2], [-1])):
+        with pytest.raises(ValueError):
+            dec.verify_tree(0, toks, par)
+        with pytest.raises(ValueError):
+            dec.accept_tree(0, toks, par, [0] * len(toks))
+        with pytest.raises(ValueError):
+            dec.tree_step(0, toks, par)
+    for start in (-1, 19, 20):
+        with pytest.raises(ValueError):
+            dec.verify_tree(start, [1, 2], [-1, 0])
+    with pytest.raises(ValueError):
+        dec.accept_tree(0, [1, 2], [-1, 0], [0])
+    with pytest.raises(ValueError):
+        dec.tree_step(0, [1], [-1], repetition_penalty=0.0)
+    with pytest.raises(tb.UnsupportedOpError):
+        dec.tree_step(0, [1], [-1], allowed=np.zeros(5, np.int32))
+    with pytest.raises(tb.UnsupportedOpError):
+        dec.tree_step(0, [1], [-1], allowed=np.zeros((V + 31) // 32, np.int64))
+    dec.set_attention_cap(10)
+    with pytest.raises(tb.UnsupportedOpError, match="cap"):
+        dec.verify_tree(9, [1, 2], [-1, 0])
+    dec.set_attention_cap(0)
+    assert dec.verify_tree(18, [1, 2], [-1, 0]).shape == (2, V)
+    # two roots: node 1 starts a second sequence behind the same prefix
+    rows = dec.verify_tree(0, [3, 4], [-1, -1]).numpy()
+    for i, t in enumerate((3, 4)):
+        assert rel(rows[i], ref.step(t, 0)) < 2e-4
+    # nothing allowed: no token
+    none = np.zeros((2, (V + 31) // 32), np.int32)
+    assert dec.tree_step(0, [3, 4], [-1, 0], allowed=none) == ([0], -1)
+    ref.close()
+    dec.close()

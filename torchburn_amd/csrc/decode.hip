@@ -732,17 +732,20 @@ __global__ __launch_bounds__(256) void k_rmsnorm_rows(const float *__restrict__ 
 // RoPE of the q and k heads of row m (position start + m) and the KV-cache
 // append, as the decode epilogue does it (decoder.rs:28-68, 1137-1146):
 // q1' = q1 c[i] - q2 s[i], q2' = q2 c[i + d/2] + q1 s[i + d/2], products
-// rounded separately.  Grid (M, hq + 2 hkv), hd / 2 threads.
+// rounded separately.  With `depth` (the nodes of a drafted tree) row m is rotated
+// for position start + depth[m] and still appended at start + m.
+// Grid (M, hq + 2 hkv), hd / 2 threads.
 __global__ void k_rope_rows(const float *__restrict__ qkv, int nq, float *__restrict__ q,
                             float *__restrict__ kc, float *__restrict__ vc,
                             const float *__restrict__ cos_t, const float *__restrict__ sin_t,
-                            int start, int hq, int hkv, int hd, int max_seq) {
+                            int start, const int32_t *__restrict__ depth, int hq, int hkv, int hd,
+                            int max_seq) {
     const int m = blockIdx.x, head = blockIdx.y, i = threadIdx.x, half = hd >> 1;
-    const int pos = start + m;
+    const int pos = start + m, turn = depth ? start + depth[m] : pos;
     const float *src = qkv + (size_t)m * nq + (size_t)head * hd;
     const float x1 = src[i], x2 = src[i + half];
     if (head < hq + hkv) {
-        const float *cr = cos_t + (size_t)pos * hd, *sr = sin_t + (size_t)pos * hd;
+        const float *cr = cos_t + (size_t)turn * hd, *sr = sin_t + (size_t)turn * hd;
         const float y1 = __fsub_rn(__fmul_rn(x1, cr[i]), __fmul_rn(x2, sr[i]));
         const float y2 = __fadd_rn(__fmul_rn(x2, cr[i + half]), __fmul_rn(x1, sr[i + half]));
         float *dst = head < hq ? q + ((size_t)m * hq + head) * hd
@@ -1291,11 +1294,11 @@ int launch_rmsnorm_rows(const float *X, const float *w, float *Xn, int M, int H,
 }
 
 int launch_rope_rows(const float *qkv, float *q, float *kc, float *vc, const float *cos_t,
-                     const float *sin_t, int start, int M, int hq, int hkv, int hd, int max_seq,
-                     hipStream_t s) {
+                     const float *sin_t, int start, const int32_t *depth, int M, int hq, int hkv,
+                     int hd, int max_seq, hipStream_t s) {
     const int nq = (hq + 2 * hkv) * hd;
     hipLaunchKernelGGL(k_rope_rows, dim3(M, hq + 2 * hkv), dim3(hd / 2), 0, s, qkv, nq, q, kc, vc,
-                       cos_t, sin_t, start, hq, hkv, hd, max_seq);
+                       cos_t, sin_t, start, depth, hq, hkv, hd, max_seq);
     TB_LAUNCHED();
     return TB_OK;
 }

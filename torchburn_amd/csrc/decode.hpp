@@ -46,9 +46,10 @@ int launch_embed_rows(const int *tok, const float *embed, float *X, int M, int H
 int launch_rmsnorm_rows(const float *X, const float *w, float *Xn, int M, int H, float eps,
                         hipStream_t s);
 // qkv [M][(hq + 2 hkv) hd] -> q [M][hq][hd] rotated; k (rotated) and v into the caches.
+// depth (device [M], or null): row m is rotated for position start + depth[m].
 int launch_rope_rows(const float *qkv, float *q, float *kc, float *vc, const float *cos_t,
-                     const float *sin_t, int start, int M, int hq, int hkv, int hd, int max_seq,
-                     hipStream_t s);
+                     const float *sin_t, int start, const int32_t *depth, int M, int hq, int hkv,
+                     int hd, int max_seq, hipStream_t s);
 // Causal attention of the M rows of q over cache positions 0 .. start + m; out [M][hq hd].
 // With scratch (prefill_attention_scratch bytes) the key range is split over
 // blocks when few query tiles meet a long cache; without, one block per tile

@@ -34,6 +34,8 @@
 #include "w4_limb.hpp"
 #include "v2_layout.hpp"
 #include "sample.hpp"
+#include "logits.hpp"
+#include "tree.hpp"
 
 struct tb_decoder;
 
@@ -130,6 +132,8 @@ struct Decoder {
         if (pf_slab) (void)hipFree(pf_slab);
         if (pf_attn) (void)hipFree(pf_attn);
         if (pf_rows) (void)hipFree(pf_rows);
+        if (pf_tree) (void)hipFree(pf_tree);
+        if (pf_tattn) (void)hipFree(pf_tattn);
         if (hstate) (void)hipHostFree(hstate);
         if (host_logits) (void)hipHostFree(host_logits);
         if (ev0) (void)hipEventDestroy(ev0);
@@ -873,12 +877,143 @@ struct Decoder {
         return TB_OK;
     }
 
+    // ---- Drafted trees --------------------------------------------------------
+    // The device side of one: parents, ancestor masks, depths, drafted tokens, next
+    // tokens, path, path length and token, and the logits' lists, one allocation.
+    struct Tree {
+        int n = 0;
+        int32_t *parents = nullptr, *mask = nullptr, *depth = nullptr, *path = nullptr,
+                *n_path = nullptr, *allowed = nullptr;
+        int64_t *draft = nullptr, *next = nullptr, *token = nullptr, *history = nullptr;
+        void *scratch = nullptr;
+    };
+    char *pf_tree = nullptr;
+    size_t pf_tree_bytes = 0;
+    float *pf_tattn = nullptr;   // the tree attention's split partials
+    size_t pf_tattn_bytes = 0;
+
+    // Whether trees of n nodes from start can be run forward.
+    int tree_runs(int64_t start, int64_t n) const {
+        TB_REQUIRE(under_cap(start, n), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: a tree's positions must lie below the attention cap");
+        TB_REQUIRE(!a8_wanted(), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: trees are not verified with W4A8 semantics");
+        TB_REQUIRE(!(wbits == 8 && wide_layers()), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: trees on INT8 layers wider than " + std::to_string(kMaxGemvK));
+        return TB_OK;
+    }
+
+    // Checks a tree (every node real, node 0 a root, its tokens in the vocabulary, its
+    // positions in the cache) and copies it to the device; n_hist and allow_words: room
+    // for the logits' lists.
+    int tree_upload(Tree &t, int64_t start, const int64_t *tokens, const int32_t *parents,
+                    int64_t n, int64_t n_hist = 0, int64_t allow_words = 0) {
+        TB_REQUIRE(n >= 1 && n <= kMaxTreeNodes, TB_ERR_VALUE,
+                   "tree of " + std::to_string(n) + " nodes outside 1.." +
+                       std::to_string(kMaxTreeNodes));
+        TB_REQUIRE(start >= 0 && start + n <= max_seq, TB_ERR_VALUE, "tree exceeds max_seq_len");
+        for (int64_t i = 0; i < n; ++i) {
+            TB_REQUIRE(parents[i] >= -1 && parents[i] < i && (i || parents[i] == -1), TB_ERR_VALUE,
+                       "tree node " + std::to_string(i) + ": parent " + std::to_string(parents[i]) +
+                           " is neither -1 nor an earlier node");
+            TB_REQUIRE(tokens[i] >= 0 && tokens[i] < V, TB_ERR_VALUE,
+                       "tree node " + std::to_string(i) + ": token outside the vocabulary");
+        }
+        const int64_t words = (n + 31) / 32;
+        const size_t scr = logits_scratch((int)n, V, true);
+        const size_t sizes[11] = {(size_t)n * 4,     (size_t)n * words * 4, (size_t)n * 4,
+                                  (size_t)n * 8,     (size_t)n * 8,         (size_t)n * 4,
+                                  8,                 8,                     (size_t)n_hist * 8,
+                                  (size_t)allow_words * 4, scr};
+        size_t total = 0;
+        for (size_t b : sizes) total += up256(b);
+        int rc = regrow(&pf_tree, &pf_tree_bytes, total);
+        if (rc) return rc;
+        char *p = pf_tree;
+        auto carve = [&](int i) {
+            char *q = p;
+            p += up256(sizes[i]);
+            return q;
+        };
+        t.n = (int)n;
+        t.parents = reinterpret_cast<int32_t *>(carve(0));
+        t.mask = reinterpret_cast<int32_t *>(carve(1));
+        t.depth = reinterpret_cast<int32_t *>(carve(2));
+        t.draft = reinterpret_cast<int64_t *>(carve(3));
+        t.next = reinterpret_cast<int64_t *>(carve(4));
+        t.path = reinterpret_cast<int32_t *>(carve(5));
+        t.n_path = reinterpret_cast<int32_t *>(carve(6));
+        t.token = reinterpret_cast<int64_t *>(carve(7));
+        t.history = reinterpret_cast<int64_t *>(carve(8));
+        t.allowed = reinterpret_cast<int32_t *>(carve(9));
+        t.scratch = carve(10);
+        TB_HIP(hipMemcpyAsync(t.parents, parents, (size_t)n * 4, hipMemcpyHostToDevice, st));
+        TB_HIP(hipMemcpyAsync(t.draft, tokens, (size_t)n * 8, hipMemcpyHostToDevice, st));
+        return TB_OK;
+    }
+
+    // Every node's logits into pf_rows by one batched forward, K / V rows start .. start +
+    // n - 1 holding the nodes in their order.
+    int tree_forward(Tree &t, const int64_t *tokens, int64_t start) {
+        int rc = launch_tree_masks(t.parents, t.mask, t.depth, 1, t.n, st);
+        if (!rc) rc = regrow(&pf_rows, &pf_rows_bytes, (size_t)t.n * V * 4);
+        if (!rc)
+            rc = regrow(&pf_tattn, &pf_tattn_bytes,
+                        tree_attention_scratch(1, t.n, hq, hkv, hd, (int)(start + t.n)));
+        return rc ? rc : prefill_batched(tokens, t.n, start, pf_rows, &t);
+    }
+
+    int tree_attention(const Tree &t, const float *kcl, const float *vcl, int start) {
+        const int64_t sh = (int64_t)max_seq * hd, sb = sh * hkv;
+        TreeAttn a{};
+        a.q = pf_q;
+        a.k = {kcl, sb, sh, hd};
+        a.v = {vcl, sb, sh, hd};
+        a.mask = t.mask;
+        a.kv_len = start;
+        a.out = pf_a;
+        a.batch = 1; a.n = t.n; a.hq = hq; a.hkv = hkv; a.hd = hd; a.max_seq = max_seq;
+        a.scale = 1.0f / sqrtf((float)hd);
+        return launch_tree_attention(a, start + t.n, pf_tattn, st);
+    }
+
+    // The accepted path given t.next: moved to the end of the prefix in every layer's
+    // cache, and reported.
+    int tree_keep(const Tree &t, int64_t start, int32_t *path, int64_t *n_path, int64_t *token) {
+        const int64_t sh = (int64_t)max_seq * hd, sb = sh * hkv;
+        std::vector<float *> k(L), v(L);
+        for (int l = 0; l < L; ++l) {
+            k[l] = kc + (size_t)l * hkv * max_seq * hd;
+            v[l] = vc + (size_t)l * hkv * max_seq * hd;
+        }
+        TreeAccept a{};
+        a.parents = t.parents; a.draft = t.draft; a.next = t.next;
+        a.kv_len = (int)start;
+        a.path = t.path; a.n_path = t.n_path; a.token = t.token;
+        a.batch = 1; a.n = t.n; a.hkv = hkv; a.hd = hd; a.max_seq = max_seq; a.layers = L;
+        a.k = {nullptr, sb, sh, hd};
+        a.v = {nullptr, sb, sh, hd};
+        int rc = launch_tree_accept(a, k.data(), v.data(), st);
+        if (rc) return rc;
+        int32_t n = 0;
+        TB_HIP(hipMemcpyAsync(path, t.path, (size_t)t.n * 4, hipMemcpyDeviceToHost, st));
+        TB_HIP(hipMemcpyAsync(&n, t.n_path, 4, hipMemcpyDeviceToHost, st));
+        TB_HIP(hipMemcpyAsync(token, t.token, 8, hipMemcpyDeviceToHost, st));
+        TB_HIP(hipStreamSynchronize(st));
+        *n_path = n;
+        kv_used = start + n;   // the rows past the path are no longer a sequence's
+        return TB_OK;
+    }
+
     // rows_out (device [n, V]): every position's logits, as verify_tokens
     // returns them (decoder.rs:565-581); otherwise only the last position's.
+    // tree: the n positions are its nodes, one chunk.
     int prefill_batched(const int64_t *tokens, int64_t n, int64_t start,
-                        float *rows_out = nullptr) {
+                        float *rows_out = nullptr, const Tree *tree = nullptr) {
         int rc = layers_set(), rows = 0;
         if (rc || (rc = prefill_alloc(n, start, &rows))) return rc;
+        TB_REQUIRE(!tree || rows >= n, TB_ERR_MEMORY,
+                   "Out of memory for a tree of " + std::to_string(n) + " nodes in one batch");
         pf_fixed = rows_out || n >= kFixedPrompt;
         const int nq = (hq + 2 * hkv) * hd;
         // Host copy of the whole prompt, alive until the closing synchronize.
@@ -896,10 +1031,12 @@ struct Decoder {
                 if ((rc = launch_rmsnorm_rows(pf_x, y.in_norm, pf_xn, M, H, eps, st)) ||
                     (rc = gemm(pf_xn, y.qkv_w, y.qkv_s, y.qkv_b, nullptr, nullptr, nullptr, pf_qkv,
                                M, nq, H, EPI_PLAIN)) ||
-                    (rc = launch_rope_rows(pf_qkv, pf_q, kcl, vcl, cos_t, sin_t, pos0, M, hq, hkv,
-                                           hd, max_seq, st)) ||
-                    (rc = launch_prefill_attention(pf_q, kcl, vcl, pf_a, pos0, M, hq, hkv, hd,
-                                                   max_seq, pf_attn, st)) ||
+                    (rc = launch_rope_rows(pf_qkv, pf_q, kcl, vcl, cos_t, sin_t, pos0,
+                                           tree ? tree->depth : nullptr, M, hq, hkv, hd, max_seq,
+                                           st)) ||
+                    (rc = tree ? tree_attention(*tree, kcl, vcl, pos0)
+                               : launch_prefill_attention(pf_q, kcl, vcl, pf_a, pos0, M, hq, hkv,
+                                                          hd, max_seq, pf_attn, st)) ||
                     (rc = gemm(pf_a, y.o_w, y.o_s, nullptr, nullptr, nullptr, pf_x, pf_x, M, H,
                                hq * hd, EPI_RESID)) ||
                     (rc = launch_rmsnorm_rows(pf_x, y.post_norm, pf_xn, M, H, eps, st)) ||
@@ -1538,6 +1675,71 @@ int tb_decoder_speculative_accept(tb_decoder *d, int64_t offset, const int64_t *
     for (auto &v : u) v = spec_uniform(d->seed, d->draws++);
     return spec_accept(rows.data(), draft_tokens, draft_probs, k, d->V, temperature, top_p,
                        u.data(), (int64_t)u.size(), accepted, bonus);
+}
+
+int tb_decoder_verify_tree(tb_decoder *d, int64_t start_offset, const int64_t *tokens,
+                           const int32_t *parents, int64_t n, float *logits_out) {
+    TB_REQUIRE(d && tokens && parents && logits_out, TB_ERR_VALUE, "null argument");
+    Decoder::Tree t;
+    int rc = d->tree_runs(start_offset, n);
+    if (rc || (rc = d->tree_upload(t, start_offset, tokens, parents, n)) ||
+        (rc = d->tree_forward(t, tokens, start_offset)))
+        return rc;
+    TB_HIP(hipMemcpy(logits_out, d->pf_rows, (size_t)n * d->V * 4, hipMemcpyDeviceToHost));
+    return TB_OK;
+}
+
+int tb_decoder_accept_tree(tb_decoder *d, int64_t start_offset, const int64_t *tokens,
+                           const int32_t *parents, const int64_t *next_tokens, int64_t n,
+                           int32_t *path_out, int64_t *n_path_out, int64_t *token_out) {
+    TB_REQUIRE(d && tokens && parents && next_tokens && path_out && n_path_out && token_out,
+               TB_ERR_VALUE, "null argument");
+    Decoder::Tree t;
+    int rc = d->tree_upload(t, start_offset, tokens, parents, n);
+    if (rc) return rc;
+    TB_HIP(hipMemcpyAsync(t.next, next_tokens, (size_t)n * 8, hipMemcpyHostToDevice, d->st));
+    return d->tree_keep(t, start_offset, path_out, n_path_out, token_out);
+}
+
+int tb_decoder_tree_step(tb_decoder *d, int64_t start_offset, const int64_t *tokens,
+                         const int32_t *parents, int64_t n, const int64_t *history,
+                         int64_t n_history, int64_t prompt_len, float repetition_penalty,
+                         float presence_penalty, float frequency_penalty, const int32_t *allowed,
+                         int32_t *path_out, int64_t *n_path_out, int64_t *token_out) {
+    TB_REQUIRE(d && tokens && parents && path_out && n_path_out && token_out &&
+                   (n_history == 0 || history),
+               TB_ERR_VALUE, "null argument");
+    TB_REQUIRE(n_history >= 0 && n_history <= (1 << 29) && repetition_penalty > 0.f, TB_ERR_VALUE,
+               "tree_step: bad history length or repetition penalty");
+    Decoder::Tree t;
+    const int64_t words = ((int64_t)d->V + 31) / 32;
+    int rc = d->tree_runs(start_offset, n);
+    if (rc || (rc = d->tree_upload(t, start_offset, tokens, parents, n, n_history,
+                                   allowed ? n * words : 0)))
+        return rc;
+    if (n_history)
+        TB_HIP(hipMemcpyAsync(t.history, history, (size_t)n_history * 8, hipMemcpyHostToDevice, d->st));
+    if (allowed)
+        TB_HIP(hipMemcpyAsync(t.allowed, allowed, (size_t)n * words * 4, hipMemcpyHostToDevice, d->st));
+    if ((rc = d->tree_forward(t, tokens, start_offset))) return rc;
+    LogitsParams p{};
+    p.x = d->pf_rows; p.tokens = t.next;
+    p.rows = (int)n; p.vocab = d->V;
+    p.history = t.history; p.groups = 1; p.hist = (int)n_history;
+    p.prompt = (int)std::min<int64_t>(std::max<int64_t>(prompt_len, 0), n_history);
+    p.rep = repetition_penalty; p.pres = presence_penalty; p.freq = frequency_penalty;
+    p.bias_groups = 1;
+    p.allowed = allowed ? t.allowed : nullptr; p.allowed_stride = words;
+    p.draft = t.draft; p.tree_mask = t.mask; p.nodes = (int)n;
+    if ((rc = launch_logits(p, t.scratch, d->st)) ||
+        (rc = d->tree_keep(t, start_offset, path_out, n_path_out, token_out)))
+        return rc;
+    // get_logits: the row that the next token came from
+    const float *row = d->pf_rows + (size_t)path_out[*n_path_out - 1] * d->V;
+    TB_HIP(hipMemcpyAsync(d->logits, row, (size_t)d->V * 4, hipMemcpyDeviceToDevice, d->st));
+    TB_HIP(hipMemcpyAsync(d->host_logits, row, (size_t)d->V * 4, hipMemcpyDeviceToHost, d->st));
+    TB_HIP(hipStreamSynchronize(d->st));
+    return TB_OK;
 }
 
 int tb_decoder_prefill(tb_decoder *d, const int64_t *tokens, int64_t n, int64_t start_offset,

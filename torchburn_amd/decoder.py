@@ -48,6 +48,10 @@ def _bind():
                                           C.POINTER(i64), C.POINTER(i64)],
         "tb_speculative_accept_rows": [p, p, p, i64, i64, C.c_float, C.c_float, p, i64,
                                        C.POINTER(i64), C.POINTER(i64)],
+        "tb_decoder_verify_tree": [p, i64, p, p, i64, p],
+        "tb_decoder_accept_tree": [p, i64, p, p, p, i64, p, C.POINTER(i64), C.POINTER(i64)],
+        "tb_decoder_tree_step": [p, i64, p, p, i64, p, i64, i64, C.c_float, C.c_float, C.c_float,
+                                 p, p, C.POINTER(i64), C.POINTER(i64)],
         "tb_decoder_reset_kv": [p],
         "tb_decoder_copy_kv": [p, i64, p, p, i64, i64],
         "tb_decoder_kv_len": [p, C.POINTER(i64)],
@@ -96,7 +100,8 @@ def decoder_symbols() -> list:
             "tb_decoder_get_logits", "tb_decoder_set_seed", "tb_decoder_time_greedy",
             "tb_decoder_destroy", "tb_decoder_generate_sampled", "tb_decoder_verify",
             "tb_decoder_speculative_accept", "tb_speculative_accept_rows", "tb_spec_uniform",
-            "tb_decoder_set_rope_tables", "tb_decoder_set_attention_cap"]
+            "tb_decoder_set_rope_tables", "tb_decoder_set_attention_cap",
+            "tb_decoder_verify_tree", "tb_decoder_accept_tree", "tb_decoder_tree_step"]
 
 
 _NP_TO_TORCH = {"float32": "float32", "uint8": "uint8", "int8": "int8", "int64": "int64"}
@@ -370,6 +375,72 @@ class RustQwenDecoder:
             probs.ctypes.data if probs.size else None, float(temperature), float(top_p),
             C.byref(a), C.byref(b)))
         return int(a.value), int(b.value)
+
+    # -- drafted trees (no reference counterpart: it verifies chains only) -----
+
+    def _tree(self, tokens: Sequence[int], parents: Sequence[int]):
+        t = np.asarray(list(tokens), dtype=np.int64)
+        par = np.asarray(list(parents), dtype=np.int32)
+        if t.size != par.size:
+            raise ValueError(f"{t.size} tree tokens against {par.size} parents")
+        return t, par
+
+    def verify_tree(self, start_offset: int, tokens: Sequence[int], parents: Sequence[int]):
+        """Logits [n, vocab] (a float32 torch tensor) of every node of a drafted tree, in one
+        batched forward.  ``parents[i]`` is -1 or an earlier node; node 0 is a root, usually
+        the last token chosen, whose K / V row is not in the cache yet.  Node i has position
+        start_offset + its depth and sees the positions below start_offset and its own
+        ancestors.  The cache holds the nodes in their order until accept_tree keeps a path."""
+        import torch
+        t, par = self._tree(tokens, parents)
+        out = np.empty((t.size, self.vocab_size), np.float32)
+        _lib.check(_bind().tb_decoder_verify_tree(self._h, int(start_offset), t.ctypes.data,
+                                                  par.ctypes.data, t.size, out.ctypes.data))
+        return torch.from_numpy(out)
+
+    def accept_tree(self, start_offset: int, tokens: Sequence[int], parents: Sequence[int],
+                    next_tokens: Sequence[int]) -> Tuple[List[int], int]:
+        """(path, token): the nodes from node 0 along ``next_tokens``, the token chosen at each
+        node (sampled from its row of verify_tree, say), and the next token of the last one.
+        The path's K / V rows are kept: the sequence goes on at start_offset + len(path)."""
+        t, par = self._tree(tokens, parents)
+        nx = np.asarray(list(next_tokens), dtype=np.int64)
+        if nx.size != t.size:
+            raise ValueError(f"{nx.size} next tokens against {t.size} tree tokens")
+        path = np.empty(max(t.size, 1), np.int32)
+        n, tok = C.c_int64(), C.c_int64()
+        _lib.check(_bind().tb_decoder_accept_tree(
+            self._h, int(start_offset), t.ctypes.data, par.ctypes.data, nx.ctypes.data, t.size,
+            path.ctypes.data, C.byref(n), C.byref(tok)))
+        return path[:n.value].tolist(), int(tok.value)
+
+    def tree_step(self, start_offset: int, tokens: Sequence[int], parents: Sequence[int],
+                  history: Optional[Sequence[int]] = None, prompt_len: int = 0,
+                  repetition_penalty: float = 1.0, presence_penalty: float = 0.0,
+                  frequency_penalty: float = 0.0, allowed=None) -> Tuple[List[int], int]:
+        """One greedy speculative step over a drafted tree: verify_tree, the best token of
+        every node, accept_tree, without reading the logits back.  The penalties cover
+        ``history`` (its first ``prompt_len`` tokens as prompt) and the node's own path;
+        ``allowed`` is None or int32 [n, ceil(vocab / 32)], the tokens a grammar allows after
+        each node (process_logits).  Returns (path, token) as accept_tree; token is -1 when
+        the mask leaves nothing."""
+        t, par = self._tree(tokens, parents)
+        h = np.asarray(list(history if history is not None else []), dtype=np.int64)
+        words = (self.vocab_size + 31) // 32
+        al = None
+        if allowed is not None:
+            al, keep, _ = _as_buffer(allowed, None, t.size * words, "allowed")
+            if str(keep.dtype).replace("torch.", "") != "int32" or getattr(keep, "is_cuda", False):
+                raise _lib.UnsupportedOpError(
+                    f"{_lib.UNSUPPORTED_MARKER} allowed must be int32 on the host")
+        path = np.empty(max(t.size, 1), np.int32)
+        n, tok = C.c_int64(), C.c_int64()
+        _lib.check(_bind().tb_decoder_tree_step(
+            self._h, int(start_offset), t.ctypes.data, par.ctypes.data, t.size,
+            h.ctypes.data if h.size else None, h.size, int(prompt_len),
+            float(repetition_penalty), float(presence_penalty), float(frequency_penalty), al,
+            path.ctypes.data, C.byref(n), C.byref(tok)))
+        return path[:n.value].tolist(), int(tok.value)
 
     # -- KV cache -------------------------------------------------------------
 
