@@ -407,8 +407,10 @@ TB_API int tb_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, 
  * contiguous; mask_sb words between the sequences' masks (0: one mask for all).
  * kv_lens: device i32 [batch], clamped to [0, max_seq] (nodes past the cache's
  * end do not exist), or NULL: kv_len for every sequence, and TB_ERR_VALUE when
- * kv_len + n > max_seq.  head_dim a multiple of 32 up to 256; q, out and the
- * caches 16-byte aligned.
+ * kv_len + n > max_seq.  The two may differ in their last bits on long caches:
+ * the work is split by the length that the call knows.  head_dim a multiple of 32
+ * up to 256, num_heads up to 1024, positions up to 2^27 elements apart; q, out
+ * and the caches 16-byte aligned.
  * scratch: tb_tree_attention_scratch bytes of device memory, 16-byte aligned
  * (max_len: kv_len + n, or max_seq with kv_lens); NULL: the stream's workspace
  * (TB_ERR_UNSUPPORTED while capturing, since graphs that are replayed side by
@@ -435,7 +437,8 @@ TB_API int tb_tree_attention(const float *q, const float *k_cache, const float *
  * In each of the `layers` caches (host arrays of device pointers; layers may be
  * 0) K / V row kv_len + path[j] moves to kv_len + j, so that the accepted rows
  * follow the prefix; rows past the path keep what they held, and rows past
- * max_seq do not exist.  Strides, kv_lens and kv_len as above.
+ * max_seq do not exist.  No cache may share memory with another.  Strides,
+ * kv_lens and kv_len as above.
  */
 TB_API int tb_tree_accept(const int32_t *parents, const int64_t *draft_tokens,
                           const int64_t *next_tokens, const int32_t *kv_lens, int64_t kv_len,

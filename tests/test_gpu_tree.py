@@ -141,6 +141,12 @@ CASES = [
     (1, 256, 8, 8, 64, [40], 300),
     (1, 130, 16, 2, 128, [2500], 2700),    # more rows than one tile, a long prefix
     (1, 2, 32, 8, 128, [9000], 9100),
+    (1, 50, 8, 2, 64, [1500], 1600),       # two and four row tiles
+    (1, 50, 16, 2, 64, [1500], 1600),
+    (1, 30, 8, 2, 128, [700], 800),
+    (1, 70, 16, 4, 128, [700], 800),
+    (2, 30, 8, 2, 256, [700, 90], 800),
+    (1, 17, 16, 2, 160, [300], 400),
 ]
 
 
@@ -159,6 +165,37 @@ def test_attention(cuda, B, N, H, KVH, D, lens, S):
         assert torch.equal(tb.tree_attention(*a, lens[0]), out[0])
         assert torch.equal(tb.tree_attention(*a, torch.tensor(lens, device=cuda)), out[0])
         assert torch.equal(tb.tree_attention(*a, lens[0], scale=D ** -0.5), out[0])
+
+
+@pytest.mark.parametrize("N,H,KVH,D,lens,S", [
+    (70, 16, 2, 64, [1000], 131072),       # two tiles of 256 rows, the last one ragged
+    (40, 16, 4, 64, [0, 2100, 63, 1, 9], 13120),
+    (19, 16, 2, 128, [700], 65600),        # 152 rows: some waves have none
+    (70, 8, 2, 96, [31, 129], 32800),
+])
+def test_attention_of_many_rows_over_a_large_cache(cuda, N, H, KVH, D, lens, S):
+    """Blocks of eight waves.  The first K and V rows of every other 4 positions are larger,
+    so that the parts of a tile have scales of their own; one node has infinities."""
+    B = len(lens)
+    print(f"case tree_attention large cache N={N} H={H}/{KVH} D={D} lens={lens} S={S}", flush=True)
+    q, k, v, bits = inputs(N + D, B, N, H, KVH, D, max(lens) + N, [N - 3] * B)
+    at = np.arange(k.shape[2])
+    k[:, :, at % 8 < 4] *= 1.5
+    v[:, :, at % 8 >= 4] *= 300.0
+    want, bound = reference(q, k, v, bits, lens, D ** -0.5)
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    kc, vc = (torch.full((B, KVH, S, D), float("nan"), device=cuda) for _ in range(2))
+    kc[:, :, :k.shape[2]], vc[:, :, :k.shape[2]] = T(k), T(v)
+    a = (T(q), kc, vc, T(words(bits)), torch.tensor(lens, device=cuda))
+    check(tb.tree_attention(*a), want, bound)
+    node = 2
+    for b, ln in enumerate(lens):
+        kc[b, :, ln + node] = float("inf")
+        vc[b, :, ln + node] = float("nan")
+    got = tb.tree_attention(*a).cpu().numpy()
+    on = bits[:, :, node]
+    assert np.isnan(got[on]).all() and np.isfinite(got[~on]).all()
+    assert (np.abs(got - want)[~on] <= bound[~on]).all()
 
 
 @pytest.mark.parametrize("D,N,kv", [(64, 6, 40), (128, 70, 300), (96, 33, 1000)])
@@ -190,6 +227,55 @@ def test_attention_unseen_positions(cuda, D, N, kv):
             assert np.isnan(on).all(-1).all()
         elif np.isinf(y):
             assert not np.isfinite(on).any()
+
+
+@pytest.mark.parametrize("D,N,kv,S", [(64, 6, 40, 46), (128, 7, 0, 7), (128, 25, 90, 115),
+                                      (96, 60, 200, 260), (256, 33, 65, 98), (64, 80, 30, 131072)])
+@pytest.mark.parametrize("big", [1e6, 3e38])
+def test_attention_large_values_beside_the_path(cuda, D, N, kv, S, big):
+    """Nodes whose K and V are very large cost the rows that do not see them no bits, and the
+    rows that see one get its V."""
+    print(f"case tree_attention large nodes D={D} N={N} kv={kv} big={big}", flush=True)
+    H, KVH = 8, 2
+    q, k, v, bits = inputs(D + N, 1, N, H, KVH, D, kv + N, [N - 1])
+    nodes = [2, N - 1] if N < 10 else [2, 5, N // 2, N - 1]   # the last one is padding
+    small = v.copy()
+    for j in nodes:
+        k[:, :, kv + j] = np.clip(k[:, :, kv + j], -1, 1) * np.float32(big)
+        v[:, :, kv + j] = np.clip(v[:, :, kv + j], -1, 1) * np.float32(big)
+    v[:, :, kv + N // 3] = 0.0       # scales of their own in both directions
+    v[:, :, kv + N // 4] *= 1e-30
+    want, bound = reference(q, k, v, bits, [kv], D ** -0.5)
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    kc, vc = (torch.zeros((1, KVH, S, D), device=cuda) for _ in range(2))
+    kc[:, :, :kv + N], vc[:, :, :kv + N] = T(k), T(v)
+    ln = torch.tensor([kv], device=cuda)
+    got = tb.tree_attention(T(q), kc, vc, T(words(bits)), ln).cpu().numpy()
+    on = bits[0][:, nodes].any(-1)
+    assert on.any() and not on.all()
+    assert (np.abs(got - want)[0, ~on] <= bound[0, ~on]).all()
+    # only V: the scores of the rows that see it are ordinary
+    k[:, :, [kv + j for j in nodes]] = small[:, :, [kv + j for j in nodes]]
+    kc[:, :, :kv + N] = T(k)
+    want, bound = reference(q, k, v, bits, [kv], D ** -0.5)
+    got = tb.tree_attention(T(q), kc, vc, T(words(bits)), ln)
+    # 2^-32 of the largest V seen, for every position
+    top = np.where(on, np.float64(big), 0.0)[None, :, None, None] * (kv + N) * 2.0 ** -32
+    check(got, want, bound + top)
+
+
+def test_attention_weights_of_zero_values(cuda):
+    """Positions whose V is zero count in the sum, however large other positions' V is."""
+    print("case tree_attention zero values", flush=True)
+    for N, H, D in ((2, 4, 128), (40, 8, 64), (60, 16, 128)):
+        KVH, kv, S = 2, 4000, 4100
+        q, k, v, bits = inputs(31, 1, N, H, KVH, D, S)
+        v[:, :, :kv] = 0.0
+        v[:, :, 3900:3904] = 1e7
+        want, bound = reference(q, k, v, bits, [kv], D ** -0.5)
+        T = lambda a: torch.from_numpy(a).to(cuda)
+        got = tb.tree_attention(T(q), T(k), T(v), T(words(bits)), kv)
+        check(got, want, bound + 1e7 * 2.0 ** -32 * (kv + N))
 
 
 @pytest.mark.parametrize("kscale,vscale", [(1e-20, 1e-30), (1e18, 1e30), (1e-38, 1e-38), (30.0, 1.0)])
@@ -275,6 +361,20 @@ def test_attention_empty(cuda):
     assert out.shape == (0, 3, 4, 64)
     out = tb.tree_attention(z(3, 4, 64) + 1, z(2, 8, 64) + 1, z(2, 8, 64) + 1, m(3, 1), 3)
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("N,kv", [(4, 40), (4, 3000), (20, 3000), (60, 3000), (90, 1000)])
+def test_attention_not_finite_queries(cuda, N, kv):
+    """A NaN in a query makes its row NaN and no other, with one block and with many."""
+    print(f"case tree_attention NaN query N={N} kv={kv}", flush=True)
+    H, KVH, D, S = 8, 2, 64, kv + N
+    q, k, v, bits = inputs(N, 1, N, H, KVH, D, S)
+    q[0, N // 2, 3, 5] = np.nan
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    out = tb.tree_attention(T(q), T(k), T(v), T(words(bits)), kv).cpu().numpy()
+    nan = np.zeros(out.shape, bool)
+    nan[0, N // 2, 3] = True
+    assert np.array_equal(np.isnan(out), nan)
 
 
 def test_attention_past_32_bits(cuda):
@@ -367,6 +467,10 @@ def test_accept_cache_end_and_host(cuda):
         assert torch.equal(c[:, :8], w[:, :8]) and torch.equal(c[:, 9], w[:, 9])
     with pytest.raises(ValueError, match="exceed"):
         tb.tree_accept(par, draft, nxt, 6, [k], [v])
+    # the layers' caches stacked in one tensor
+    ks, vs = torch.stack((k0, v0)).to(cuda), torch.stack((v0, k0)).to(cuda)
+    tb.tree_accept(par.to(cuda), draft.to(cuda), nxt.to(cuda), torch.tensor([7], device=cuda), ks, vs)
+    assert torch.equal(ks.cpu(), torch.stack((k, v))) and torch.equal(vs.cpu(), torch.stack((v, k)))
 
 
 # ---- streams, graphs -------------------------------------------------------------

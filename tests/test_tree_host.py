@@ -61,6 +61,11 @@ U, V = _lib.TB_ERR_UNSUPPORTED, _lib.TB_ERR_VALUE
     (attention, dict(kv_len=-1), V, b"exceed"), (attention, dict(max_seq=(1 << 30) + 1), U, b"max_seq"),
     (attention, dict(scratch=A, size=8, max_seq=4096, kv_len=2000), U, b"scratch"),
     (attention, dict(scratch=A + 8, size=1 << 40, max_seq=4096, kv_len=2000), U, b"scratch"),
+    (attention, dict(kv_len=2 ** 63 - 2), V, b"exceed"), (attention, dict(heads=1026), U, b"1024"),
+    (attention, dict(k_ss=(1 << 27) + 4), U, b"2^27"), (attention, dict(v_ss=1 << 40), U, b"2^27"),
+    (attention, dict(mask_sb=-4), U, b"mask"), (attention, dict(mask=A + 2), U, b"misaligned"),
+    (attention, dict(kv_lens=A + 1), U, b"misaligned"),
+    (accept, dict(kv_len=2 ** 63 - 2), V, b"exceed"),
     (accept, dict(parents=None), U, b"null"), (accept, dict(token=None), U, b"null"),
     (accept, dict(n=0), U, b"empty"), (accept, dict(n=1025), U, b"1024"),
     (accept, dict(kv_len=30), V, b"exceed"), (accept, dict(layers=-1), U, b"layers"),
@@ -78,6 +83,7 @@ U, V = _lib.TB_ERR_UNSUPPORTED, _lib.TB_ERR_VALUE
     (logits, dict(allowed=A, stride=3), U, b"mask rows"), (logits, dict(x=A + 2), U, b"misaligned"),
     (logits, dict(history=A + 4), U, b"misaligned"),
     (logits, dict(tokens=A, scratch=A, size=1), U, b"scratch"),
+    (logits, dict(out=A + 400), U, b"overlap"), (logits, dict(out=A - 1596), U, b"overlap"),
 ])
 def test_c_refusals(call, kw, code, msg):
     assert call(**kw) == code, kw

@@ -1235,7 +1235,7 @@ int tb_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, int64_t
 int64_t tb_tree_attention_scratch(int64_t batch, int64_t n, int64_t num_heads,
                                   int64_t num_kv_heads, int64_t head_dim, int64_t max_len) {
     if (batch <= 0 || batch > 65535 || n <= 0 || n > kMaxTreeNodes || num_kv_heads <= 0 ||
-        num_heads <= 0 || num_heads > 65535 || num_heads % num_kv_heads || head_dim <= 0 ||
+        num_heads <= 0 || num_heads > kMaxTreeHeads || num_heads % num_kv_heads || head_dim <= 0 ||
         head_dim > 256 || max_len < 0 || max_len > (1 << 30))
         return 0;
     return (int64_t)tree_attention_scratch((int)batch, (int)n, (int)num_heads, (int)num_kv_heads,
@@ -1252,10 +1252,15 @@ int tb_tree_attention(const float *q, const float *k_cache, const float *v_cache
     if (!rc) rc = check_cache("tree_attention", num_kv_heads, head_dim, max_seq, {k_sb, k_sh, k_ss},
                               {v_sb, v_sh, v_ss});
     if (rc) return rc;
-    TB_REQUIRE(num_heads > 0 && num_heads <= 65535 && num_heads % num_kv_heads == 0,
+    TB_REQUIRE(num_heads > 0 && num_heads <= kMaxTreeHeads && num_heads % num_kv_heads == 0,
                TB_ERR_UNSUPPORTED,
-               "TB_UNSUPPORTED: tree_attention: num_heads must be a multiple of num_kv_heads");
-    TB_REQUIRE(kv_lens || (kv_len >= 0 && kv_len + n <= max_seq), TB_ERR_VALUE,
+               "TB_UNSUPPORTED: tree_attention: num_heads must be a multiple of num_kv_heads, up to " +
+                   std::to_string(kMaxTreeHeads));
+    // a tile's offsets are 32 bits of 16-byte units
+    TB_REQUIRE(k_ss <= (1 << 27) && v_ss <= (1 << 27), TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: tree_attention: positions more than 2^27 elements apart");
+    TB_REQUIRE(mask_sb >= 0, TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: tree_attention: negative mask stride");
+    TB_REQUIRE(kv_lens || (kv_len >= 0 && kv_len <= max_seq - n), TB_ERR_VALUE,
                "tree_attention: " + std::to_string(n) + " nodes at position " +
                    std::to_string(kv_len) + " exceed the cache's " + std::to_string(max_seq));
     if (batch == 0 || n == 0) return TB_OK;
@@ -1264,6 +1269,8 @@ int tb_tree_attention(const float *q, const float *k_cache, const float *v_cache
     TB_REQUIRE(aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16),
                TB_ERR_UNSUPPORTED,
                "TB_UNSUPPORTED: tree_attention: q, out and the caches must be 16-byte aligned");
+    TB_REQUIRE(aligned(mask, 4) && aligned(kv_lens, 4), TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: tree_attention: misaligned device pointer");
     TreeAttn a{};
     a.q = q;
     a.k = {k_cache, k_sb, k_sh, k_ss};
@@ -1307,7 +1314,7 @@ int tb_tree_accept(const int32_t *parents, const int64_t *draft_tokens, const in
         if ((rc = check_cache("tree_accept", num_kv_heads, head_dim, max_seq, {k_sb, k_sh, k_ss},
                               {v_sb, v_sh, v_ss})))
             return rc;
-        TB_REQUIRE(kv_lens || (kv_len >= 0 && kv_len + n <= max_seq), TB_ERR_VALUE,
+        TB_REQUIRE(kv_lens || (kv_len >= 0 && kv_len <= max_seq - n), TB_ERR_VALUE,
                    "tree_accept: " + std::to_string(n) + " nodes at position " +
                        std::to_string(kv_len) + " exceed the cache's " + std::to_string(max_seq));
         TB_REQUIRE(k_caches && v_caches, TB_ERR_UNSUPPORTED,
@@ -1377,13 +1384,16 @@ int tb_process_logits(const float *logits, float *out, int64_t *tokens, int64_t 
                    aligned(draft_tokens, 8) && aligned(bias_ids, 8) && aligned(bias, 4) &&
                    aligned(allowed, 4) && aligned(tree_mask, 4),
                TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: process_logits: misaligned device pointer");
+    const int64_t apart = reinterpret_cast<intptr_t>(out) - reinterpret_cast<intptr_t>(logits);
+    TB_REQUIRE(!out || apart == 0 || std::abs(apart) >= rows * vocab * 4, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: process_logits: out and logits overlap without being the same");
     TB_REQUIRE(allowed_stride == 0 || allowed_stride >= (vocab + 31) / 32, TB_ERR_UNSUPPORTED,
                "TB_UNSUPPORTED: process_logits: mask rows shorter than the vocabulary");
     LogitsParams p{};
     p.x = logits; p.y = out; p.tokens = tokens;
     p.rows = (int)rows; p.vocab = (int)vocab;
     p.history = history; p.history_len = history_len; p.prompt_len = prompt_len;
-    p.groups = (int)groups; p.hist = (int)hist; p.prompt = (int)std::min<int64_t>(prompt, hist);
+    p.groups = (int)groups; p.hist = (int)hist; p.prompt = (int)std::clamp<int64_t>(prompt, 0, hist);
     p.rep = repetition_penalty; p.pres = presence_penalty; p.freq = frequency_penalty;
     p.rep_rows = repetition_rows; p.pres_rows = presence_rows; p.freq_rows = frequency_rows;
     p.bias_ids = bias_ids; p.bias = bias; p.bias_groups = (int)bias_groups; p.n_bias = (int)n_bias;

@@ -10,10 +10,14 @@
 // as two f16 limbs, x 2^s = hi + lo, and three products, hi hi + hi lo + lo hi:
 // 22 bits and more of each factor, so that an error against exact arithmetic
 // stays that of an f32 product, at a third of the f16 rate (the f32 MFMA has a
-// sixteenth of it).  s puts the largest factor of a tile (K, V) or row (Q) at
-// 2^14, so factors down to 2^-25 of it keep both limbs whole and smaller ones an
-// error of 2^-39 of it.  Weights are taken as w 2^7 for the same reason.  Scores,
-// running maxima, sums and outputs are f32.
+// sixteenth of it).  s puts the largest factor of a few positions (K, V) or a row
+// (Q) at 2^14, so factors down to 2^-17 of it keep both limbs whole and smaller ones
+// an error of 2^-39 of it.  Weights are taken as w 2^7 for the same reason, less
+// where the positions' V is smaller than others': an error of 2^-32 of the largest
+// V.  Behind the prefix, where rows see different positions, a tile whose K or V
+// spread wider than that is worked in f32 (as one with infinities is), so that
+// nothing that a row does not see costs it bits.  Scores, running maxima, sums and
+// outputs are f32.
 #include <math.h>
 
 #include <algorithm>
@@ -32,6 +36,10 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// For lambdas that are called more than once, which would become functions with their
+// captures in memory.
+#define TB_INLINE __attribute__((always_inline))
+
 constexpr int kMaxSplits = 128;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kTop = 14;         // factors are scaled to below 2^(kTop + 1)
@@ -42,10 +50,13 @@ constexpr int kTop = 14;         // factors are scaled to below 2^(kTop + 1)
 constexpr float kLag = 8.f;
 constexpr int kWeight = 7;
 
+constexpr int kNoV = -1000;          // in place of an exponent: none yet
+constexpr int kLeast = kTop - 127;   // the smallest exponent()
+
 // Exponent of the largest magnitude given its bits, such that 2^(kTop - e) is a
 // normal f32 (values below 2^-113 keep an error below the smallest f32).
 __device__ __forceinline__ int exponent(uint32_t bits) {
-    return min(max((int)(bits >> 23) - 127, kTop - 127), 127);
+    return min(max((int)(bits >> 23) - 127, kLeast), 127);
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
@@ -97,6 +108,23 @@ __device__ __forceinline__ void max3_abs(float &m, float a, float b) {
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 constexpr uint32_t kInf = 0x7F800000u;
+template <int N>
+__device__ __forceinline__ uint32_t top_bits(const float (&x)[N]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) top = max(top, abs_bits(x[j]));
+    return top;
+}
+// low takes the bits of the smallest magnitude but 0, turned over.
+__device__ __forceinline__ void low_bits(uint32_t &low, uint32_t bits) {
+    low = max(low, bits ? ~bits : 0u);
+}
+// Whether the smallest of some positions' magnitudes is so far below 2^top that limbs in
+// one scale would not keep it whole (they do down to 2^-17), with a margin: 6 bits of
+// the outputs' scale, and that the smallest is one over a few dimensions.
+__device__ __forceinline__ bool spread(int top, uint32_t low) {
+    return low && top - exponent(~low) > 10;
+}
 
 // Over the lanes c, c + 16, c + 32, c + 48: a swap of 16- or 32-lane halves of a
 // register with itself leaves both halves' values in every lane.
@@ -132,6 +160,13 @@ __device__ __forceinline__ void wave_max_bits(uint32_t &a, uint32_t &b) {
     s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
     a = __builtin_amdgcn_readfirstlane(max(r[0], r[1]));
     b = __builtin_amdgcn_readfirstlane(max(s[0], s[1]));
+}
+
+// What this wave wrote to LDS before is there for what it reads after.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // x, which the compiler must take as new: what follows from it is worked out where
@@ -223,30 +258,41 @@ __device__ __forceinline__ void scores_in_f32(const TreeAttn &a, int b, int kvh,
     }
 }
 
-// Adds the values of a tile's V that are not finite, with their weights (row c's in
-// lane group `from` for its positions), to the outputs of row c.
-template <int NB, int KT>
-__device__ __forceinline__ void add_not_finite(const TreeAttn &a, const float *vb, int p0, int end,
-                                               int g, int c, const f16x8 *ph, const f16x8 *pl,
-                                               f32x4 (&o)[NB][4]) {
-    for (int i = 0; i < 32 * KT; ++i) {
+// The least exponent of a weight's scale.  Where V is that small against the outputs'
+// scale 2^(kTop - oe), the limbs (below 2^(kTop + 1)) come out too large, by less than
+// 2^(oe - 60), and the sum still gets every weight down to 2^-66.
+constexpr int kWeightLow = -60;
+
+// Adds a tile's V, taken in f32, with its weights (row c's in lane group `from` for its
+// positions) to the outputs of row c, whose scale is `by`.  The scale is such that no V
+// passes 2^90 in it (raise()).
+template <int NB, int N>
+__device__ __forceinline__ void add_in_f32(const TreeAttn &a, const float *vb, int p0, int end,
+                                           int g, int c, const float (&p)[N], float by,
+                                           f32x4 (&o)[NB][4]) {
+    for (int i = 0; i < 4 * N; ++i) {
         const int sub = i >> 5, from = i >> 3 & 3, j = i & 7;
         const float *v = vb + min(p0 + 32 * sub + position(j, from), end - 1) * a.v.ss;
         float w = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8 * KT; ++k)
-            if (k == j + 8 * sub) w = (float)ph[k >> 3][k & 7] + (float)pl[k >> 3][k & 7];
+        for (int k = 0; k < N; ++k)
+            if (k == j + 8 * sub) w = p[k];
         w = __shfl(w, c + 16 * from);
-        if (w == 0.f) continue;
+        if (w == 0.f) continue;   // not seen, NaN or not
 #pragma unroll
         for (int q = 0; q < NB; ++q)
 #pragma unroll
             for (int y = 0; y < 16; ++y)
-                if (64 * q + 16 * g < a.hd) {
-                    const float x = v[64 * q + 16 * g + y];
-                    if (abs_bits(x) >= kInf) o[q][y & 3][y >> 2] = fmaf(w, x, o[q][y & 3][y >> 2]);
-                }
+                if (64 * q + 16 * g < a.hd)
+                    o[q][y & 3][y >> 2] = fmaf(w, v[64 * q + 16 * g + y] * by, o[q][y & 3][y >> 2]);
     }
+}
+
+// What a partial result's maximum is merged as: -inf when it saw nothing, infinity
+// when its sum is NaN without a score to refer to (a NaN among the queries), which
+// makes the row NaN.
+__device__ __forceinline__ float reference(bool live, float m, float sum) {
+    return !live ? -INFINITY : sum != sum && m == -INFINITY ? INFINITY : m;
 }
 
 // The outputs' scale 2^(kTop - oe) for a tile of V's exponent ve: how far it moves
@@ -256,6 +302,15 @@ __device__ __forceinline__ int rescale(int ve, int &oe, int &oe_top) {
     oe_top = max(oe_top, ve);
     if (ve <= oe && ve >= oe - 6) return 0;
     const int to = max(ve, oe_top - 64), down = oe - to;
+    oe = to;
+    return down;
+}
+
+// The same before add_in_f32, of V up to 2^ve: it may stay up to 90 below, so that the
+// largest V of one row and the ordinary ones of another both fit f32.
+__device__ __forceinline__ int raise(int ve, int &oe, int &oe_top) {
+    oe_top = max(oe_top, ve);
+    const int to = max(oe, ve - 90), down = oe - to;
     oe = to;
     return down;
 }
@@ -270,14 +325,15 @@ __host__ __device__ inline int tiles_per_split(int tiles, int cap) {
     return t < kMinTiles ? kMinTiles : t;
 }
 
-// A block takes 64 * RB query rows of one KV head, a row being a (node, head of
-// the group) pair i = node * G + head, 16 * RB of them a wave, and a range of
-// the positions in tiles of TK.  Per tile the four waves build the limbs of a
-// quarter of K and of V each, in LDS and in MFMA operand order, and then every
-// wave multiplies all of them with its rows: so each f32 of the cache is read
-// and split once a block.  Two buffers, one barrier a tile: while tile i is
-// multiplied, tile i + 1 goes from registers to the other buffer and tile i + 2
-// is requested.
+// A block of NW waves takes 16 * RB * NW query rows of one KV head, a row being a
+// (node, head of the group) pair i = node * G + head, 16 * RB of them a wave, and a
+// range of the positions in tiles of TK.  Per tile the waves build the limbs of an
+// NW-th of K and of V each, in LDS and in MFMA operand order, and then every wave
+// multiplies all of them with its rows: so each f32 of the cache is read and split
+// once a block.  Two buffers, one barrier a tile: while tile i is multiplied, tile
+// i + 1 goes from registers to the other buffer and tile i + 2 is requested.  Where
+// one block has a CU to itself (NW = 8) half of its waves multiply first and half
+// build first, so that a SIMD's two waves want its matrix and its vector unit in turn.
 //   Lane (g, c) = (lane / 16, lane % 16) has A[c][8g ..] and B[8g ..][c] of a
 //   product of depth 32, and gets D[4g + r][c] in register r:
 //   S^T = K Q^T: A = 16 positions, position c with the 8 dimensions 16 x + 4g ..
@@ -287,45 +343,62 @@ __host__ __device__ inline int tiles_per_split(int tiles, int cap) {
 //     depth 8g + i is position 4g + i (i < 4) or 16 + 4g + i - 4 of 32: the
 //     positions whose scores the lane holds for row c, so P^T needs no exchange
 //     and V rows are read in whole 256-byte pieces.
-// Each wave's quarter has a scale of its own: a quarter of K is 8 positions
-// 16 (w / 2) + 8 (w % 2) .. of every 32, one of V the positions of lane group
-// g = w, so a lane needs two scales for its scores and one for its weights.
+// What a wave builds has a scale of its own: of every 32 positions, K's 32 / NW from
+// w * 32 / NW on, and V's of lane group g = w (NW = 4), or of half h and group g,
+// w = 4 h + g (NW = 8).
 //
 // A tile with infinities (or NaN, behind the prefix) takes its sums one by one
 // in f32, so that positions that a row does not see stay out of its result.
-template <int DP, int RB>
-__global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
+template <int DP, int RB, int NW>
+__global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_attn(
     TreeAttn a, int cap, float *__restrict__ part, float *__restrict__ pml) {
     constexpr int NS = DP / 32, NB = DP / 64, TK = tile_of(DP), KT = TK / 32;
-    constexpr int KU = KT * NS / 2, VU = KT * NB / 2;   // operands of 8 K values, 16 V values a lane
-    constexpr int KG = RB == 1 ? 2 : 1, VG = RB == 1 ? 4 : 2;   // operands read at a time
+    constexpr int PW = 32 / NW, LX = 16 / PW;   // K positions a wave, operands of one side by side
+    constexpr int KU = KT * NS / LX;            // K operands (8 values) a lane
+    constexpr int VU = KT * NB / 2, VP = 16 / NW;   // V: columns of 4 a lane, positions of each
+    constexpr int KG = RB == 1 ? 2 : 1, VG = RB == 1 ? 4 : NW == 4 && DP == 128 ? 1 : 2;   // operands read at a time
     __shared__ f16x8 sk[2][KT * 2 * NS * 2 * 64];       // [32 positions][16][32 dims][limb][lane]
     __shared__ f16x8 sv[2][KT * NB * 4 * 2 * 64];       // [32 positions][64 dims][j][limb][lane]
-    __shared__ int se[2][2][4], bad[2][2][4];           // K's, V's quarters: exponent, not finite
+    __shared__ int se[2][2][NW], bad[2][2][NW];         // K's, V's shares: exponent, for f32
+    // A share's largest and least exponent of V in the tiles behind the prefix so far.
+    __shared__ int behind[2][2][NW];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, g = lane >> 4;
     const int G = a.hq / a.hkv, R = a.n * G, D = a.hd, words = (a.n + 31) / 32;
     const int split = blockIdx.x, kvh = blockIdx.y % a.hkv, b = blockIdx.z;
-    const int w0 = (blockIdx.y / a.hkv * 4 + wave) * 16 * RB;   // the wave's first row
+    const int w0 = (blockIdx.y / a.hkv * NW + wave) * 16 * RB;   // the wave's first row
     const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
     const int tiles = (end + TK - 1) / TK, tps = tiles_per_split(tiles, cap);
     const int t0 = split * tps, t1 = min(tiles, t0 + tps);
     if (split > 0 && t0 >= t1) return;   // the merge skips this split
     const float *kb = a.k.p + b * a.k.sb + kvh * a.k.sh, *vb = a.v.p + b * a.v.sb + kvh * a.v.sh;
 
-    // ---- this thread's part of a tile
-    const int kkey = 16 * (wave >> 1) + 8 * (wave & 1) + (lane & 7), kg = lane >> 3 & 3;
-    const int kx = lane >> 5;             // K: dimension block's parity
-    const int half = lane & 1, vc = lane >> 1 & 15, vx = lane >> 5;
-    float kr[KU][8], vr[VU][4][4];
+    // ---- this thread's part of a tile: operand (sub, s) of K position kpos, column (sub, q)
+    // of V positions vpos ..
+    auto kpos = [&](int ln) { return wave * PW + (ln & (PW - 1)); };
+    auto kgrp = [](int ln) { return ln / PW & 3; };
+    auto kop = [](int ln, int u) { return u * LX + ln / (4 * PW); };   // sub * NS + s
+    auto vpos = [&](int ln) {
+        return NW == 4 ? 16 * (ln & 1) + 4 * wave : 4 * wave + 2 * (ln & 1);
+    };
+    auto vcol = [](int ln) { return ln >> 1 & 15; };
+    auto vsub = [](int ln) { return KT == 2 ? ln >> 5 : 0; };
+    auto vq = [](int ln, int u) { return KT == 2 ? 0 : (ln >> 5) + 2 * u; };
+    float kr[KU][8], vr[VU][VP][4];
     // Its addresses, in 16-byte units from the tile's first row.  Dimensions past head_dim
-    // repeat its last ones: the query limbs are zero there, and those outputs are not kept.
+    // repeat others: the query limbs are zero there, and those outputs are not kept.
     const uint32_t ks4 = (uint32_t)(a.k.ss / 4), vs4 = (uint32_t)(a.v.ss / 4);
-    const uint32_t koff = kkey * ks4 + 4 * kx + kg;
-    uint32_t voff[VU];
+    uint32_t koff[KU], koff2[KU], voff[VU];
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+        const int s = kop(lane, u) % NS, d = 64 * (s >> 1);
+        koff[u] = (32 * (kop(lane, u) / NS) + kpos(lane)) * ks4 + 4 * (s & 1) + kgrp(lane) +
+                  (d < D ? d / 4 : 0);
+        koff2[u] = d + 32 < D ? 8 : 0;
+    }
 #pragma unroll
     for (int u = 0; u < VU; ++u)
-        voff[u] = (32 * (KT == 2 ? vx : 0) + 16 * half + 4 * wave) * vs4 +
-                  min(16 * (KT == 2 ? 0 : vx + 2 * u) + vc, D / 4 - 1);
+        voff[u] = (32 * vsub(lane) + vpos(lane)) * vs4 +
+                  min(16 * vq(lane, u) + vcol(lane), D / 4 - 1);
     auto load_k = [&](int tile) {
         const float4 *kt = reinterpret_cast<const float4 *>(kb + (int64_t)tile * TK * a.k.ss);
         const int last = end - 1 - tile * TK;   // the last tile repeats the last position
@@ -333,12 +406,9 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
         const int ln = fresh_lane();
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
-            const int sub = KT == 2 ? u : 0, d = KT == 2 ? 0 : 64 * u;   // 64 dimensions from d
-            uint32_t at = (uint32_t)fresh((int)koff) + sub * 32 * ks4;
-            if (!whole)
-                at -= max(32 * sub + 16 * (wave >> 1) + 8 * (wave & 1) + (ln & 7) - last, 0) * ks4;
-            const float4 x = kt[at + (d < D ? d / 4 : 0)];
-            const float4 y = kt[at + (d + 32 < D ? d / 4 + 8 : 0)];
+            uint32_t at = (uint32_t)fresh((int)koff[u]);
+            if (!whole) at -= max(32 * (kop(ln, u) / NS) + kpos(ln) - last, 0) * ks4;
+            const float4 x = kt[at], y = kt[at + koff2[u]];
             kr[u][0] = x.x; kr[u][1] = x.y; kr[u][2] = x.z; kr[u][3] = x.w;
             kr[u][4] = y.x; kr[u][5] = y.y; kr[u][6] = y.z; kr[u][7] = y.w;
         }
@@ -351,19 +421,16 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
 #pragma unroll
         for (int u = 0; u < VU; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < VP; ++i) {
                 uint32_t at = (uint32_t)fresh((int)voff[u]) + i * vs4;
-                if (!whole)
-                    at -= max(32 * (KT == 2 ? ln >> 5 : 0) + 16 * (ln & 1) + 4 * wave + i - last,
-                              0) * vs4;
+                if (!whole) at -= max(32 * vsub(ln) + vpos(ln) + i - last, 0) * vs4;
                 const float4 x = vt[at];
                 vr[u][i][0] = x.x; vr[u][i][1] = x.y; vr[u][i][2] = x.z; vr[u][i][3] = x.w;
             }
     };
     // The tile's limbs to a buffer; the registers then take the next tile's values.
     auto store = [&](int tile, int buf) {
-        const int ln = fresh_lane(), kx = ln >> 5, kg = ln >> 3 & 3, vx = ln >> 5, vc = ln >> 1 & 15,
-                  half = ln & 1;
+        const int ln = fresh_lane();
         const bool open = (tile + 1) * TK <= len;
         float km = 0.f, vm = 0.f, kn = 0.f, vn = 0.f;
 #pragma unroll
@@ -376,69 +443,93 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
 #pragma unroll
         for (int u = 0; u < VU; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < VP; ++i) {
                 max3_abs(vm, vr[u][i][0], vr[u][i][1]);
                 max3_abs(vn, vr[u][i][2], vr[u][i][3]);
             }
         uint32_t kt = max(abs_bits(km), abs_bits(kn)), vt = max(abs_bits(vm), abs_bits(vn));
+        bool slow_k = false, slow_v = false;
         if (!open) {   // NaN in V too: a row that does not see its position must not get it
+            uint32_t k_low = 0, v_low = 0;
 #pragma unroll
-            for (int u = 0; u < VU; ++u)
+            for (int u = 0; u < KU; ++u) low_bits(k_low, top_bits(kr[u]));
 #pragma unroll
-                for (int i = 0; i < 16; ++i) vt = max(vt, abs_bits(vr[u][i >> 2][i & 3]));
+            for (int i = 0; i < VP; ++i) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int u = 0; u < VU; ++u) top = max(top, top_bits(vr[u][i]));
+                vt = max(vt, top);
+                low_bits(v_low, top);
+            }
+            wave_max_bits(kt, vt);
+            wave_max_bits(k_low, v_low);
+            slow_k = spread(exponent(kt), k_low);
+            slow_v = spread(exponent(vt), v_low);
+        } else {
+            wave_max_bits(kt, vt);
         }
-        wave_max_bits(kt, vt);
-        const bool bad_k = kt >= kInf, bad_v = vt >= kInf;
-        if (__builtin_expect(bad_k | bad_v, 0)) {
-            // Out of the limbs: the tile's scores are summed in f32, and what of V has weight
-            // is added in f32.
-#pragma unroll
-            for (int u = 0; u < KU; ++u)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) kr[u][j] = bad_k ? 0.f : kr[u][j];
-            kt = bad_k ? 0 : kt;
+        slow_k |= kt >= kInf;
+        slow_v |= vt >= kInf;
+        if (__builtin_expect(vt >= kInf, 0)) {   // the largest finite one
             vt = 0;
 #pragma unroll
             for (int u = 0; u < VU; ++u)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < 4 * VP; ++i) {
                     float &x = vr[u][i >> 2][i & 3];
                     x = abs_bits(x) < kInf ? x : 0.f;
                     vt = max(vt, abs_bits(x));
                 }
-            uint32_t k2 = kt;
-            wave_max_bits(k2, vt);
+            uint32_t v2 = vt;
+            wave_max_bits(vt, v2);
         }
         const int ke = exponent(kt), ve = exponent(vt);
+        int high = kNoV, low = -kNoV;
+        if (!open) {
+            if (tile > t0) {   // what those before it were, it is
+                high = behind[buf ^ 1][0][wave];
+                low = behind[buf ^ 1][1][wave];
+                slow_v |= (tile * TK > len && bad[buf ^ 1][1][wave]) ||
+                          ve - se[buf ^ 1][1][wave] > 20;
+            }
+            high = max(high, ve);
+            low = min(low, ve == kLeast ? -kNoV : ve);
+        }
         if (ln == 0) {
+            behind[buf][0][wave] = high;
+            behind[buf][1][wave] = low;
             se[buf][0][wave] = ke;
             se[buf][1][wave] = ve;
-            bad[buf][0][wave] = bad_k;
-            bad[buf][1][wave] = bad_v;
+            bad[buf][0][wave] = slow_k;
+            bad[buf][1][wave] = slow_v;
         }
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
-            const int sub = KT == 2 ? u : 0, s = KT == 2 ? kx : kx + 2 * u;
+            const int sub = kop(ln, u) / NS, s = kop(ln, u) % NS, p = kpos(ln);
             f16x8 hi, lo;
             split_to_lds<8>(kr[u], pow2(kTop - ke), hi, lo);
-            f16x8 *d = sk[buf] + (((sub * 2 + (wave >> 1)) * NS + s) * 2) * 64 + 16 * kg +
-                       8 * (wave & 1) + (ln & 7);
+            f16x8 *d = sk[buf] + (((sub * 2 + (p >> 4)) * NS + s) * 2) * 64 + 16 * kgrp(ln) + (p & 15);
             d[0] = hi;
             d[64] = lo;
         }
         if (tile + 1 < t1) load_k(tile + 1);
 #pragma unroll
         for (int u = 0; u < VU; ++u) {
-            const int sub = KT == 2 ? vx : 0, q = KT == 2 ? 0 : vx + 2 * u;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float x[4] = {vr[u][0][j], vr[u][1][j], vr[u][2][j], vr[u][3][j]};
-                f16x4 hi, lo;
-                split_to_lds<4>(x, pow2(kTop - ve), hi, lo);
-                f16x4 *d = reinterpret_cast<f16x4 *>(
-                               sv[buf] + (((sub * NB + q) * 4 + j) * 2) * 64 + 16 * wave + vc) + half;
+                float x[VP];
+#pragma unroll
+                for (int i = 0; i < VP; ++i) x[i] = vr[u][i][j];
+                f16v<VP> hi, lo;
+                split_to_lds<VP>(x, pow2(kTop - ve), hi, lo);
+                const int p = vpos(ln);   // half p / 16, group p % 16 / 4, first of it p % 4
+                f16v<VP> *d = reinterpret_cast<f16v<VP> *>(
+                    reinterpret_cast<_Float16 *>(
+                        sv[buf] + (((vsub(ln) * NB + vq(ln, u)) * 4 + j) * 2) * 64 +
+                        16 * (p >> 2 & 3) + vcol(ln)) +
+                    4 * (p >> 4) + (p & 3));
                 d[0] = hi;
-                d[128] = lo;
+                d[64 * 8 / VP] = lo;
             }
         }
         if (tile + 1 < t1) load_v(tile + 1);
@@ -469,15 +560,26 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[rb][q][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    int oe = 0, oe_top = -1000;   // exponent of the outputs' scale; the largest V's so far
+    int oe = 0, oe_top = kNoV;   // exponent of the outputs' scale; the largest V's so far
     const float f = fabsf(a.scale) * kLog2e;
 
     if (t0 < t1) {
         store(t0, 0);
         __syncthreads();
     }
-    for (int tile = t0; tile < t1; ++tile) {
-        const int buf = (tile - t0) & 1, p0 = tile * TK;
+    // Without the positions that the row does not see.
+    auto mask_scores = [&](int rb, int p0, int g, float (&s)[8 * KT]) TB_INLINE {
+#pragma unroll
+        for (int sub = 0; sub < KT; ++sub) {
+            const uint32_t see =
+                live[rb] ? seen(mask + mrow[rb], words, p0 + 32 * sub, len, end) : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!(see >> position(j, g) & 1)) s[8 * sub + j] = -INFINITY;
+        }
+    };
+    auto multiply = [&](int tile, int buf) {
+        const int p0 = tile * TK;
         if (busy) {
             const bool open = p0 + TK <= len;   // every live row sees every position
             const int ln = fresh_lane(), g = ln >> 4;
@@ -534,12 +636,24 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
                         vf[grp & 1][j][y] = sv[buf][((grp * VG + j) * 2 + y) * 64 + ln];
             };
             read_v(0);
-            const int ke[2] = {se[buf][0][g >> 1], se[buf][0][2 + (g >> 1)]};
-            const int ve = se[buf][1][g];
-            const int vtop = __builtin_amdgcn_readfirstlane(max(
-                max(se[buf][1][0], se[buf][1][1]), max(se[buf][1][2], se[buf][1][3])));
-            const bool slow_k = bad[buf][0][0] | bad[buf][0][1] | bad[buf][0][2] | bad[buf][0][3];
-            const bool slow_v = bad[buf][1][0] | bad[buf][1][1] | bad[buf][1][2] | bad[buf][1][3];
+            const int ke[2] = {se[buf][0][4 * g / PW], se[buf][0][(16 + 4 * g) / PW]};
+            const int ve[2] = {se[buf][1][g], se[buf][1][NW == 4 ? g : 4 + g]};
+            int vtop = se[buf][1][0], slow_k = bad[buf][0][0], slow_v = bad[buf][1][0];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) {
+                vtop = max(vtop, se[buf][1][w]);
+                slow_k |= bad[buf][0][w];
+                slow_v |= bad[buf][1][w];
+            }
+            vtop = __builtin_amdgcn_readfirstlane(vtop);
+            slow_k = __builtin_amdgcn_readfirstlane(slow_k);
+            int high = behind[buf][0][0], low = behind[buf][1][0];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) {
+                high = max(high, behind[buf][0][w]);
+                low = min(low, behind[buf][1][w]);
+            }
+            slow_v = __builtin_amdgcn_readfirstlane(slow_v | (high - low > 8));
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 const float sx[2] = {ldexpf(f, qe[rb] + ke[0] - 2 * kTop),
@@ -559,16 +673,7 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
             bool moved = false;
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                if (!open) {
-#pragma unroll
-                    for (int sub = 0; sub < KT; ++sub) {
-                        const uint32_t see =
-                            live[rb] ? seen(mask + mrow[rb], words, p0 + 32 * sub, len, end) : 0;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (!(see >> position(j, g) & 1)) s8[rb][8 * sub + j] = -INFINITY;
-                    }
-                }
+                if (!open) mask_scores(rb, p0, g, s8[rb]);
                 float top = s8[rb][0];
 #pragma unroll
                 for (int j = 1; j < 8 * KT; ++j) top = fmaxf(top, s8[rb][j]);
@@ -577,7 +682,7 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
                 m[rb] = top > m[rb] + kLag ? top : m[rb];
                 moved |= m[rb] != was[rb];
             }
-            const int down = rescale(vtop, oe, oe_top);
+            const int down = slow_v ? raise(vtop, oe, oe_top) : rescale(vtop, oe, oe_top);
             if (__any(moved) || down != 0) {
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
@@ -593,18 +698,21 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
             }
             // ---- weights, in the scale of the positions' V: 2^pe w
             f16x8 ph[RB][KT], pl[RB][KT];
-            const int pe = max(kWeight + ve - oe, -126);
-            const float back = pow2(-pe);
+            const int pe[2] = {max(kWeight + ve[0] - oe, kWeightLow),
+                               max(kWeight + ve[1] - oe, kWeightLow)};
+            const float back[2] = {pow2(-pe[0]), pow2(-pe[1])};
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                const float base = (float)pe - (m[rb] == -INFINITY ? 0.f : m[rb]);
+                float top = m[rb] == -INFINITY ? 0.f : m[rb];   // nothing seen: weights 0
+                if (slow_v) top = INFINITY;   // V in f32 below: weights 0 here
+                const float base[2] = {(float)pe[0] - top, (float)pe[1] - top};
 #pragma unroll
                 for (int sub = 0; sub < KT; ++sub) {
                     float p8[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        p8[j] = __builtin_amdgcn_exp2f(s8[rb][8 * sub + j] + base);
-                        l[rb] = fmaf(p8[j], back, l[rb]);
+                        p8[j] = __builtin_amdgcn_exp2f(s8[rb][8 * sub + j] + base[j >> 2]);
+                        l[rb] = fmaf(p8[j], back[j >> 2], l[rb]);
                     }
                     split8(p8, 1.f, ph[rb][sub], pl[rb][sub]);
                 }
@@ -628,14 +736,40 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
                         }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (__builtin_expect(slow_v, 0)) {
+            if (__builtin_expect(slow_v, 0)) {   // weights anew: nothing waits for this in registers
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-                    add_not_finite<NB, KT>(a, vb, p0, end, g, c, ph[rb], pl[rb], o[rb]);
+                for (int rb = 0; rb < RB; ++rb) {
+                    float p[8 * KT];
+                    scores_in_f32<8 * KT>(a, b, kvh, min(w0 + 16 * rb + c, R - 1), p0, end, g, p);
+                    if (!open) mask_scores(rb, p0, g, p);
+                    const float base = (float)kWeight - (m[rb] == -INFINITY ? 0.f : m[rb]);
+#pragma unroll
+                    for (int j = 0; j < 8 * KT; ++j) {
+                        p[j] = __builtin_amdgcn_exp2f(p[j] + base);
+                        l[rb] = fmaf(p[j], pow2(-kWeight), l[rb]);
+                    }
+                    add_in_f32<NB, 8 * KT>(a, vb, p0, end, g, c, p, pow2(kTop - oe), o[rb]);
+                }
             }
         }
-        if (tile + 1 < t1) store(tile + 1, buf ^ 1);
-        __syncthreads();
+    };
+    if constexpr (NW == 4) {
+        for (int tile = t0; tile < t1; ++tile) {
+            const int buf = (tile - t0) & 1;
+            multiply(tile, buf);
+            if (tile + 1 < t1) store(tile + 1, buf ^ 1);
+            __syncthreads();
+        }
+    } else {
+        for (int step = 0; step < 2 * (t1 - t0); ++step) {
+            const int tile = t0 + (step >> 1), buf = step >> 1 & 1;
+            if ((step ^ wave >> 2) & 1) {
+                if (tile + 1 < t1) store(tile + 1, buf ^ 1);
+            } else {
+                multiply(tile, buf);
+            }
+            if (step & 1) __syncthreads();
+        }
     }
     if (!busy) return;
 
@@ -646,11 +780,11 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
         const float sum = live[rb] ? sum_over_groups(l[rb]) : 0.f;
         if (i >= R) continue;
         const size_t at = (((size_t)b * a.hkv + kvh) * gridDim.x + split) * R + i;
-        float *to = part ? part + at * D
+        float *to = part ? part + at * D   // normalised, so that the largest V do not overflow
                          : a.out + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D;
-        const float x = part ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;
+        const float x = sum == 0.f ? 0.f : 1.0f / sum;
         if (part && g == 0) {
-            pml[2 * at] = live[rb] ? m[rb] : -INFINITY;
+            pml[2 * at] = reference(live[rb], m[rb], sum);
             pml[2 * at + 1] = sum;
         }
 #pragma unroll
@@ -659,10 +793,10 @@ __global__ __launch_bounds__(256, DP * RB <= 256 ? 2 : 1) void k_tree_attn(
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float4 y;
-                    y.x = ldexpf(o[rb][q][0][r], oe - kTop - kWeight) * x;
-                    y.y = ldexpf(o[rb][q][1][r], oe - kTop - kWeight) * x;
-                    y.z = ldexpf(o[rb][q][2][r], oe - kTop - kWeight) * x;
-                    y.w = ldexpf(o[rb][q][3][r], oe - kTop - kWeight) * x;
+                    y.x = ldexpf(o[rb][q][0][r] * x, oe - kTop - kWeight);
+                    y.y = ldexpf(o[rb][q][1][r] * x, oe - kTop - kWeight);
+                    y.z = ldexpf(o[rb][q][2][r] * x, oe - kTop - kWeight);
+                    y.w = ldexpf(o[rb][q][3][r] * x, oe - kTop - kWeight);
                     if (!live[rb]) y = make_float4(0.f, 0.f, 0.f, 0.f);
                     reinterpret_cast<float4 *>(to + 64 * q + 16 * g)[r] = y;
                 }
@@ -744,7 +878,9 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[rb][q][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    int oe = 0, oe_top = -1000;   // exponent of the outputs' scale; the largest V's so far
+    int oe = 0, oe_top = kNoV;   // exponent of the outputs' scale; the largest V's so far
+    // The largest V's behind the prefix so far; the first tile there whose V went in f32.
+    int behind = kNoV, f32_since = t1;
     const float f = fabsf(a.scale) * kLog2e;
 
     for (int tile = first; tile < t1; tile += 4) {
@@ -759,10 +895,14 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
                 max3_abs(km, kr[0][s][j], kr[0][s][j + 1]);
                 max3_abs(kn, kr[1][s][j], kr[1][s][j + 1]);
             }
-        uint32_t kt = max(abs_bits(km), abs_bits(kn)), zero = 0;
-        wave_max_bits(kt, zero);
-        const bool bad_k = kt >= kInf;
+        uint32_t kt = max(abs_bits(km), abs_bits(kn)), k_low = 0;
+        if (!open) {
+            low_bits(k_low, abs_bits(km));
+            low_bits(k_low, abs_bits(kn));
+        }
+        wave_max_bits(kt, k_low);
         const int ke = exponent(kt);
+        const bool slow_k = kt >= kInf || spread(ke, k_low);
         // ---- scores, in powers of two
         f32x4 acc[RB][2];
 #pragma unroll
@@ -790,7 +930,7 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
 #pragma unroll
             for (int j = 0; j < 8; ++j) s8[rb][j] = acc[rb][j >> 2][j & 3] * sx;
         }
-        if (__builtin_expect(bad_k, 0)) {
+        if (__builtin_expect(slow_k, 0)) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
                 scores_in_f32<8>(a, b, kvh, min(16 * rb + c, R - 1), p0, end, g, s8[rb]);
@@ -822,18 +962,20 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
                 max3_abs(vm, vr[i][q][0], vr[i][q][1]);
                 max3_abs(vn, vr[i][q][2], vr[i][q][3]);
             }
-        uint32_t vt = max(abs_bits(vm), abs_bits(vn));
+        uint32_t vt = max(abs_bits(vm), abs_bits(vn)), v_low = 0;
         if (!open) {   // NaN too: a row that does not see its position must not get it
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 8; ++i) {
+                uint32_t top = 0;
 #pragma unroll
-                for (int q = 0; q < NB; ++q)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) vt = max(vt, abs_bits(vr[i][q][j]));
+                for (int q = 0; q < NB; ++q) top = max(top, top_bits(vr[i][q]));
+                vt = max(vt, top);
+                low_bits(v_low, top);
+            }
         }
-        wave_max_bits(vt, zero);
-        const bool bad_v = vt >= kInf;
-        if (__builtin_expect(bad_v, 0)) {   // out of the limbs; what has weight is added in f32
+        wave_max_bits(vt, v_low);
+        bool slow_v = vt >= kInf;
+        if (__builtin_expect(slow_v, 0)) {   // the largest finite one
             vt = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -841,12 +983,19 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
                 for (int q = 0; q < NB; ++q)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        vr[i][q][j] = abs_bits(vr[i][q][j]) < kInf ? vr[i][q][j] : 0.f;
-                        vt = max(vt, abs_bits(vr[i][q][j]));
+                        const uint32_t x = abs_bits(vr[i][q][j]);
+                        vt = max(vt, x < kInf ? x : 0);
                     }
-            wave_max_bits(vt, zero);
+            uint32_t v2 = vt;
+            wave_max_bits(vt, v2);
         }
-        const int ve = exponent(vt), down = rescale(ve, oe, oe_top);
+        const int ve = exponent(vt);
+        if (!open) {
+            behind = max(behind, ve);
+            slow_v |= f32_since < tile || spread(behind, v_low) || (oe_top != kNoV && ve - oe > 20);
+            if (slow_v) f32_since = min(f32_since, tile);
+        }
+        const int down = slow_v ? raise(ve, oe, oe_top) : rescale(ve, oe, oe_top);
         if (__any(moved) || down != 0) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
@@ -860,19 +1009,26 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
             }
         }
         // ---- weights 2^kWeight w
-        f16x8 ph[RB], pl[RB];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             const float base = (float)kWeight - (m[rb] == -INFINITY ? 0.f : m[rb]);
-            float p8[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                p8[j] = __builtin_amdgcn_exp2f(s8[rb][j] + base);
-                l[rb] += p8[j];
+                s8[rb][j] = __builtin_amdgcn_exp2f(s8[rb][j] + base);
+                l[rb] += s8[rb][j];
             }
-            split8(p8, 1.f, ph[rb], pl[rb]);
         }
         // ---- outputs; V takes the outputs' scale
+        if (__builtin_expect(slow_v, 0)) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+                add_in_f32<NB, 8>(a, vb, p0, end, g, c, s8[rb], pow2(kTop - oe), o[rb]);
+            if (tile + 4 < t1) load_v(tile + 4);
+            continue;
+        }
+        f16x8 ph[RB], pl[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) split8(s8[rb], 1.f, ph[rb], pl[rb]);
 #pragma unroll
         for (int q = 0; q < NB; ++q) {
             f16x8 vh[4], vl[4];
@@ -892,33 +1048,42 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
                             x == 0 ? vl[j] : vh[j], x == 1 ? pl[rb] : ph[rb], o[rb][q][j], 0, 0, 0);
         }
         if (tile + 4 < t1) load_v(tile + 4);
-        if (__builtin_expect(bad_v, 0)) {
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
-                add_not_finite<NB, 1>(a, vb, p0, end, g, c, &ph[rb], &pl[rb], o[rb]);
-        }
     }
 
-    // ---- the four waves' outputs, brought to one maximum and summed in wave order
+    // ---- the four waves' outputs, normalised, in the shares of their sums, in wave order
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        if (!live[rb]) m[rb] = -INFINITY;
         const float sum = sum_over_groups(l[rb]);
         l[rb] = live[rb] ? sum : 0.f;
+        m[rb] = reference(live[rb], m[rb], sum);
         if (g == 0) {
             lm[wave][16 * rb + c] = m[rb];
             ls[wave][16 * rb + c] = l[rb];
         }
     }
     __syncthreads();
+    // Row r's maximum, sum and share of wave w.
+    auto shares = [&](int r, int w, float &top, float &sum) {
+        top = fmaxf(fmaxf(lm[0][r], lm[1][r]), fmaxf(lm[2][r], lm[3][r]));
+        sum = 0.f;
+        float mine = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const float y =
+                lm[x][r] == -INFINITY ? 0.f : ls[x][r] * __builtin_amdgcn_exp2f(lm[x][r] - top);
+            sum += y;
+            mine = x == w ? y : mine;
+        }
+        return sum == 0.f ? 0.f : mine / sum;
+    };
+    float top, sum;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         if (wave == w) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 const int r = 16 * rb + c;
-                const float top = fmaxf(fmaxf(lm[0][r], lm[1][r]), fmaxf(lm[2][r], lm[3][r]));
-                const float x = m[rb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rb] - top);
+                const float x = shares(r, w, top, sum), inv = l[rb] == 0.f ? 0.f : 1.0f / l[rb];
 #pragma unroll
                 for (int q = 0; q < NB; ++q)
 #pragma unroll
@@ -926,10 +1091,10 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
                         float4 *d = reinterpret_cast<float4 *>(&lo[r][64 * q + 16 * g]) + i;
                         float4 y = w ? *d : make_float4(0.f, 0.f, 0.f, 0.f);
                         if (x != 0.f) {
-                            y.x = fmaf(ldexpf(o[rb][q][0][i], oe - kTop), x, y.x);
-                            y.y = fmaf(ldexpf(o[rb][q][1][i], oe - kTop), x, y.y);
-                            y.z = fmaf(ldexpf(o[rb][q][2][i], oe - kTop), x, y.z);
-                            y.w = fmaf(ldexpf(o[rb][q][3][i], oe - kTop), x, y.w);
+                            y.x = fmaf(ldexpf(o[rb][q][0][i] * inv, oe - kTop), x, y.x);
+                            y.y = fmaf(ldexpf(o[rb][q][1][i] * inv, oe - kTop), x, y.y);
+                            y.z = fmaf(ldexpf(o[rb][q][2][i] * inv, oe - kTop), x, y.z);
+                            y.w = fmaf(ldexpf(o[rb][q][3][i] * inv, oe - kTop), x, y.w);
                         }
                         *d = y;
                     }
@@ -941,33 +1106,24 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
     for (int x = t; x < ROWS * cols; x += 256) {
         const int r = x / cols, d = x % cols;
         if (r >= R) break;
-        const float top = fmaxf(fmaxf(lm[0][r], lm[1][r]), fmaxf(lm[2][r], lm[3][r]));
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-            if (lm[w][r] != -INFINITY)
-                sum = fmaf(ls[w][r], __builtin_amdgcn_exp2f(lm[w][r] - top), sum);
         const float4 y = *reinterpret_cast<const float4 *>(&lo[r][4 * d]);
         if (part) {
             const size_t at = (((size_t)b * a.hkv + kvh) * gridDim.x + split) * R + r;
-            // sums and outputs as the other kernel leaves them, without 2^kWeight
-            reinterpret_cast<float4 *>(part + at * D)[d] =
-                make_float4(y.x * pow2(-kWeight), y.y * pow2(-kWeight), y.z * pow2(-kWeight), y.w * pow2(-kWeight));
+            reinterpret_cast<float4 *>(part + at * D)[d] = y;
             if (d == 0) {
+                shares(r, 0, top, sum);
                 pml[2 * at] = top;
-                pml[2 * at + 1] = sum * pow2(-kWeight);
+                pml[2 * at + 1] = sum;
             }
         } else {
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
             float *out = a.out + (((size_t)b * a.n + r / G) * a.hq + kvh * G + r % G) * D;
-            reinterpret_cast<float4 *>(out)[d] =
-                make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+            reinterpret_cast<float4 *>(out)[d] = y;
         }
     }
 }
 
-// The splits' outputs brought to one maximum, a block per row.  Each wave works
-// out every split's weight (lane s: splits s and s + 64); the columns are taken by
+// The splits' outputs, normalised, in the shares of their sums, a block per row.  Each
+// wave works out every split's share (lane s: splits s and s + 64); the columns are taken by
 // 256 / LC groups of LC lanes, group i with the splits i, i + 256 / LC, ...  The first
 // of those are requested before the weights are known: every split's place in the
 // scratch can be read, and what was not written has weight 0.
@@ -1007,15 +1163,15 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int tk, int cap,
     float sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-        const float y = m[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[x] - top);
-        w[wave][lane + 64 * x] = y;
-        if (y != 0.f) sum = fmaf(l[x], y, sum);
+        m[x] = m[x] == -INFINITY ? 0.f : l[x] * __builtin_amdgcn_exp2f(m[x] - top);
+        sum += m[x];
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) sum += gemv::shfl_xor_u(sum, o);
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // w: written and read by this wave
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) w[wave][lane + 64 * x] = m[x] * inv;
+    wave_fence();
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](int s, const float4 &v) {
         const float x = w[wave][s];
@@ -1040,17 +1196,16 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int tk, int cap,
     if (lane < LC) col[wave][lane] = y;
     __syncthreads();
     if ((int)threadIdx.x >= cols) return;
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
     const float4 y0 = col[0][d], y1 = col[1][d], y2 = col[2][d], y3 = col[3][d];
     float *out = a.out + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * a.hd;
     reinterpret_cast<float4 *>(out)[d] =
-        make_float4(((y0.x + y1.x) + (y2.x + y3.x)) * inv, ((y0.y + y1.y) + (y2.y + y3.y)) * inv,
-                    ((y0.z + y1.z) + (y2.z + y3.z)) * inv, ((y0.w + y1.w) + (y2.w + y3.w)) * inv);
+        make_float4((y0.x + y1.x) + (y2.x + y3.x), (y0.y + y1.y) + (y2.y + y3.y),
+                    (y0.z + y1.z) + (y2.z + y3.z), (y0.w + y1.w) + (y2.w + y3.w));
 }
 
 struct Plan {
     bool few;
-    int dp, rb, tk, rtiles, cap, nsplit;
+    int dp, rb, nw, tk, rtiles, cap, nsplit;
 };
 
 Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len) {
@@ -1060,15 +1215,20 @@ Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len) {
     p.few = R <= 32 && p.dp <= 128;
     p.rb = p.few ? (R <= 16 ? 1 : 2) : R <= 64 || p.dp == 256 ? 1 : 2;
     p.tk = p.few ? 32 : tile_of(p.dp);
-    p.rtiles = p.few ? 1 : (R + 64 * p.rb - 1) / (64 * p.rb);
-    // As many blocks as run at once: two per CU, or one where registers or LDS allow one
-    // (few rows, head_dim past 128).  us at half as many / this / half as many again, 8
-    // heads of 128: 4096 + 49 nodes 41.7 / 43.4 / 51.5, 32767 + 64 198 / 178 / 201, 8
-    // sequences of up to 6000 + 16 100 / 73 / 78; head_dim 256, 8192 + 16: - / 37.1 / 43.9.
-    const int64_t want =
-        (p.few || p.dp == 256 ? 256 : 512) / ((int64_t)p.rtiles * hkv * batch);
-    p.cap = (int)std::max<int64_t>(1, std::min<int64_t>(want, kMaxSplits));
     const int tiles = (max_len + p.tk - 1) / p.tk;
+    // Eight waves build a tile's limbs for 256 rows, half as much a row, where that leaves
+    // each of 256 blocks 16 tiles.  us with four / eight, 8 heads of 128 and groups of 4: 64
+    // nodes on 32767 180 / 164, 60 on 16384 94 / 92, on 4096 45.4 / 45.9, on 1024 28 / 33.
+    p.nw = p.rb == 2 && R > 128 && (int64_t)tiles * hkv * batch >= 16 * 256 ? 8 : 4;
+    const int rows = 16 * p.rb * p.nw;
+    p.rtiles = p.few ? 1 : (R + rows - 1) / rows;
+    // As many blocks as run at once: two per CU, or one where registers or LDS allow one
+    // (few rows, eight waves, head_dim past 128).  us at half as many / this / half as many
+    // again, 8 heads of 128: 4096 + 49 nodes 41.7 / 43.4 / 51.5, 32767 + 64 198 / 178 / 201, 8
+    // sequences of up to 6000 + 16 100 / 73 / 78; head_dim 256, 8192 + 16: - / 37.1 / 43.9.
+    const int64_t want = (p.few || p.nw == 8 || p.dp == 256 ? 256 : 512) /
+                         ((int64_t)p.rtiles * hkv * batch);
+    p.cap = (int)std::max<int64_t>(1, std::min<int64_t>(want, kMaxSplits));
     p.nsplit = std::max(1, std::min(p.cap, (tiles + kMinTiles - 1) / kMinTiles));
     return p;
 }
@@ -1088,18 +1248,20 @@ int launch_tree_attention(const TreeAttn &a, int max_len, float *scratch, hipStr
 #define TB_TF(DP, RB)                                                                        \
     if (p.few && p.dp == DP && p.rb == RB)                                                   \
     hipLaunchKernelGGL((k_tree_attn_few<DP, RB>), grid, dim3(256), 0, s, a, p.cap, part, pml)
-#define TB_TA(DP, RB)                                                                        \
-    if (!p.few && p.dp == DP && p.rb == RB)                                                  \
-    hipLaunchKernelGGL((k_tree_attn<DP, RB>), grid, dim3(256), 0, s, a, p.cap, part, pml)
+#define TB_TA(DP, RB, NW)                                                                    \
+    if (!p.few && p.dp == DP && p.rb == RB && p.nw == NW)                                    \
+    hipLaunchKernelGGL((k_tree_attn<DP, RB, NW>), grid, dim3(64 * NW), 0, s, a, p.cap, part, pml)
     TB_TF(64, 1);
     TB_TF(64, 2);
     TB_TF(128, 1);
     TB_TF(128, 2);
-    TB_TA(64, 1);
-    TB_TA(64, 2);
-    TB_TA(128, 1);
-    TB_TA(128, 2);
-    TB_TA(256, 1);
+    TB_TA(64, 1, 4);
+    TB_TA(64, 2, 4);
+    TB_TA(64, 2, 8);
+    TB_TA(128, 1, 4);
+    TB_TA(128, 2, 4);
+    TB_TA(128, 2, 8);
+    TB_TA(256, 1, 4);
 #undef TB_TA
 #undef TB_TF
     TB_LAUNCHED();

@@ -88,7 +88,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     for every bit j of its row, and a row without bits gives zeros.  Positions that a row
     does not see take no part, whatever the caches hold there.  ``kv_len`` is a number
     (ValueError when kv_len + n exceeds max_seq) or a tensor with one per sequence (clamped
-    on the device).  ``scale`` defaults to head_dim ** -0.5.  f32, in q's shape; caches may
+    on the device); the two may differ in their last bits on long caches, where the work is
+    split by the length known at the call.  ``scale`` defaults to head_dim ** -0.5.  f32, in q's shape; caches may
     have any strides of 16-byte rows.  Does not wait for the device."""
     op = "tree_attention"
     if q.ndim not in (3, 4):
@@ -135,7 +136,8 @@ def tree_accept(parents: torch.Tensor, draft_tokens: torch.Tensor, next_tokens: 
     int64 (..): the next token of the path's last node; -1 without a path).
 
     ``k_caches`` / ``v_caches``: every layer's cache, as tree_attention takes them (all of
-    one shape and one layout); row kv_len + path[j] moves to kv_len + j in each of them, in
+    one shape and one layout, none sharing memory with another), as lists or stacked in one
+    tensor; row kv_len + path[j] moves to kv_len + j in each of them, in
     place, so the sequence's new length is kv_len + n_path.  Rows past the path keep what
     they held.  Does not wait for the device."""
     op = "tree_accept"
@@ -151,7 +153,7 @@ def tree_accept(parents: torch.Tensor, draft_tokens: torch.Tensor, next_tokens: 
     if n == 0 and batch:
         raise _bad(op, "empty trees")
     lens, ln = _kv_len(op, kv_len, batch, dev)
-    ks_in, vs_in = list(k_caches or ()), list(v_caches or ())
+    ks_in, vs_in = ([] if c is None else list(c) for c in (k_caches, v_caches))
     if len(ks_in) != len(vs_in):
         raise _bad(op, f"{len(ks_in)} k_caches against {len(vs_in)} v_caches")
     layers, given, caches = len(ks_in), ks_in + vs_in, ()
