@@ -50,6 +50,7 @@ constexpr int kTop = 14;         // factors are scaled to below 2^(kTop + 1)
 constexpr float kLag = 8.f;
 constexpr int kWeight = 7;
 
+constexpr int kBias = 1 << 10, kSlow = 1 << 20;
 constexpr int kNoV = -1000;          // in place of an exponent: none yet
 constexpr int kLeast = kTop - 127;   // the smallest exponent()
 
@@ -318,7 +319,8 @@ __device__ __forceinline__ int raise(int ve, int &oe, int &oe_top) {
 // Positions per tile: the same bytes for every head_dim up to 128.
 __host__ __device__ constexpr int tile_of(int dp) { return dp == 64 ? 64 : 32; }
 // Tiles per split where at most `cap` splits are wanted.  Only the sequence's own
-// length counts, so a result is the same whatever the cache's size.
+// length counts, so that within one plan a result is the same whatever the bound.
+// With 2 or 8 tiles at least, 49 nodes on 512 positions take 3 and 6 us longer.
 constexpr int kMinTiles = 4;
 __host__ __device__ inline int tiles_per_split(int tiles, int cap) {
     const int t = (tiles + cap - 1) / cap;
@@ -347,8 +349,18 @@ __host__ __device__ inline int tiles_per_split(int tiles, int cap) {
 // w * 32 / NW on, and V's of lane group g = w (NW = 4), or of half h and group g,
 // w = 4 h + g (NW = 8).
 //
-// A tile with infinities (or NaN, behind the prefix) takes its sums one by one
-// in f32, so that positions that a row does not see stay out of its result.
+// A tile with infinities, and one behind the prefix with NaN in V or with K or V too
+// far apart for limbs in common scales, goes in f32, as do those after such a one
+// behind the prefix: its scores come from f32 sums, its weights leave the MFMAs as 0,
+// and then V is added in f32.  (Positions behind the prefix are few, and this is rare.)
+//
+// Bound by what a SIMD can issue: a wave has 96 MFMAs and some 470 vector
+// instructions (limbs, exponentials, maxima, sums) a tile of 32 positions of 128 and
+// 32 rows, and the two overlap in part only: loops of MFMAs for 36.8 ns and vector
+// instructions for 46 take 60.7 together on one SIMD.  8 KV heads of 128 in groups of
+// 4: 49 nodes on 4096 positions 40 us, 64 on 32767 137 us (2.0 TB/s of K and V, 251
+// TFLOP/s of f32 products on three times that of f16 ones, of 1186 that a large
+// product reaches); VALU sums in f32, one wave a row, took 1344 and 14693 us.
 template <int DP, int RB, int NW>
 __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_attn(
     TreeAttn a, int cap, float *__restrict__ part, float *__restrict__ pml) {
@@ -359,7 +371,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
     constexpr int KG = RB == 1 ? 2 : 1, VG = RB == 1 ? 4 : NW == 4 && DP == 128 ? 1 : 2;   // operands read at a time
     __shared__ f16x8 sk[2][KT * 2 * NS * 2 * 64];       // [32 positions][16][32 dims][limb][lane]
     __shared__ f16x8 sv[2][KT * NB * 4 * 2 * 64];       // [32 positions][64 dims][j][limb][lane]
-    __shared__ int se[2][2][NW], bad[2][2][NW];         // K's, V's shares: exponent, for f32
+    // The shares' exponents, K's and V's; V's + kBias again with kSlow where K or V is for f32.
+    __shared__ int se[2][2][NW], sw[2][NW];
     // A share's largest and least exponent of V in the tiles behind the prefix so far.
     __shared__ int behind[2][2][NW];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, g = lane >> 4;
@@ -448,7 +461,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
                 max3_abs(vn, vr[u][i][2], vr[u][i][3]);
             }
         uint32_t kt = max(abs_bits(km), abs_bits(kn)), vt = max(abs_bits(vm), abs_bits(vn));
-        bool slow_k = false, slow_v = false;
+        bool slow = false;
         if (!open) {   // NaN in V too: a row that does not see its position must not get it
             uint32_t k_low = 0, v_low = 0;
 #pragma unroll
@@ -463,13 +476,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
             }
             wave_max_bits(kt, vt);
             wave_max_bits(k_low, v_low);
-            slow_k = spread(exponent(kt), k_low);
-            slow_v = spread(exponent(vt), v_low);
+            slow = spread(exponent(kt), k_low) || spread(exponent(vt), v_low);
         } else {
             wave_max_bits(kt, vt);
         }
-        slow_k |= kt >= kInf;
-        slow_v |= vt >= kInf;
+        slow |= kt >= kInf || vt >= kInf;
         if (__builtin_expect(vt >= kInf, 0)) {   // the largest finite one
             vt = 0;
 #pragma unroll
@@ -489,8 +500,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
             if (tile > t0) {   // what those before it were, it is
                 high = behind[buf ^ 1][0][wave];
                 low = behind[buf ^ 1][1][wave];
-                slow_v |= (tile * TK > len && bad[buf ^ 1][1][wave]) ||
-                          ve - se[buf ^ 1][1][wave] > 20;
+                slow |= (tile * TK > len && sw[buf ^ 1][wave] >= kSlow) ||
+                        ve - se[buf ^ 1][1][wave] > 20;
             }
             high = max(high, ve);
             low = min(low, ve == kLeast ? -kNoV : ve);
@@ -500,8 +511,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
             behind[buf][1][wave] = low;
             se[buf][0][wave] = ke;
             se[buf][1][wave] = ve;
-            bad[buf][0][wave] = slow_k;
-            bad[buf][1][wave] = slow_v;
+            sw[buf][wave] = ve + kBias + (slow ? kSlow : 0);
         }
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
@@ -638,22 +648,24 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
             read_v(0);
             const int ke[2] = {se[buf][0][4 * g / PW], se[buf][0][(16 + 4 * g) / PW]};
             const int ve[2] = {se[buf][1][g], se[buf][1][NW == 4 ? g : 4 + g]};
-            int vtop = se[buf][1][0], slow_k = bad[buf][0][0], slow_v = bad[buf][1][0];
+            int word = sw[buf][0];
 #pragma unroll
-            for (int w = 1; w < NW; ++w) {
-                vtop = max(vtop, se[buf][1][w]);
-                slow_k |= bad[buf][0][w];
-                slow_v |= bad[buf][1][w];
-            }
+            for (int w = 1; w < NW; ++w) word = max(word, sw[buf][w]);
+            word = __builtin_amdgcn_readfirstlane(word);
+            bool slow = word >= kSlow;
+            int vtop = se[buf][1][0];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) vtop = max(vtop, se[buf][1][w]);
             vtop = __builtin_amdgcn_readfirstlane(vtop);
-            slow_k = __builtin_amdgcn_readfirstlane(slow_k);
-            int high = behind[buf][0][0], low = behind[buf][1][0];
+            if (NW == 4 || !open) {   // (a branch has four waves of 32 rows spill 160 registers)
+                int high = behind[buf][0][0], low = behind[buf][1][0];
 #pragma unroll
-            for (int w = 1; w < NW; ++w) {
-                high = max(high, behind[buf][0][w]);
-                low = min(low, behind[buf][1][w]);
+                for (int w = 1; w < NW; ++w) {
+                    high = max(high, behind[buf][0][w]);
+                    low = min(low, behind[buf][1][w]);
+                }
+                slow |= __builtin_amdgcn_readfirstlane(high - low) > 8;
             }
-            slow_v = __builtin_amdgcn_readfirstlane(slow_v | (high - low > 8));
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 const float sx[2] = {ldexpf(f, qe[rb] + ke[0] - 2 * kTop),
@@ -662,7 +674,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
                 for (int j = 0; j < 8 * KT; ++j)
                     s8[rb][j] = acc[rb][j >> 3][j >> 2 & 1][j & 3] * sx[j >> 2 & 1];
             }
-            if (__builtin_expect(slow_k, 0)) {
+            if (__builtin_expect(slow, 0)) {
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb)
                     scores_in_f32<8 * KT>(a, b, kvh, min(w0 + 16 * rb + c, R - 1), p0, end, g,
@@ -682,7 +694,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
                 m[rb] = top > m[rb] + kLag ? top : m[rb];
                 moved |= m[rb] != was[rb];
             }
-            const int down = slow_v ? raise(vtop, oe, oe_top) : rescale(vtop, oe, oe_top);
+            const int down = slow ? raise(vtop, oe, oe_top) : rescale(vtop, oe, oe_top);
             if (__any(moved) || down != 0) {
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
@@ -704,7 +716,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 float top = m[rb] == -INFINITY ? 0.f : m[rb];   // nothing seen: weights 0
-                if (slow_v) top = INFINITY;   // V in f32 below: weights 0 here
+                if (slow) top = INFINITY;   // V in f32 below: weights 0 here
                 const float base[2] = {(float)pe[0] - top, (float)pe[1] - top};
 #pragma unroll
                 for (int sub = 0; sub < KT; ++sub) {
@@ -736,7 +748,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
                         }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (__builtin_expect(slow_v, 0)) {   // weights anew: nothing waits for this in registers
+            if (__builtin_expect(slow, 0)) {   // weights anew: nothing waits for this in registers
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
                     float p[8 * KT];
@@ -1078,12 +1090,17 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
     };
     float top, sum;
 #pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const float x = shares(16 * rb + c, wave, top, sum);
+        l[rb] = l[rb] == 0.f ? 0.f : x / l[rb];
+    }
+#pragma unroll
     for (int w = 0; w < 4; ++w) {
         if (wave == w) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 const int r = 16 * rb + c;
-                const float x = shares(r, w, top, sum), inv = l[rb] == 0.f ? 0.f : 1.0f / l[rb];
+                const float x = l[rb];
 #pragma unroll
                 for (int q = 0; q < NB; ++q)
 #pragma unroll
@@ -1091,10 +1108,10 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
                         float4 *d = reinterpret_cast<float4 *>(&lo[r][64 * q + 16 * g]) + i;
                         float4 y = w ? *d : make_float4(0.f, 0.f, 0.f, 0.f);
                         if (x != 0.f) {
-                            y.x = fmaf(ldexpf(o[rb][q][0][i] * inv, oe - kTop), x, y.x);
-                            y.y = fmaf(ldexpf(o[rb][q][1][i] * inv, oe - kTop), x, y.y);
-                            y.z = fmaf(ldexpf(o[rb][q][2][i] * inv, oe - kTop), x, y.z);
-                            y.w = fmaf(ldexpf(o[rb][q][3][i] * inv, oe - kTop), x, y.w);
+                            y.x += ldexpf(o[rb][q][0][i] * x, oe - kTop);
+                            y.y += ldexpf(o[rb][q][1][i] * x, oe - kTop);
+                            y.z += ldexpf(o[rb][q][2][i] * x, oe - kTop);
+                            y.w += ldexpf(o[rb][q][3][i] * x, oe - kTop);
                         }
                         *d = y;
                     }
