@@ -168,13 +168,18 @@ def test_attention(cuda, B, N, H, KVH, D, lens, S):
 
 
 @pytest.mark.parametrize("N,H,KVH,D,lens,S", [
-    (70, 16, 2, 64, [1000], 131072),       # two tiles of 256 rows, the last one ragged
+    (70, 16, 2, 64, [1000], 131072),
     (40, 16, 4, 64, [0, 2100, 63, 1, 9], 13120),
-    (19, 16, 2, 128, [700], 65600),        # 152 rows: some waves have none
+    (19, 16, 2, 128, [700], 65600),
     (70, 8, 2, 96, [31, 129], 32800),
+    # blocks of eight waves (the ones above are of four: too many of 256 rows would be empty)
+    (28, 16, 2, 64, [1000], 131072),
+    (60, 16, 4, 64, [0, 2100, 63, 1, 9], 13120),
+    (25, 16, 2, 128, [700], 65600),        # 200 rows: some waves have few or none
+    (120, 8, 2, 96, [31, 129], 32800),     # two tiles of rows
 ])
 def test_attention_of_many_rows_over_a_large_cache(cuda, N, H, KVH, D, lens, S):
-    """Blocks of eight waves.  The first K and V rows of every other 4 positions are larger,
+    """Blocks of four and of eight waves.  The first K and V rows of every other 4 positions are larger,
     so that the parts of a tile have scales of their own; one node has infinities."""
     B = len(lens)
     print(f"case tree_attention large cache N={N} H={H}/{KVH} D={D} lens={lens} S={S}", flush=True)
@@ -230,7 +235,7 @@ def test_attention_unseen_positions(cuda, D, N, kv):
 
 
 @pytest.mark.parametrize("D,N,kv,S", [(64, 6, 40, 46), (128, 7, 0, 7), (128, 25, 90, 115),
-                                      (96, 60, 200, 260), (256, 33, 65, 98), (64, 80, 30, 131072)])
+                                      (96, 60, 200, 260), (256, 33, 65, 98), (64, 80, 30, 131072), (64, 60, 30, 131072)])
 @pytest.mark.parametrize("big", [1e6, 3e38])
 def test_attention_large_values_beside_the_path(cuda, D, N, kv, S, big):
     """Nodes whose K and V are very large cost the rows that do not see them no bits, and the

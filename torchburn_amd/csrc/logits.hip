@@ -82,7 +82,11 @@ __device__ float add_biases(float y, int t, const Biases &b) {
 // pass through once, 16 bytes a lane, four loads in flight (a lane whose four
 // tokens the mask excludes reads none).  A word of LDS per token holds what the
 // history, the tree path and the biases say of it; the block reads those lists
-// whole, which is why chunks are as large as the row count lets them be.
+// whole, which is why chunks are as large as the row count lets them be.  64 rows of
+// 128256 tokens with one history of 2048 take 22 us (67 MB, 3.0 TB/s), 192 with one of
+// 1500 each 59 (202 MB, 3.4 TB/s), where a large copy reaches 5.1; chunks half as large
+// change neither, and loads ahead of the lists win 0.7 us on the first and lose 2 on the
+// second.
 // Vectors start where the row's address is a multiple of 16 bytes, `lead` tokens
 // into it; LDS word 4 is the chunk's first vector, the words before it are chunk
 // 0's tokens ahead of that.  The last vector may be cut.

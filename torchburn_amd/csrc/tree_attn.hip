@@ -320,7 +320,8 @@ __device__ __forceinline__ int raise(int ve, int &oe, int &oe_top) {
 __host__ __device__ constexpr int tile_of(int dp) { return dp == 64 ? 64 : 32; }
 // Tiles per split where at most `cap` splits are wanted.  Only the sequence's own
 // length counts, so that within one plan a result is the same whatever the bound.
-// With 2 or 8 tiles at least, 49 nodes on 512 positions take 3 and 6 us longer.
+// us with 2 / 4 / 8 tiles at least, groups of 4 heads of 128: 60 nodes on 512 positions
+// 25 / 26 / 34, 32 on 4096 38 / 34 / 36; groups of 7 heads of 64, 16 on 1000 21 / 21 / 31.
 constexpr int kMinTiles = 4;
 __host__ __device__ inline int tiles_per_split(int tiles, int cap) {
     const int t = (tiles + cap - 1) / cap;
@@ -822,7 +823,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
 // in the loop waits for another wave.  The next tile's K is requested when this
 // one's scores are on their way, its V when this one's limbs are built.  Every K and
 // V row is read once: non-temporal loads (8 rows of each KV head over 32775 positions of
-// 8 heads of 128: 62 us, 67 with ordinary ones).
+// 8 heads of 128: 62 us and 4.3 TB/s, 67 with ordinary ones).  Bound by the loads that
+// its waves keep on their way, and on short caches by the two launches: 8 nodes on
+// 4096 positions take 27 us, 1 node 21.
 template <int DP, int RB>
 __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
                                                           float *__restrict__ part,
@@ -1143,7 +1146,8 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
 // wave works out every split's share (lane s: splits s and s + 64); the columns are taken by
 // 256 / LC groups of LC lanes, group i with the splits i, i + 256 / LC, ...  The first
 // of those are requested before the weights are known: every split's place in the
-// scratch can be read, and what was not written has weight 0.
+// scratch can be read, and what was not written has weight 0.  Bound by the launch and
+// the way of those reads: 7.1 us for 1568 rows of 26 splits, 8.6 for 2048 of 32.
 template <int LC>
 __global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int tk, int cap, int nsplit,
                                                     const float *__restrict__ part,
@@ -1234,9 +1238,11 @@ Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len) {
     p.tk = p.few ? 32 : tile_of(p.dp);
     const int tiles = (max_len + p.tk - 1) / p.tk;
     // Eight waves build a tile's limbs for 256 rows, half as much a row, where that leaves
-    // each of 256 blocks 16 tiles.  us with four / eight, 8 heads of 128 and groups of 4: 64
-    // nodes on 32767 180 / 164, 60 on 16384 94 / 92, on 4096 45.4 / 45.9, on 1024 28 / 33.
-    p.nw = p.rb == 2 && R > 128 && (int64_t)tiles * hkv * batch >= 16 * 256 ? 8 : 4;
+    // each of 256 blocks 16 tiles and few of the rows empty.  us with four / eight, 8 heads of
+    // 128 and groups of 4: 64 nodes on 32767 positions 180 / 164, 60 on 16384 94 / 92, on
+    // 4096 45.4 / 45.9, on 1024 28 / 33; groups of 7, 12 sequences of 21 nodes (147 rows) on
+    // up to 6000 142 / 147.
+    p.nw = p.rb == 2 && (R + 63) / 64 % 4 == 0 && (int64_t)tiles * hkv * batch >= 16 * 256 ? 8 : 4;
     const int rows = 16 * p.rb * p.nw;
     p.rtiles = p.few ? 1 : (R + rows - 1) / rows;
     // As many blocks as run at once: two per CU, or one where registers or LDS allow one
