@@ -250,13 +250,23 @@ __device__ __forceinline__ void scores_in_f32(const TreeAttn &a, int b, int kvh,
     i = fresh(i);
     const float *q = a.q + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D;
     const float *kb = a.k.p + b * a.k.sb + kvh * a.k.sh;
+    uint32_t off[N];   // in 16-byte units from the tile's first row
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        const float *k = kb + min(p0 + position(j, g), end - 1) * a.k.ss;
-        float s = 0.f;
-        for (int d = 0; d < D; ++d) s = fmaf(q[d], k[d], s);
-        s8[j] = s * a.scale * kLog2e;
+        off[j] = min(position(j, g), end - 1 - p0) * (uint32_t)(a.k.ss / 4);
+        s8[j] = 0.f;
     }
+    const float4 *k = reinterpret_cast<const float4 *>(kb + p0 * a.k.ss);
+    for (int d = 0; d < D / 4; ++d) {
+        const float4 x = reinterpret_cast<const float4 *>(q)[d];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float4 y = k[off[j] + d];
+            s8[j] = fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, fmaf(x.x, y.x, s8[j]))));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) s8[j] *= a.scale * kLog2e;
 }
 
 // The least exponent of a weight's scale.  Where V is that small against the outputs'
@@ -353,7 +363,8 @@ __host__ __device__ inline int tiles_per_split(int tiles, int cap) {
 // A tile with infinities, and one behind the prefix with NaN in V or with K or V too
 // far apart for limbs in common scales, goes in f32, as do those after such a one
 // behind the prefix: its scores come from f32 sums, its weights leave the MFMAs as 0,
-// and then V is added in f32.  (Positions behind the prefix are few, and this is rare.)
+// and then V is added in f32.  (Positions behind the prefix are few, and this is rare:
+// 49 nodes on 4096 positions take 259 us with such a node and 45 without.)
 //
 // Bound by what a SIMD can issue: a wave has 96 MFMAs and some 470 vector
 // instructions (limbs, exponentials, maxima, sums) a tile of 32 positions of 128 and
