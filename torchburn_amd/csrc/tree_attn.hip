@@ -329,7 +329,8 @@ __device__ __forceinline__ int raise(int ve, int &oe, int &oe_top) {
 // Positions per tile: the same bytes for every head_dim up to 128.
 __host__ __device__ constexpr int tile_of(int dp) { return dp == 64 ? 64 : 32; }
 // Tiles per split where at most `cap` splits are wanted.  Only the sequence's own
-// length counts, so that within one plan a result is the same whatever the bound.
+// length counts, so that within one plan a result is the same whatever the bound and
+// the batch.
 // us with 2 / 4 / 8 tiles at least, groups of 4 heads of 128: 60 nodes on 512 positions
 // 25 / 26 / 34, 32 on 4096 38 / 34 / 36; groups of 7 heads of 64, 16 on 1000 21 / 21 / 31.
 constexpr int kMinTiles = 4;
@@ -389,8 +390,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
     __shared__ int behind[2][2][NW];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, g = lane >> 4;
     const int G = a.hq / a.hkv, R = a.n * G, D = a.hd, words = (a.n + 31) / 32;
-    const int split = blockIdx.x, kvh = blockIdx.y % a.hkv, b = blockIdx.z;
-    const int w0 = (blockIdx.y / a.hkv * NW + wave) * 16 * RB;   // the wave's first row
+    const int split = blockIdx.y, kvh = blockIdx.x % a.hkv, b = blockIdx.z;
+    const int w0 = ((int)blockIdx.x / a.hkv * NW + wave) * 16 * RB;   // the wave's first row
     const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
     const int tiles = (end + TK - 1) / TK, tps = tiles_per_split(tiles, cap);
     const int t0 = split * tps, t1 = min(tiles, t0 + tps);
@@ -803,7 +804,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
         const int i = w0 + 16 * rb + c;
         const float sum = live[rb] ? sum_over_groups(l[rb]) : 0.f;
         if (i >= R) continue;
-        const size_t at = (((size_t)b * a.hkv + kvh) * gridDim.x + split) * R + i;
+        const size_t at = (((size_t)b * a.hkv + kvh) * gridDim.y + split) * R + i;
         float *to = part ? part + at * D   // normalised, so that the largest V do not overflow
                          : a.out + (((size_t)b * a.n + i / G) * a.hq + kvh * G + i % G) * D;
         const float x = sum == 0.f ? 0.f : 1.0f / sum;
@@ -846,7 +847,7 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
     __shared__ float lm[4][ROWS], ls[4][ROWS];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, g = lane >> 4;
     const int G = a.hq / a.hkv, R = a.n * G, D = a.hd, words = (a.n + 31) / 32;
-    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    const int split = blockIdx.y, kvh = blockIdx.x, b = blockIdx.z;
     const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
     const int tiles = (end + TK - 1) / TK, tps = tiles_per_split(tiles, cap);
     const int t0 = split * tps, t1 = min(tiles, t0 + tps);
@@ -1139,7 +1140,7 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
         if (r >= R) break;
         const float4 y = *reinterpret_cast<const float4 *>(&lo[r][4 * d]);
         if (part) {
-            const size_t at = (((size_t)b * a.hkv + kvh) * gridDim.x + split) * R + r;
+            const size_t at = (((size_t)b * a.hkv + kvh) * gridDim.y + split) * R + r;
             reinterpret_cast<float4 *>(part + at * D)[d] = y;
             if (d == 0) {
                 shares(r, 0, top, sum);
@@ -1278,7 +1279,10 @@ int launch_tree_attention(const TreeAttn &a, int max_len, float *scratch, hipStr
     const Plan p = plan(a.batch, a.n, a.hq, a.hkv, a.hd, max_len);
     float *part = p.nsplit > 1 ? scratch : nullptr;
     float *pml = part ? part + (size_t)a.batch * a.hq * a.n * p.nsplit * a.hd : nullptr;
-    const dim3 grid(p.nsplit, a.hkv * p.rtiles, a.batch);
+    // Heads first: the row tiles of a KV head, which read the same K and V, on one of the
+    // eight dies (block i goes to die i % 8), and the splits that a sequence has not on all of
+    // them.  Splits first, 24 nodes on 4096 positions of 8 heads take 31.7 us instead of 28.3.
+    const dim3 grid(a.hkv * p.rtiles, p.nsplit, a.batch);
 #define TB_TF(DP, RB)                                                                        \
     if (p.few && p.dp == DP && p.rb == RB)                                                   \
     hipLaunchKernelGGL((k_tree_attn_few<DP, RB>), grid, dim3(256), 0, s, a, p.cap, part, pml)
