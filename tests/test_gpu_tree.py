@@ -357,6 +357,19 @@ def test_attention_lengths_are_clamped(cuda):
         tb.tree_attention(T(q), T(k), T(v), T(words(bits)), 45)
 
 
+def test_indices_past_32_bits(cuda):
+    """int64 parents and lengths that int32 does not hold are padding and clamped lengths."""
+    print("case int64 parents and lengths", flush=True)
+    par = torch.tensor([-1, 0, 1 << 32, (1 << 32) - 1, 2, -(1 << 40), 1], device=cuda)
+    mask, depth = tb.tree_masks(par)
+    assert mask[:, 0].tolist() == [1, 3, 0, 0, 0, 0, 67] and depth.tolist() == [0, 1, 0, 0, 0, 0, 2]
+    q, k, v, bits = inputs(2, 2, 5, 4, 2, 64, 20)
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    a = [T(q), T(k), T(v), T(words(bits))]
+    far = tb.tree_attention(*a, torch.tensor([(1 << 32) + 3, -(1 << 33)], device=cuda))
+    assert torch.equal(far, tb.tree_attention(*a, torch.tensor([20, 0], device=cuda)))
+
+
 def test_attention_empty(cuda):
     print("case tree_attention empty", flush=True)
     z = lambda *s: torch.zeros(s, device=cuda)

@@ -367,9 +367,9 @@ __host__ __device__ inline int tiles_per_split(int tiles, int cap) {
 // and then V is added in f32.  (Positions behind the prefix are few, and this is rare:
 // 49 nodes on 4096 positions take 259 us with such a node and 45 without.)
 //
-// Bound by what a SIMD can issue: a wave has 96 MFMAs and some 470 vector
-// instructions (limbs, exponentials, maxima, sums) a tile of 32 positions of 128 and
-// 32 rows, and the two overlap in part only: loops of MFMAs for 36.8 ns and vector
+// Bound by what a SIMD can issue: a wave has 96 MFMAs and 410 to 470 vector
+// instructions (limbs, exponentials, maxima, sums; eight waves, four) a tile of 32
+// positions of 128 and 32 rows, and the two overlap in part only: loops of MFMAs for 36.8 ns and vector
 // instructions for 46 take 60.7 together on one SIMD.  8 KV heads of 128 in groups of
 // 4: 49 nodes on 4096 positions 40 us, 64 on 32767 137 us (2.0 TB/s of K and V, 251
 // TFLOP/s of f32 products on three times that of f16 ones, of 1186 that a large

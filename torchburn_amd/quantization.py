@@ -37,6 +37,14 @@ def _on_gpu(t: Optional[torch.Tensor], dtype: torch.dtype, dev: torch.device):
     return t.contiguous()
 
 
+def _int32_on_gpu(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """Indices and lengths as int32: what int64 holds past its range becomes the nearest
+    value, not another index."""
+    if t.dtype is torch.int64:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1)
+    return _on_gpu(t, torch.int32, dev)
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

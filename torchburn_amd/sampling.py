@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._lib import UnsupportedOpError
-from .quantization import _on_gpu, _ptr, _stream, _target
+from .quantization import _int32_on_gpu, _on_gpu, _ptr, _stream, _target
 
 
 def sample_uniform(seed: int, counter: int) -> float:
@@ -69,7 +69,7 @@ def _lengths(op: str, name: str, t, groups: int, dev):
         return None, int(t)
     if t.numel() != groups:
         raise _bad(op, f"{name} must have {groups} elements, got {list(t.shape)}")
-    return _on_gpu(t.reshape(-1), torch.int32, dev), 0
+    return _int32_on_gpu(t.reshape(-1), dev), 0
 
 
 def _penalty(op: str, name: str, t, rows: int, dev):

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import UnsupportedOpError
-from .quantization import _on_gpu, _ptr, _stream, _target, _write_back
+from .quantization import _int32_on_gpu, _on_gpu, _ptr, _stream, _target, _write_back
 
 
 _dtype = attrgetter("dtype")
@@ -34,7 +34,7 @@ def _trees(op: str, t: torch.Tensor, dtype, dev) -> torch.Tensor:
     """Per-node values (n,) or (batch, n) as a device tensor."""
     if t.ndim not in (1, 2):
         raise _bad(op, f"trees must be (n,) or (batch, n), got {list(t.shape)}")
-    return _on_gpu(t, dtype, dev)
+    return _int32_on_gpu(t, dev) if dtype is torch.int32 else _on_gpu(t, dtype, dev)
 
 
 def _cache(op: str, name: str, c: torch.Tensor, batched: bool, dev: torch.device) -> torch.Tensor:
@@ -58,7 +58,7 @@ def _kv_len(op: str, kv_len, batch: int, dev) -> Tuple[Optional[torch.Tensor], i
         return None, int(kv_len)
     if kv_len.numel() != batch:
         raise _bad(op, f"kv_len must have {batch} elements, got {list(kv_len.shape)}")
-    return _on_gpu(kv_len.reshape(-1), torch.int32, dev), 0
+    return _int32_on_gpu(kv_len.reshape(-1), dev), 0
 
 
 def tree_masks(parents: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
