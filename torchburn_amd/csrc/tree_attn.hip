@@ -369,9 +369,9 @@ __host__ __device__ inline int tiles_per_split(int tiles, int cap) {
 //
 // Bound by what a SIMD can issue: a wave has 96 MFMAs and 410 to 470 vector
 // instructions (limbs, exponentials, maxima, sums; eight waves, four) a tile of 32
-// positions of 128 and 32 rows, and the two overlap in part only: loops of MFMAs for 36.8 ns and vector
-// instructions for 46 take 60.7 together on one SIMD.  8 KV heads of 128 in groups of
-// 4: 49 nodes on 4096 positions 40 us, 64 on 32767 137 us (2.0 TB/s of K and V, 251
+// positions of 128 and 32 rows, and the two overlap in part only: loops of MFMAs for
+// 36.8 ns and vector instructions for 46 take 60.7 together on one SIMD.  8 KV heads
+// of 128 in groups of 4: 49 nodes on 4096 positions 40 us, 64 on 32767 137 us (2.0 TB/s of K and V, 251
 // TFLOP/s of f32 products on three times that of f16 ones, of 1186 that a large
 // product reaches); VALU sums in f32, one wave a row, took 1344 and 14693 us.
 template <int DP, int RB, int NW>
@@ -381,7 +381,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
     constexpr int PW = 32 / NW, LX = 16 / PW;   // K positions a wave, operands of one side by side
     constexpr int KU = KT * NS / LX;            // K operands (8 values) a lane
     constexpr int VU = KT * NB / 2, VP = 16 / NW;   // V: columns of 4 a lane, positions of each
-    constexpr int KG = RB == 1 ? 2 : 1, VG = RB == 1 ? 4 : NW == 4 && DP == 128 ? 1 : 2;   // operands read at a time
+    // Operands read at a time.  (With 2 of V the four-wave block of 32 rows and 128 dimensions
+    // spills 149 registers, with 1 it spills 4.)
+    constexpr int KG = RB == 1 ? 2 : 1, VG = RB == 1 ? 4 : NW == 4 && DP == 128 ? 1 : 2;
     __shared__ f16x8 sk[2][KT * 2 * NS * 2 * 64];       // [32 positions][16][32 dims][limb][lane]
     __shared__ f16x8 sv[2][KT * NB * 4 * 2 * 64];       // [32 positions][64 dims][j][limb][lane]
     // The shares' exponents, K's and V's; V's + kBias again with kSlow where K or V is for f32.
