@@ -328,15 +328,23 @@ __device__ __forceinline__ int raise(int ve, int &oe, int &oe_top) {
 
 // Positions per tile: the same bytes for every head_dim up to 128.
 __host__ __device__ constexpr int tile_of(int dp) { return dp == 64 ? 64 : 32; }
-// Tiles per split where at most `cap` splits are wanted.  Only the sequence's own
-// length counts, so that within one plan a result is the same whatever the bound and
-// the batch.
-// us with 2 / 4 / 8 tiles at least, groups of 4 heads of 128: 60 nodes on 512 positions
-// 25 / 26 / 34, 32 on 4096 38 / 34 / 36; groups of 7 heads of 64, 16 on 1000 21 / 21 / 31.
+// A split's tiles t0 .. t1 - 1 of a sequence, and how many splits it has where at most
+// `cap` are wanted.  Tiles behind the prefix, whose masks are read and applied, count
+// twice: they take 6 us where others take 3, and the splits that have them would end
+// last (49 nodes on 4096 positions: at 36 us, the others at 28; a call 40.9 us, so 39.6).  Only the sequence's own
+// lengths count, so that within one plan a result is the same whatever the bound and
+// the batch.  us with 2 / 4 / 8 at least, groups of 4 heads of 128: 60 nodes on 512
+// positions 25 / 26 / 34, 32 on 4096 38 / 34 / 36; groups of 7 heads of 64, 16 on 1000
+// 21 / 21 / 31.
 constexpr int kMinTiles = 4;
-__host__ __device__ inline int tiles_per_split(int tiles, int cap) {
-    const int t = (tiles + cap - 1) / cap;
-    return t < kMinTiles ? kMinTiles : t;
+struct Range {
+    int t0, t1, splits;
+};
+__device__ __forceinline__ Range split_range(int len, int end, int tk, int cap, int split) {
+    const int tiles = (end + tk - 1) / tk, open = min(len / tk, tiles), units = 2 * tiles - open;
+    const int each = max((units + cap - 1) / cap, kMinTiles);
+    auto tile = [&](int unit) { return unit <= open ? unit : open + (unit - open) / 2; };
+    return {tile(split * each), tile(min(units, (split + 1) * each)), (units + each - 1) / each};
 }
 
 // A block of NW waves takes 16 * RB * NW query rows of one KV head, a row being a
@@ -395,9 +403,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
     const int split = blockIdx.y, kvh = blockIdx.x % a.hkv, b = blockIdx.z;
     const int w0 = ((int)blockIdx.x / a.hkv * NW + wave) * 16 * RB;   // the wave's first row
     const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
-    const int tiles = (end + TK - 1) / TK, tps = tiles_per_split(tiles, cap);
-    const int t0 = split * tps, t1 = min(tiles, t0 + tps);
-    if (split > 0 && t0 >= t1) return;   // the merge skips this split
+    const Range range = split_range(len, end, TK, cap, split);
+    const int t0 = range.t0, t1 = range.t1;
+    if (split > 0 && split >= range.splits) return;   // the merge skips this split
     const float *kb = a.k.p + b * a.k.sb + kvh * a.k.sh, *vb = a.v.p + b * a.v.sb + kvh * a.v.sh;
 
     // ---- this thread's part of a tile: operand (sub, s) of K position kpos, column (sub, q)
@@ -851,9 +859,9 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
     const int G = a.hq / a.hkv, R = a.n * G, D = a.hd, words = (a.n + 31) / 32;
     const int split = blockIdx.y, kvh = blockIdx.x, b = blockIdx.z;
     const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
-    const int tiles = (end + TK - 1) / TK, tps = tiles_per_split(tiles, cap);
-    const int t0 = split * tps, t1 = min(tiles, t0 + tps);
-    if (split > 0 && t0 >= t1) return;   // the merge skips this split
+    const Range range = split_range(len, end, TK, cap, split);
+    const int t0 = range.t0, t1 = range.t1;
+    if (split > 0 && split >= range.splits) return;   // the merge skips this split
     const float *kb = a.k.p + b * a.k.sb + kvh * a.k.sh, *vb = a.v.p + b * a.v.sb + kvh * a.v.sh;
     const int32_t *mask = a.mask + b * a.mask_sb;
 
@@ -1187,8 +1195,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int tk, int cap,
         l[x] = p[1];
     }
     const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
-    const int tiles = (end + tk - 1) / tk, tps = tiles_per_split(tiles, cap);
-    const int used = (tiles + tps - 1) / tps;
+    const int used = split_range(len, end, tk, cap, 0).splits;
 #pragma unroll
     for (int x = 0; x < 2; ++x)
         if (lane + 64 * x >= used) m[x] = -INFINITY;
@@ -1266,7 +1273,9 @@ Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len) {
     const int64_t want = (p.few || p.nw == 8 || p.dp == 256 ? 256 : 512) /
                          ((int64_t)p.rtiles * hkv * batch);
     p.cap = (int)std::max<int64_t>(1, std::min<int64_t>(want, kMaxSplits));
-    p.nsplit = std::max(1, std::min(p.cap, (tiles + kMinTiles - 1) / kMinTiles));
+    const int units = tiles + (n + p.tk - 1) / p.tk + 1;   // of a sequence at most (split_range)
+    if (tiles <= kMinTiles) p.cap = 1;
+    p.nsplit = std::max(1, std::min(p.cap, (units + kMinTiles - 1) / kMinTiles));
     return p;
 }
 
