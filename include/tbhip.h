@@ -407,8 +407,8 @@ TB_API int tb_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, 
  * contiguous; mask_sb words between the sequences' masks (0: one mask for all).
  * kv_lens: device i32 [batch], clamped to [0, max_seq] (nodes past the cache's
  * end do not exist), or NULL: kv_len for every sequence, and TB_ERR_VALUE when
- * kv_len + n > max_seq.  The two may differ in their last bits on long caches:
- * the work is split by the length that the call knows.  head_dim a multiple of 32
+ * kv_len + n > max_seq.  The two may differ in their last bits: the work is split
+ * by the length that the call knows.  head_dim a multiple of 32
  * up to 256, num_heads up to 1024, positions up to 2^27 elements apart; q, out
  * and the caches 16-byte aligned.
  * scratch: tb_tree_attention_scratch bytes of device memory, 16-byte aligned

@@ -331,11 +331,11 @@ __host__ __device__ constexpr int tile_of(int dp) { return dp == 64 ? 64 : 32; }
 // A split's tiles t0 .. t1 - 1 of a sequence, and how many splits it has where at most
 // `cap` are wanted.  Tiles behind the prefix, whose masks are read and applied, count
 // twice: they take 6 us where others take 3, and the splits that have them would end
-// last (49 nodes on 4096 positions: at 36 us, the others at 28; a call 40.9 us, so 39.6).  Only the sequence's own
-// lengths count, so that within one plan a result is the same whatever the bound and
-// the batch.  us with 2 / 4 / 8 at least, groups of 4 heads of 128: 60 nodes on 512
-// positions 25 / 26 / 34, 32 on 4096 38 / 34 / 36; groups of 7 heads of 64, 16 on 1000
-// 21 / 21 / 31.
+// last (49 nodes on 4096 positions: at 36 us, the others at 28; a call 40.9 us, so
+// 39.6).  Only the sequence's own lengths count, so that within one plan a result is
+// the same whatever the bound and the batch.  us with 2 / 4 / 8 tiles at least, groups
+// of 4 heads of 128: 60 nodes on 512 positions 25 / 26 / 34, 32 on 4096 38 / 34 / 36;
+// groups of 7 heads of 64, 16 on 1000 21 / 21 / 31.
 constexpr int kMinTiles = 4;
 struct Range {
     int t0, t1, splits;

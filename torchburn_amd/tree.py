@@ -88,8 +88,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     for every bit j of its row, and a row without bits gives zeros.  Positions that a row
     does not see take no part, whatever the caches hold there.  ``kv_len`` is a number
     (ValueError when kv_len + n exceeds max_seq) or a tensor with one per sequence (clamped
-    on the device); the two may differ in their last bits on long caches, where the work is
-    split by the length known at the call.  ``scale`` defaults to head_dim ** -0.5.  f32, in q's shape; caches may
+    on the device); the two may differ in their last bits, since the work is split by the
+    length known at the call.  ``scale`` defaults to head_dim ** -0.5.  f32, in q's shape; caches may
     have any strides of 16-byte rows.  Does not wait for the device."""
     op = "tree_attention"
     if q.ndim not in (3, 4):
