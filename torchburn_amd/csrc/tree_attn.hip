@@ -401,7 +401,10 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, g = lane >> 4;
     const int G = a.hq / a.hkv, R = a.n * G, D = a.hd, words = (a.n + 31) / 32;
     const int split = blockIdx.y, kvh = blockIdx.x % a.hkv, b = blockIdx.z;
-    const int w0 = ((int)blockIdx.x / a.hkv * NW + wave) * 16 * RB;   // the wave's first row
+    // The row tile: the last one, which may be mostly empty, is another block's in every split,
+    // or some dies would have nothing else (12 sequences, 147 rows 147 us instead of 137).
+    const int rtiles = gridDim.x / a.hkv, rtile = ((int)blockIdx.x / a.hkv + split + b) % rtiles;
+    const int w0 = (rtile * NW + wave) * 16 * RB;   // the wave's first row
     const int len = prefix_len(a.kv_lens, a.kv_len, b, a.max_seq), end = min(len + a.n, a.max_seq);
     const Range range = split_range(len, end, TK, cap, split);
     const int t0 = range.t0, t1 = range.t1;
@@ -1250,7 +1253,7 @@ struct Plan {
     int dp, rb, nw, tk, rtiles, cap, nsplit;
 };
 
-Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len) {
+Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len, bool ragged) {
     Plan p;
     p.dp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
     const int R = n * (hq / hkv);
@@ -1273,6 +1276,12 @@ Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len) {
     const int64_t want = (p.few || p.nw == 8 || p.dp == 256 ? 256 : 512) /
                          ((int64_t)p.rtiles * hkv * batch);
     p.cap = (int)std::max<int64_t>(1, std::min<int64_t>(want, kMaxSplits));
+    // Twice as many for sequences of different lengths where the longest's splits would still
+    // have 16 tiles: the call ends with them.  us without / with: 12 sequences of up to 6000
+    // positions, 147 rows (38 tiles) 148 / 136, 28 rows of up to 3000 (47) 72 / 70; 8 of up to
+    // 6000, 64 rows (23) 76 / 78, 4 of them, 128 rows (12) 61 / 74; equal lengths gain nothing
+    // (12 of 6123, 147 rows 174 / 202) and are better given as a number.
+    if (ragged && batch > 1 && tiles >= 32 * p.cap) p.cap = std::min(2 * p.cap, kMaxSplits);
     const int units = tiles + (n + p.tk - 1) / p.tk + 1;   // of a sequence at most (split_range)
     if (tiles <= kMinTiles) p.cap = 1;
     p.nsplit = std::max(1, std::min(p.cap, (units + kMinTiles - 1) / kMinTiles));
@@ -1282,12 +1291,12 @@ Plan plan(int batch, int n, int hq, int hkv, int hd, int max_len) {
 }  // namespace
 
 size_t tree_attention_scratch(int batch, int n, int hq, int hkv, int hd, int max_len) {
-    const int ns = plan(batch, n, hq, hkv, hd, max_len).nsplit;
+    const int ns = plan(batch, n, hq, hkv, hd, max_len, true).nsplit;   // the more of the two
     return ns > 1 ? (size_t)batch * hq * n * ns * (hd + 2) * sizeof(float) : 0;
 }
 
 int launch_tree_attention(const TreeAttn &a, int max_len, float *scratch, hipStream_t s) {
-    const Plan p = plan(a.batch, a.n, a.hq, a.hkv, a.hd, max_len);
+    const Plan p = plan(a.batch, a.n, a.hq, a.hkv, a.hd, max_len, a.kv_lens != nullptr);
     float *part = p.nsplit > 1 ? scratch : nullptr;
     float *pml = part ? part + (size_t)a.batch * a.hq * a.n * p.nsplit * a.hd : nullptr;
     // Heads first: the row tiles of a KV head, which read the same K and V, on one of the
