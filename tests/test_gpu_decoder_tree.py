@@ -168,9 +168,13 @@ def test_tree_refusals(cuda):
             dec.accept_tree(0, toks, par, [0] * len(toks))
         with pytest.raises(ValueError):
             dec.tree_step(0, toks, par)
-    for start in (-1, 19, 20):
+    for start in (-1, 19, 20, 2 ** 63 - 1):
         with pytest.raises(ValueError):
             dec.verify_tree(start, [1, 2], [-1, 0])
+        with pytest.raises(ValueError):
+            dec.accept_tree(start, [1, 2], [-1, 0], [0, 0])
+        with pytest.raises(ValueError):
+            dec.tree_step(start, [1, 2], [-1, 0])
     with pytest.raises(ValueError):
         dec.accept_tree(0, [1, 2], [-1, 0], [0])
     with pytest.raises(ValueError):

@@ -894,6 +894,9 @@ struct Decoder {
 
     // Whether trees of n nodes from start can be run forward.
     int tree_runs(int64_t start, int64_t n) const {
+        TB_REQUIRE(n >= 0 && n <= kMaxTreeNodes && start >= 0 && start <= max_seq - n, TB_ERR_VALUE,
+                   "tree of " + std::to_string(n) + " nodes at " + std::to_string(start) +
+                       " exceeds max_seq_len or " + std::to_string(kMaxTreeNodes) + " nodes");
         TB_REQUIRE(under_cap(start, n), TB_ERR_UNSUPPORTED,
                    "TB_UNSUPPORTED: a tree's positions must lie below the attention cap");
         TB_REQUIRE(!a8_wanted(), TB_ERR_UNSUPPORTED,
@@ -911,7 +914,7 @@ struct Decoder {
         TB_REQUIRE(n >= 1 && n <= kMaxTreeNodes, TB_ERR_VALUE,
                    "tree of " + std::to_string(n) + " nodes outside 1.." +
                        std::to_string(kMaxTreeNodes));
-        TB_REQUIRE(start >= 0 && start + n <= max_seq, TB_ERR_VALUE, "tree exceeds max_seq_len");
+        TB_REQUIRE(start >= 0 && start <= max_seq - n, TB_ERR_VALUE, "tree exceeds max_seq_len");
         for (int64_t i = 0; i < n; ++i) {
             TB_REQUIRE(parents[i] >= -1 && parents[i] < i && (i || parents[i] == -1), TB_ERR_VALUE,
                        "tree node " + std::to_string(i) + ": parent " + std::to_string(parents[i]) +
