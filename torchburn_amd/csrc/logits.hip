@@ -25,7 +25,7 @@ constexpr int kThreads = 512;
 constexpr uint32_t kSeen = 1u << 31;   // of a token's LDS word: occurs in the history
 constexpr uint32_t kBias = 1u << 30;   // has a bias; the rest: its count
 constexpr uint32_t kCount = kBias - 1;
-constexpr int kBiasList = 512;         // biases of one block kept in LDS
+constexpr int kBiasList = kThreads;    // biases of one block kept in LDS
 
 // Orders as the values do, ties to the lower index; 0: nothing to take.
 __device__ __forceinline__ uint64_t best_item(float y, int t) {
@@ -45,48 +45,20 @@ __device__ __forceinline__ uint64_t max_over_wave(uint64_t v) {
 }
 
 struct Biases {
-    const int64_t *ids;
-    const float *val;
-    int n;              // entries of the row's list
-    int at[kBiasList], token[kBiasList];   // those of the block's tokens, in any order
-    int count;          // how many there are (past kBiasList: not listed)
+    int at[kBiasList], token[kBiasList];   // the entries of the block's tokens
+    int count;                             // how many there are (past kBiasList: not all listed)
 };
-
-// Token t's biases added to y in the order of the list.
-__device__ float add_biases(float y, int t, const Biases &b) {
-    float s = 0.f;
-    bool any = false;
-    if (b.count <= kBiasList) {
-        for (int last = -1;;) {   // the lowest entry past the last one taken
-            int next = b.n;
-            for (int j = 0; j < b.count; ++j) {
-                const int i = b.at[j];
-                if (b.token[j] == t && i > last && i < next) next = i;
-            }
-            if (next == b.n) break;
-            s = any ? __fadd_rn(s, b.val[next]) : b.val[next];
-            any = true;
-            last = next;
-        }
-    } else {
-        for (int i = 0; i < b.n; ++i)
-            if (b.ids[i] == t) {
-                s = any ? __fadd_rn(s, b.val[i]) : b.val[i];
-                any = true;
-            }
-    }
-    return any ? __fadd_rn(y, s) : y;
-}
 
 // One block per row and chunk of the vocabulary.  Bound by the logits' bytes: they
 // pass through once, 16 bytes a lane, four loads in flight (a lane whose four
 // tokens the mask excludes reads none).  A word of LDS per token holds what the
-// history, the tree path and the biases say of it; the block reads those lists
+// history, the tree path and the biases say of it (tokens with a bias are left to a
+// second pass, a thread for each: 200 biases of one block of 1500 tokens take 30 us,
+// 180 where the threads that meet such tokens look them up); the block reads those lists
 // whole, which is why chunks are as large as the row count lets them be.  64 rows of
-// 128256 tokens with one history of 2048 take 22 us (67 MB, 3.0 TB/s), 192 with one of
-// 1500 each 59 (202 MB, 3.4 TB/s), where a large copy reaches 5.1; chunks half as large
-// change neither, and loads ahead of the lists win 0.7 us on the first and lose 2 on the
-// second.
+// 128256 tokens with one history of 2048 take 17.6 us (67 MB, 3.8 TB/s), 192 with one of
+// 1500 and 64 biases each 53 (202 MB, 3.8 TB/s), where a large copy reaches 5.1; chunks
+// half as large change neither.
 // Vectors start where the row's address is a multiple of 16 bytes, `lead` tokens
 // into it; LDS word 4 is the chunk's first vector, the words before it are chunk
 // 0's tokens ahead of that.  The last vector may be cut.
@@ -132,11 +104,6 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, 
     if (p.n_bias) {
         const size_t g = r / (p.rows / p.bias_groups);
         const int64_t *ids = p.bias_ids + g * p.n_bias;
-        if (tid == 0) {
-            bias.ids = ids;
-            bias.val = p.bias + g * p.n_bias;
-            bias.n = p.n_bias;
-        }
         for (int i = tid; i < p.n_bias; i += kThreads) {
             const int64_t t = ids[i];
             if (t < t0 || t >= t1) continue;
@@ -155,18 +122,21 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, 
     const uint32_t *allow =
         p.allowed ? reinterpret_cast<const uint32_t *>(p.allowed) + r * p.allowed_stride : nullptr;
     uint64_t best = 0;
+    auto penalised = [&](float v, uint32_t w) {
+        if (w & ~kBias) v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+        const uint32_t n = w & kCount;
+        return n ? __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)n)), pres) : v;
+    };
+    auto candidate = [&](float v, int t) {
+        if (!part) return;
+        const uint64_t it = best_item(v, t);
+        best = it > best ? it : best;
+    };
     auto one = [&](float v, int t, uint32_t w, bool ok) {
-        if (w) {
-            if (w & ~kBias) v = v > 0.f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-            const uint32_t n = w & kCount;
-            if (n) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)n)), pres);
-            if (w & kBias) v = add_biases(v, t, bias);
-        }
+        if (ok && (w & kBias)) return v;   // as it is, for the second pass
+        if (w) v = penalised(v, w);
         v = ok ? v : -INFINITY;
-        if (part) {
-            const uint64_t it = best_item(v, t);
-            best = it > best ? it : best;
-        }
+        candidate(v, t);
         return v;
     };
     auto scalar = [&](int t) {
@@ -221,6 +191,48 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, 
         if (rest + tid < t1) scalar(rest + tid);
     } else {
         for (int t = t0 + tid; t < t1; t += kThreads) scalar(t);
+    }
+    if (p.n_bias) {
+        __syncthreads();
+        // The first entry of a token adds up all of its entries, in the order of the list.
+        auto biased = [&](int n, int j, auto token, auto value) {
+            const int t = token(j);
+            if (t < t0 || t >= t1 || (allow && !(allow[t >> 5] >> (t & 31) & 1))) return;
+            for (int k = 0; k < j; ++k)
+                if (token(k) == t) return;
+            float s = value(j);
+            for (int k = j + 1; k < n; ++k)
+                if (token(k) == t) s = __fadd_rn(s, value(k));
+            const float v = __fadd_rn(penalised(x[t], at[t]), s);
+            if (y) y[t] = v;
+            candidate(v, t);
+        };
+        const size_t g = r / (p.rows / p.bias_groups);
+        const int64_t *ids = p.bias_ids + g * p.n_bias;
+        const float *val = p.bias + g * p.n_bias;
+        const int n = bias.count;
+        if (n <= kBiasList) {   // one entry a thread: into the list's order, then added up
+            int mine = 0, token = 0, rank = 0;
+            if (tid < n) {
+                mine = bias.at[tid];
+                token = bias.token[tid];
+                for (int k = 0; k < n; ++k) rank += bias.at[k] < mine;
+            }
+            __syncthreads();
+            if (tid < n) {
+                bias.at[rank] = mine;
+                bias.token[rank] = token;
+            }
+            __syncthreads();
+            if (tid < n)
+                biased(n, tid, [&](int k) { return bias.token[k]; },
+                       [&](int k) { return val[bias.at[k]]; });
+        } else {
+            for (int j = tid; j < p.n_bias; j += kThreads)
+                biased(p.n_bias, j,
+                       [&](int k) { return ids[k] < 0 || ids[k] >= V ? -1 : (int)ids[k]; },
+                       [&](int k) { return val[k]; });
+        }
     }
     if (!part) return;
     best = max_over_wave(best);
