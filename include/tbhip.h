@@ -603,7 +603,10 @@ TB_API int tb_decoder_verify_tree(tb_decoder *d, int64_t start_offset, const int
 /* The path of that tree along next_tokens (host [n], the token chosen at each node),
  * as tb_tree_accept walks it: its rows move to start_offset .. in every layer's cache
  * and kv_len becomes start_offset + *n_path_out.  path_out host [n] (-1 behind the
- * path), *token_out the next token of its last node. */
+ * path), *token_out the next token of its last node.  TB_ERR_VALUE unless the cache
+ * still holds that tree: the last one verified, at that position with those tokens and
+ * parents, none of its rows written since (a path is kept once, here or by
+ * tb_decoder_tree_step). */
 TB_API int tb_decoder_accept_tree(tb_decoder *d, int64_t start_offset, const int64_t *tokens,
                                   const int32_t *parents, const int64_t *next_tokens, int64_t n,
                                   int32_t *path_out, int64_t *n_path_out, int64_t *token_out);

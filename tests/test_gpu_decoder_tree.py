@@ -197,3 +197,57 @@ def test_tree_refusals(cuda):
     assert dec.tree_step(0, [3, 4], [-1, 0], allowed=none) == ([0], -1)
     ref.close()
     dec.close()
+
+
+def test_accept_tree_takes_the_tree_that_the_cache_holds(cuda):
+    """A path is kept once, and only of the tree verified last at that position whose rows
+    nothing has been written to since: a second acceptance would move rows that have moved
+    already.  A refused call leaves the cache as it was."""
+    print("case accept_tree of trees that the cache does not hold", flush=True)
+    ref, dec, _ = make(4, 4)
+    g = np.random.default_rng(5)
+    prefix(ref, dec, g, 10)
+    toks, par, nxt = [7, 8, 9, 10, 11], [-1, 0, 0, 2, 3], [9, 0, 10, 11, 3]
+
+    def refused(start=10, t=toks, p=par):
+        before = dec.kv_len()
+        with pytest.raises(ValueError, match="does not hold"):
+            dec.accept_tree(start, t, p, nxt)
+        assert dec.kv_len() == before
+
+    refused()                                     # no tree yet
+    dec.verify_tree(10, toks, par)
+    refused(9)
+    refused(10, [7, 8, 9, 10, 12])
+    refused(10, toks, [-1, 0, 0, 2, 2])
+    with pytest.raises(ValueError, match="does not hold"):
+        dec.accept_tree(10, toks[:4], par[:4], nxt[:4])
+    assert dec.accept_tree(10, toks, par, nxt) == ([0, 2, 3, 4], 3)
+    refused()                                     # accepted already
+    for depth, t in enumerate((7, 9, 10, 11)):
+        ref.step(t, 10 + depth)
+    for i, t in enumerate((3, 5, 17)):            # the refusals moved nothing
+        lg, _ = dec._step(t, 14 + i, True)
+        assert rel(lg, ref.step(t, 14 + i)) < 2e-4
+    dec.tree_step(17, toks, par)
+    refused(17)                                   # tree_step has kept its path
+    kv = [torch.zeros(2, 18, 64)] * 2
+    for write in (lambda: dec._step(1, 21, False), lambda: dec.prefill_tokens([1] * 5, 15),
+                  lambda: dec.verify_tokens(21, [1, 2]), lambda: dec.verify_tree(20, [1], [-1]),
+                  lambda: dec.generate_loop(1, 19, 2, temperature=0.0),
+                  lambda: dec.generate_loop(1, 21, 2, top_k=5), lambda: dec.reset_kv_cache(),
+                  lambda: dec.time_greedy(1, 18, 1),
+                  lambda: dec.copy_kv_cache_from_tensors(kv, kv, 18),
+                  lambda: dec.tree_step(16, [1, 2], [-1, 0])):
+        dec.verify_tree(17, toks, par)
+        write()
+        refused(17)
+    # rows before and behind the nodes are not theirs
+    dec.verify_tree(17, toks, par)
+    dec._step(1, 16, False)
+    dec._step(1, 22, False)
+    dec.prefill_tokens([1, 2, 3, 4], 13)
+    dec.copy_kv_cache_from_tensors(kv, kv, 17)
+    assert dec.accept_tree(17, toks, par, nxt) == ([0, 2, 3, 4], 3)
+    ref.close()
+    dec.close()

@@ -891,6 +891,17 @@ struct Decoder {
     size_t pf_tree_bytes = 0;
     float *pf_tattn = nullptr;   // the tree attention's split partials
     size_t pf_tattn_bytes = 0;
+    // The tree whose nodes the cache holds from row held_start on (none: empty), until
+    // its path is kept or something else is written to one of those rows.
+    int64_t held_start = 0;
+    std::vector<int64_t> held_tokens;
+    std::vector<int32_t> held_parents;
+
+    // Rows from .. to - 1 of the cache are about to be written.
+    void overwrites(int64_t from, int64_t to) {
+        if (from < to && from < held_start + (int64_t)held_tokens.size() && to > held_start)
+            held_tokens.clear();
+    }
 
     // Whether trees of n nodes from start can be run forward.
     int tree_runs(int64_t start, int64_t n) const {
@@ -957,13 +968,24 @@ struct Decoder {
 
     // Every node's logits into pf_rows by one batched forward, K / V rows start .. start +
     // n - 1 holding the nodes in their order.
-    int tree_forward(Tree &t, const int64_t *tokens, int64_t start) {
+    int tree_forward(Tree &t, const int64_t *tokens, const int32_t *parents, int64_t start) {
         int rc = launch_tree_masks(t.parents, t.mask, t.depth, 1, t.n, st);
         if (!rc) rc = regrow(&pf_rows, &pf_rows_bytes, (size_t)t.n * V * 4);
         if (!rc)
             rc = regrow(&pf_tattn, &pf_tattn_bytes,
                         tree_attention_scratch(1, t.n, hq, hkv, hd, (int)(start + t.n)));
-        return rc ? rc : prefill_batched(tokens, t.n, start, pf_rows, &t);
+        if (rc || (rc = prefill_batched(tokens, t.n, start, pf_rows, &t))) return rc;
+        held_start = start;
+        held_tokens.assign(tokens, tokens + t.n);
+        held_parents.assign(parents, parents + t.n);
+        return TB_OK;
+    }
+
+    // Whether the cache holds that tree from row start on.
+    bool holds(int64_t start, const int64_t *tokens, const int32_t *parents, int64_t n) const {
+        return n == (int64_t)held_tokens.size() && start == held_start &&
+               std::equal(tokens, tokens + n, held_tokens.begin()) &&
+               std::equal(parents, parents + n, held_parents.begin());
     }
 
     int tree_attention(const Tree &t, const float *kcl, const float *vcl, int start) {
@@ -996,6 +1018,7 @@ struct Decoder {
         a.batch = 1; a.n = t.n; a.hkv = hkv; a.hd = hd; a.max_seq = max_seq; a.layers = L;
         a.k = {nullptr, sb, sh, hd};
         a.v = {nullptr, sb, sh, hd};
+        held_tokens.clear();   // its rows move
         int rc = launch_tree_accept(a, k.data(), v.data(), st);
         if (rc) return rc;
         int32_t n = 0;
@@ -1017,6 +1040,7 @@ struct Decoder {
         if (rc || (rc = prefill_alloc(n, start, &rows))) return rc;
         TB_REQUIRE(!tree || rows >= n, TB_ERR_MEMORY,
                    "Out of memory for a tree of " + std::to_string(n) + " nodes in one batch");
+        overwrites(start, start + n);
         pf_fixed = rows_out || n >= kFixedPrompt;
         const int nq = (hq + 2 * hkv) * hd;
         // Host copy of the whole prompt, alive until the closing synchronize.
@@ -1086,6 +1110,7 @@ struct Decoder {
             if (argmax) *argmax = 0;
             return TB_OK;
         }
+        overwrites(pos, pos + 1);
         kv_used = std::max<int64_t>(kv_used, pos + 1);
         rc = set_state((int)token, (int)pos);
         if (rc) return rc;
@@ -1423,6 +1448,7 @@ int tb_decoder_generate_sampled(tb_decoder *d, int64_t first_token, int64_t seq_
                                   : 0;
         if (valid > 0) {
             if ((rc = d->set_state((int)first_token, (int)seq_len))) return rc;
+            d->overwrites(seq_len, seq_len + valid);
             if (eos_token_id < 0) {
                 for (int64_t i = 0; i < valid; ++i) TB_HIP(hipGraphLaunch(d->sampled_graph(), d->st));
                 std::vector<int> hist((size_t)valid);
@@ -1481,6 +1507,7 @@ int tb_decoder_generate(tb_decoder *d, int64_t first_token, int64_t seq_len,
         if (valid > 0) {
             rc = d->set_state((int)first_token, (int)seq_len);
             if (rc) return rc;
+            d->overwrites(seq_len, seq_len + valid);
             for (int64_t i = 0; i < valid; ++i) TB_HIP(hipGraphLaunch(d->exec, d->st));
             std::vector<int> hist((size_t)valid);
             TB_HIP(hipMemcpyAsync(hist.data(), d->history, (size_t)valid * 4,
@@ -1686,7 +1713,7 @@ int tb_decoder_verify_tree(tb_decoder *d, int64_t start_offset, const int64_t *t
     Decoder::Tree t;
     int rc = d->tree_runs(start_offset, n);
     if (rc || (rc = d->tree_upload(t, start_offset, tokens, parents, n)) ||
-        (rc = d->tree_forward(t, tokens, start_offset)))
+        (rc = d->tree_forward(t, tokens, parents, start_offset)))
         return rc;
     TB_HIP(hipMemcpy(logits_out, d->pf_rows, (size_t)n * d->V * 4, hipMemcpyDeviceToHost));
     return TB_OK;
@@ -1700,6 +1727,9 @@ int tb_decoder_accept_tree(tb_decoder *d, int64_t start_offset, const int64_t *t
     Decoder::Tree t;
     int rc = d->tree_upload(t, start_offset, tokens, parents, n);
     if (rc) return rc;
+    TB_REQUIRE(d->holds(start_offset, tokens, parents, n), TB_ERR_VALUE,
+               "accept_tree: the cache does not hold this tree's nodes from position " +
+                   std::to_string(start_offset) + " (verify_tree first; a tree is accepted once)");
     TB_HIP(hipMemcpyAsync(t.next, next_tokens, (size_t)n * 8, hipMemcpyHostToDevice, d->st));
     return d->tree_keep(t, start_offset, path_out, n_path_out, token_out);
 }
@@ -1724,7 +1754,7 @@ int tb_decoder_tree_step(tb_decoder *d, int64_t start_offset, const int64_t *tok
         TB_HIP(hipMemcpyAsync(t.history, history, (size_t)n_history * 8, hipMemcpyHostToDevice, d->st));
     if (allowed)
         TB_HIP(hipMemcpyAsync(t.allowed, allowed, (size_t)n * words * 4, hipMemcpyHostToDevice, d->st));
-    if ((rc = d->tree_forward(t, tokens, start_offset))) return rc;
+    if ((rc = d->tree_forward(t, tokens, parents, start_offset))) return rc;
     LogitsParams p{};
     p.x = d->pf_rows; p.tokens = t.next;
     p.rows = (int)n; p.vocab = d->V;
@@ -1772,6 +1802,7 @@ int tb_decoder_prefill(tb_decoder *d, const int64_t *tokens, int64_t n, int64_t 
 int tb_decoder_reset_kv(tb_decoder *d) {
     TB_REQUIRE(d, TB_ERR_VALUE, "null decoder");
     const size_t kv = (size_t)d->L * d->hkv * d->max_seq * d->hd * sizeof(float);
+    d->overwrites(0, d->max_seq);
     if (d->kv_used > 0) {
         TB_HIP(hipMemsetAsync(d->kc, 0, kv, d->st));
         TB_HIP(hipMemsetAsync(d->vc, 0, kv, d->st));
@@ -1790,6 +1821,7 @@ int tb_decoder_copy_kv(tb_decoder *d, int64_t layer, const float *k, const float
     // Source [hkv, src_max, hd] per layer (decoder.rs:479-523).
     int rc = d->settle();   // device sources that the null stream is still writing
     if (rc) return rc;
+    d->overwrites(0, seq_len);
     const size_t row = (size_t)d->hd * 4;
     for (int hh = 0; hh < d->hkv; ++hh) {
         const size_t so = (size_t)hh * src_max * d->hd;
@@ -1856,6 +1888,7 @@ int tb_decoder_time_greedy(tb_decoder *d, int64_t first_token, int64_t offset, i
     if (rc) return rc;
     rc = d->set_state((int)first_token, (int)offset);
     if (rc) return rc;
+    d->overwrites(offset, offset + n_steps);
     TB_HIP(hipEventRecord(d->ev0, d->st));
     for (int64_t i = 0; i < n_steps; ++i) TB_HIP(hipGraphLaunch(d->exec, d->st));
     TB_HIP(hipEventRecord(d->ev1, d->st));

@@ -402,7 +402,9 @@ class RustQwenDecoder:
                     next_tokens: Sequence[int]) -> Tuple[List[int], int]:
         """(path, token): the nodes from node 0 along ``next_tokens``, the token chosen at each
         node (sampled from its row of verify_tree, say), and the next token of the last one.
-        The path's K / V rows are kept: the sequence goes on at start_offset + len(path)."""
+        The path's K / V rows are kept: the sequence goes on at start_offset + len(path).
+        The tree is the last one verified, its rows not written since, and a path of it is kept
+        once: ValueError otherwise."""
         t, par = self._tree(tokens, parents)
         nx = np.asarray(list(next_tokens), dtype=np.int64)
         if nx.size != t.size:
