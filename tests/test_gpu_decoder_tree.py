@@ -251,3 +251,51 @@ def test_accept_tree_takes_the_tree_that_the_cache_holds(cuda):
     assert dec.accept_tree(17, toks, par, nxt) == ([0, 2, 3, 4], 3)
     ref.close()
     dec.close()
+
+
+def test_verify_tree_of_large_layers_is_no_less_exact(cuda):
+    """9 nodes through layers of more than 2^24 weights, as a tree and as the steps that it
+    stands for: over all nodes, the tree's error against float64 is not the larger one."""
+    H, I, hd, n = 2048, 8320, 128, 9
+    cfg = dict(num_layers=1, hidden=H, intermediate=I, num_heads=16, num_kv_heads=4, head_dim=hd,
+               vocab=1024, eps=1e-6, rope_theta=1e6, qkv_bias=False)
+    w = synth.decoder_weights(cfg, 97, 4, 32, 32)
+    y = w["layers"][0]
+    y["post_norm"][::128] = 12.0      # large channels, and outputs of about unit size
+    for t in ("qkv_s", "o_s", "gate_s", "up_s", "down_s"):
+        y[t] *= 0.1
+    dec = decoder_from_weights(w, cfg, group_size=32, max_seq_len=32)
+    toks = [int(t) for t in np.random.default_rng(97).integers(0, cfg["vocab"], n)]
+    par = [-1, 0, 0, 1, 1, 3, 2, 5, 7]
+    tree = dec.verify_tree(0, toks, par).numpy()
+    steps = np.empty_like(tree)
+    for i in range(n):
+        for depth, j in enumerate(branch(par, i)):
+            steps[i], _ = dec._step(toks[j], depth, True)
+    dec.close()
+
+    f = lambda a: np.asarray(a, np.float64)
+    deq = lambda p, s: (np.stack((p & 15, p >> 4), -1).reshape(p.shape[0], -1) - 8.0) * \
+        np.repeat(f(s), 32, 1)
+    lin = lambda a, t: a @ deq(y[t + "_w"], y[t + "_s"]).T
+    rms = lambda v, g: v / np.sqrt((v * v).mean(1, keepdims=True) + cfg["eps"]) * f(g)
+    x = f(w["embed"])[toks]
+    depth = np.array([len(branch(par, i)) - 1 for i in range(n)])
+    ang = depth[:, None] / cfg["rope_theta"] ** (np.arange(0, hd, 2) / hd)
+    cos, sin = (np.tile(fn(ang), (1, 2))[:, None] for fn in (np.cos, np.sin))
+    turn = lambda v: v * cos + np.concatenate((-v[..., hd // 2:], v[..., :hd // 2]), -1) * sin
+    q, k, v = (a.reshape(n, -1, hd)
+               for a in np.split(lin(rms(x, y["in_norm"]), "qkv"), (H, H + 4 * hd), 1))
+    q, k, v = turn(q), np.repeat(turn(k), 4, 1), np.repeat(v, 4, 1)
+    see = np.array([[j in branch(par, i) for j in range(n)] for i in range(n)])
+    s = np.einsum("ihd,jhd->hij", q, k) / np.sqrt(hd) + np.where(see, 0.0, -np.inf)
+    p = np.exp(s - s.max(-1, keepdims=True))
+    a = np.einsum("hij,jhd->ihd", p / p.sum(-1, keepdims=True), v).reshape(n, -1)
+    x = x + lin(a, "o")
+    xn = rms(x, y["post_norm"])
+    g, u = lin(xn, "gate"), lin(xn, "up")
+    x = x + lin(g / (1 + np.exp(-g)) * u, "down")
+    want = rms(x, w["final_norm"]) @ f(w["lm_head_w"]).T
+    err = [np.linalg.norm(f(t) - want) / np.linalg.norm(want) for t in (tree, steps)]
+    print(f"case verify_tree errors: tree {err[0]:.2e}, steps {err[1]:.2e}", flush=True)
+    assert err[0] <= 1.02 * err[1]

@@ -687,7 +687,7 @@ struct Decoder {
             if ((rc = alloc(&pf_part, pf_part_bytes))) return rc;
         }
         if (wbits == 4 && !pf_limb_bytes) {
-            // 3..16 rows (verify_tokens, short chunks) take the small-batch
+            // 3..16 rows (verify_tokens, the last rows of longer prompts) take the small-batch
             // projection: records + split partials of the largest of its shapes
             size_t lb = 0;
             for (int m = 3; m <= kLimbMaxM; ++m) {
@@ -722,8 +722,8 @@ struct Decoder {
     uint8_t *pf_hrec = nullptr;   // records of h, [kLimbMaxM, I]
     size_t pf_limb_bytes = 0;
     // Whether the batch may take it: its activations are in fixed point, one step per
-    // 64 elements, where the steps that a prompt of up to 15 tokens stands for have one
-    // per 16 (error of eight Llama-3-8B layers' logits at 9 tokens: steps 1.98e-6, this
+    // 64 elements, where the steps that a prompt of up to 15 tokens or a drafted tree
+    // stands for have one per 16 (error of eight Llama-3-8B layers' logits at 9 tokens: steps 1.98e-6, this
     // 2.15e-6, the GEMM 1.55e-6; us for two layers 1262 / 354 / 407).
     bool pf_fixed = false;
     static constexpr int kFixedPrompt = 16;
@@ -1041,7 +1041,7 @@ struct Decoder {
         TB_REQUIRE(!tree || rows >= n, TB_ERR_MEMORY,
                    "Out of memory for a tree of " + std::to_string(n) + " nodes in one batch");
         overwrites(start, start + n);
-        pf_fixed = rows_out || n >= kFixedPrompt;
+        pf_fixed = !tree && (rows_out || n >= kFixedPrompt);
         const int nq = (hq + 2 * hkv) * hd;
         // Host copy of the whole prompt, alive until the closing synchronize.
         std::vector<int> tok32(tokens, tokens + n);
