@@ -574,3 +574,20 @@ def test_step_in_graphs(cuda):
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want)), rnd
             assert all(torch.equal(a, b) for a, b in zip(st["k"] + st["v"], n["k"] + n["v"]))
+
+
+def test_attention_of_misaligned_queries(cuda):
+    """A contiguous q that does not start at a multiple of 16 bytes is copied, as misaligned
+    caches are."""
+    print("case tree_attention misaligned q", flush=True)
+    N, H, KVH, D, S, kv = 5, 4, 2, 64, 60, 40
+    q, k, v, bits = inputs(21, 1, N, H, KVH, D, S)
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    a = (T(k[0]), T(v[0]), T(words(bits[0])), kv)
+    want = tb.tree_attention(T(q[0]), *a)
+    for off in (1, 2, 3):
+        buf = torch.empty(N * H * D + 4, device=cuda)
+        x = buf[off:off + N * H * D].view(N, H, D)
+        x.copy_(T(q[0]))
+        assert x.is_contiguous() and x.data_ptr() % 16
+        assert torch.equal(tb.tree_attention(x, *a), want)

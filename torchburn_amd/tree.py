@@ -99,6 +99,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     n, heads, hd = (int(s) for s in q.shape[-3:])
     batch = int(q.shape[0]) if batched else 1
     x = _on_gpu(q.detach(), torch.float32, dev)
+    if x.data_ptr() % 16:      # a view that starts inside a 16-byte unit
+        x = x.clone()
     kc = _cache(op, "k_cache", k_cache, batched, dev)
     vc = _cache(op, "v_cache", v_cache, batched, dev)
     if kc.shape != vc.shape or kc.shape[0] != batch or kc.shape[3] != hd:
