@@ -591,3 +591,27 @@ def test_attention_of_misaligned_queries(cuda):
         x.copy_(T(q[0]))
         assert x.is_contiguous() and x.data_ptr() % 16
         assert torch.equal(tb.tree_attention(x, *a), want)
+
+
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("bad", [0, 1, 2, 3])
+def test_accept_of_misaligned_caches(cuda, bad, strided):
+    """One cache among the layers' that does not start at a multiple of 16 bytes, the first or
+    a later one, contiguous or not: copied and written back."""
+    print(f"case tree_accept misaligned cache {bad} strided={strided}", flush=True)
+    KVH, S, D = 2, 12, 32
+    g = torch.Generator().manual_seed(3)
+    was = [torch.randn((KVH, S, D), generator=g) for _ in range(4)]
+    caches = []
+    for i, w in enumerate(was):
+        at = int(i == bad)
+        c = torch.empty(KVH * S * D + 4, device=cuda)[at:at + KVH * S * D]
+        caches.append(c.view(S, KVH, D).transpose(0, 1) if strided else c.view(KVH, S, D))
+        caches[i].copy_(w)
+    T = lambda a: torch.tensor(a, device=cuda)
+    path, n, tok = tb.tree_accept(T([-1, 0, 0, 2]), T([0, 1, 2, 3]), T([2, 0, 3, 9]), 6, caches[:2],
+                                  caches[2:])
+    assert path.tolist() == [0, 2, 3, -1] and int(n) == 3 and int(tok) == 9
+    for c, w in zip(caches, was):
+        w[:, 7:9] = w[:, 8:10].clone()
+        assert torch.equal(c.cpu(), w)

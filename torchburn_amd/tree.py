@@ -24,6 +24,7 @@ from .quantization import _int32_on_gpu, _on_gpu, _ptr, _stream, _target, _write
 
 
 _dtype = attrgetter("dtype")
+_ALIGNED = bytes(range(0, 256, 16))   # the low bytes of 16-byte aligned addresses
 
 
 def _bad(op: str, msg: str) -> UnsupportedOpError:
@@ -165,14 +166,20 @@ def tree_accept(parents: torch.Tensor, draft_tokens: torch.Tensor, next_tokens: 
         # Device caches of one layout are used as they are (checked as whole lists: a cache
         # more costs 0.3 us, 1.5 through _cache).
         k0, v0, T = given[0], given[layers], torch.Tensor
+        ptrs = (C.c_void_p * len(given))(*map(T.data_ptr, given))
         alike = set(map(T.get_device, given)) == {dev.index} and \
             set(map(_dtype, given)) == {torch.float32} and \
             list(map(T.size, given)) == [k0.shape] * len(given) and \
             list(map(T.stride, ks_in)) == [k0.stride()] * layers and \
             list(map(T.stride, vs_in)) == [v0.stride()] * layers and \
+            not bytes(ptrs)[::8].translate(None, _ALIGNED) and \
             _cache(op, "cache", k0, batched, dev).data_ptr() == k0.data_ptr() and \
             _cache(op, "cache", v0, batched, dev).data_ptr() == v0.data_ptr()
         caches = given if alike else [_cache(op, "cache", x, batched, dev) for x in given]
+        for part in () if alike else (slice(0, layers), slice(layers, None)):
+            # a copy beside caches of other strides: those are copied too
+            if any(c.data_ptr() != x.data_ptr() for c, x in zip(caches[part], given[part])):
+                caches[part] = [c.contiguous() for c in caches[part]]
         if caches is not given and any(c.shape != caches[0].shape or
                                        c.stride() != caches[i // layers * layers].stride()
                                        for i, c in enumerate(caches)):
@@ -183,9 +190,10 @@ def tree_accept(parents: torch.Tensor, draft_tokens: torch.Tensor, next_tokens: 
         shape, ks, vs = k0.shape, k0.stride(), v0.stride()
         if shape[0] != batch:
             raise _bad(op, f"caches {list(given[0].shape)} do not fit {batch} trees")
-        ptrs = list(map(T.data_ptr, caches))
-        kp = (C.c_void_p * layers)(*ptrs[:layers])
-        vp = (C.c_void_p * layers)(*ptrs[layers:])
+        if caches is not given:
+            ptrs = (C.c_void_p * len(caches))(*map(T.data_ptr, caches))
+        kp = C.addressof(ptrs)
+        vp = kp + layers * C.sizeof(C.c_void_p)
     path = torch.empty(p.shape, dtype=torch.int32, device=dev)
     count = torch.empty(p.shape[:-1], dtype=torch.int32, device=dev)
     token = torch.empty(p.shape[:-1], dtype=torch.int64, device=dev)
