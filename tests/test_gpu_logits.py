@@ -233,3 +233,68 @@ def test_alignment_and_many_biases(cuda):
         assert tb.greedy_tokens(xs, **kw).tolist() == best(y)
         tb.process_logits(xs, **kw, out=xs)
         assert torch.equal(xs, want)
+
+
+@pytest.mark.parametrize("R,V,n,style", [
+    (3, 700, 5000, "few"), (2, 2053, 1537, "one"), (2, 33333, 33333, "all"),
+    (512, 5000, 900, "few"),        # blocks of 8192 tokens
+    (1, 9000, 20000, "mixed"), (5, 40, 513, "few"),
+])
+def test_long_bias_lists(cuda, R, V, n, style):
+    """More biases than a block lists, in the order of the list: every sum is the one of f32
+    additions one after the other, bit by bit, with and without 16-byte vectors."""
+    print(f"case process_logits long bias list R={R} V={V} n={n} {style}", flush=True)
+    g = np.random.default_rng(V + n)
+    if style == "all":
+        ids = g.permutation(V)
+    elif style == "one":
+        ids = np.full(n, 1234)
+    else:
+        ids = g.integers(-3, min(V, 300) + 3, n)
+        if style == "mixed":
+            ids[n // 2:] = g.integers(0, V, n - n // 2)
+            ids[::7] = 5
+    bias = g.standard_normal(n).astype(np.float32)
+    x = g.standard_normal((R, V)).astype(np.float32)
+    total, named = np.zeros(V, np.float32), np.zeros(V, bool)
+    for t, b in zip(ids, bias):
+        if 0 <= t < V:
+            total[t] = total[t] + b if named[t] else b
+            named[t] = True
+    allowed = g.random(V) < 0.8
+    want = np.where(allowed, np.where(named, x + total, x), -np.inf).astype(np.float32)
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    kw = dict(bias_ids=T(ids), bias_values=T(bias), allowed=T(pack(allowed)))
+    assert np.array_equal(tb.process_logits(T(x), **kw).cpu().numpy(), want)
+    out = torch.empty(R * V + 1, device=cuda)[1:].view(R, V)
+    assert np.array_equal(tb.process_logits(T(x), **kw, out=out).cpu().numpy(), want)
+    assert tb.greedy_tokens(T(x), **kw).tolist() == best(want)
+    own = dict(bias_ids=T(ids).repeat(R, 1), bias_values=T(bias).repeat(R, 1),
+               allowed=T(pack(allowed)))
+    assert np.array_equal(tb.process_logits(T(x), **own).cpu().numpy(), want)
+
+
+def test_long_bias_lists_take_time_in_their_length(cuda):
+    """Ten times as many biases for as many tokens take no more than ten times as long (twice,
+    measured; 50 times where each entry looked through the whole list)."""
+    print("case process_logits long bias lists, time", flush=True)
+    g = np.random.default_rng(9)
+    x = torch.zeros(1, 2053, device=cuda)
+
+    def time(n):
+        kw = dict(bias_ids=torch.from_numpy(g.integers(0, 300, n)).to(cuda),
+                  bias_values=torch.zeros(n, device=cuda))
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        least = 1e9
+        for _ in range(5):
+            a.record()
+            for _ in range(20):
+                tb.process_logits(x, **kw)
+            b.record()
+            torch.cuda.synchronize()
+            least = min(least, a.elapsed_time(b))
+        return least
+
+    few, many = time(400), time(4000)
+    print(f"400 biases {few * 50:.1f} us, 4000 {many * 50:.1f} us", flush=True)
+    assert many <= 10 * few

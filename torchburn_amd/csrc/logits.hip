@@ -26,6 +26,7 @@ constexpr uint32_t kSeen = 1u << 31;   // of a token's LDS word: occurs in the h
 constexpr uint32_t kBias = 1u << 30;   // has a bias; the rest: its count
 constexpr uint32_t kCount = kBias - 1;
 constexpr int kBiasList = kThreads;    // biases of one block kept in LDS
+constexpr int kSums = 2048;            // tokens whose biases are added up at once, past that many
 
 // Orders as the values do, ties to the lower index; 0: nothing to take.
 __device__ __forceinline__ uint64_t best_item(float y, int t) {
@@ -44,6 +45,13 @@ __device__ __forceinline__ uint64_t max_over_wave(uint64_t v) {
     return v;
 }
 
+// What this wave wrote to LDS before is there for what it reads after.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 struct Biases {
     int at[kBiasList], token[kBiasList];   // the entries of the block's tokens
     int count;                             // how many there are (past kBiasList: not all listed)
@@ -53,8 +61,11 @@ struct Biases {
 // pass through once, 16 bytes a lane, four loads in flight (a lane whose four
 // tokens the mask excludes reads none).  A word of LDS per token holds what the
 // history, the tree path and the biases say of it (tokens with a bias are left to a
-// second pass, a thread for each: 200 biases of one block of 1500 tokens take 30 us,
-// 180 where the threads that meet such tokens look them up); the block reads those lists
+// second pass, a thread for each: 200 biases of one block of 1500 tokens take 26 us,
+// 180 where the threads that meet such tokens look them up; past kBiasList biases of a
+// block, MANY, a sum for each token: 500 in a list 53 us, 520 as sums 17, 4000 for 300
+// tokens 91, all 151936 of a vocabulary 214, where the list's threads search it whole
+// 4000 took 2556; sums need LDS, and blocks of few biases have none to give); the block reads those lists
 // whole, which is why chunks are as large as the row count lets them be.  64 rows of
 // 128256 tokens with one history of 2048 take 17.6 us (67 MB, 3.8 TB/s), 192 with one of
 // 1500 and 64 biases each 53 (202 MB, 3.8 TB/s), where a large copy reaches 5.1; chunks
@@ -62,7 +73,7 @@ struct Biases {
 // Vectors start where the row's address is a multiple of 16 bytes, `lead` tokens
 // into it; LDS word 4 is the chunk's first vector, the words before it are chunk
 // 0's tokens ahead of that.  The last vector may be cut.
-template <bool VEC>
+template <bool VEC, bool MANY>
 __global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, uint64_t *part) {
     extern __shared__ uint32_t word[];
     __shared__ uint64_t red[kThreads / 64];
@@ -194,15 +205,9 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, 
     }
     if (p.n_bias) {
         __syncthreads();
-        // The first entry of a token adds up all of its entries, in the order of the list.
-        auto biased = [&](int n, int j, auto token, auto value) {
-            const int t = token(j);
-            if (t < t0 || t >= t1 || (allow && !(allow[t >> 5] >> (t & 31) & 1))) return;
-            for (int k = 0; k < j; ++k)
-                if (token(k) == t) return;
-            float s = value(j);
-            for (int k = j + 1; k < n; ++k)
-                if (token(k) == t) s = __fadd_rn(s, value(k));
+        // The entries of a token are added up in the order of the list.
+        auto biased = [&](int t, float s) {
+            if (allow && !(allow[t >> 5] >> (t & 31) & 1)) return;
             const float v = __fadd_rn(penalised(x[t], at[t]), s);
             if (y) y[t] = v;
             candidate(v, t);
@@ -211,7 +216,7 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, 
         const int64_t *ids = p.bias_ids + g * p.n_bias;
         const float *val = p.bias + g * p.n_bias;
         const int n = bias.count;
-        if (n <= kBiasList) {   // one entry a thread: into the list's order, then added up
+        if (!MANY || n <= kBiasList) {   // one entry a thread: into the list's order, then added up
             int mine = 0, token = 0, rank = 0;
             if (tid < n) {
                 mine = bias.at[tid];
@@ -224,14 +229,51 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, 
                 bias.token[rank] = token;
             }
             __syncthreads();
-            if (tid < n)
-                biased(n, tid, [&](int k) { return bias.token[k]; },
-                       [&](int k) { return val[bias.at[k]]; });
-        } else {
-            for (int j = tid; j < p.n_bias; j += kThreads)
-                biased(p.n_bias, j,
-                       [&](int k) { return ids[k] < 0 || ids[k] >= V ? -1 : (int)ids[k]; },
-                       [&](int k) { return val[k]; });
+            bool first = tid < n;
+            if (first) token = bias.token[tid];
+            for (int k = 0; first && k < tid; ++k) first = bias.token[k] != token;
+            if (first) {
+                float v = val[bias.at[tid]];
+                for (int k = tid + 1; k < n; ++k)
+                    if (bias.token[k] == token) v = __fadd_rn(v, val[bias.at[k]]);
+                biased(token, v);
+            }
+        } else if (MANY) {
+            // kSums tokens at a time: each one's sum of biases, and whose turn it is to add to
+            // it.  The list goes by in windows of an entry a thread; the entries of one token
+            // take turns by their place in it, wave by wave and then lane by lane.
+            float *sum = reinterpret_cast<float *>(word + chunk + 4);
+            uint32_t *next = word + chunk + 4 + kSums;
+            const uint32_t wave = tid >> 6, lane = tid & 63;
+            for (int s0 = t0; s0 < t1; s0 += kSums) {
+                const int s1 = min(t1, s0 + kSums);
+                __syncthreads();
+                for (int i = tid; i < kSums; i += kThreads) {
+                    sum[i] = -0.f;   // -0 + v is v
+                    next[i] = ~0u;
+                }
+                for (int i0 = 0; i0 < p.n_bias; i0 += kThreads) {
+                    const int64_t id = i0 + tid < p.n_bias ? ids[i0 + tid] : -1;
+                    bool waits = id >= s0 && id < s1;
+                    const int i = waits ? (int)id - s0 : 0;
+                    const float v = waits ? val[i0 + tid] : 0.f;
+                    while (__syncthreads_or(waits)) {
+                        if (waits) atomicMin(&next[i], wave);
+                        __syncthreads();
+                        const bool mine = waits && next[i] == wave;
+                        __syncthreads();
+                        waits = waits && !mine;
+                        if (mine) next[i] = ~0u;
+                        for (uint64_t todo = __ballot(mine); todo; todo &= todo - 1) {
+                            wave_fence();
+                            if (lane == (uint32_t)__builtin_ctzll(todo))
+                                sum[i] = __fadd_rn(sum[i], v);
+                        }
+                    }
+                }
+                for (int t = s0 + tid; t < s1; t += kThreads)
+                    if (at[t] & kBias) biased(t, sum[t - s0]);
+            }
         }
     }
     if (!part) return;
@@ -275,13 +317,14 @@ size_t logits_scratch(int rows, int vocab, bool tokens) {
 int launch_logits(const LogitsParams &p, void *scratch, hipStream_t s) {
     const int chunk = chunk_tokens(p.rows, p.vocab), chunks = (p.vocab + chunk - 1) / chunk;
     uint64_t *part = p.tokens ? static_cast<uint64_t *>(scratch) : nullptr;
-    const size_t lds = p.hist || p.nodes || p.n_bias ? (size_t)(chunk + 4) * 4 : 0;
+    size_t lds = p.hist || p.nodes || p.n_bias ? (size_t)(chunk + 4) * 4 : 0;
     // Rows of x and y are equally far from a 16-byte boundary, or go word by word.
     const bool vec = !p.y || (reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.y)) % 16 == 0;
-    if (vec)
-        hipLaunchKernelGGL(k_logits<true>, dim3(chunks, p.rows), dim3(kThreads), lds, s, p, chunk, part);
-    else
-        hipLaunchKernelGGL(k_logits<false>, dim3(chunks, p.rows), dim3(kThreads), lds, s, p, chunk, part);
+    const bool many = p.n_bias > kBiasList;   // a block may have more than its list holds
+    if (many) lds += 2 * kSums * 4;
+    auto *k = vec ? (many ? k_logits<true, true> : k_logits<true, false>)
+                  : (many ? k_logits<false, true> : k_logits<false, false>);
+    hipLaunchKernelGGL(k, dim3(chunks, p.rows), dim3(kThreads), lds, s, p, chunk, part);
     TB_LAUNCHED();
     if (part) {
         hipLaunchKernelGGL(k_best_token, dim3(p.rows), dim3(64), 0, s, part, chunks, p.tokens);
