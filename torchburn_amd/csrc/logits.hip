@@ -60,16 +60,17 @@ struct Biases {
 // One block per row and chunk of the vocabulary.  Bound by the logits' bytes: they
 // pass through once, 16 bytes a lane, four loads in flight (a lane whose four
 // tokens the mask excludes reads none).  A word of LDS per token holds what the
-// history, the tree path and the biases say of it (tokens with a bias are left to a
-// second pass, a thread for each: 200 biases of one block of 1500 tokens take 26 us,
-// 180 where the threads that meet such tokens look them up; past kBiasList biases of a
-// block, MANY, a sum for each token: 500 in a list 53 us, 520 as sums 17, 4000 for 300
-// tokens 91, all 151936 of a vocabulary 214, where the list's threads search it whole
-// 4000 took 2556; sums need LDS, and blocks of few biases have none to give); the block reads those lists
-// whole, which is why chunks are as large as the row count lets them be.  64 rows of
-// 128256 tokens with one history of 2048 take 17.6 us (67 MB, 3.8 TB/s), 192 with one of
-// 1500 and 64 biases each 53 (202 MB, 3.8 TB/s), where a large copy reaches 5.1; chunks
-// half as large change neither.
+// history, the tree path and the biases say of it; the block reads those lists whole,
+// which is why chunks are as large as the row count lets them be.  64 rows of 128256
+// tokens with one history of 2048 take 17.6 us (67 MB, 3.8 TB/s), 192 with one of 1500
+// and 64 biases each 53 (202 MB, 3.8 TB/s), where a large copy reaches 5.1; chunks half
+// as large change neither.
+// Tokens with a bias are left to a second pass, a thread for each from a list in LDS:
+// 200 biases of one block of 1500 tokens take 26 us, 180 where the threads that meet
+// such tokens look them up.  MANY, where a call has more biases than that list holds:
+// blocks with too many of them keep a sum for each of their tokens (500 in the list
+// take 53 us, 520 as sums 17, 4000 for 300 tokens 91, all 151936 of a vocabulary 214).
+// It is a kernel of its own, because its registers and LDS cost the others 4 us.
 // Vectors start where the row's address is a multiple of 16 bytes, `lead` tokens
 // into it; LDS word 4 is the chunk's first vector, the words before it are chunk
 // 0's tokens ahead of that.  The last vector may be cut.
@@ -264,6 +265,8 @@ __global__ __launch_bounds__(kThreads) void k_logits(LogitsParams p, int chunk, 
                         __syncthreads();
                         waits = waits && !mine;
                         if (mine) next[i] = ~0u;
+                        // lane by lane, the loop's end known to all of them: one that each lane
+                        // left after its own turn could be compiled into a wait for itself
                         for (uint64_t todo = __ballot(mine); todo; todo &= todo - 1) {
                             wave_fence();
                             if (lane == (uint32_t)__builtin_ctzll(todo))
