@@ -161,3 +161,8 @@ def test_python_refusals(host, call):
 def test_python_value_errors(host):
     with pytest.raises(ValueError, match="history_len"):
         tb.process_logits(f(4, 100), ints(5), history_len=6)
+
+
+def test_no_rows_have_no_lists():
+    """A batch without rows comes with as many histories and bias lists: none."""
+    assert logits(rows=0, x=None, groups=0, bias_groups=0, n_bias=2) == _lib.TB_OK

@@ -1364,10 +1364,11 @@ int tb_process_logits(const float *logits, float *out, int64_t *tokens, int64_t 
                "TB_UNSUPPORTED: process_logits: rows outside 0..65535 or vocabulary outside 1..2^30");
     TB_REQUIRE(hist >= 0 && hist <= (1 << 29) && n_bias >= 0 && n_bias <= (1 << 29),
                TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: process_logits: bad history or bias length");
-    TB_REQUIRE(hist == 0 || (groups > 0 && rows % groups == 0), TB_ERR_UNSUPPORTED,
+    TB_REQUIRE(rows == 0 || hist == 0 || (groups > 0 && rows % groups == 0), TB_ERR_UNSUPPORTED,
                "TB_UNSUPPORTED: process_logits: " + std::to_string(groups) +
                    " histories do not divide " + std::to_string(rows) + " rows");
-    TB_REQUIRE(n_bias == 0 || (bias_groups > 0 && rows % bias_groups == 0), TB_ERR_UNSUPPORTED,
+    TB_REQUIRE(rows == 0 || n_bias == 0 || (bias_groups > 0 && rows % bias_groups == 0),
+               TB_ERR_UNSUPPORTED,
                "TB_UNSUPPORTED: process_logits: " + std::to_string(bias_groups) +
                    " bias lists do not divide " + std::to_string(rows) + " rows");
     TB_REQUIRE(nodes >= 0 && nodes <= kMaxTreeNodes && (nodes == 0 || rows % nodes == 0),
