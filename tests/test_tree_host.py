@@ -166,3 +166,15 @@ def test_python_value_errors(host):
 def test_no_rows_have_no_lists():
     """A batch without rows comes with as many histories and bias lists: none."""
     assert logits(rows=0, x=None, groups=0, bias_groups=0, n_bias=2) == _lib.TB_OK
+
+
+@pytest.mark.parametrize("call", [
+    lambda: tb.process_logits(f(1, 20), allowed=torch.tensor(3, dtype=i32)),
+    lambda: tb.greedy_tokens(f(1, 20), allowed=torch.tensor(3, dtype=i32)),
+    lambda: tb.process_logits(f(1, 20), draft_tokens=torch.tensor(3), tree_mask=ints(1)),
+    lambda: tb.process_logits(f(1, 20), torch.tensor(3)),
+    lambda: tb.process_logits(f(1, 20), bias_ids=torch.tensor(3), bias_values=torch.tensor(1.0)),
+])
+def test_tensors_without_dimensions(host, call):
+    with pytest.raises(tb.UnsupportedOpError, match="TB_UNSUPPORTED"):
+        call()

@@ -112,7 +112,7 @@ def _process(op: str, want_tokens: bool, logits, history, history_len, prompt_le
                        f"{list(bias_values.shape)} differ")
     am, words = None, (vocab + 31) // 32
     if allowed is not None:
-        if allowed.dtype != torch.int32 or allowed.shape[-1] != words or \
+        if allowed.dtype != torch.int32 or allowed.shape[-1:] != (words,) or \
                 allowed.numel() not in (words, rows * words):
             raise _bad(op, f"allowed must be int32 [{words}] or [{rows}, {words}], got "
                            f"{allowed.dtype} {list(allowed.shape)}")
@@ -121,8 +121,8 @@ def _process(op: str, want_tokens: bool, logits, history, history_len, prompt_le
     if (draft_tokens is None) != (tree_mask is None):
         raise _bad(op, "draft_tokens and tree_mask come together")
     if draft_tokens is not None:
-        nodes = int(draft_tokens.shape[-1])
-        if tree_mask.dtype != torch.int32 or draft_tokens.numel() != rows or \
+        nodes = int(draft_tokens.shape[-1]) if draft_tokens.ndim else 0
+        if tree_mask.dtype != torch.int32 or draft_tokens.numel() != rows or not draft_tokens.ndim or \
                 tuple(tree_mask.shape) != (*draft_tokens.shape, (nodes + 31) // 32):
             raise _bad(op, f"draft_tokens [.., n] of {rows} nodes in all and tree_mask int32 "
                            f"[.., n, ceil(n / 32)] needed, got {list(draft_tokens.shape)} and "
