@@ -178,3 +178,17 @@ def test_no_rows_have_no_lists():
 def test_tensors_without_dimensions(host, call):
     with pytest.raises(tb.UnsupportedOpError, match="TB_UNSUPPORTED"):
         call()
+
+
+@pytest.mark.parametrize("n,given", [(2 ** 64 + 3, 2 ** 63 - 1), (-2 ** 64 + 3, -2 ** 63),
+                                     (2 ** 63, 2 ** 63 - 1), (-1, -1), (3, 3)])
+def test_numbers_past_64_bits(host, monkeypatch, n, given):
+    """Lengths reach the C entry points, which refuse or clamp them, as the nearest number,
+    not as another one with the same low bits."""
+    calls = []
+    monkeypatch.setattr(_lib, "call_on", lambda dev, name, *a: calls.append((name, a)))
+    tb.tree_attention(f(4, 4, 64), f(2, 32, 64), f(2, 32, 64), ints(4, 1), n)
+    tb.tree_accept(ints(4), ints(4), ints(4), n)
+    tb.process_logits(f(4, 100), ints(5), prompt_len=n)
+    (_, a), (_, b), (_, c) = calls
+    assert a[12] == given and b[4] == given and c[10] == given

@@ -126,6 +126,12 @@ def check(rc: int) -> None:
     raise RuntimeError(f"HIP error: {msg}")
 
 
+def int64(x) -> int:
+    """A number as the C entry points take it: past 64 bits the nearest one, where ctypes
+    keeps the low bits."""
+    return max(-1 << 63, min(int(x), (1 << 63) - 1))
+
+
 def call_on(dev, name: str, *args) -> None:
     """call() with ``dev`` as the current device, for kernels launched on one of its streams."""
     import torch

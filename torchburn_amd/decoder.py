@@ -394,8 +394,9 @@ class RustQwenDecoder:
         import torch
         t, par = self._tree(tokens, parents)
         out = np.empty((t.size, self.vocab_size), np.float32)
-        _lib.check(_bind().tb_decoder_verify_tree(self._h, int(start_offset), t.ctypes.data,
-                                                  par.ctypes.data, t.size, out.ctypes.data))
+        _lib.check(_bind().tb_decoder_verify_tree(
+            self._h, _lib.int64(start_offset), t.ctypes.data, par.ctypes.data, t.size,
+            out.ctypes.data))
         return torch.from_numpy(out)
 
     def accept_tree(self, start_offset: int, tokens: Sequence[int], parents: Sequence[int],
@@ -412,8 +413,8 @@ class RustQwenDecoder:
         path = np.empty(max(t.size, 1), np.int32)
         n, tok = C.c_int64(), C.c_int64()
         _lib.check(_bind().tb_decoder_accept_tree(
-            self._h, int(start_offset), t.ctypes.data, par.ctypes.data, nx.ctypes.data, t.size,
-            path.ctypes.data, C.byref(n), C.byref(tok)))
+            self._h, _lib.int64(start_offset), t.ctypes.data, par.ctypes.data, nx.ctypes.data,
+            t.size, path.ctypes.data, C.byref(n), C.byref(tok)))
         return path[:n.value].tolist(), int(tok.value)
 
     def tree_step(self, start_offset: int, tokens: Sequence[int], parents: Sequence[int],
@@ -438,8 +439,8 @@ class RustQwenDecoder:
         path = np.empty(max(t.size, 1), np.int32)
         n, tok = C.c_int64(), C.c_int64()
         _lib.check(_bind().tb_decoder_tree_step(
-            self._h, int(start_offset), t.ctypes.data, par.ctypes.data, t.size,
-            h.ctypes.data if h.size else None, h.size, int(prompt_len),
+            self._h, _lib.int64(start_offset), t.ctypes.data, par.ctypes.data, t.size,
+            h.ctypes.data if h.size else None, h.size, _lib.int64(prompt_len),
             float(repetition_penalty), float(presence_penalty), float(frequency_penalty), al,
             path.ctypes.data, C.byref(n), C.byref(tok)))
         return path[:n.value].tolist(), int(tok.value)

@@ -66,7 +66,7 @@ def _groups(op: str, name: str, t: Optional[torch.Tensor], rows: int, dtype, dev
 def _lengths(op: str, name: str, t, groups: int, dev):
     """(device int32 [groups] or None, host int) of lengths given as a tensor or a number."""
     if not isinstance(t, torch.Tensor):
-        return None, int(t)
+        return None, _lib.int64(t)
     if t.numel() != groups:
         raise _bad(op, f"{name} must have {groups} elements, got {list(t.shape)}")
     return _int32_on_gpu(t.reshape(-1), dev), 0

@@ -56,7 +56,7 @@ def _cache(op: str, name: str, c: torch.Tensor, batched: bool, dev: torch.device
 
 def _kv_len(op: str, kv_len, batch: int, dev) -> Tuple[Optional[torch.Tensor], int]:
     if not isinstance(kv_len, torch.Tensor):
-        return None, int(kv_len)
+        return None, _lib.int64(kv_len)
     if kv_len.numel() != batch:
         raise _bad(op, f"kv_len must have {batch} elements, got {list(kv_len.shape)}")
     return _int32_on_gpu(kv_len.reshape(-1), dev), 0
