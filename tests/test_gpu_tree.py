@@ -615,3 +615,120 @@ def test_accept_of_misaligned_caches(cuda, bad, strided):
     for c, w in zip(caches, was):
         w[:, 7:9] = w[:, 8:10].clone()
         assert torch.equal(c.cpu(), w)
+
+
+def weight_floor(q, k, v, bits, lens, scale, slack):
+    """What the bound leaves to weights that are small beside their tile's reference, row by
+    row.  A weight's two limbs have 22 bits down to 2^-21 of the reference and an error of
+    2^-43 of it below; times the largest V of the 64 positions and 2^slack, where the outputs'
+    scale is up to that far above it.  The reference is at most the row's largest score, and
+    at most 2^24 above the tile's largest one while that is 2^-36 of the largest or more."""
+    out = np.zeros((*q.shape[:3], 1))
+    G = q.shape[2] // k.shape[1]
+    for b, i, h in np.ndindex(*q.shape[:3]):
+        if not bits[b, i].any():
+            continue
+        n = bits.shape[1]
+        s = k[b, h // G, :lens[b] + n].astype(np.float64) @ q[b, i, h].astype(np.float64) * scale
+        s[lens[b]:][~bits[b, i]] = -np.inf
+        w = np.exp(s - s.max())
+        big = np.abs(v[b, h // G, :lens[b] + n]).max(-1)
+        for t in range(0, len(w), 64):
+            top = w[t:t + 64].max()
+            out[b, i, h] += 64 * 2.0 ** (slack - 43) * big[t:t + 64].max() * \
+                min(1.0, max(2.0 ** 24 * top, 2.0 ** -36))
+    return out
+
+
+@pytest.mark.parametrize("N,H,KVH,D,kv,S", [
+    (2, 4, 2, 128, 9000, 9100), (8, 8, 2, 64, 3000, 3100),          # few rows
+    (40, 8, 2, 64, 5000, 5100), (49, 8, 2, 128, 2000, 2100), (17, 4, 1, 224, 1500, 1600),
+    (64, 8, 2, 64, 3000, 131072), (64, 4, 1, 128, 1500, 131200),    # blocks of eight waves
+])
+@pytest.mark.parametrize("gap", [8.0, 14.0, 21.1, 39.0])
+def test_attention_of_small_weights(cuda, N, H, KVH, D, kv, S, gap):
+    """One position whose V is zero takes nearly all of the weight; the result is that of the
+    others, each with e^-gap of it, all of them alike, so that their errors add up."""
+    print(f"case tree_attention small weights N={N} H={H}/{KVH} D={D} kv={kv} gap={gap}", flush=True)
+    g = np.random.default_rng(N)
+    bits = ancestors(tree(g, N))[0][None]
+    q = np.zeros((1, N, H, D), np.float32)
+    k, v = np.zeros((1, KVH, kv + N, D), np.float32), np.ones((1, KVH, kv + N, D), np.float32)
+    q[..., 0] = 1.0
+    for at in (0, kv // 2 + 5):      # in the first split and in another
+        k[..., 0] = 0.0
+        k[:, :, at, 0] = gap
+        v[:] = 1.0
+        v[:, :, at] = 0.0
+        want, bound = reference(q, k, v, bits, [kv], 1.0)
+        bound += weight_floor(q, k, v, bits, [kv], 1.0, 1)
+        # sharp: 2 ds is 3.4e-4 at most, and the tile of the large weight leaves 64 2^-42
+        assert (bound < 1e-3 * want + 2e-11).all()
+        T = lambda a: torch.from_numpy(a).to(cuda)
+        kc, vc = (torch.zeros((1, KVH, S, D), device=cuda) for _ in range(2))
+        kc[:, :, :kv + N], vc[:, :, :kv + N] = T(k), T(v)
+        got = tb.tree_attention(T(q), kc, vc, T(words(bits)), torch.tensor([kv], device=cuda), 1.0)
+        check(got, want, bound)
+
+
+@pytest.mark.parametrize("N,H,KVH,D,kv,S", [
+    (2, 4, 2, 128, 700, 800), (8, 8, 2, 64, 700, 800), (40, 8, 2, 64, 700, 800),
+    (49, 8, 2, 128, 700, 800), (17, 4, 1, 224, 700, 800), (64, 8, 2, 64, 700, 131072),
+])
+@pytest.mark.parametrize("fall,rise", [(30.0, 0.0), (60.0, 50.0), (100.0, 90.0), (40.0, -80.0),
+                                       (-80.0, 60.0), (-60.0, -60.0)])
+def test_attention_of_falling_scores(cuda, N, H, KVH, D, kv, S, fall, rise):
+    """Scores that fall by `fall` powers of two over the cache (or rise, up and down again in
+    every fourth position), V that grows or shrinks by `rise` of them: small weights of large
+    V, and references and scales that follow both."""
+    print(f"case tree_attention falling scores N={N} H={H}/{KVH} D={D} {fall} {rise}", flush=True)
+    q, k, v, bits = inputs(N + D, 1, N, H, KVH, D, kv + N)
+    x = np.arange(kv + N) / (kv + N)
+    k *= 0.05
+    q[..., 0] = 1.0
+    k[..., 0] = (-fall * np.log(2) * x)[None, None]
+    k[:, :, 3::4, 0] *= 0.5
+    v *= (2.0 ** (rise * x))[None, None, :, None].astype(np.float32)
+    want, bound = reference(q, k, v, bits, [kv], 1.0)
+    bound += weight_floor(q, k, v, bits, [kv], 1.0, 8)
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    kc, vc = (torch.zeros((1, KVH, S, D), device=cuda) for _ in range(2))
+    kc[:, :, :kv + N], vc[:, :, :kv + N] = T(k), T(v)
+    got = tb.tree_attention(T(q), kc, vc, T(words(bits)), torch.tensor([kv], device=cuda), 1.0)
+    check(got, want, bound)
+
+
+def test_attention_sums_of_zero_values(cuda):
+    """As test_attention_weights_of_zero_values, with an allowance for the positions whose V is
+    large alone: what is lost from the sum of weights would show."""
+    print("case tree_attention sums of zero values", flush=True)
+    for N, H, D in ((2, 4, 128), (40, 8, 64), (60, 16, 128)):
+        KVH, kv, S = 2, 4000, 4100
+        q, k, v, bits = inputs(31, 1, N, H, KVH, D, S)
+        v[:, :, :kv] = 0.0
+        v[:, :, 3900:3904] = 1e7
+        want, bound = reference(q, k, v, bits, [kv], D ** -0.5)
+        floor = weight_floor(q, k, v, bits, [kv], D ** -0.5, 1)
+        assert floor.max() < 1e-3
+        T = lambda a: torch.from_numpy(a).to(cuda)
+        check(tb.tree_attention(T(q), T(k), T(v), T(words(bits)), kv), want, bound + floor)
+
+
+@pytest.mark.parametrize("D,N,kv,S", [(64, 6, 40, 46), (128, 25, 90, 115), (96, 60, 200, 260),
+                                      (256, 33, 65, 98), (64, 60, 30, 131072)])
+@pytest.mark.parametrize("big", [1e6, 3e38])
+def test_attention_large_values_seen(cuda, D, N, kv, S, big):
+    """Rows that see nodes of very large V, with no allowance beside the bound: those tiles are
+    worked in f32."""
+    print(f"case tree_attention large values seen D={D} N={N} kv={kv} big={big}", flush=True)
+    H, KVH = 8, 2
+    q, k, v, bits = inputs(D + N + 1, 1, N, H, KVH, D, kv + N, [N - 1])
+    nodes = [0, N // 2, N - 1]
+    for j in nodes:
+        v[:, :, kv + j] = np.clip(v[:, :, kv + j], -1, 1) * np.float32(big)
+    want, bound = reference(q, k, v, bits, [kv], D ** -0.5)
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    kc, vc = (torch.zeros((1, KVH, S, D), device=cuda) for _ in range(2))
+    kc[:, :, :kv + N], vc[:, :, :kv + N] = T(k), T(v)
+    check(tb.tree_attention(T(q), kc, vc, T(words(bits)), torch.tensor([kv], device=cuda)), want,
+          bound)

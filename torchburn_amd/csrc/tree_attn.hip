@@ -13,8 +13,11 @@
 // sixteenth of it).  s puts the largest factor of a few positions (K, V) or a row
 // (Q) at 2^14, so factors down to 2^-17 of it keep both limbs whole and smaller ones
 // an error of 2^-39 of it.  Weights are taken as w 2^7 for the same reason, less
-// where the positions' V is smaller than others': an error of 2^-32 of the largest
-// V.  Behind the prefix, where rows see different positions, a tile whose K or V
+// where the positions' V is smaller than others', with low limbs times 2^11: 22 bits
+// down to 2^-21 of the row's reference score's weight, and an error of 2^-43 of that one
+// times the largest V for every position below, which add up.  The reference falls with
+// the scores (kDrop), so that only the tile of a large weight whose V is zero shows it.
+// Behind the prefix, where rows see different positions, a tile whose K or V
 // spread wider than that is worked in f32 (as one with infinities is), so that
 // nothing that a row does not see costs it bits.  Scores, running maxima, sums and
 // outputs are f32.
@@ -49,6 +52,18 @@ constexpr int kTop = 14;         // factors are scaled to below 2^(kTop + 1)
 // are scaled by 2^kWeight, so that they stay below 2^(kTop + 2), the f16 range.
 constexpr float kLag = 8.f;
 constexpr int kWeight = 7;
+// The low limb of a weight is kept times 2^kLow, as f16's smallest steps would take what
+// is below 2^-32 of the reference; V's high limb is divided by it for that product.
+// (32767 positions 21.1 below a score whose V is zero: 1.53e-5 without, the result is
+// 2.27e-5.)  It costs 40 vector instructions a tile: 40.0 / 139 us without, 41.2 / 144.
+constexpr int kLow = 11;
+// The reference also follows down, to a tile's largest score that is more than 2^kDrop
+// below it: where the largest weights meet a V of zero, the small ones are the result.
+// As far down as the sum of weights stays below 2^kRoom and the outputs within f32.
+// Scores whose standard deviation is 11 powers of two take 148 us with 24, 150 with 20
+// and 136 without, ordinary ones the same.
+constexpr float kDrop = 24.f;
+constexpr int kRoom = 36;
 
 constexpr int kBias = 1 << 10, kSlow = 1 << 20;
 constexpr int kNoV = -1000;          // in place of an exponent: none yet
@@ -102,6 +117,25 @@ __device__ __forceinline__ void split_to_lds(const float (&x)[N], float sc, f16v
         lo[j] = r.x; lo[j + 1] = r.y;
     }
 }
+
+// The limbs of 8 weights given times 2^kLow, the low one times 2^kLow.
+__device__ __forceinline__ void split_weights(const float (&y)[8], f16x8 &hi, f16x8 &lo) {
+    float up = (float)(1 << kLow), down = 1.f / (1 << kLow);
+    asm("" : "+s"(up));
+    asm("" : "+s"(down));
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        f16x2 h = {(_Float16)__builtin_fmaf(y[j], down, 0.f),
+                   (_Float16)__builtin_fmaf(y[j + 1], down, 0.f)};
+        asm("" : "+v"(h));
+        hi[j] = h.x; hi[j + 1] = h.y;
+        lo[j] = (_Float16)__builtin_fmaf(-(float)h.x, up, y[j]);
+        lo[j + 1] = (_Float16)__builtin_fmaf(-(float)h.y, up, y[j + 1]);
+    }
+}
+
+// V's high limbs for the weights' low ones.
+__device__ __forceinline__ f16x8 low(const f16x8 &v) { return v * (_Float16)(1.f / (1 << kLow)); }
 
 // max(m, |a|, |b|) of loaded values without the canonicalising moves of fmaxf.
 __device__ __forceinline__ void max3_abs(float &m, float a, float b) {
@@ -306,6 +340,16 @@ __device__ __forceinline__ float reference(bool live, float m, float sum) {
     return !live ? -INFINITY : sum != sum && m == -INFINITY ? INFINITY : m;
 }
 
+// A row's reference m, of sum `sum` so far, for a tile whose largest score is `top`: down
+// to that where it is more than 2^kDrop below, but the outputs, at most sum 2^(kWeight +
+// kTop + 1 + oe_top - oe) and through rescale() 2^64 times as much, stay below 2^127.
+__device__ __forceinline__ float drop(float m, float top, float sum, int oe, int oe_top) {
+    const int least = (int)(__float_as_uint(sum) >> 23) - 127;
+    const int room = min(kRoom, 96 - (oe_top - oe)) - least;
+    const float to = fmaxf(top, m - (float)min(room, kRoom));
+    return top < m - kDrop && top > -INFINITY && room > 0 ? to : m;
+}
+
 // The outputs' scale 2^(kTop - oe) for a tile of V's exponent ve: how far it moves
 // down.  It stays while the tile fits it and loses at most 6 bits of range to it, and
 // stays 64 bits below the largest one so far (the outputs' f32 must not overflow).
@@ -373,7 +417,7 @@ __device__ __forceinline__ Range split_range(int len, int end, int tk, int cap, 
 // far apart for limbs in common scales, goes in f32, as do those after such a one
 // behind the prefix: its scores come from f32 sums, its weights leave the MFMAs as 0,
 // and then V is added in f32.  (Positions behind the prefix are few, and this is rare:
-// 49 nodes on 4096 positions take 259 us with such a node and 45 without.)
+// 49 nodes on 4096 positions take 146 us with such a node and 44 without.)
 //
 // Bound by what a SIMD can issue: a wave has 96 MFMAs and 410 to 470 vector
 // instructions (limbs, exponentials, maxima, sums; eight waves, four) a tile of 32
@@ -389,9 +433,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
     constexpr int PW = 32 / NW, LX = 16 / PW;   // K positions a wave, operands of one side by side
     constexpr int KU = KT * NS / LX;            // K operands (8 values) a lane
     constexpr int VU = KT * NB / 2, VP = 16 / NW;   // V: columns of 4 a lane, positions of each
-    // Operands read at a time.  (With 2 of V the four-wave block of 32 rows and 128 dimensions
-    // spills 149 registers, with 1 it spills 4.)
-    constexpr int KG = RB == 1 ? 2 : 1, VG = RB == 1 ? 4 : NW == 4 && DP == 128 ? 1 : 2;
+    // Operands read at a time.  (32 rows of 128 dimensions have all 256 registers: 3 to 5 spill.
+    // With 1 of V the four-wave block spills none, and is no faster: 41.1 us both, 137 / 132.)
+    constexpr int KG = RB == 1 ? 2 : 1, VG = RB == 1 ? 4 : 2;
     __shared__ f16x8 sk[2][KT * 2 * NS * 2 * 64];       // [32 positions][16][32 dims][limb][lane]
     __shared__ f16x8 sv[2][KT * NB * 4 * 2 * 64];       // [32 positions][64 dims][j][limb][lane]
     // The shares' exponents, K's and V's; V's + kBias again with kSlow where K or V is for f32.
@@ -708,17 +752,28 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
             }
             // ---- running maxima
             float was[RB];
-            bool moved = false;
+            bool moved = false, below = false;
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 if (!open) mask_scores(rb, p0, g, s8[rb]);
-                float top = s8[rb][0];
+                float t = s8[rb][0];
 #pragma unroll
-                for (int j = 1; j < 8 * KT; ++j) top = fmaxf(top, s8[rb][j]);
+                for (int j = 1; j < 8 * KT; ++j) t = fmaxf(t, s8[rb][j]);
                 was[rb] = m[rb];
-                top = max_over_groups(top);
-                m[rb] = top > m[rb] + kLag ? top : m[rb];
+                t = max_over_groups(t);
+                below |= t < m[rb] - kDrop;
+                m[rb] = t > m[rb] + kLag ? t : m[rb];
                 moved |= m[rb] != was[rb];
+            }
+            if (__builtin_expect(__any(below), 0)) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    float t = s8[rb][0];
+#pragma unroll
+                    for (int j = 1; j < 8 * KT; ++j) t = fmaxf(t, s8[rb][j]);
+                    m[rb] = drop(m[rb], max_over_groups(t), sum_over_groups(l[rb]), oe, oe_top);
+                    moved |= m[rb] != was[rb];
+                }
             }
             const int down = slow ? raise(vtop, oe, oe_top) : rescale(vtop, oe, oe_top);
             if (__any(moved) || down != 0) {
@@ -738,12 +793,12 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
             f16x8 ph[RB][KT], pl[RB][KT];
             const int pe[2] = {max(kWeight + ve[0] - oe, kWeightLow),
                                max(kWeight + ve[1] - oe, kWeightLow)};
-            const float back[2] = {pow2(-pe[0]), pow2(-pe[1])};
+            const float back[2] = {pow2(-pe[0] - kLow), pow2(-pe[1] - kLow)};
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 float top = m[rb] == -INFINITY ? 0.f : m[rb];   // nothing seen: weights 0
                 if (slow) top = INFINITY;   // V in f32 below: weights 0 here
-                const float base[2] = {(float)pe[0] - top, (float)pe[1] - top};
+                const float base[2] = {(float)(pe[0] + kLow) - top, (float)(pe[1] + kLow) - top};
 #pragma unroll
                 for (int sub = 0; sub < KT; ++sub) {
                     float p8[8];
@@ -752,7 +807,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
                         p8[j] = __builtin_amdgcn_exp2f(s8[rb][8 * sub + j] + base[j >> 2]);
                         l[rb] = fmaf(p8[j], back[j >> 2], l[rb]);
                     }
-                    split8(p8, 1.f, ph[rb][sub], pl[rb][sub]);
+                    split_weights(p8, ph[rb][sub], pl[rb][sub]);
                 }
             }
             // ---- outputs
@@ -769,7 +824,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_
                             const int at = grp * VG + j;   // [32 positions][64 dims][j]
                             f32x4 &d = o[rb][at / 4 % NB][at % 4];
                             d = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                vf[grp & 1][j][y == 0],
+                                y == 1 ? low(vf[grp & 1][j][0]) : vf[grp & 1][j][y == 0],
                                 y == 1 ? pl[rb][at / (4 * NB)] : ph[rb][at / (4 * NB)], d, 0, 0, 0);
                         }
                 __builtin_amdgcn_sched_barrier(0);
@@ -977,7 +1032,7 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
         }
         // ---- running maxima
         float was[RB];
-        bool moved = false;
+        bool moved = false, below = false;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             if (!open) {
@@ -986,13 +1041,24 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
                 for (int j = 0; j < 8; ++j)
                     if (!(see >> position(j, g) & 1)) s8[rb][j] = -INFINITY;
             }
-            float top = s8[rb][0];
+            float t = s8[rb][0];
 #pragma unroll
-            for (int j = 1; j < 8; ++j) top = fmaxf(top, s8[rb][j]);
+            for (int j = 1; j < 8; ++j) t = fmaxf(t, s8[rb][j]);
             was[rb] = m[rb];
-            top = max_over_groups(top);
-            m[rb] = top > m[rb] + kLag ? top : m[rb];
+            t = max_over_groups(t);
+            below |= t < m[rb] - kDrop;
+            m[rb] = t > m[rb] + kLag ? t : m[rb];
             moved |= m[rb] != was[rb];
+        }
+        if (__builtin_expect(__any(below), 0)) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                float t = s8[rb][0];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) t = fmaxf(t, s8[rb][j]);
+                m[rb] = drop(m[rb], max_over_groups(t), sum_over_groups(l[rb]), oe, oe_top);
+                moved |= m[rb] != was[rb];
+            }
         }
         // ---- V's scale and the outputs'
 #pragma unroll
@@ -1048,27 +1114,27 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
                     for (int j = 0; j < 4; ++j) o[rb][q][j] *= x;
             }
         }
-        // ---- weights 2^kWeight w
+        // ---- weights 2^(kWeight + kLow) w, their sums of 2^kWeight w
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            const float base = (float)kWeight - (m[rb] == -INFINITY ? 0.f : m[rb]);
+            const float base = (float)(kWeight + kLow) - (m[rb] == -INFINITY ? 0.f : m[rb]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 s8[rb][j] = __builtin_amdgcn_exp2f(s8[rb][j] + base);
-                l[rb] += s8[rb][j];
+                l[rb] = fmaf(s8[rb][j], 1.f / (1 << kLow), l[rb]);
             }
         }
         // ---- outputs; V takes the outputs' scale
         if (__builtin_expect(slow_v, 0)) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
-                add_in_f32<NB, 8>(a, vb, p0, end, g, c, s8[rb], pow2(kTop - oe), o[rb]);
+                add_in_f32<NB, 8>(a, vb, p0, end, g, c, s8[rb], pow2(kTop - kLow - oe), o[rb]);
             if (tile + 4 < t1) load_v(tile + 4);
             continue;
         }
         f16x8 ph[RB], pl[RB];
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) split8(s8[rb], 1.f, ph[rb], pl[rb]);
+        for (int rb = 0; rb < RB; ++rb) split_weights(s8[rb], ph[rb], pl[rb]);
 #pragma unroll
         for (int q = 0; q < NB; ++q) {
             f16x8 vh[4], vl[4];
@@ -1085,7 +1151,7 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb)
                         o[rb][q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            x == 0 ? vl[j] : vh[j], x == 1 ? pl[rb] : ph[rb], o[rb][q][j], 0, 0, 0);
+                            x == 0 ? vl[j] : x == 1 ? low(vh[j]) : vh[j], x == 1 ? pl[rb] : ph[rb], o[rb][q][j], 0, 0, 0);
         }
         if (tile + 4 < t1) load_v(tile + 4);
     }
