@@ -428,7 +428,8 @@ TB_API int tb_tree_attention(const float *q, const float *k_cache, const float *
                              int64_t scratch_bytes, void *stream);
 
 /*
- * Acceptance: the path starts at node 0 (which must be a root) and goes from a
+ * Acceptance: the path starts at node 0 (which must be a root; no path leads to other
+ * roots) and goes from a
  * node to its lowest child whose draft token is the node's next token, the one
  * that the model chose there (a negative token matches none).  path i32
  * [batch, n] receives the path's nodes, then -1; n_path i32 [batch] its length (0
@@ -471,7 +472,8 @@ TB_API int tb_tree_accept(const int32_t *parents, const int64_t *draft_tokens,
  * mask for all); NULL: every token.  draft_tokens i64 [rows / nodes, nodes] and
  * tree_mask [rows / nodes, nodes, ceil(nodes / 32)]: row r is node r % nodes of
  * tree r / nodes, and the draft tokens of its mask bits are part of its generated
- * history.  nodes 0: no trees.
+ * history, after the list (which ends before node 0's token, or that counts twice).
+ * nodes 0: no trees.
  * scratch: tb_process_logits_scratch bytes of device memory, needed with tokens
  * only; NULL: the stream's workspace (TB_ERR_UNSUPPORTED while capturing, since
  * graphs that are replayed side by side would share it).
@@ -613,7 +615,7 @@ TB_API int tb_decoder_accept_tree(tb_decoder *d, int64_t start_offset, const int
 
 /* Both with greedy next tokens, without reading the logits back: the forward, each
  * node's best token after the penalties over `history` (host [n_history], the first
- * prompt_len tokens prompt) and the node's own path, and the grammar mask `allowed`
+ * prompt_len tokens prompt; it ends before node 0's token) and the node's own path, and the grammar mask `allowed`
  * (host i32 [n, ceil(vocab / 32)] or NULL; tb_process_logits), then the acceptance.
  * tb_decoder_get_logits then gives the row of the path's last node (after
  * tb_decoder_verify_tree: of the tree's last one). */

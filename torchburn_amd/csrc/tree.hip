@@ -25,9 +25,11 @@ namespace {
 // a chain, so a row's words come one after the other: a thread first walks its
 // chain to the end of its own 32 nodes (at most 31 steps), and then takes whole
 // words from the nodes where the chain enters them (at most 31 more, where a walk
-// by single nodes takes 1023 twice).  Bound by the LDS reads of that chain, each
-// waiting for the one before: 3.2 us on a chain of 64 nodes (8.3 node by node), 19.7
-// on one of 1024 (117); a drafter's tree of 26 takes 1.9, the launch alone.
+// by single nodes takes 1023 twice).  A drafter's tree of 26 takes 1.9 us, the launch alone,
+// a chain of 64 nodes 3.2 (8.3 node by node).  Large trees are bound by the LDS reads
+// of the chains, each waiting for the one before, and then by the rows' words, which
+// leave one by one, a row apart from lane to lane: 64 trees of 512 take 7.7 us (5.2
+// without those stores), a chain of 1024 19.2 (8.8; 117 node by node).
 __global__ void k_tree_masks(const int32_t *__restrict__ parents, int32_t *__restrict__ mask,
                              int32_t *__restrict__ depth, int n) {
     __shared__ int par[kMaxTreeNodes], up[kMaxTreeNodes];

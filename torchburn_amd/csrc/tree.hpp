@@ -8,7 +8,7 @@
 namespace tb {
 
 constexpr int kMaxTreeNodes = 1024;      // nodes of one draft tree
-constexpr int kMaxTreeHeads = 1024;      // query heads: its row tiles fit a grid's y
+constexpr int kMaxTreeHeads = 1024;      // query heads: rows of a KV head stay below 2^20
 constexpr int kTreeLayersPerLaunch = 64; // caches that one accept launch moves rows in
 
 // parents [batch][n] -> ancestor-or-self bit masks [batch][n][ceil(n / 32)] and

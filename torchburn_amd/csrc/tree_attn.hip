@@ -1151,7 +1151,8 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb)
                         o[rb][q][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            x == 0 ? vl[j] : x == 1 ? low(vh[j]) : vh[j], x == 1 ? pl[rb] : ph[rb], o[rb][q][j], 0, 0, 0);
+                            x == 0 ? vl[j] : x == 1 ? low(vh[j]) : vh[j],
+                            x == 1 ? pl[rb] : ph[rb], o[rb][q][j], 0, 0, 0);
         }
         if (tile + 4 < t1) load_v(tile + 4);
     }
@@ -1238,7 +1239,7 @@ __global__ __launch_bounds__(256, 1) void k_tree_attn_few(TreeAttn a, int cap,
 // 256 / LC groups of LC lanes, group i with the splits i, i + 256 / LC, ...  The first
 // of those are requested before the weights are known: every split's place in the
 // scratch can be read, and what was not written has weight 0.  Bound by the launch and
-// the way of those reads: 7.1 us for 1568 rows of 26 splits, 8.6 for 2048 of 32.
+// the way of those reads: 7.1 us for 1568 rows of 27 splits, 8.6 for 2048 of 32.
 template <int LC>
 __global__ __launch_bounds__(256) void k_tree_merge(TreeAttn a, int tk, int cap, int nsplit,
                                                     const float *__restrict__ part,

@@ -423,7 +423,8 @@ class RustQwenDecoder:
                   frequency_penalty: float = 0.0, allowed=None) -> Tuple[List[int], int]:
         """One greedy speculative step over a drafted tree: verify_tree, the best token of
         every node, accept_tree, without reading the logits back.  The penalties cover
-        ``history`` (its first ``prompt_len`` tokens as prompt) and the node's own path;
+        ``history`` (its first ``prompt_len`` tokens as prompt) and the node's own path,
+        node 0's token among it: the history ends before that, or it counts twice;
         ``allowed`` is None or int32 [n, ceil(vocab / 32)], the tokens a grammar allows after
         each node (process_logits).  Returns (path, token) as accept_tree; token is -1 when
         the mask leaves nothing."""

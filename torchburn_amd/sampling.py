@@ -122,7 +122,8 @@ def _process(op: str, want_tokens: bool, logits, history, history_len, prompt_le
         raise _bad(op, "draft_tokens and tree_mask come together")
     if draft_tokens is not None:
         nodes = int(draft_tokens.shape[-1]) if draft_tokens.ndim else 0
-        if tree_mask.dtype != torch.int32 or draft_tokens.numel() != rows or not draft_tokens.ndim or \
+        if tree_mask.dtype != torch.int32 or not draft_tokens.ndim or \
+                draft_tokens.numel() != rows or \
                 tuple(tree_mask.shape) != (*draft_tokens.shape, (nodes + 31) // 32):
             raise _bad(op, f"draft_tokens [.., n] of {rows} nodes in all and tree_mask int32 "
                            f"[.., n, ceil(n / 32)] needed, got {list(draft_tokens.shape)} and "
@@ -186,7 +187,8 @@ def process_logits(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
     word t // 32 set where token t may be taken; a row without bits becomes all
     -inf.  ``draft_tokens`` (.., n) and ``tree_mask`` (.., n, ceil(n / 32)) of
     tree_masks(): row r is node r % n of tree r // n, and the tokens of the node
-    and its ancestors are part of its generated history.
+    and its ancestors are part of its generated history, after ``history`` (which
+    ends before node 0's token, or that counts twice).
 
     Returns y, a new tensor or ``out`` (which may be ``logits`` itself).  Does not
     wait for the device.  No reference counterpart beyond the repetition penalty

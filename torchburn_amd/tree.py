@@ -8,6 +8,12 @@ A tree's nodes are in topological order: ``parents[i]`` is -1 (a root: a child o
 the prefix's last token) or the index of an earlier node; anything else marks
 node i as padding, and its descendants with it.  Node i's K / V row is in the
 caches at position kv_len + i.  Batches hold trees of one node count, padded.
+Acceptance starts at node 0, usually the last token chosen: other roots are
+verified, but no path leads to them.
+
+Caches are used where they are when they are f32 on q's (parents') device with
+16-byte rows, contiguous or not.  Any others are converted whole, max_seq rows of
+them, at every call (and written back by tree_accept): keep them in that form.
 """
 from __future__ import annotations
 
@@ -90,8 +96,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     does not see take no part, whatever the caches hold there.  ``kv_len`` is a number
     (ValueError when kv_len + n exceeds max_seq) or a tensor with one per sequence (clamped
     on the device); the two may differ in their last bits, since the work is split by the
-    length known at the call.  ``scale`` defaults to head_dim ** -0.5.  f32, in q's shape; caches may
-    have any strides of 16-byte rows.  Does not wait for the device."""
+    length known at the call.  ``scale`` defaults to head_dim ** -0.5.  f32, in q's shape.
+    Does not wait for the device."""
     op = "tree_attention"
     if q.ndim not in (3, 4):
         raise _bad(op, f"q must be [n, num_heads, head_dim] or [batch, n, num_heads, head_dim], "
