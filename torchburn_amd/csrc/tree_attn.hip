@@ -419,13 +419,13 @@ __device__ __forceinline__ Range split_range(int len, int end, int tk, int cap, 
 // and then V is added in f32.  (Positions behind the prefix are few, and this is rare:
 // 49 nodes on 4096 positions take 146 us with such a node and 44 without.)
 //
-// Bound by what a SIMD can issue: a wave has 96 MFMAs and 410 to 470 vector
+// Bound by what a SIMD can issue: a wave has 96 MFMAs and 450 to 510 vector
 // instructions (limbs, exponentials, maxima, sums; eight waves, four) a tile of 32
 // positions of 128 and 32 rows, and the two overlap in part only: loops of MFMAs for
 // 36.8 ns and vector instructions for 46 take 60.7 together on one SIMD.  8 KV heads
-// of 128 in groups of 4: 49 nodes on 4096 positions 40 us, 64 on 32767 137 us (2.0 TB/s of K and V, 251
-// TFLOP/s of f32 products on three times that of f16 ones, of 1186 that a large
-// product reaches); VALU sums in f32, one wave a row, took 1344 and 14693 us.
+// of 128 in groups of 4: 49 nodes on 4096 positions 41 us, 64 on 32767 143 us (1.9 TB/s
+// of K and V, 242 TFLOP/s of f32 products on three times that of f16 ones, of 1186 that
+// a large product reaches); VALU sums in f32, one wave a row, took 1344 and 14693 us.
 template <int DP, int RB, int NW>
 __global__ __launch_bounds__(64 * NW, DP <= 128 || NW == 8 ? 2 : 1) void k_tree_attn(
     TreeAttn a, int cap, float *__restrict__ part, float *__restrict__ pml) {
