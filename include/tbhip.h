@@ -491,6 +491,108 @@ TB_API int tb_process_logits(const float *logits, float *out, int64_t *tokens, i
                              void *scratch, int64_t scratch_bytes, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/*
+ * Decoding several sequences from one shared prompt: samples side by side, or the
+ * beams of a beam search (the reference decodes one sequence over one cache,
+ * src/llm/decoder.rs:788-832).  The sequences of a group share the cache of their
+ * prompt (the prefix) and have a cache each for what they added.  Nothing here
+ * waits for the device, so all of it can be captured into a graph.  Strides are in
+ * elements, head_dim is contiguous everywhere.
+ *
+ * tb_norm_rope: head norms and position rotation of n tokens.  q f32 with strides
+ * q_st between tokens and q_sh between its num_heads heads, k and v likewise (num_kv_heads
+ * heads each).  With q_weight / k_weight f32 [head_dim] (NULL: no norm) a head x
+ * becomes x / sqrt(mean(x^2) + eps) * weight.  Then pair i of its first rotary_dim
+ * dimensions, (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1), turns by
+ * positions[token] * inv_freq[i] (f64 [rotary_dim / 2]; angles are worked out in 64
+ * bits) and is multiplied by attention_factor.  q_out f32 [n, num_heads, head_dim];
+ * k_out f32 [n, num_kv_heads, head_dim], or NULL: key and value rows go to the
+ * tokens' caches (strides sb between tokens, sh between KV heads, ss between
+ * positions) at position kv_lens[token] (device i32 [n]; where it is outside of
+ * [0, max_seq) nothing is written), or kv_len for all of them with kv_lens NULL
+ * (TB_ERR_VALUE outside).  No two cache rows may share memory.  head_dim and
+ * rotary_dim even, head_dim up to 512.
+ */
+TB_API int tb_norm_rope(const float *q, const float *k, const float *v, const int64_t *positions,
+                        const double *inv_freq, const float *q_weight, const float *k_weight,
+                        float *q_out, float *k_out, float *k_cache, float *v_cache,
+                        const int32_t *kv_lens, int64_t n, int64_t num_heads,
+                        int64_t num_kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t q_st,
+                        int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                        int64_t kc_sb, int64_t kc_sh, int64_t kc_ss, int64_t vc_sb, int64_t vc_sh,
+                        int64_t vc_ss, int64_t max_seq, int64_t kv_len, int interleaved,
+                        float attention_factor, double eps, void *stream);
+
+/*
+ * GQA attention of one token of each sequence: row r of group s sees the first
+ * prefix_lens[s] positions of its group's prefix, whose K and V are read once for
+ * all of its rows, and the first kv_lens[s * rows + r] of its own cache.  Positions
+ * past those take no part, whatever the caches hold; a row that sees none gives
+ * zeros.  q and out f32 [groups, rows, num_heads, head_dim] (query head h reads KV
+ * head h / (num_heads / num_kv_heads)); prefixes f32 with strides for group (sb),
+ * KV head (sh) and position (ss), own caches with strides for sequence (sb), KV
+ * head and position, all multiples of 4.  prefix_lens device i32 [groups], clamped
+ * to [0, max_prefix], or NULL: prefix_len for every group; kv_lens device i32
+ * [groups * rows], clamped to [0, max_seq], or NULL: kv_len for every row
+ * (TB_ERR_VALUE past the caches).  max_seq 0: no own caches.  head_dim a multiple
+ * of 32 up to 256, num_heads up to 1024; q, out and the caches 16-byte aligned.
+ * scratch: tb_prefix_attention_scratch bytes of device memory, 16-byte aligned
+ * (prefix: prefix_len, or max_prefix with prefix_lens; own: kv_len, or max_seq with
+ * kv_lens); NULL: the stream's workspace (TB_ERR_UNSUPPORTED while capturing, since
+ * graphs that are replayed side by side would share it).
+ */
+TB_API int64_t tb_prefix_attention_scratch(int64_t groups, int64_t rows, int64_t num_heads,
+                                           int64_t num_kv_heads, int64_t head_dim, int64_t prefix,
+                                           int64_t own);
+TB_API int tb_prefix_attention(const float *q, const float *k_prefix, const float *v_prefix,
+                               const int32_t *prefix_lens, const float *k_cache,
+                               const float *v_cache, const int32_t *kv_lens, float *out,
+                               int64_t groups, int64_t rows, int64_t num_heads,
+                               int64_t num_kv_heads, int64_t head_dim, int64_t max_prefix,
+                               int64_t max_seq, int64_t prefix_len, int64_t kv_len, int64_t kp_sb,
+                               int64_t kp_sh, int64_t kp_ss, int64_t vp_sb, int64_t vp_sh,
+                               int64_t vp_ss, int64_t k_sb, int64_t k_sh, int64_t k_ss,
+                               int64_t v_sb, int64_t v_sh, int64_t v_ss, float scale,
+                               void *scratch, int64_t scratch_bytes, void *stream);
+
+/*
+ * The k best continuations of each group of beams, best first.  Token t after beam
+ * b has the value scores[b] + x[b][t] - log sum_u exp x[b][u], x = logits f32
+ * [groups, beams, vocab], scores f32 [groups, beams]; worked out in 64 bits.  Of
+ * equal values the lowest beam's and then the lowest token is taken.  A beam that
+ * is finished (u8 [groups, beams], or NULL) has the one continuation eos, at its
+ * score.  Logits of -inf are never taken; a beam whose score is infinite or NaN, or
+ * that has a logit of NaN or +inf, has no continuation.  out_scores f32, tokens and
+ * beams_out i64, each [groups, k]; where fewer than k are left, -inf, -1 and -1.
+ * Up to 64 beams, k up to 64, vocabulary up to 2^20.
+ * scratch: tb_beam_select_scratch bytes of device memory, 16-byte aligned; NULL: the
+ * stream's workspace (TB_ERR_UNSUPPORTED while capturing).
+ */
+TB_API int64_t tb_beam_select_scratch(int64_t groups, int64_t beams, int64_t vocab, int64_t k);
+TB_API int tb_beam_select(const float *logits, const float *scores, const uint8_t *finished,
+                          float *out_scores, int64_t *tokens, int64_t *beams_out, int64_t groups,
+                          int64_t beams, int64_t vocab, int64_t k, int64_t eos, void *scratch,
+                          int64_t scratch_bytes, void *stream);
+
+/*
+ * Beam j of each group takes over the first kv_lens[beams_in[j]] positions (device
+ * i32 [groups, beams], the beams' lengths before the step, clamped to [0, max_seq];
+ * NULL: kv_len, TB_ERR_VALUE past max_seq) of beam beams_in[j]'s rows in each of the
+ * `layers` caches (host arrays of device pointers), in place: all beams are read
+ * before any is written, and one may be taken over many times.  beams_in i64
+ * [groups, beams]; a beam whose entry is itself or outside of [0, beams) keeps its
+ * rows, as all rows past the lengths do.  Caches f32 with strides for group (sg),
+ * beam (sb), KV head (sh) and position (ss), multiples of 4, head_dim a multiple of
+ * 32 up to 256; no cache may share memory with another or overlap itself.  Up to 64
+ * beams.
+ */
+TB_API int tb_beam_reorder(const int64_t *beams_in, const int32_t *kv_lens, int64_t kv_len,
+                           float *const *k_caches, float *const *v_caches, int64_t layers,
+                           int64_t groups, int64_t beams, int64_t num_kv_heads, int64_t head_dim,
+                           int64_t max_seq, int64_t k_sg, int64_t k_sb, int64_t k_sh, int64_t k_ss,
+                           int64_t v_sg, int64_t v_sb, int64_t v_sh, int64_t v_ss, void *stream);
+
+/* ------------------------------------------------------------------------ */
 
 typedef struct tb_decoder tb_decoder;
 

@@ -1,0 +1,211 @@
+"""beam_select and beam_reorder against their definitions: tokens, beams and moved rows have to
+be equal; a score is rounded once (2^-24 of it) and its sum of exponentials kept in 64
+bits (1e-9 allows for every rounding there)."""
+import numpy as np
+import pytest
+import torch
+
+import torchburn_amd as tb
+
+pytestmark = pytest.mark.gpu
+
+
+def select(x, scores, k, ended=None, eos=None):
+    """(scores, tokens, beams) of one group, in float64: x [B, V]."""
+    x = x.astype(np.float64)
+    B, V = x.shape
+    items = []
+    for b in range(B):
+        s = float(scores[b])
+        if not np.isfinite(s):
+            continue
+        if ended is not None and ended[b]:
+            items.append((-s, b, 0.0, eos))
+            continue
+        if np.isnan(x[b]).any() or (x[b] == np.inf).any() or (x[b] == -np.inf).all():
+            continue
+        top = x[b].max()
+        lse = np.log(np.exp(x[b] - top).sum()) + top
+        for t in np.argsort(-x[b], kind="stable")[:k]:
+            if x[b, t] > -np.inf:
+                items.append((-(x[b, t] - lse + s), b, -x[b, t], int(t)))
+    items = sorted(items)[:k]
+    items += [(np.inf, -1, 0.0, -1)] * (k - len(items))
+    return (np.array([-i[0] for i in items]), np.array([i[3] for i in items]),
+            np.array([i[1] for i in items]))
+
+
+def check(got, x, scores, k, ended=None, eos=None):
+    s, t, b = (a.cpu().numpy() for a in got)
+    G = x.shape[0]
+    assert s.shape == t.shape == b.shape == (G, k)
+    for g in range(G):
+        ws, wt, wb = select(x[g], scores[g], k, None if ended is None else ended[g], eos)
+        assert np.array_equal(t[g], wt) and np.array_equal(b[g], wb), (g, t[g], wt, b[g], wb)
+        real = wt >= 0
+        assert (np.abs(s[g][real] - ws[real]) <= 2.0 ** -24 * np.abs(ws[real]) + 1e-9).all()
+        assert np.isneginf(s[g][~real]).all()
+
+
+CASES = [
+    # groups, beams, vocab, k
+    (1, 1, 1, 1), (1, 1, 3, 5), (1, 2, 5, 4), (2, 3, 1000, 3), (1, 4, 1023, 8), (1, 4, 1024, 8),
+    (3, 4, 1025, 8), (1, 4, 32003, 8), (5, 8, 4099, 16), (2, 16, 50257, 32), (1, 64, 3001, 64),
+    (1, 1, 151936, 64), (2, 5, 128256, 10), (40, 16, 9001, 1), (1, 3, 1 << 20, 64),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("kind", ["plain", "ties", "masked"])
+def test_select(cuda, case, kind):
+    G, B, V, k = case
+    print(f"case beam_select {case} {kind}", flush=True)
+    g = np.random.default_rng(V + k)
+    x = (3 * g.standard_normal((G, B, V))).astype(np.float32)
+    scores = -np.cumsum(3 * g.random((G, B)), -1).astype(np.float32)
+    ended, eos = None, None
+    if kind == "ties":      # a few values many times, beams alike in part
+        x = np.round(x * 2) / 2
+        x[:, B // 2:] = x[:, :1]
+        scores[:, B // 2:] = scores[:, :1]
+        x[x == 0] = -0.0
+    if kind == "masked":
+        x[g.random(x.shape) < 0.7] = -np.inf
+        x[0, 0] = -np.inf           # a row without any
+        x[0, -1, 1:] = -np.inf      # and one with a single token
+        ended = g.random((G, B)) < 0.3
+        eos = V - 1
+    T = lambda a: None if a is None else torch.from_numpy(a).to(cuda)
+    got = tb.beam_select(T(x), T(scores), k=k, finished=T(ended), eos=eos)
+    check(got, x, scores, k, ended, eos)
+    if G > 1:
+        return
+    one = tb.beam_select(T(x[0]), T(scores[0]), k=k, finished=T(None if ended is None else ended[0]),
+                         eos=eos)
+    for a, b in zip(got, one):
+        assert torch.equal(a[0], b)
+
+
+def test_select_values_out_of_range(cuda):
+    """Scores of -inf, NaN, inf and very low ones; logits with NaN, inf, the lowest number; rows
+    of equal logits; the largest spread."""
+    g = np.random.default_rng(5)
+    B, V, k = 12, 5001, 24
+    x = (3 * g.standard_normal((1, B, V))).astype(np.float32)
+    scores = np.array([[0, -np.inf, np.nan, np.inf, -1e9, -3e38, -1, -2, -3, -4, -5, -6]],
+                      np.float32)
+    x[0, 6, 17] = np.nan
+    x[0, 7, 4000] = np.inf
+    x[0, 8] = np.finfo(np.float32).min      # masked by the lowest value, but for two
+    x[0, 8, 100] = x[0, 8, 99] = 2.0
+    x[0, 9] = 0.25
+    x[0, 10] = np.linspace(-3e38, 3e38, V)
+    x[0, 11] *= 200
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    check(tb.beam_select(T(x), T(scores), k=k), x, scores, k)
+    only = tb.beam_select(T(x[:, 8:10]), T(scores[:, 8:10]), k=64)
+    check(only, x[:, 8:10], scores[:, 8:10], 64)
+    # the first step: every beam the same, one of them alive
+    x[0, :] = x[0, :1]
+    scores = np.full((1, B), -np.inf, np.float32)
+    scores[0, 0] = 0
+    got = tb.beam_select(T(x), T(scores))
+    check(got, x, scores, B)
+    assert (got[2] == 0).all()
+
+
+def test_select_forms(cuda):
+    """Host tensors, halves, unaligned views, k past the candidates, no groups."""
+    x = torch.randn((2, 3, 41), dtype=torch.float16)
+    scores = torch.tensor([[0.0, -1, -2], [-3, -4, -5]])
+    got = tb.beam_select(x, scores, k=50)
+    assert all(t.device.type == "cpu" for t in got)
+    check(got, x.numpy(), scores.numpy(), 50)
+    wide = torch.randn((2, 3, 45), device=cuda)
+    check(tb.beam_select(wide[..., 1:42], scores.to(cuda), k=7), wide[..., 1:42].cpu().numpy(),
+          scores.numpy(), 7)
+    flat = torch.randn(1 + 6 * 4097, device=cuda)[1:].view(2, 3, 4097)      # 4 bytes off
+    check(tb.beam_select(flat, scores.to(cuda), k=7), flat.cpu().numpy(), scores.numpy(), 7)
+    none = tb.beam_select(torch.zeros((0, 3, 41), device=cuda), torch.zeros((0, 3), device=cuda))
+    assert none[0].shape == none[1].shape == (0, 3)
+
+
+@pytest.mark.parametrize("beams", [1, 2, 3, 4, 5, 8, 13, 16, 31, 33, 64])
+@pytest.mark.parametrize("form", ["number", "lengths"])
+def test_reorder(cuda, beams, form):
+    print(f"case beam_reorder {beams} {form}", flush=True)
+    g = np.random.default_rng(beams)
+    G, L, H, S, D = 2, 3, 2, 21, 96
+    k, v = (torch.randn((L, G, beams, H, S, D), device=cuda) for _ in range(2))
+    par = g.integers(-2, beams + 2, (G, beams))
+    par[0] = g.permutation(beams)      # a permutation in one group
+    lens = g.integers(0, S + 1, (G, beams))
+    if form == "number":
+        lens[:] = 17
+    want = []
+    for c in (k, v):
+        was, c = c.cpu().numpy(), c.cpu().numpy().copy()
+        for i in range(G):
+            for j in range(beams):
+                p = par[i, j]
+                if 0 <= p < beams:
+                    c[:, i, j, :, :lens[i, p]] = was[:, i, p, :, :lens[i, p]]
+        want.append(c)
+    n = 17 if form == "number" else torch.from_numpy(lens).to(cuda)
+    tb.beam_reorder(torch.from_numpy(par).to(cuda), list(k), list(v), n)
+    assert np.array_equal(k.cpu().numpy(), want[0]) and np.array_equal(v.cpu().numpy(), want[1])
+
+
+def test_reorder_layouts(cuda):
+    """Positions before heads, spare rows, one group without its dimension, lengths past the
+    cache, caches that are converted and written back, more layers than a launch takes."""
+    par = torch.tensor([2, 0, 0, 3], device=cuda)
+    base = torch.randn((2, 4, 11, 3, 64), device=cuda)
+    k, v = (c[:, :9].transpose(1, 2) for c in base)      # [4, 3, 9, 64]
+    rows = base.clone()
+    tb.beam_reorder(par, [k], [v], torch.tensor([5, 7, 100, -3], device=cuda))
+    want = rows.clone()
+    want[:, 0, :9] = rows[:, 2, :9]
+    want[:, 1, :5] = rows[:, 0, :5]
+    want[:, 2, :5] = rows[:, 0, :5]
+    assert torch.equal(base, want)
+    hk, hv = rows[0, :, :9].transpose(1, 2).cpu(), rows[1, :, :9].transpose(1, 2).double()
+    tb.beam_reorder(par, [hk], [hv], torch.tensor([5, 7, 100, -3], device=cuda))
+    assert torch.equal(hk, k.cpu()) and torch.equal(hv, v.double())
+    many = torch.randn((2, 70, 4, 1, 3, 32), device=cuda)
+    was = many.clone()
+    tb.beam_reorder(par, many[0], many[1], 3)
+    assert torch.equal(many, was[:, :, par])
+    tb.beam_reorder(par, [], [], 3)
+
+
+def test_captured_and_two_streams(cuda):
+    x = torch.randn((2, 4, 5000), device=cuda)
+    scores = torch.zeros((2, 4), device=cuda)
+    k, v = (torch.randn((2, 2, 4, 2, 8, 64), device=cuda) for _ in range(2))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            _, _, b = tb.beam_select(x, scores)
+            tb.beam_reorder(b, list(k), list(v), 5)
+    torch.cuda.current_stream().wait_stream(s)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = tb.beam_select(x, scores)
+            tb.beam_reorder(out[2], list(k), list(v), 5)
+        graphs.append((graph, out))
+    for step in range(4):
+        x.normal_()
+        was = k.clone()
+        graph, out = graphs[step % 2]
+        graph.replay()
+        want = tb.beam_select(x, scores)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+        for i in range(2):
+            assert torch.equal(k[:, i, :, :, :5], was[:, i, out[2][i], :, :5])
+            assert torch.equal(k[:, i, :, :, 5:], was[:, i, :, :, 5:])

@@ -8,6 +8,8 @@ meaning and error behaviour.
 from ._lib import UnsupportedOpError
 from .decoder import RustQwenDecoder, create_rust_qwen_decoder
 from .sampling import greedy_tokens, process_logits, sample_logits, sample_uniform
+from .beams import beam_reorder, beam_select, prefix_attention
+from .rotary import norm_rope, norm_rope_append, rope_frequencies
 from .tree import tree_accept, tree_attention, tree_masks
 from .quantization import (
     QuantizedLinear,
@@ -77,4 +79,10 @@ __all__ = [
     "tree_masks",
     "tree_attention",
     "tree_accept",
+    "rope_frequencies",
+    "norm_rope",
+    "norm_rope_append",
+    "prefix_attention",
+    "beam_select",
+    "beam_reorder",
 ]

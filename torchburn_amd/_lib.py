@@ -72,6 +72,10 @@ _SIGS = {
     "tb_tree_accept": [_p] * 4 + [_i64] + [_p] * 5 + [_i64] * 12 + [_p],
     "tb_process_logits": [_p] * 3 + [_i64] * 2 + [_p] * 3 + [_i64] * 3 + [C.c_float] * 3 +
                          [_p] * 5 + [_i64] * 2 + [_p, _i64, _p, _p, _i64, _p, _i64, _p],
+    "tb_norm_rope": [_p] * 12 + [_i64] * 19 + [C.c_int, C.c_float, C.c_double, _p],
+    "tb_prefix_attention": [_p] * 8 + [_i64] * 21 + [C.c_float, _p, _i64, _p],
+    "tb_beam_select": [_p] * 6 + [_i64] * 5 + [_p, _i64, _p],
+    "tb_beam_reorder": [_p, _p, _i64, _p, _p] + [_i64] * 14 + [_p],
 }
 
 
@@ -79,6 +83,7 @@ def declared_symbols() -> list:
     """Every entry point the Python layer binds (all are declared in include/tbhip.h)."""
     return ["tb_last_error", "tb_version", "tb_x_records_bytes", "tb_sample_uniform",
             "tb_w4_kernel", "tb_process_logits_scratch", "tb_tree_attention_scratch",
+            "tb_prefix_attention_scratch", "tb_beam_select_scratch",
             *_SIGS.keys()]
 
 
@@ -103,6 +108,10 @@ def lib():
             L.tb_process_logits_scratch.argtypes = [C.c_int64] * 2
             L.tb_tree_attention_scratch.restype = C.c_int64
             L.tb_tree_attention_scratch.argtypes = [C.c_int64] * 6
+            L.tb_prefix_attention_scratch.restype = C.c_int64
+            L.tb_prefix_attention_scratch.argtypes = [C.c_int64] * 7
+            L.tb_beam_select_scratch.restype = C.c_int64
+            L.tb_beam_select_scratch.argtypes = [C.c_int64] * 4
             L.tb_sample_uniform.restype = C.c_float
             L.tb_sample_uniform.argtypes = [C.c_uint64, C.c_uint64]
             for name, args in _SIGS.items():

@@ -28,6 +28,9 @@
 #include "sample.hpp"
 #include "logits.hpp"
 #include "tree.hpp"
+#include "rope.hpp"
+#include "prefix.hpp"
+#include "beam.hpp"
 
 namespace tb {
 
@@ -1210,10 +1213,12 @@ static int check_cache(const char *what, int64_t hkv, int64_t hd, int64_t max_se
 }
 
 // Whether no two elements of a cache of this geometry share memory.
-static bool disjoint(const int64_t (&st)[3], const int64_t (&size)[3], int64_t hd) {
-    std::pair<int64_t, int64_t> d[3];
-    for (int i = 0; i < 3; ++i) d[i] = {st[i], size[i]};
-    std::sort(d, d + 3);
+}  // extern "C"
+template <size_t N>
+static bool disjoint(const int64_t (&st)[N], const int64_t (&size)[N], int64_t hd) {
+    std::pair<int64_t, int64_t> d[N];
+    for (size_t i = 0; i < N; ++i) d[i] = {st[i], size[i]};
+    std::sort(d, d + N);
     int64_t extent = hd;
     for (const auto &[stride, n] : d) {
         if (n <= 1) continue;
@@ -1222,6 +1227,7 @@ static bool disjoint(const int64_t (&st)[3], const int64_t (&size)[3], int64_t h
     }
     return true;
 }
+extern "C" {
 
 int tb_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, int64_t batch, int64_t n,
                   void *stream) {
@@ -1414,6 +1420,280 @@ int tb_process_logits(const float *logits, float *out, int64_t *tokens, int64_t 
                    "TB_UNSUPPORTED: process_logits: scratch too short or not 16-byte aligned");
     }
     return launch_logits(p, scratch, st);
+}
+
+// ---- several sequences from one prompt --------------------------------------
+
+static bool strides_ok(std::initializer_list<int64_t> st) {
+    for (int64_t s : st)
+        if (s < 0 || s > ((int64_t)1 << 40)) return false;
+    return true;
+}
+
+int tb_norm_rope(const float *q, const float *k, const float *v, const int64_t *positions,
+                 const double *inv_freq, const float *q_weight, const float *k_weight,
+                 float *q_out, float *k_out, float *k_cache, float *v_cache, const int32_t *kv_lens,
+                 int64_t n, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                 int64_t rotary_dim, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+                 int64_t v_st, int64_t v_sh, int64_t kc_sb, int64_t kc_sh, int64_t kc_ss,
+                 int64_t vc_sb, int64_t vc_sh, int64_t vc_ss, int64_t max_seq, int64_t kv_len,
+                 int interleaved, float attention_factor, double eps, void *stream) {
+    const bool append = k_cache || v_cache;
+    TB_REQUIRE(head_dim > 0 && head_dim <= kMaxRopeHeadDim && head_dim % 2 == 0, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: norm_rope: head_dim must be even and up to " +
+                   std::to_string(kMaxRopeHeadDim) + ", got " + std::to_string(head_dim));
+    TB_REQUIRE(rotary_dim >= 0 && rotary_dim <= head_dim && rotary_dim % 2 == 0, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: norm_rope: rotary_dim must be even and up to head_dim, got " +
+                   std::to_string(rotary_dim));
+    TB_REQUIRE(num_heads >= 0 && num_heads <= 65535 && num_kv_heads >= 0 && num_kv_heads <= 65535,
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: norm_rope: heads outside 0..65535");
+    TB_REQUIRE(n >= 0 && n <= (1 << 28) && n * (num_heads + 2 * num_kv_heads) <= (1 << 28),
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: norm_rope: more than 2^28 heads in all");
+    TB_REQUIRE(strides_ok({q_st, q_sh, k_st, k_sh, v_st, v_sh, kc_sb, kc_sh, kc_ss, vc_sb, vc_sh,
+                           vc_ss}),
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: norm_rope: bad strides");
+    TB_REQUIRE(eps >= 0.0, TB_ERR_VALUE, "norm_rope: eps must not be negative");
+    if (append) {
+        TB_REQUIRE(max_seq >= 0 && max_seq <= (1 << 30), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: norm_rope: max_seq outside 0..2^30");
+        TB_REQUIRE(kv_lens || (kv_len >= 0 && kv_len < max_seq), TB_ERR_VALUE,
+                   "norm_rope: position " + std::to_string(kv_len) + " is outside the cache's " +
+                       std::to_string(max_seq));
+    }
+    if (n == 0 || num_heads + num_kv_heads == 0) return TB_OK;
+    TB_REQUIRE((q || !num_heads) && (q_out || !num_heads) && (k || !num_kv_heads) && positions &&
+                   (inv_freq || !rotary_dim) &&
+                   (append ? v && k_cache && v_cache && !k_out : k_out || !num_kv_heads),
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: norm_rope: null pointer, or caches beside k_out");
+    TB_REQUIRE(aligned(q, 4) && aligned(k, 4) && aligned(v, 4) && aligned(positions, 8) &&
+                   aligned(inv_freq, 8) && aligned(q_weight, 4) && aligned(k_weight, 4) &&
+                   aligned(q_out, 4) && aligned(k_out, 4) && aligned(k_cache, 4) &&
+                   aligned(v_cache, 4) && aligned(kv_lens, 4),
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: norm_rope: misaligned device pointer");
+    RopeParams p{};
+    p.q = {q, q_st, q_sh};
+    p.k = {k, k_st, k_sh};
+    p.positions = positions; p.inv_freq = inv_freq; p.qw = q_weight; p.kw = k_weight;
+    p.q_out = q_out; p.k_out = k_out;
+    if (append) {
+        // rows are written side by side: no two may share memory
+        const int64_t size[3] = {n, num_kv_heads, max_seq};
+        TB_REQUIRE(disjoint({kc_sb, kc_sh, kc_ss}, size, head_dim) &&
+                       disjoint({vc_sb, vc_sh, vc_ss}, size, head_dim) &&
+                       k_cache != v_cache,
+                   TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: norm_rope: a cache overlaps itself");
+        p.v = {v, v_st, v_sh};
+        p.kc = {k_cache, kc_sb, kc_sh, kc_ss};
+        p.vc = {v_cache, vc_sb, vc_sh, vc_ss};
+        p.at = kv_lens; p.at_all = kv_lens ? 0 : (int)kv_len; p.max_seq = (int)max_seq;
+    }
+    p.n = (int)n; p.hq = (int)num_heads; p.hkv = (int)num_kv_heads; p.hd = (int)head_dim;
+    p.rotary = (int)rotary_dim; p.interleaved = interleaved != 0;
+    p.attention_factor = attention_factor; p.eps = eps;
+    p.append = append;
+    return launch_norm_rope(p, (hipStream_t)stream);
+}
+
+// The shape of a call over `groups` prefixes of `rows` sequences each.
+static int check_prefix(int64_t groups, int64_t rows, int64_t hq, int64_t hkv, int64_t hd,
+                        int64_t prefix, int64_t own) {
+    TB_REQUIRE(hkv > 0 && hq > 0 && hq <= kMaxPrefixHeads && hq % hkv == 0, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: prefix_attention: num_heads must be a multiple of num_kv_heads, up to " +
+                   std::to_string(kMaxPrefixHeads));
+    TB_REQUIRE(groups >= 0 && groups <= 65535 && rows >= 0 && rows <= 65535 &&
+                   groups * rows * hq <= kMaxPrefixRows,
+               TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: prefix_attention: " + std::to_string(groups) + " groups of " +
+                   std::to_string(rows) + " rows; up to 65535 each, and 2^23 query heads in all");
+    TB_REQUIRE(hd >= 32 && hd <= 256 && hd % 32 == 0, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: prefix_attention: head_dim must be a multiple of 32 in 32..256, got " +
+                   std::to_string(hd));
+    TB_REQUIRE(prefix >= 0 && prefix <= (1 << 30) && own >= 0 && own <= (1 << 30), TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: prefix_attention: positions outside 0..2^30");
+    return TB_OK;
+}
+
+int64_t tb_prefix_attention_scratch(int64_t groups, int64_t rows, int64_t num_heads,
+                                    int64_t num_kv_heads, int64_t head_dim, int64_t prefix,
+                                    int64_t own) {
+    if (check_prefix(groups, rows, num_heads, num_kv_heads, head_dim, prefix, own) ||
+        groups * rows == 0)
+        return 0;
+    return (int64_t)prefix_attention_scratch((int)groups, (int)rows, (int)num_heads,
+                                             (int)num_kv_heads, (int)head_dim, (int)prefix, (int)own);
+}
+
+int tb_prefix_attention(const float *q, const float *k_prefix, const float *v_prefix,
+                        const int32_t *prefix_lens, const float *k_cache, const float *v_cache,
+                        const int32_t *kv_lens, float *out, int64_t groups, int64_t rows,
+                        int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                        int64_t max_prefix, int64_t max_seq, int64_t prefix_len, int64_t kv_len,
+                        int64_t kp_sb, int64_t kp_sh, int64_t kp_ss, int64_t vp_sb, int64_t vp_sh,
+                        int64_t vp_ss, int64_t k_sb, int64_t k_sh, int64_t k_ss, int64_t v_sb,
+                        int64_t v_sh, int64_t v_ss, float scale, void *scratch,
+                        int64_t scratch_bytes, void *stream) {
+    int rc = check_prefix(groups, rows, num_heads, num_kv_heads, head_dim, max_prefix, max_seq);
+    if (rc) return rc;
+    TB_REQUIRE(prefix_lens || (prefix_len >= 0 && prefix_len <= max_prefix), TB_ERR_VALUE,
+               "prefix_attention: a prefix of " + std::to_string(prefix_len) +
+                   " exceeds the cache's " + std::to_string(max_prefix));
+    TB_REQUIRE(kv_lens || (kv_len >= 0 && kv_len <= max_seq), TB_ERR_VALUE,
+               "prefix_attention: " + std::to_string(kv_len) + " positions exceed the cache's " +
+                   std::to_string(max_seq));
+    const int64_t strides[] = {kp_sb, kp_sh, kp_ss, vp_sb, vp_sh, vp_ss,
+                               k_sb,  k_sh,  k_ss,  v_sb,  v_sh,  v_ss};
+    for (int64_t st : strides)
+        TB_REQUIRE(st >= 0 && st % 4 == 0 && strides_ok({st}), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: prefix_attention: cache strides must be multiples of 4 elements");
+    if (groups == 0 || rows == 0) return TB_OK;
+    TB_REQUIRE(q && out && (max_prefix == 0 || (k_prefix && v_prefix)) &&
+                   (max_seq == 0 || (k_cache && v_cache)),
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: prefix_attention: null pointer");
+    TB_REQUIRE(aligned(q, 16) && aligned(out, 16) && aligned(k_prefix, 16) && aligned(v_prefix, 16) &&
+                   aligned(k_cache, 16) && aligned(v_cache, 16),
+               TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: prefix_attention: q, out and the caches must be 16-byte aligned");
+    TB_REQUIRE(aligned(prefix_lens, 4) && aligned(kv_lens, 4), TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: prefix_attention: misaligned device pointer");
+    PrefixAttn a{};
+    a.q = q; a.out = out;
+    a.kp = {k_prefix, kp_sb, kp_sh, kp_ss};
+    a.vp = {v_prefix, vp_sb, vp_sh, vp_ss};
+    a.k = {k_cache, k_sb, k_sh, k_ss};
+    a.v = {v_cache, v_sb, v_sh, v_ss};
+    a.prefix_lens = prefix_lens; a.prefix_len = prefix_lens ? 0 : (int)prefix_len;
+    a.own_lens = kv_lens; a.own_len = kv_lens ? 0 : (int)kv_len;
+    a.max_prefix = (int)max_prefix; a.max_own = (int)max_seq;
+    a.groups = (int)groups; a.rows = (int)rows;
+    a.hq = (int)num_heads; a.hkv = (int)num_kv_heads; a.hd = (int)head_dim; a.scale = scale;
+    const size_t need = prefix_attention_scratch(
+        a.groups, a.rows, a.hq, a.hkv, a.hd, prefix_lens ? a.max_prefix : a.prefix_len,
+        kv_lens ? a.max_own : a.own_len);
+    hipStream_t st = (hipStream_t)stream;
+    WsLease lease;
+    if (need && !scratch) {
+        TB_REQUIRE(!capturing(st), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: prefix_attention: a captured call needs scratch of its own");
+        if ((rc = workspace(need, st, lease))) return rc;
+        scratch = lease.ptr;
+    } else if (need) {
+        TB_REQUIRE(scratch_bytes >= (int64_t)need && aligned(scratch, 16), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: prefix_attention: scratch too short or not 16-byte aligned");
+    }
+    return launch_prefix_attention(a, static_cast<float *>(scratch), st);
+}
+
+static int check_beams(const char *what, int64_t groups, int64_t beams) {
+    TB_REQUIRE(beams >= 0 && beams <= kMaxBeams && groups >= 0 && groups <= 65535,
+               TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: " + std::string(what) + ": " + std::to_string(groups) +
+                   " groups of " + std::to_string(beams) + " beams; up to 65535 and " +
+                   std::to_string(kMaxBeams));
+    return TB_OK;
+}
+
+static int check_select(int64_t groups, int64_t beams, int64_t vocab, int64_t k) {
+    int rc = check_beams("beam_select", groups, beams);
+    if (rc) return rc;
+    TB_REQUIRE(groups * beams <= 65535, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: beam_select: more than 65535 rows");
+    TB_REQUIRE(vocab > 0 && vocab <= kMaxBeamVocab, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: beam_select: vocabulary outside 1..2^20");
+    TB_REQUIRE(k > 0 && k <= kMaxBeamResults, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: beam_select: k outside 1.." + std::to_string(kMaxBeamResults));
+    return TB_OK;
+}
+
+int64_t tb_beam_select_scratch(int64_t groups, int64_t beams, int64_t vocab, int64_t k) {
+    if (check_select(groups, beams, vocab, k) || groups * beams == 0) return 0;
+    return (int64_t)beam_select_scratch((int)groups, (int)beams, (int)vocab, (int)k);
+}
+
+int tb_beam_select(const float *logits, const float *scores, const uint8_t *finished,
+                   float *out_scores, int64_t *tokens, int64_t *beams_out, int64_t groups,
+                   int64_t beams, int64_t vocab, int64_t k, int64_t eos, void *scratch,
+                   int64_t scratch_bytes, void *stream) {
+    int rc = check_select(groups, beams, vocab, k);
+    if (rc) return rc;
+    TB_REQUIRE(beams > 0 || groups == 0, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: beam_select: no beams");
+    TB_REQUIRE(!finished || (eos >= 0 && eos < vocab), TB_ERR_VALUE,
+               "beam_select: eos " + std::to_string(eos) + " is outside the vocabulary");
+    if (groups == 0) return TB_OK;
+    TB_REQUIRE(logits && scores && out_scores && tokens && beams_out, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: beam_select: null pointer");
+    TB_REQUIRE(aligned(logits, 4) && aligned(scores, 4) && aligned(out_scores, 4) &&
+                   aligned(tokens, 8) && aligned(beams_out, 8),
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: beam_select: misaligned device pointer");
+    BeamSelect p{};
+    p.logits = logits; p.scores = scores; p.finished = finished; p.eos = finished ? eos : 0;
+    p.out_scores = out_scores; p.tokens = tokens; p.parents = beams_out;
+    p.groups = (int)groups; p.beams = (int)beams; p.vocab = (int)vocab; p.k = (int)k;
+    const size_t need = beam_select_scratch(p.groups, p.beams, p.vocab, p.k);
+    hipStream_t st = (hipStream_t)stream;
+    WsLease lease;
+    if (!scratch) {
+        TB_REQUIRE(!capturing(st), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: beam_select: a captured call needs scratch of its own");
+        if ((rc = workspace(need, st, lease))) return rc;
+        scratch = lease.ptr;
+    } else {
+        TB_REQUIRE(scratch_bytes >= (int64_t)need && aligned(scratch, 16), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: beam_select: scratch too short or not 16-byte aligned");
+    }
+    return launch_beam_select(p, scratch, st);
+}
+
+int tb_beam_reorder(const int64_t *beams_in, const int32_t *kv_lens, int64_t kv_len,
+                    float *const *k_caches, float *const *v_caches, int64_t layers, int64_t groups,
+                    int64_t beams, int64_t num_kv_heads, int64_t head_dim, int64_t max_seq,
+                    int64_t k_sg, int64_t k_sb, int64_t k_sh, int64_t k_ss, int64_t v_sg,
+                    int64_t v_sb, int64_t v_sh, int64_t v_ss, void *stream) {
+    int rc = check_beams("beam_reorder", groups, beams);
+    if (!rc)
+        rc = check_cache("beam_reorder", num_kv_heads, head_dim, max_seq, {k_sb, k_sh, k_ss},
+                         {v_sb, v_sh, v_ss});
+    if (rc) return rc;
+    TB_REQUIRE(layers >= 0 && layers <= 65535, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: beam_reorder: layers outside 0..65535");
+    TB_REQUIRE(k_sg >= 0 && v_sg >= 0 && k_sg % 4 == 0 && v_sg % 4 == 0 &&
+                   strides_ok({k_sg, k_sb, k_sh, k_ss, v_sg, v_sb, v_sh, v_ss}),
+               TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: beam_reorder: cache strides must be multiples of 4 elements");
+    TB_REQUIRE(kv_lens || (kv_len >= 0 && kv_len <= max_seq), TB_ERR_VALUE,
+               "beam_reorder: " + std::to_string(kv_len) + " positions exceed the cache's " +
+                   std::to_string(max_seq));
+    if (groups == 0 || beams == 0 || layers == 0 || max_seq == 0 || (!kv_lens && kv_len == 0))
+        return TB_OK;
+    TB_REQUIRE(beams_in && k_caches && v_caches, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: beam_reorder: null pointer");
+    TB_REQUIRE(aligned(beams_in, 8) && aligned(kv_lens, 4), TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: beam_reorder: misaligned device pointer");
+    for (int64_t l = 0; l < layers; ++l)
+        TB_REQUIRE(k_caches[l] && v_caches[l] && aligned(k_caches[l], 16) && aligned(v_caches[l], 16),
+                   TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: beam_reorder: the caches must be 16-byte aligned");
+    // rows change places: no two may share memory
+    const int64_t size[4] = {groups, beams, num_kv_heads, max_seq};
+    TB_REQUIRE(disjoint({k_sg, k_sb, k_sh, k_ss}, size, head_dim) &&
+                   disjoint({v_sg, v_sb, v_sh, v_ss}, size, head_dim),
+               TB_ERR_UNSUPPORTED, "TB_UNSUPPORTED: beam_reorder: a cache overlaps itself");
+    try {
+        std::vector<const float *> all(k_caches, k_caches + layers);
+        all.insert(all.end(), v_caches, v_caches + layers);
+        std::sort(all.begin(), all.end());
+        TB_REQUIRE(std::adjacent_find(all.begin(), all.end()) == all.end(), TB_ERR_UNSUPPORTED,
+                   "TB_UNSUPPORTED: beam_reorder: a cache is given twice");
+    } catch (const std::bad_alloc &) {
+        return fail(TB_ERR_MEMORY, "beam_reorder: out of host memory");
+    }
+    BeamReorder p{};
+    p.parents = beams_in; p.lens = kv_lens; p.len = kv_lens ? 0 : (int)kv_len;
+    p.groups = (int)groups; p.beams = (int)beams; p.layers = (int)layers;
+    p.hkv = (int)num_kv_heads; p.hd = (int)head_dim; p.max_seq = (int)max_seq;
+    p.ksg = k_sg; p.ksb = k_sb; p.ksh = k_sh; p.kss = k_ss;
+    p.vsg = v_sg; p.vsb = v_sb; p.vsh = v_sh; p.vss = v_ss;
+    return launch_beam_reorder(p, k_caches, v_caches, (hipStream_t)stream);
 }
 
 }  // extern "C"
