@@ -15,7 +15,6 @@ beam_reorder): keep them in that form.
 from __future__ import annotations
 
 import ctypes as C
-import math
 from operator import attrgetter
 from typing import Optional, Sequence, Tuple, Union
 
@@ -33,41 +32,48 @@ def _bad(op: str, msg: str) -> UnsupportedOpError:
     return UnsupportedOpError(f"{_lib.UNSUPPORTED_MARKER} {op}: {msg}")
 
 
-def _usable(c: torch.Tensor, dev: torch.device) -> bool:
-    """Whether the kernels can take a cache where it is."""
-    st = c.stride()
-    return c.dtype is torch.float32 and c.device == dev and c.data_ptr() % 16 == 0 and \
-        (st[-1] == 1 or c.shape[-1] == 1) and not any(s % 4 for s in st[:-1])
+def _usable(c: torch.Tensor, st, dev: torch.device) -> bool:
+    """Whether the kernels can take a cache of strides st where it is."""
+    if c.dtype is not torch.float32 or c.get_device() != dev.index or c.data_ptr() % 16 or \
+            (st[-1] != 1 and c.shape[-1] != 1):
+        return False
+    for s in st[:-1]:
+        if s % 4:
+            return False
+    return True
 
 
 def _copied(c: torch.Tensor, dev: torch.device) -> torch.Tensor:
-    return c.to(device=dev, dtype=torch.float32, copy=True).contiguous()
+    return c.detach().to(device=dev, dtype=torch.float32, copy=True).contiguous()
 
 
-def _cache(op: str, name: str, c: torch.Tensor, ndim: int, dev: torch.device) -> torch.Tensor:
-    if c.ndim != ndim:
+def _cache(op: str, name: str, c: torch.Tensor, ndim: int, dev: torch.device):
+    """A cache that the kernels can take, and its strides."""
+    st = c.stride()
+    if len(st) != ndim:
         raise _bad(op, f"{name} must have {ndim} dimensions, got {list(c.shape)}")
-    c = c.detach()
-    return c if _usable(c, dev) else _copied(c, dev)
+    if not _usable(c, st, dev):
+        c = _copied(c, dev)
+        st = c.stride()
+    return c, st
 
 
 def _sequences(op: str, name: str, c: torch.Tensor, batched: bool, dev: torch.device):
     """A cache of every sequence and its strides of sequence, KV head and position."""
-    c = _cache(op, name, c, 5 if batched else 4, dev)
-    st = c.stride()
+    c, st = _cache(op, name, c, 5 if batched else 4, dev)
     if not batched:
         return c, st
-    if c.shape[0] > 1 and st[0] != c.shape[1] * st[1]:      # groups apart
+    if st[0] != c.shape[1] * st[1] and c.shape[0] > 1:      # groups apart
         c = _copied(c, dev)
         st = c.stride()
     return c, st[1:]
 
 
-def _lengths(op: str, name: str, t, shape, dev) -> Tuple[Optional[torch.Tensor], int]:
+def _lengths(op: str, name: str, t, count: int, dev) -> Tuple[Optional[torch.Tensor], int]:
     if not isinstance(t, torch.Tensor):
         return None, _lib.int64(t)
-    if t.numel() != math.prod(shape) or t.dtype.is_floating_point:
-        raise _bad(op, f"{name} must be a number or {math.prod(shape)} integers, got {t.dtype} "
+    if t.numel() != count or t.dtype.is_floating_point:
+        raise _bad(op, f"{name} must be a number or {count} integers, got {t.dtype} "
                        f"{list(t.shape)}")
     return _int32_on_gpu(t, dev), 0
 
@@ -90,23 +96,24 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     same length may differ in their last bits, since the work is split by what the call
     knows.  Does not wait for the device."""
     op = "prefix_attention"
-    if q.ndim not in (3, 4):
+    shape = q.shape
+    if len(shape) not in (3, 4):
         raise _bad(op, f"q must be [rows, num_heads, head_dim] or [groups, rows, num_heads, "
-                       f"head_dim], got {list(q.shape)}")
-    dev, batched = _target(q), q.ndim == 4
-    rows, heads, hd = q.shape[-3:]
-    groups = q.shape[0] if batched else 1
-    x = _on_gpu(q.detach(), torch.float32, dev)
+                       f"head_dim], got {list(shape)}")
+    dev, batched = _target(q), len(shape) == 4
+    rows, heads, hd = shape[-3:]
+    groups = shape[0] if batched else 1
+    x = _on_gpu(q, torch.float32, dev)
     if x.data_ptr() % 16:      # a view that starts inside a 16-byte unit
-        x = x.clone()
-    kp = _cache(op, "k_prefix", k_prefix, 4 if batched else 3, dev)
-    vp = _cache(op, "v_prefix", v_prefix, 4 if batched else 3, dev)
-    kvh, max_prefix = kp.shape[-3:-1]
-    if kp.shape != vp.shape or kp.shape[-1] != hd or (batched and kp.shape[0] != groups):
+        x = x.detach().clone()
+    kp, kps = _cache(op, "k_prefix", k_prefix, 4 if batched else 3, dev)
+    vp, vps = _cache(op, "v_prefix", v_prefix, 4 if batched else 3, dev)
+    kvh, max_prefix, width = kp.shape[-3:]
+    if kp.shape != vp.shape or width != hd or (batched and kp.shape[0] != groups):
         raise _bad(op, f"prefixes {list(k_prefix.shape)} / {list(v_prefix.shape)} do not fit q "
-                       f"{list(q.shape)}")
-    kps, vps = ((kp.stride(), vp.stride()) if batched else
-                ((0, *kp.stride()), (0, *vp.stride())))
+                       f"{list(shape)}")
+    if not batched:
+        kps, vps = (0, *kps), (0, *vps)
     if (k_cache is None) != (v_cache is None):
         raise _bad(op, "k_cache and v_cache come together")
     max_own, kc, vc, ks, vs = 0, None, None, (0, 0, 0), (0, 0, 0)
@@ -114,22 +121,22 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
         kc, ks = _sequences(op, "k_cache", k_cache, batched, dev)
         vc, vs = _sequences(op, "v_cache", v_cache, batched, dev)
         max_own = kc.shape[-2]
-        if kc.shape != vc.shape or kc.shape != (*q.shape[:-2], kvh, max_own, hd):
+        if kc.shape != vc.shape or kc.shape != (*shape[:-2], kvh, max_own, hd):
             raise _bad(op, f"caches {list(k_cache.shape)} / {list(v_cache.shape)} do not fit q "
-                           f"{list(q.shape)} and {kvh} KV heads")
-    pl, p = _lengths(op, "prefix_len", prefix_len, q.shape[:-3], dev)
-    ol, o = _lengths(op, "kv_len", kv_len, q.shape[:-2], dev)
-    out = torch.empty(x.shape, dtype=torch.float32, device=dev)
+                           f"{list(shape)} and {kvh} KV heads")
+    pl, p = _lengths(op, "prefix_len", prefix_len, groups, dev)
+    ol, o = _lengths(op, "kv_len", kv_len, groups * rows, dev)
+    out = x.new_empty(shape)
     # scratch of this call's own, so that graphs captured on one stream share none
     size = _lib.lib().tb_prefix_attention_scratch(groups, rows, heads, kvh, hd,
                                                   p if pl is None else max_prefix,
                                                   o if ol is None else max_own)
-    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
-    _lib.call_on(dev, "tb_prefix_attention", _ptr(x), _ptr(kp), _ptr(vp), _ptr(pl), _ptr(kc),
-                 _ptr(vc), _ptr(ol), _ptr(out), groups, rows, heads, kvh, hd, max_prefix, max_own,
-                 p, o, kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], ks[0], ks[1], ks[2], vs[0],
-                 vs[1], vs[2], hd ** -0.5 if scale is None else float(scale), _ptr(scratch), size,
-                 _stream(dev))
+    scratch = x.new_empty((size + 3) // 4) if size > 0 else None
+    _lib.call_on(dev, "tb_prefix_attention", x.data_ptr(), kp.data_ptr(), vp.data_ptr(), _ptr(pl),
+                 _ptr(kc), _ptr(vc), _ptr(ol), out.data_ptr(), groups, rows, heads, kvh, hd,
+                 max_prefix, max_own, p, o, kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], ks[0],
+                 ks[1], ks[2], vs[0], vs[1], vs[2], hd ** -0.5 if scale is None else float(scale),
+                 _ptr(scratch), size, _stream(dev))
     return out if q.is_cuda else out.to(q.device)
 
 
@@ -150,30 +157,29 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = N
     left, tokens and beams are -1 and scores -inf.  Up to 64 beams, k up to 64.  Does not wait
     for the device."""
     op = "beam_select"
-    if logits.ndim not in (2, 3) or scores.shape != logits.shape[:-1]:
+    shape = logits.shape
+    if len(shape) not in (2, 3) or scores.shape != shape[:-1]:
         raise _bad(op, f"logits must be [.., beams, vocab] and scores [.., beams], got "
-                       f"{list(logits.shape)} and {list(scores.shape)}")
+                       f"{list(shape)} and {list(scores.shape)}")
     dev = _target(logits)
-    beams, vocab = logits.shape[-2:]
-    groups = logits.shape[0] if logits.ndim == 3 else 1
+    beams, vocab = shape[-2:]
+    groups = shape[0] if len(shape) == 3 else 1
     k = beams if k is None else _lib.int64(k)
-    x = _on_gpu(logits.detach(), torch.float32, dev)
-    sc = _on_gpu(scores.detach(), torch.float32, dev)
+    x, sc = _on_gpu(logits, torch.float32, dev), _on_gpu(scores, torch.float32, dev)
     done = None
     if finished is not None:
         if finished.shape != scores.shape or eos is None:
             raise _bad(op, f"finished {list(finished.shape)} needs the scores' shape "
                            f"{list(scores.shape)}, and eos")
         done = _on_gpu(finished if finished.dtype is torch.bool else finished != 0, torch.bool, dev)
-    shape = (*logits.shape[:-2], max(k, 0))
-    out = torch.empty(shape, dtype=torch.float32, device=dev)
-    tokens = torch.empty((2, *shape), dtype=torch.int64, device=dev)
-    tokens, parents = tokens[0], tokens[1]
+    lead = (*shape[:-2], max(k, 0))
+    out = x.new_empty(lead)
+    tokens, parents = x.new_empty((2, *lead), dtype=torch.int64).unbind(0)
     size = _lib.lib().tb_beam_select_scratch(groups, beams, vocab, k)
-    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
-    _lib.call_on(dev, "tb_beam_select", _ptr(x), _ptr(sc), _ptr(done), _ptr(out), _ptr(tokens),
-                 _ptr(parents), groups, beams, vocab, k, 0 if done is None else _lib.int64(eos),
-                 _ptr(scratch), size, _stream(dev))
+    scratch = x.new_empty(size // 4) if size > 0 else None
+    _lib.call_on(dev, "tb_beam_select", x.data_ptr(), sc.data_ptr(), _ptr(done), out.data_ptr(),
+                 tokens.data_ptr(), parents.data_ptr(), groups, beams, vocab, k,
+                 0 if done is None else _lib.int64(eos), _ptr(scratch), size, _stream(dev))
     if logits.is_cuda:
         return out, tokens, parents
     to = logits.device
@@ -203,7 +209,7 @@ def beam_reorder(beams: torch.Tensor, k_caches: Sequence[torch.Tensor],
     ks_in, vs_in = list(k_caches), list(v_caches)
     if len(ks_in) != len(vs_in):
         raise _bad(op, f"{len(ks_in)} k_caches against {len(vs_in)} v_caches")
-    lens, ln = _lengths(op, "kv_len", kv_len, beams.shape, dev)
+    lens, ln = _lengths(op, "kv_len", kv_len, groups * n, dev)
     layers, given = len(ks_in), ks_in + vs_in
     if not layers:
         return
@@ -218,12 +224,13 @@ def beam_reorder(beams: torch.Tensor, k_caches: Sequence[torch.Tensor],
         list(map(T.size, given)) == [k0.shape] * len(given) and \
         list(map(T.stride, ks_in)) == [k0.stride()] * layers and \
         list(map(T.stride, vs_in)) == [v0.stride()] * layers and \
-        not bytes(ptrs)[::8].translate(None, _ALIGNED) and _usable(k0, dev) and _usable(v0, dev)
+        not bytes(ptrs)[::8].translate(None, _ALIGNED) and _usable(k0, k0.stride(), dev) and \
+        _usable(v0, v0.stride(), dev)
     caches = given
     if not alike:
         if any(c.shape != k0.shape for c in given):
             raise _bad(op, "the layers' caches differ in shape")
-        caches = [_copied(c.detach(), dev) for c in given]
+        caches = [_copied(c, dev) for c in given]
         k0, v0 = caches[0], caches[layers]
         ptrs = (C.c_void_p * len(given))(*map(T.data_ptr, caches))
     ks, vs = k0.stride(), v0.stride()

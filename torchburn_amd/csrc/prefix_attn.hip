@@ -18,7 +18,11 @@ namespace tb {
 
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMaxSplits = 64;   // of the prefix, and of a row's own cache
@@ -46,24 +50,43 @@ __device__ __forceinline__ int length(const int32_t *lens, int len, int i, int m
     return min(max(lens ? lens[i] : len, 0), most);
 }
 
-// What one block works on: query rows i0 .. i1 - 1 of one KV head of one group (row i is
-// sequence i / G's query head i % G of the KV head's G) over the positions of one cache.
-struct Job {
-    const float *k, *v;   // the KV head's rows
+// One cache's rows of a KV head, of which the first len positions count.
+struct Rows {
+    const float *k, *v;
     int64_t ks, vs;
+    int len;
+};
+
+__device__ __forceinline__ Rows prefix_rows(const PrefixAttn &a, int group, int kvh) {
+    return {a.kp.p + group * a.kp.sb + kvh * a.kp.sh, a.vp.p + group * a.vp.sb + kvh * a.vp.sh,
+            a.kp.ss, a.vp.ss, length(a.prefix_lens, a.prefix_len, group, a.max_prefix)};
+}
+__device__ __forceinline__ Rows own_rows(const PrefixAttn &a, int seq, int kvh) {
+    return {a.k.p + seq * a.k.sb + kvh * a.k.sh, a.v.p + seq * a.v.sb + kvh * a.v.sh, a.k.ss,
+            a.v.ss, length(a.own_lens, a.own_len, seq, a.max_own)};
+}
+
+// What one block works on: query rows i0 .. i1 - 1 of one KV head of one group (row i is
+// sequence i / G's query head i % G of the KV head's G) over tiles t0 .. t1 - 1 of the positions
+// of x, followed by all of y's.
+struct Job {
+    Rows x, y;
     int group, kvh, i0, i1;
-    int slot;             // its place among the partial results
-    int t0, t1, len;      // tiles of the positions below len
-    bool none;            // this split is not among the cache's
+    int slot;   // its place among the partial results
+    int t0, t1;
+    bool none;  // nothing to do: this split is not among the cache's, and the merge skips it
 };
 
 // The plan of a launch; the blocks' order: the prefix's, then the sequences' own.
 struct Plan {
-    int rb;               // 16 * rb rows a block
+    int rb, nw;           // 16 * rb rows of a sequence a block, nw waves
+    int prows;            // rows of a group a block
     int ptiles, gtiles;   // row tiles of a group's rows, of a sequence's
     int pcap, ocap;       // splits at most
     int pblocks, oblocks;
     int slots;            // partial results a row; 1: none, the output itself
+    bool joined;          // the sequences' blocks take the prefix too
+    bool dense;           // the prefix's blocks share limbs in LDS
 };
 
 // Split `split` of a cache of len positions where at most cap are wanted: only the length
@@ -74,34 +97,33 @@ struct Range {
 };
 __device__ __forceinline__ Range split_range(int len, int cap, int split) {
     const int tiles = (len + kTile - 1) / kTile;
-    const int each = max((tiles + cap - 1) / cap, kMinTiles);
+    const int each = max(((tiles + cap - 1) / cap + 3) & ~3, kMinTiles);   // the waves' alike
     return {min(split * each, tiles), min((split + 1) * each, tiles), (tiles + each - 1) / each};
 }
 
-// KV heads first: the row tiles that read the same K and V are a multiple of the KV
-// heads apart, on one of the eight dies (block i goes to die i % 8) where those are 8.
-__device__ __forceinline__ Job job_of(const PrefixAttn &a, const Plan &p, int block) {
+// The row tiles that read the same K and V are eight blocks apart, so that they run on the
+// same of the eight dies (block i goes to die i % 8) and share its cache.
+__device__ __forceinline__ Job job_of(const PrefixAttn &a, const Plan &p, int block, bool part) {
     Job j;
     const int G = a.hq / a.hkv, rows = 16 * p.rb;
     if (block < p.pblocks) {
-        j.kvh = block % a.hkv;
-        block /= a.hkv;
-        const int rt = block % p.ptiles;
-        block /= p.ptiles;
-        const int split = block % p.pcap;
-        j.group = block / p.pcap;
-        j.i0 = rt * rows;
-        j.i1 = min(j.i0 + rows, a.rows * G);
-        j.k = a.kp.p + j.group * a.kp.sb + j.kvh * a.kp.sh;
-        j.v = a.vp.p + j.group * a.vp.sb + j.kvh * a.vp.sh;
-        j.ks = a.kp.ss;
-        j.vs = a.vp.ss;
-        j.len = length(a.prefix_lens, a.prefix_len, j.group, a.max_prefix);
-        const Range r = split_range(j.len, p.pcap, split);
+        const int rt = block / 8 % p.ptiles, unit = block / (8 * p.ptiles) * 8 + block % 8;
+        j.kvh = unit % a.hkv;
+        const int split = unit / a.hkv % p.pcap;
+        j.group = unit / (a.hkv * p.pcap);
+        j.i0 = rt * p.prows;
+        j.i1 = min(j.i0 + p.prows, a.rows * G);
+        j.slot = split;
+        j.none = true;
+        j.t0 = j.t1 = 0;
+        if (j.group >= a.groups) return j;   // the last units make eight
+        j.x = prefix_rows(a, j.group, j.kvh);
+        j.y = j.x;
+        j.y.len = 0;
+        const Range r = split_range(j.x.len, p.pcap, split);
         j.t0 = r.t0;
         j.t1 = r.t1;
-        j.none = split >= r.splits;
-        j.slot = split;
+        j.none = split >= r.splits && part;
     } else {
         block -= p.pblocks;
         j.kvh = block % a.hkv;
@@ -113,15 +135,20 @@ __device__ __forceinline__ Job job_of(const PrefixAttn &a, const Plan &p, int bl
         const int i = (seq - j.group * a.rows) * G;
         j.i0 = i + gt * rows;
         j.i1 = min(j.i0 + rows, i + G);
-        j.k = a.k.p + seq * a.k.sb + j.kvh * a.k.sh;
-        j.v = a.v.p + seq * a.v.sb + j.kvh * a.v.sh;
-        j.ks = a.k.ss;
-        j.vs = a.v.ss;
-        j.len = length(a.own_lens, a.own_len, seq, a.max_own);
-        const Range r = split_range(j.len, p.ocap, split);
-        j.t0 = r.t0;
-        j.t1 = r.t1;
-        j.none = split >= r.splits;
+        j.y = own_rows(a, seq, j.kvh);
+        if (p.joined) {
+            j.x = prefix_rows(a, j.group, j.kvh);
+            j.t0 = 0;
+            j.t1 = (j.x.len + kTile - 1) / kTile;
+            j.none = false;
+        } else {
+            j.x = j.y;
+            j.y.len = 0;
+            const Range r = split_range(j.x.len, p.ocap, split);
+            j.t0 = r.t0;
+            j.t1 = r.t1;
+            j.none = split >= r.splits && part;
+        }
         j.slot = p.pcap + split;
     }
     return j;
@@ -132,71 +159,77 @@ __device__ __forceinline__ size_t row_of(const PrefixAttn &a, const Job &j, int 
     return ((size_t)j.group * a.rows + i / G) * a.hq + j.kvh * G + i % G;
 }
 
-// A block's four waves take tiles of 16 positions in turn, each with the block's 16 * RB
-// rows and references, sums and outputs of its own, and meet in LDS once at the end.
-// Both products run on f32 MFMA (v_mfma_f32_16x16x4_f32), whose factors are as they are
-// in memory.  Lane (g, c) = (lane / 16, lane % 16) has A[c][g] and B[g][c] of a product
-// of depth 4, and gets D[4g + r][c] in register r:
+// What 16 * RB query rows have seen so far: their references, sums, and outputs of lane
+// (g, c): dimensions 64 q + 16 g + 4 r + i of row c in register r of o[..][q][i].
+template <int DP, int RB>
+struct State {
+    float m[RB], l[RB];
+    f32x4 o[RB][DP / 64][4];
+};
+
+// A wave's pass over the tiles first, first + step .. of a job, for its rows i0 + 16 rb + c
+// (those from i1 on repeat the last).  Both products run on f32 MFMA (v_mfma_f32_16x16x4_f32),
+// whose factors are as they are in memory.  Lane (g, c) = (lane / 16, lane % 16) has A[c][g]
+// and B[g][c] of a product of depth 4, and gets D[4g + r][c] in register r:
 //   S^T = K Q^T: A = position c's dimension 16 x + 4g + j, B = row c's, so that a lane
 //     has 16-byte pieces of K and Q and the products j = 0 .. 3 take them apart;
 //   O^T = V^T P^T: product j's depth g is position 4g + j, whose score the lane holds in
 //     register j for row c, and A's row c of block (q, i) is dimension 64 q + 4 c + i.
+// The next tile's K is requested when this one's scores are on their way, its V when
+// this one's outputs are.
 template <int DP, int RB>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_prefix_attn(PrefixAttn a, Plan plan,
-                                                                        float *__restrict__ part,
-                                                                        float *__restrict__ pml) {
-    constexpr int NX = DP / 16, NB = DP / 64, ROWS = 16 * RB;
-    __shared__ __attribute__((aligned(16))) float lo[ROWS][DP + 4];
-    __shared__ float lm[4][ROWS], ls[4][ROWS];
-    const Job job = job_of(a, plan, blockIdx.x);
-    if (job.none && part) return;   // the merge skips this split
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, g = lane >> 4;
-    const int D = a.hd;
+__device__ __forceinline__ void stream(const PrefixAttn &a, const Job &job, int i0, int i1, int first,
+                                       int step, State<DP, RB> &st) {
+    constexpr int NX = DP / 16, NB = DP / 64;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, D = a.hd;
+    const int xt = job.t1 - job.t0, end = xt + (job.y.len + kTile - 1) / kTile;
     float4 kr[NX], vr[4][NB];
-    auto load_k = [&](int tile) {
-        const float *r = job.k + min(tile * kTile + c, job.len - 1) * job.ks + 4 * g;
+    // Tile t of the job: its cache and first position.
+    auto rows = [&](int t) { return t < xt ? job.x : job.y; };
+    auto place = [&](int t) { return kTile * (t < xt ? job.t0 + t : t - xt); };
+    auto load_k = [&](int t) {
+        const Rows x = rows(t);
+        const float *r = x.k + min(place(t) + c, x.len - 1) * x.ks + 4 * g;
 #pragma unroll
-        for (int x = 0; x < NX; ++x)
-            if (16 * x < D) kr[x] = *reinterpret_cast<const float4 *>(r + 16 * x);
+        for (int i = 0; i < NX; ++i)
+            if (16 * i < D) kr[i] = *reinterpret_cast<const float4 *>(r + 16 * i);
     };
-    auto load_v = [&](int tile) {
+    auto load_v = [&](int t) {
+        const Rows x = rows(t);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int at = tile * kTile + 4 * g + j;
-            const float *r = job.v + min(at, job.len - 1) * job.vs;
+            const int at = place(t) + 4 * g + j;
+            const float *r = x.v + min(at, x.len - 1) * x.vs;
 #pragma unroll
             for (int q = 0; q < NB; ++q) {
                 vr[j][q] = *reinterpret_cast<const float4 *>(r + min(64 * q + 4 * c, D - 4));
                 // weight 0 must meet no infinity or NaN
-                if (at >= job.len) vr[j][q] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (at >= x.len) vr[j][q] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
         }
     };
-    const int first = job.t0 + wave;
-    if (first < job.t1) {
+    if (first < end) {
         load_k(first);
         load_v(first);
     }
     float4 qr[RB][NX];
-    float m[RB], l[RB];
-    f32x4 o[RB][NB][4];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        const int i = min(job.i0 + 16 * rb + c, job.i1 - 1);   // rows past the last repeat it
+        const int i = min(i0 + 16 * rb + c, i1 - 1);
         const float *q = a.q + row_of(a, job, i) * D + 4 * g;
 #pragma unroll
         for (int x = 0; x < NX; ++x)
             if (16 * x < D) qr[rb][x] = *reinterpret_cast<const float4 *>(q + 16 * x);
-        m[rb] = -INFINITY;
-        l[rb] = 0.f;
+        st.m[rb] = -INFINITY;
+        st.l[rb] = 0.f;
 #pragma unroll
         for (int q2 = 0; q2 < NB; ++q2)
 #pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) o[rb][q2][i2] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i2 = 0; i2 < 4; ++i2) st.o[rb][q2][i2] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const float f = a.scale * kLog2e;
 
-    for (int tile = first; tile < job.t1; tile += 4) {
+    for (int t = first; t < end; t += step) {
         // ---- scores, in powers of two
         f32x4 s[RB];
 #pragma unroll
@@ -214,41 +247,41 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_prefix_attn(PrefixAt
                         s[rb] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[j], q1, s[rb], 0, 0, 0);
                     }
             }
-        if (tile + 4 < job.t1) load_k(tile + 4);
+        if (t + step < end) load_k(t + step);
         // ---- the rows' references
         bool moved = false;
         float was[RB];
-        const int left = job.len - tile * kTile - 4 * g;
+        const int left = rows(t).len - place(t) - 4 * g;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[rb][r] = r < left ? s[rb][r] * f : -INFINITY;
-            const float top = max_over_groups(
-                fmaxf(fmaxf(s[rb][0], s[rb][1]), fmaxf(s[rb][2], s[rb][3])));
-            was[rb] = m[rb];
-            if (top > m[rb]) m[rb] = top + kLead;
-            moved |= m[rb] != was[rb];
+            const float top =
+                max_over_groups(fmaxf(fmaxf(s[rb][0], s[rb][1]), fmaxf(s[rb][2], s[rb][3])));
+            was[rb] = st.m[rb];
+            if (top > st.m[rb]) st.m[rb] = top + kLead;
+            moved |= st.m[rb] != was[rb];
         }
         if (__any(moved)) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
                 const float alpha =
-                    was[rb] == m[rb] ? 1.f : __builtin_amdgcn_exp2f(was[rb] - m[rb]);
-                l[rb] *= alpha;
+                    was[rb] == st.m[rb] ? 1.f : __builtin_amdgcn_exp2f(was[rb] - st.m[rb]);
+                st.l[rb] *= alpha;
 #pragma unroll
                 for (int q = 0; q < NB; ++q)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[rb][q][i] *= alpha;
+                    for (int i = 0; i < 4; ++i) st.o[rb][q][i] *= alpha;
             }
         }
         // ---- weights and outputs
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-            const float base = m[rb] == -INFINITY ? 0.f : m[rb];
+            const float base = st.m[rb] == -INFINITY ? 0.f : st.m[rb];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 s[rb][r] = __builtin_amdgcn_exp2f(s[rb][r] - base);
-                l[rb] += s[rb][r];
+                st.l[rb] += s[rb][r];
             }
         }
 #pragma unroll
@@ -260,80 +293,92 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_prefix_attn(PrefixAt
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int rb = 0; rb < RB; ++rb)
-                        o[rb][q][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v4[i], s[rb][j],
-                                                                          o[rb][q][i], 0, 0, 0);
+                        st.o[rb][q][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            v4[i], s[rb][j], st.o[rb][q][i], 0, 0, 0);
             }
-        if (tile + 4 < job.t1) load_v(tile + 4);
+        if (t + step < end) load_v(t + step);
     }
-
-    // ---- the four waves' outputs, normalised, in the shares of their sums, in wave order
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        l[rb] = sum_over_groups(l[rb]);
-        if (l[rb] != l[rb] && m[rb] == -INFINITY) m[rb] = INFINITY;   // only NaN seen: NaN
+        st.l[rb] = sum_over_groups(st.l[rb]);
+        // NaN and nothing else: the reference of a row that is NaN
+        if (st.l[rb] != st.l[rb] && st.m[rb] == -INFINITY) st.m[rb] = INFINITY;
+    }
+}
+
+// LDS of a block of NW waves that meet: their outputs, references, sums and shares.
+template <int DP, int RB, int NW>
+struct Meeting {
+    float o[NW][16 * RB][DP + 4];
+    float m[NW][16 * RB], l[NW][16 * RB], share[NW][16 * RB], top[16 * RB], sum[16 * RB];
+};
+
+// A block's NW waves take tiles of 16 positions in turn, each with the block's rows and a
+// state of its own, and meet in LDS once at the end.
+template <int DP, int RB, int NW>
+__device__ __forceinline__ void stream_block(const PrefixAttn &a, const Plan &plan, const Job &job,
+                                             Meeting<DP, RB, NW> &lds, float *part, float *pml) {
+    constexpr int NB = DP / 64;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, g = lane >> 4;
+    const int D = a.hd;
+    State<DP, RB> st;
+    stream<DP, RB>(a, job, job.i0, job.i1, wave, NW, st);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int r = 16 * rb + c;
         if (g == 0) {
-            lm[wave][16 * rb + c] = m[rb];
-            ls[wave][16 * rb + c] = l[rb];
+            lds.m[wave][r] = st.m[rb];
+            lds.l[wave][r] = st.l[rb];
         }
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)   // dimensions 64 q + 16 g + 4 i .. + 3
+                *reinterpret_cast<float4 *>(&lds.o[wave][r][64 * q + 16 * g + 4 * i]) =
+                    make_float4(st.o[rb][q][0][i], st.o[rb][q][1][i], st.o[rb][q][2][i],
+                                st.o[rb][q][3][i]);
     }
     __syncthreads();
-    // Row r's reference, sum and share of wave w.
-    auto shares = [&](int r, int w, float &top, float &sum) {
-        top = fmaxf(fmaxf(lm[0][r], lm[1][r]), fmaxf(lm[2][r], lm[3][r]));
-        sum = 0.f;
-        float mine = 0.f;
+    // ---- each row's reference, sum and the waves' factors: e^(m - top) over the sum
+    if (t < 16 * RB) {
+        float top = -INFINITY, sum = 0.f, e[NW];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const float y =
-                lm[x][r] == -INFINITY ? 0.f : ls[x][r] * __builtin_amdgcn_exp2f(lm[x][r] - top);
-            sum += y;
-            mine = x == w ? y : mine;
+        for (int w = 0; w < NW; ++w) top = fmaxf(top, lds.m[w][t]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float m = lds.m[w][t];
+            e[w] = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            if (e[w] != 0.f) sum = fmaf(lds.l[w][t], e[w], sum);
         }
-        return sum == 0.f ? 0.f : mine / sum;
-    };
-    float top, sum;
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const float x = shares(16 * rb + c, wave, top, sum);
-        l[rb] = l[rb] == 0.f ? 0.f : x / l[rb];
+        for (int w = 0; w < NW; ++w) lds.share[w][t] = e[w] * inv;
+        lds.top[t] = top;
+        lds.sum[t] = sum;
     }
+    __syncthreads();
+    const int cols = D / 4, n = job.i1 - job.i0, R = a.rows * (a.hq / a.hkv);
+    for (int x = t; x < n * cols; x += 64 * NW) {
+        const int r = x / cols, d = x - r * cols;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (wave == w) {
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                const int r = 16 * rb + c;
-                const float x = l[rb];
-#pragma unroll
-                for (int q = 0; q < NB; ++q)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {   // dimensions 64 q + 16 g + 4 i .. + 3
-                        float4 *d = reinterpret_cast<float4 *>(&lo[r][64 * q + 16 * g]) + i;
-                        float4 y = w ? *d : make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (x != 0.f) {
-                            y.x = fmaf(o[rb][q][0][i], x, y.x);
-                            y.y = fmaf(o[rb][q][1][i], x, y.y);
-                            y.z = fmaf(o[rb][q][2][i], x, y.z);
-                            y.w = fmaf(o[rb][q][3][i], x, y.w);
-                        }
-                        *d = y;
-                    }
+        for (int w = 0; w < NW; ++w) {
+            const float4 z = *reinterpret_cast<const float4 *>(&lds.o[w][r][4 * d]);
+            const float k = lds.share[w][r];
+            if (k != 0.f) {   // a wave that saw nothing of the row counts for nothing
+                y.x = fmaf(z.x, k, y.x);
+                y.y = fmaf(z.y, k, y.y);
+                y.z = fmaf(z.z, k, y.z);
+                y.w = fmaf(z.w, k, y.w);
             }
         }
-        __syncthreads();
-    }
-    const int cols = D / 4, n = job.i1 - job.i0, R = a.rows * (a.hq / a.hkv);
-    for (int x = t; x < n * cols; x += 256) {
-        const int r = x / cols, d = x - r * cols;
-        const float4 y = *reinterpret_cast<const float4 *>(&lo[r][4 * d]);
         if (part) {
             const size_t at =
                 (((size_t)job.group * a.hkv + job.kvh) * plan.slots + job.slot) * R + job.i0 + r;
             reinterpret_cast<float4 *>(part + at * D)[d] = y;
             if (d == 0) {
-                shares(r, 0, top, sum);
-                pml[2 * at] = top;
-                pml[2 * at + 1] = sum;
+                pml[2 * at] = lds.top[r];
+                pml[2 * at + 1] = lds.sum[r];
             }
         } else {
             reinterpret_cast<float4 *>(a.out + row_of(a, job, job.i0 + r) * D)[d] = y;
@@ -341,36 +386,325 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_prefix_attn(PrefixAt
     }
 }
 
-// A row's partial results, normalised, in the shares of their sums, a wave per row: lanes of
-// LC columns of four dimensions, 64 / LC slots side by side.
-template <int LC>
+template <int DP, int RB, int NW>
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_prefix_stream(
+    PrefixAttn a, Plan plan, float *__restrict__ part, float *__restrict__ pml) {
+    __shared__ __attribute__((aligned(16))) Meeting<DP, RB, NW> lds;
+    const Job job = job_of(a, plan, blockIdx.x, part != nullptr);
+    if (job.none) return;
+    stream_block<DP, RB, NW>(a, plan, job, lds, part, pml);
+}
+
+// ---- many rows: bf16 MFMA -------------------------------------------------------
+
+// 8 values as three bf16 limbs, x = hi + mid + lo but for 2^-27 of x: each is the
+// rounded rest of those before.  bf16 has f32's exponents, so that nothing is scaled.
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 &hi, bf16x8 &mid, bf16x8 &lo) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const f32x2 y = {x[j], x[j + 1]};
+        const bf16x2 h = __builtin_convertvector(y, bf16x2);
+        const f32x2 r = {y.x - (float)h.x, y.y - (float)h.y};
+        const bf16x2 m = __builtin_convertvector(r, bf16x2);
+        const f32x2 e = {r.x - (float)m.x, r.y - (float)m.y};
+        const bf16x2 l = __builtin_convertvector(e, bf16x2);
+        hi[j] = h.x; hi[j + 1] = h.y;
+        mid[j] = m.x; mid[j + 1] = m.y;
+        lo[j] = l.x; lo[j + 1] = l.y;
+    }
+}
+
+// d += a b of two factors of three limbs: all products but those below 2^-25 of it.
+__device__ __forceinline__ f32x16 mfma6(const bf16x8 (&a)[3], const bf16x8 (&b)[3], f32x16 d) {
+    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[2], b[0], d, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[2], d, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[1], d, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[0], d, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[1], d, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], d, 0, 0, 0);
+}
+
+// The largest of the two lanes that share a row.
+__device__ __forceinline__ float max_of_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// LDS of a dense block: a tile's limbs of 32 positions in operand order.
+template <int DP>
+struct Limbs {
+    bf16x8 k[DP / 16][3][64];      // [16 dimensions][limb][lane]
+    bf16x8 v[2][DP / 32][3][64];   // [16 positions][32 dimensions][limb][lane]
+};
+
+// A block of four waves takes 128 rows of a group, 32 a wave, and a split of the prefix in
+// tiles of 32 positions.  Per tile its waves build the limbs of K and V, a quarter each, in
+// LDS, and then every wave multiplies all of them with its rows, so that each f32 of the
+// prefix is read and split once for 128 rows; the next tile is requested before.
+// Products are of depth 16 (v_mfma_f32_32x32x16_bf16): lane (h, c) = (lane / 32, lane % 32)
+// has A[c][8h ..] and B[8h ..][c] and gets D[8 (r / 4) + 4h + r % 4][c] in register r:
+//   S^T = K Q^T: A = position c's dimensions 16 x + 8h .., B = row c's, in registers;
+//   O^T = V^T P^T: A = dimension 32 y + c's positions 16 t + 4h + (0 .. 3, 8 .. 11), which
+//     are those whose scores the lane holds for row c.
+// Every product of f32 factors is six of limbs (mfma6): 22 bits and more of it, at a sixth
+// of the bf16 rate, where the f32 MFMA has a sixteenth.  An infinity or NaN among K, V or
+// the queries makes NaN of the limbs' products: a wave that has one in its results
+// works its rows out anew in f32 (stream()).
+template <int DP>
+__device__ __forceinline__ void dense_block(const PrefixAttn &a, const Plan &plan, const Job &job,
+                                            Limbs<DP> &lds, float *part, float *pml) {
+    constexpr int NX = DP / 16, NY = DP / 32, KD = DP / 8, U = DP / 64;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 31, h = lane >> 5;
+    const int D = a.hd, G = a.hq / a.hkv, R = a.rows * G;
+    const int t0 = job.t0 / 2, t1 = (job.t1 + 1) / 2, len = job.x.len;
+
+    // ---- this thread's parts of a tile: 8 dimensions kd .. of position kp, and 8 positions
+    // of dimension vd
+    float kr[U][8], vr[U][8];
+    auto load = [&](int tile) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int kd = t % KD, kp = (t + 256 * u) / KD;
+            const float *k = job.x.k + min(32 * tile + kp, len - 1) * job.x.ks + min(8 * kd, D - 8);
+            const float4 x = reinterpret_cast<const float4 *>(k)[0];
+            const float4 y = reinterpret_cast<const float4 *>(k)[1];
+            kr[u][0] = x.x; kr[u][1] = x.y; kr[u][2] = x.z; kr[u][3] = x.w;
+            kr[u][4] = y.x; kr[u][5] = y.y; kr[u][6] = y.z; kr[u][7] = y.w;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int vd = t % DP, th = (t + 256 * u) / DP;   // positions 16 (th / 2) + 4 (th % 2) ..
+            const int p0 = 32 * tile + 16 * (th >> 1) + 4 * (th & 1);
+            const float *v = job.x.v + min(vd, D - 1);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int at = p0 + 8 * (i >> 2) + (i & 3);
+                vr[u][i] = v[min(at, len - 1) * job.x.vs];
+                if (at >= len) vr[u][i] = 0.f;   // weight 0 must meet no infinity or NaN
+            }
+        }
+    };
+    auto store = [&]() {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            // lanes are swapped within 16 by the dimensions, or a wave's stores would meet in
+            // a quarter of the banks
+            const int kd = t % KD, kp = (t + 256 * u) / KD;
+            const int at = (kp + 32 * (kd & 1)) ^ (kd * (16 / KD));
+            bf16x8 x[3];
+            split8(kr[u], x[0], x[1], x[2]);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) lds.k[kd >> 1][i][at] = x[i];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int vd = t % DP, th = (t + 256 * u) / DP;
+            bf16x8 x[3];
+            split8(vr[u], x[0], x[1], x[2]);
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                lds.v[th >> 1][vd >> 5][i][(vd & 31) + 32 * (th & 1)] = x[i];
+        }
+    };
+    if (t0 < t1) load(t0);
+
+    // ---- the wave's query rows, row c in this lane; with the sign of the score's factor
+    const int w0 = job.i0 + 32 * wave;
+    const bool busy = w0 < job.i1;
+    const float f = fabsf(a.scale) * kLog2e;
+    bf16x8 q[NX][3];
+    {
+        const float *x = a.q + row_of(a, job, min(w0 + c, R - 1)) * D + 8 * h;
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+            float y[8];
+            const bool in = 16 * i < D;
+            const float4 u = reinterpret_cast<const float4 *>(x + (in ? 16 * i : 0))[0];
+            const float4 v = reinterpret_cast<const float4 *>(x + (in ? 16 * i : 0))[1];
+            y[0] = u.x; y[1] = u.y; y[2] = u.z; y[3] = u.w;
+            y[4] = v.x; y[5] = v.y; y[6] = v.z; y[7] = v.w;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = a.scale < 0.f ? -y[j] : y[j];
+            split8(y, q[i][0], q[i][1], q[i][2]);
+        }
+    }
+    float m = -INFINITY, l = 0.f;
+    f32x16 o[NY];
+#pragma unroll
+    for (int y = 0; y < NY; ++y)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[y][r] = 0.f;
+
+    for (int tile = t0; tile < t1; ++tile) {
+        __syncthreads();
+        store();
+        if (tile + 1 < t1) load(tile + 1);
+        __syncthreads();
+        if (!busy) continue;
+        // ---- scores
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int x = 0; x < NX; ++x)
+            if (16 * x < D) {
+                bf16x8 k[3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) k[i] = lds.k[x][i][lane ^ ((2 * x + h) * (16 / KD))];
+                s = mfma6(k, q[x], s);
+            }
+        // ---- the rows' references, in powers of two
+        const int left = len - 32 * tile - 4 * h;
+        if (left < 32 - 4 * h) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (8 * (r >> 2) + (r & 3) >= left) s[r] = -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+        top = max_of_halves(top) * f;
+        if (__any(top > m)) {
+            const float was = m;
+            if (top > m) m = top + kLead;
+            const float alpha = was == m ? 1.f : __builtin_amdgcn_exp2f(was - m);
+            l *= alpha;
+#pragma unroll
+            for (int y = 0; y < NY; ++y)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[y][r] *= alpha;
+        }
+        // ---- weights and outputs
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + i], f, -base));
+                l += w[i];
+            }
+            bf16x8 p[3];
+            split8(w, p[0], p[1], p[2]);
+#pragma unroll
+            for (int y = 0; y < NY; ++y)
+                if (32 * y < D) {
+                    bf16x8 v[3];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) v[i] = lds.v[u][y][i][lane];
+                    o[y] = mfma6(v, p, o[y]);
+                }
+        }
+    }
+    if (!busy) return;
+    l = sum_of_halves(l);
+    const bool row = w0 + c < job.i1;
+    bool bad = !(l <= 3.4e38f);
+#pragma unroll
+    for (int y = 0; y < NY; ++y)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bad |= 32 * y < D && !(fabsf(o[y][r]) <= 3.4e38f);
+    const size_t slot = (((size_t)job.group * a.hkv + job.kvh) * plan.slots + job.slot) * R;
+    if (__builtin_expect(__any(bad && row), 0)) {
+        const int c16 = lane & 15, g16 = lane >> 4;
+        State<DP, 2> st;
+        stream<DP, 2>(a, job, w0, min(w0 + 32, job.i1), 0, 1, st);
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            const int i = w0 + 16 * rb + c16;
+            if (i >= job.i1) continue;
+            const float inv = st.l[rb] == 0.f ? 0.f : 1.0f / st.l[rb];
+            float *to = part ? part + (slot + i) * D : a.out + row_of(a, job, i) * D;
+            if (part && g16 == 0) {
+                pml[2 * (slot + i)] = st.m[rb];
+                pml[2 * (slot + i) + 1] = st.l[rb];
+            }
+#pragma unroll
+            for (int y = 0; y < DP / 64; ++y)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (64 * y + 16 * g16 < D)
+                        *reinterpret_cast<float4 *>(to + 64 * y + 16 * g16 + 4 * r) =
+                            make_float4(st.o[rb][y][0][r] * inv, st.o[rb][y][1][r] * inv,
+                                        st.o[rb][y][2][r] * inv, st.o[rb][y][3][r] * inv);
+        }
+        return;
+    }
+    if (!row) return;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const int i = w0 + c;
+    float *to = part ? part + (slot + i) * D : a.out + row_of(a, job, i) * D;
+    if (part && h == 0) {
+        pml[2 * (slot + i)] = m;
+        pml[2 * (slot + i) + 1] = l;
+    }
+#pragma unroll
+    for (int y = 0; y < NY; ++y)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            if (32 * y < D)
+                *reinterpret_cast<float4 *>(to + 32 * y + 2 * r + 4 * h) = make_float4(
+                    o[y][r] * inv, o[y][r + 1] * inv, o[y][r + 2] * inv, o[y][r + 3] * inv);
+}
+
+template <int DP, int RB>
+__global__ __launch_bounds__(256, 2) void k_prefix_dense(PrefixAttn a, Plan plan,
+                                                         float *__restrict__ part,
+                                                         float *__restrict__ pml) {
+    __shared__ __attribute__((aligned(16))) union {
+        Limbs<DP> limbs;
+        Meeting<DP, RB, 4> meeting;
+    } lds;
+    const Job job = job_of(a, plan, blockIdx.x, part != nullptr);
+    if (job.none) return;
+    if ((int)blockIdx.x < plan.pblocks)
+        dense_block<DP>(a, plan, job, lds.limbs, part, pml);
+    else
+        stream_block<DP, RB, 4>(a, plan, job, lds.meeting, part, pml);
+}
+
+// A row's partial results, normalised, in the shares of their sums, in the order of the slots, by
+// WR waves: groups of LC lanes of four dimensions each take every 64 WR / LC-th slot, the
+// first of them requested before the shares are known (every slot's place in the scratch
+// can be read, and what was not written has a share of 0).
+template <int LC, int WR>
 __global__ __launch_bounds__(256) void k_prefix_merge(PrefixAttn a, Plan plan,
                                                       const float *__restrict__ part,
                                                       const float *__restrict__ pml) {
-    constexpr int NG = 64 / LC;
+    constexpr int NG = 64 * WR / LC, AHEAD = 8;
     __shared__ float w[4][2 * kMaxSplits];
+    __shared__ float4 col[4][LC];
     const int G = a.hq / a.hkv, R = a.rows * G, cols = a.hd / 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int i = blockIdx.x * 4 + wave, kvh = blockIdx.y, group = blockIdx.z;
-    if (i >= R) return;
+    const int i = blockIdx.x * (4 / WR) + wave / WR, kvh = blockIdx.y, group = blockIdx.z;
+    if (WR == 1 && i >= R) return;
+    const size_t at = ((size_t)group * a.hkv + kvh) * plan.slots * R + i;
+    const int d = min(lane % LC, cols - 1), grp = (threadIdx.x % (64 * WR)) / LC;
+    const float4 *src = reinterpret_cast<const float4 *>(part + at * a.hd) + d;
+    const size_t step = (size_t)R * cols;
+    float4 z[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) z[k] = src[min(grp + NG * k, plan.slots - 1) * step];
+    float m[2], l[2], top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const float *p = pml + 2 * (at + (size_t)min(lane + 64 * x, plan.slots - 1) * R);
+        m[x] = p[0];
+        l[x] = p[1];
+    }
     const int pu = split_range(length(a.prefix_lens, a.prefix_len, group, a.max_prefix), plan.pcap, 0)
                        .splits;
     const int ou = split_range(length(a.own_lens, a.own_len, group * a.rows + i / G, a.max_own),
                                plan.ocap, 0)
                        .splits;
-    const int used = pu + ou;
-    auto slot = [&](int x) { return x < pu ? x : plan.pcap + x - pu; };
-    const size_t at = ((size_t)group * a.hkv + kvh) * plan.slots * R + i;
-    float m[2], l[2], top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-        m[x] = -INFINITY;
-        l[x] = 0.f;
-        if (lane + 64 * x < used) {
-            const float *p = pml + 2 * (at + (size_t)slot(lane + 64 * x) * R);
-            m[x] = p[0];
-            l[x] = p[1];
-        }
+        const int s = lane + 64 * x;
+        if (!(s < pu || (s >= plan.pcap && s < plan.pcap + ou))) m[x] = -INFINITY;
         top = fmaxf(top, m[x]);
     }
 #pragma unroll
@@ -388,27 +722,34 @@ __global__ __launch_bounds__(256) void k_prefix_merge(PrefixAttn a, Plan plan,
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const int d = min(lane % LC, cols - 1), grp = lane / LC;
-    const float4 *src = reinterpret_cast<const float4 *>(part + at * a.hd) + d;
-    const size_t step = (size_t)R * cols;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = grp; s < used; s += NG) {
+    auto add = [&](int s, const float4 &v) {
         const float x = w[wave][s];
-        const float4 v = src[slot(s) * step];
         if (x != 0.f) {   // a split that sees nothing of the row counts for nothing
             y.x = fmaf(v.x, x, y.x);
             y.y = fmaf(v.y, x, y.y);
             y.z = fmaf(v.z, x, y.z);
             y.w = fmaf(v.w, x, y.w);
         }
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+        if (grp + NG * k < plan.slots) add(grp + NG * k, z[k]);
+    for (int s = grp + NG * AHEAD; s < plan.slots; s += NG) add(s, src[s * step]);
 #pragma unroll
     for (int o = LC; o < 64; o <<= 1) {
         y.x += __shfl_xor(y.x, o);
         y.y += __shfl_xor(y.y, o);
         y.z += __shfl_xor(y.z, o);
         y.w += __shfl_xor(y.w, o);
+    }
+    if (WR == 4) {
+        if (lane < LC) col[wave][lane] = y;
+        __syncthreads();
+        if ((int)threadIdx.x >= cols) return;
+        const float4 y0 = col[0][d], y1 = col[1][d], y2 = col[2][d], y3 = col[3][d];
+        y = make_float4((y0.x + y1.x) + (y2.x + y3.x), (y0.y + y1.y) + (y2.y + y3.y),
+                        (y0.z + y1.z) + (y2.z + y3.z), (y0.w + y1.w) + (y2.w + y3.w));
     }
     if (lane >= cols) return;
     float *out = a.out + (((size_t)group * a.rows + i / G) * a.hq + kvh * G + i % G) * a.hd;
@@ -419,21 +760,43 @@ __global__ __launch_bounds__(256) void k_prefix_merge(PrefixAttn a, Plan plan,
 Plan plan_of(int groups, int rows, int hq, int hkv, int hd, int prefix, int own) {
     Plan p{};
     const int G = hq / hkv, R = rows * G;
-    p.rb = R <= 16 || hd > 128 ? 1 : 2;
-    p.ptiles = (R + 16 * p.rb - 1) / (16 * p.rb);
+    const int pt = (prefix + kTile - 1) / kTile, ot = (own + kTile - 1) / kTile;
+    const int64_t seqs = (int64_t)groups * rows;
+    // Short caches: a sequence's block reads the prefix for itself, and nothing is merged.
+    p.joined = pt + ot <= 32;
+    p.dense = !p.joined && R > 64 && hd <= 128;
+    p.rb = (p.joined || p.dense ? G : R) <= 16 || hd > 128 ? 1 : 2;
+    p.nw = p.joined && hd <= 128 ? 8 : 4;
+    p.prows = p.dense ? 128 : 16 * p.rb;
+    p.ptiles = (R + p.prows - 1) / p.prows;
     p.gtiles = (G + 16 * p.rb - 1) / (16 * p.rb);
-    auto cap = [](int64_t blocks, int len) {
-        const int tiles = (len + kTile - 1) / kTile;
+    if (p.joined) {
+        p.ocap = p.slots = 1;
+        p.oblocks = (int)(seqs * hkv * p.gtiles);
+        return p;
+    }
+    auto cap = [](int64_t want, int64_t blocks, int tiles) {
         const int64_t most = std::min<int64_t>((tiles + kMinTiles - 1) / kMinTiles, kMaxSplits);
-        return (int)std::max<int64_t>(1, std::min<int64_t>(512 / blocks, most));
+        return (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, most));
     };
-    const int64_t pb = (int64_t)groups * hkv * p.ptiles, ob = (int64_t)groups * rows * hkv * p.gtiles;
-    p.pcap = prefix || !own ? cap(pb, prefix) : 0;   // without positions: the zeros
-    p.ocap = own ? cap(ob, own) : 0;
-    p.pblocks = (int)(pb * p.pcap);
+    const int64_t units = (int64_t)groups * hkv, ob = seqs * hkv * p.gtiles;
+    p.pcap = pt ? cap(p.dense ? 512 : 256, units * p.ptiles, pt) : 0;
+    p.ocap = ot ? cap(256, ob, ot) : 0;
+    p.pblocks = (int)((units * p.pcap + 7) / 8 * 8 * p.ptiles);
     p.oblocks = (int)(ob * p.ocap);
     p.slots = p.pcap + p.ocap;
     return p;
+}
+
+template <int LC>
+void merge(const PrefixAttn &a, const Plan &p, const float *part, const float *pml, hipStream_t s) {
+    const int R = a.rows * (a.hq / a.hkv);
+    if (p.slots > 8)
+        hipLaunchKernelGGL((k_prefix_merge<LC, 4>), dim3(R, a.hkv, a.groups), dim3(256), 0, s, a, p,
+                           part, pml);
+    else
+        hipLaunchKernelGGL((k_prefix_merge<LC, 1>), dim3((R + 3) / 4, a.hkv, a.groups), dim3(256), 0,
+                           s, a, p, part, pml);
 }
 
 }  // namespace
@@ -444,35 +807,46 @@ size_t prefix_attention_scratch(int groups, int rows, int hq, int hkv, int hd, i
 }
 
 int launch_prefix_attention(const PrefixAttn &a, float *scratch, hipStream_t s) {
-    const Plan p = plan_of(a.groups, a.rows, a.hq, a.hkv, a.hd, a.prefix_lens ? a.max_prefix : a.prefix_len,
+    const Plan p = plan_of(a.groups, a.rows, a.hq, a.hkv, a.hd,
+                           a.prefix_lens ? a.max_prefix : a.prefix_len,
                            a.own_lens ? a.max_own : a.own_len);
     float *part = p.slots > 1 ? scratch : nullptr;
     const size_t rows = (size_t)a.groups * a.rows * a.hq;
     float *pml = part ? part + rows * p.slots * a.hd : nullptr;
     const dim3 grid(p.pblocks + p.oblocks);
-#define TB_PA(DP, RB)                                                                       \
-    hipLaunchKernelGGL((k_prefix_attn<DP, RB>), grid, dim3(256), 0, s, a, p, part, pml)
-    if (a.hd <= 64) {
-        if (p.rb == 1) TB_PA(64, 1);
-        else TB_PA(64, 2);
+#define TB_PS(DP, RB, NW)                                                                   \
+    if (p.rb == RB && p.nw == NW)                                                           \
+    hipLaunchKernelGGL((k_prefix_stream<DP, RB, NW>), grid, dim3(64 * NW), 0, s, a, p, part, pml)
+#define TB_PD(DP, RB)                                                                       \
+    if (p.rb == RB)                                                                         \
+    hipLaunchKernelGGL((k_prefix_dense<DP, RB>), grid, dim3(256), 0, s, a, p, part, pml)
+    if (p.dense && a.hd <= 64) {
+        TB_PD(64, 1);
+        TB_PD(64, 2);
+    } else if (p.dense) {
+        TB_PD(128, 1);
+        TB_PD(128, 2);
+    } else if (a.hd <= 64) {
+        TB_PS(64, 1, 4);
+        TB_PS(64, 2, 4);
+        TB_PS(64, 1, 8);
+        TB_PS(64, 2, 8);
     } else if (a.hd <= 128) {
-        if (p.rb == 1) TB_PA(128, 1);
-        else TB_PA(128, 2);
+        TB_PS(128, 1, 4);
+        TB_PS(128, 2, 4);
+        TB_PS(128, 1, 8);
+        TB_PS(128, 2, 8);
     } else {
-        TB_PA(256, 1);
+        TB_PS(256, 1, 4);
     }
-#undef TB_PA
+#undef TB_PD
+#undef TB_PS
     TB_LAUNCHED();
     if (part) {
-        const dim3 blocks((a.rows * (a.hq / a.hkv) + 3) / 4, a.hkv, a.groups);
-        if (a.hd <= 32)
-            hipLaunchKernelGGL(k_prefix_merge<8>, blocks, dim3(256), 0, s, a, p, part, pml);
-        else if (a.hd <= 64)
-            hipLaunchKernelGGL(k_prefix_merge<16>, blocks, dim3(256), 0, s, a, p, part, pml);
-        else if (a.hd <= 128)
-            hipLaunchKernelGGL(k_prefix_merge<32>, blocks, dim3(256), 0, s, a, p, part, pml);
-        else
-            hipLaunchKernelGGL(k_prefix_merge<64>, blocks, dim3(256), 0, s, a, p, part, pml);
+        if (a.hd <= 32) merge<8>(a, p, part, pml, s);
+        else if (a.hd <= 64) merge<16>(a, p, part, pml, s);
+        else if (a.hd <= 128) merge<32>(a, p, part, pml, s);
+        else merge<64>(a, p, part, pml, s);
         TB_LAUNCHED();
     }
     return TB_OK;

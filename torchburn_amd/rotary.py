@@ -80,72 +80,72 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optional[
 def _heads(op: str, name: str, t: torch.Tensor, lead, hd: int, dev):
     """(tensor, heads, token stride, head stride): the caller's memory where a token's heads
     are a constant number of elements apart and the tokens too, else a copy."""
-    if t.ndim < 2 or t.shape[:-2] != lead or t.shape[-1] != hd:
+    shape = t.shape
+    if len(shape) < 2 or shape[:-2] != lead or shape[-1] != hd:
         raise _bad(op, f"{name} must be [{', '.join(map(str, lead))}, heads, {hd}], got "
-                       f"{list(t.shape)}")
-    t = t.detach()
-    if t.dtype is not torch.float32 or t.device != dev or (hd > 1 and t.stride(-1) != 1):
-        t = _on_gpu(t, torch.float32, dev)
-    heads = int(t.shape[-2])
-    if t.ndim == 3:
-        st, sh, _ = t.stride()
-        return t, heads, st, sh
-    if t.ndim == 2:
-        return t, heads, 0, t.stride(0)
+                       f"{list(shape)}")
+    st = t.stride()
+    if t.dtype is not torch.float32 or t.get_device() != dev.index or (st[-1] != 1 and hd > 1):
+        t = _on_gpu(t.detach(), torch.float32, dev)
+        st = t.stride()
+    if len(shape) == 3:
+        return t, shape[1], st[0], st[1]
+    if len(shape) == 2:
+        return t, shape[0], 0, st[0]
+    flat = _flat(t.detach(), 2)
+    return flat, shape[-2], flat.stride(0), flat.stride(1)
+
+
+def _flat(t: torch.Tensor, last: int) -> torch.Tensor:
+    """t with one dimension before its last ones: a view, or a copy where there is none."""
     try:
-        flat = t.view(-1, heads, hd)
+        return t.view(-1, *t.shape[-last:])
     except RuntimeError:
-        flat = t.reshape(-1, heads, hd)
-    st, sh, _ = flat.stride()
-    return flat, heads, st, sh
+        return t.reshape(-1, *t.shape[-last:])
 
 
-def _own_caches(op: str, name: str, c: torch.Tensor, shape, dev):
+def _own_caches(op: str, name: str, c: torch.Tensor, lead, heads: int, hd: int, dev):
     """A cache [.., heads, positions, head_dim] as an f32 device tensor whose sequences are a
     constant number of elements apart, and those strides: the caller's memory or a copy."""
-    if c.ndim < 3 or (*c.shape[:-2], c.shape[-1]) != shape:
-        raise _bad(op, f"{name} must be [{', '.join(map(str, shape[:-1]))}, max_seq, {shape[-1]}], "
-                       f"got {list(c.shape)}")
-    c = c.detach()
-    if c.dtype is not torch.float32 or c.device != dev or (c.shape[-1] > 1 and c.stride(-1) != 1):
-        c = c.to(device=dev, dtype=torch.float32, copy=True).contiguous()
-    if c.ndim == 4:
-        return c, c.stride()
-    if c.ndim == 3:
-        return c, (0, *c.stride())
-    try:
-        return c, c.view(-1, *c.shape[-3:]).stride()
-    except RuntimeError:
-        c = c.clone(memory_format=torch.contiguous_format)
-        return c, c.view(-1, *c.shape[-3:]).stride()
+    shape = c.shape
+    if len(shape) < 3 or shape[:-3] != lead or shape[-3] != heads or shape[-1] != hd:
+        raise _bad(op, f"{name} must be [{', '.join(map(str, lead))}, {heads}, max_seq, {hd}], "
+                       f"got {list(shape)}")
+    st = c.stride()
+    if c.dtype is not torch.float32 or c.get_device() != dev.index or (st[-1] != 1 and hd > 1):
+        c = c.detach().to(device=dev, dtype=torch.float32, copy=True).contiguous()
+        st = c.stride()
+    if len(shape) == 4:
+        return c, st
+    if len(shape) == 3:
+        return c, (0, *st)
+    flat = _flat(c.detach(), 3)
+    return flat, flat.stride()
 
 
 def _call(op, q, k, v, positions, inv_freq, q_weight, k_weight, eps, interleaved,
           attention_factor, k_cache, v_cache, at):
     if q.ndim < 2:
         raise _bad(op, f"q must be [.., num_heads, head_dim], got {list(q.shape)}")
-    dev, lead, hd = _target(q), q.shape[:-2], int(q.shape[-1])
+    dev, lead, hd = _target(q), q.shape[:-2], q.shape[-1]
     x, hq, q_st, q_sh = _heads(op, "q", q, lead, hd, dev)
     y, hkv, k_st, k_sh = _heads(op, "k", k, lead, hd, dev)
-    n = 1
-    for s in lead:
-        n *= int(s)
     if not isinstance(positions, torch.Tensor) or positions.shape != lead or \
             positions.dtype.is_floating_point:
         raise _bad(op, f"positions must be integers {list(lead)}, one a token")
-    if inv_freq.ndim != 1 or 2 * inv_freq.shape[0] > hd:
+    pairs = inv_freq.shape[0] if inv_freq.ndim == 1 else hd
+    if 2 * pairs > hd:
         raise _bad(op, f"inv_freq must hold at most head_dim / 2 = {hd // 2} frequencies, got "
                        f"{list(inv_freq.shape)}")
     pos = _on_gpu(positions, torch.int64, dev)
-    freq = _on_gpu(inv_freq.detach(), torch.float64, dev)
-    weights = []
+    freq = _on_gpu(inv_freq, torch.float64, dev)
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and w.shape != (hd,):
+        if w is not None and (w.ndim != 1 or w.shape[0] != hd):
             raise _bad(op, f"{name} must be [{hd}], got {list(w.shape)}")
-        weights.append(None if w is None else _on_gpu(w.detach(), torch.float32, dev))
-    out = torch.empty((*lead, hq, hd), dtype=torch.float32, device=dev)
+    qw, kw = _on_gpu(q_weight, torch.float32, dev), _on_gpu(k_weight, torch.float32, dev)
+    out = x.new_empty((*lead, hq, hd))
     if v is None:
-        k_out = torch.empty((*lead, hkv, hd), dtype=torch.float32, device=dev)
+        k_out = x.new_empty((*lead, hkv, hd))
         z = kc = vc = lens = None
         v_st = v_sh = where = rows = 0
         ks = vs = (0, 0, 0, 0)
@@ -154,9 +154,9 @@ def _call(op, q, k, v, positions, inv_freq, q_weight, k_weight, eps, interleaved
         z, v_heads, v_st, v_sh = _heads(op, "v", v, lead, hd, dev)
         if v_heads != hkv:
             raise _bad(op, f"k has {hkv} heads, v {v_heads}")
-        kc, ks = _own_caches(op, "k_cache", k_cache, (*lead, hkv, hd), dev)
-        vc, vs = _own_caches(op, "v_cache", v_cache, (*lead, hkv, hd), dev)
-        rows = int(kc.shape[-2])
+        kc, ks = _own_caches(op, "k_cache", k_cache, lead, hkv, hd, dev)
+        vc, vs = _own_caches(op, "v_cache", v_cache, lead, hkv, hd, dev)
+        rows = kc.shape[-2]
         if vc.shape[-2] != rows:
             raise _bad(op, f"k_cache has {rows} positions, v_cache {vc.shape[-2]}")
         if isinstance(at, torch.Tensor):
@@ -166,14 +166,16 @@ def _call(op, q, k, v, positions, inv_freq, q_weight, k_weight, eps, interleaved
             lens, where = _int32_on_gpu(at, dev), 0
         else:
             lens, where = None, _lib.int64(at)
-    _lib.call_on(dev, "tb_norm_rope", _ptr(x), _ptr(y), _ptr(z), _ptr(pos), _ptr(freq),
-                 _ptr(weights[0]), _ptr(weights[1]), _ptr(out), _ptr(k_out), _ptr(kc), _ptr(vc),
-                 _ptr(lens), n, hq, hkv, hd, 2 * freq.shape[0], q_st, q_sh, k_st, k_sh, v_st, v_sh,
-                 ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], rows, where, int(bool(interleaved)),
-                 float(attention_factor), float(eps), _stream(dev))
+    _lib.call_on(dev, "tb_norm_rope", x.data_ptr(), y.data_ptr(), _ptr(z), pos.data_ptr(),
+                 freq.data_ptr(), _ptr(qw), _ptr(kw), out.data_ptr(), _ptr(k_out), _ptr(kc),
+                 _ptr(vc), _ptr(lens), pos.numel(), hq, hkv, hd, 2 * pairs, q_st, q_sh, k_st, k_sh,
+                 v_st, v_sh, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], rows, where,
+                 1 if interleaved else 0, float(attention_factor), float(eps), _stream(dev))
     if v is not None:
-        for c, g in ((k_cache, kc), (v_cache, vc)):
-            _write_back(c, g)
+        if kc.data_ptr() != k_cache.data_ptr():
+            _write_back(k_cache, kc)
+        if vc.data_ptr() != v_cache.data_ptr():
+            _write_back(v_cache, vc)
     if q.is_cuda:
         return out, k_out
     return out.to(q.device), None if k_out is None else k_out.to(q.device)
