@@ -79,8 +79,8 @@ struct Job {
 
 // The plan of a launch; the blocks' order: the prefix's, then the sequences' own.
 struct Plan {
-    int rb, nw;           // 16 * rb rows of a sequence a block, nw waves
-    int prows;            // rows of a group a block
+    int nw;               // waves a block
+    int rb, prows;        // 16 * rb rows of a group a block (16 of a sequence), or prows of a dense one
     int ptiles, gtiles;   // row tiles of a group's rows, of a sequence's
     int pcap, ocap;       // splits at most
     int pblocks, oblocks;
@@ -105,7 +105,7 @@ __device__ __forceinline__ Range split_range(int len, int cap, int split) {
 // same of the eight dies (block i goes to die i % 8) and share its cache.
 __device__ __forceinline__ Job job_of(const PrefixAttn &a, const Plan &p, int block, bool part) {
     Job j;
-    const int G = a.hq / a.hkv, rows = 16 * p.rb;
+    const int G = a.hq / a.hkv;
     if (block < p.pblocks) {
         const int rt = block / 8 % p.ptiles, unit = block / (8 * p.ptiles) * 8 + block % 8;
         j.kvh = unit % a.hkv;
@@ -133,8 +133,8 @@ __device__ __forceinline__ Job job_of(const PrefixAttn &a, const Plan &p, int bl
         const int split = block % p.ocap, seq = block / p.ocap;
         j.group = seq / a.rows;
         const int i = (seq - j.group * a.rows) * G;
-        j.i0 = i + gt * rows;
-        j.i1 = min(j.i0 + rows, i + G);
+        j.i0 = i + 16 * gt;
+        j.i1 = min(j.i0 + 16, i + G);
         j.y = own_rows(a, seq, j.kvh);
         if (p.joined) {
             j.x = prefix_rows(a, j.group, j.kvh);
@@ -160,14 +160,14 @@ __device__ __forceinline__ size_t row_of(const PrefixAttn &a, const Job &j, int 
 }
 
 // What 16 * RB query rows have seen so far: their references, sums, and outputs of lane
-// (g, c): dimensions 64 q + 16 g + 4 r + i of row c in register r of o[..][q][i].
-template <int DP, int RB>
+// (g, c): dimensions 64 q + 16 g + 4 r + i of row 16 b + c in register r of o[b][q][i].
+template <int D, int RB>
 struct State {
     float m[RB], l[RB];
-    f32x4 o[RB][DP / 64][4];
+    f32x4 o[RB][(D + 63) / 64][4];
 };
 
-// A wave's pass over the tiles first, first + step .. of a job, for its rows i0 + 16 rb + c
+// A wave's pass over the tiles first, first + step .. of a job, for its rows i0 + 16 b + c
 // (those from i1 on repeat the last).  Both products run on f32 MFMA (v_mfma_f32_16x16x4_f32),
 // whose factors are as they are in memory.  Lane (g, c) = (lane / 16, lane % 16) has A[c][g]
 // and B[g][c] of a product of depth 4, and gets D[4g + r][c] in register r:
@@ -177,11 +177,11 @@ struct State {
 //     register j for row c, and A's row c of block (q, i) is dimension 64 q + 4 c + i.
 // The next tile's K is requested when this one's scores are on their way, its V when
 // this one's outputs are.
-template <int DP, int RB>
+template <int D, int RB>
 __device__ __forceinline__ void stream(const PrefixAttn &a, const Job &job, int i0, int i1, int first,
-                                       int step, State<DP, RB> &st) {
-    constexpr int NX = DP / 16, NB = DP / 64;
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, D = a.hd;
+                                       int step, State<D, RB> &st) {
+    constexpr int NX = D / 16, NB = (D + 63) / 64;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int xt = job.t1 - job.t0, end = xt + (job.y.len + kTile - 1) / kTile;
     float4 kr[NX], vr[4][NB];
     // Tile t of the job: its cache and first position.
@@ -189,23 +189,23 @@ __device__ __forceinline__ void stream(const PrefixAttn &a, const Job &job, int 
     auto place = [&](int t) { return kTile * (t < xt ? job.t0 + t : t - xt); };
     auto load_k = [&](int t) {
         const Rows x = rows(t);
-        const float *r = x.k + min(place(t) + c, x.len - 1) * x.ks + 4 * g;
+        const int p0 = place(t);
+        const float *r = x.k + p0 * x.ks + (c * x.ks + 4 * g);
+        if (p0 + kTile > x.len) r -= max(p0 + c - (x.len - 1), 0) * x.ks;   // repeats the last
 #pragma unroll
-        for (int i = 0; i < NX; ++i)
-            if (16 * i < D) kr[i] = *reinterpret_cast<const float4 *>(r + 16 * i);
+        for (int i = 0; i < NX; ++i) kr[i] = *reinterpret_cast<const float4 *>(r + 16 * i);
     };
     auto load_v = [&](int t) {
         const Rows x = rows(t);
+        const int p0 = place(t);
+        const float *r = x.v + p0 * x.vs + 4 * g * x.vs;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int at = place(t) + 4 * g + j;
-            const float *r = x.v + min(at, x.len - 1) * x.vs;
+            const float *v = r + j * x.vs;
+            if (p0 + kTile > x.len) v -= max(p0 + 4 * g + j - (x.len - 1), 0) * x.vs;
 #pragma unroll
-            for (int q = 0; q < NB; ++q) {
-                vr[j][q] = *reinterpret_cast<const float4 *>(r + min(64 * q + 4 * c, D - 4));
-                // weight 0 must meet no infinity or NaN
-                if (at >= x.len) vr[j][q] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+            for (int q = 0; q < NB; ++q)
+                vr[j][q] = *reinterpret_cast<const float4 *>(v + min(64 * q + 4 * c, D - 4));
         }
     };
     if (first < end) {
@@ -213,75 +213,83 @@ __device__ __forceinline__ void stream(const PrefixAttn &a, const Job &job, int 
         load_v(first);
     }
     float4 qr[RB][NX];
+    float m[RB], l[RB];
+    f32x4(&o)[RB][NB][4] = st.o;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const int i = min(i0 + 16 * rb + c, i1 - 1);
-        const float *q = a.q + row_of(a, job, i) * D + 4 * g;
+    for (int b = 0; b < RB; ++b) {
+        const float *q = a.q + row_of(a, job, min(i0 + 16 * b + c, i1 - 1)) * D + 4 * g;
 #pragma unroll
-        for (int x = 0; x < NX; ++x)
-            if (16 * x < D) qr[rb][x] = *reinterpret_cast<const float4 *>(q + 16 * x);
-        st.m[rb] = -INFINITY;
-        st.l[rb] = 0.f;
+        for (int x = 0; x < NX; ++x) qr[b][x] = *reinterpret_cast<const float4 *>(q + 16 * x);
+        m[b] = -INFINITY;
+        l[b] = 0.f;
 #pragma unroll
-        for (int q2 = 0; q2 < NB; ++q2)
+        for (int y = 0; y < NB; ++y)
 #pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) st.o[rb][q2][i2] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 4; ++i) o[b][y][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const float f = a.scale * kLog2e;
 
     for (int t = first; t < end; t += step) {
-        // ---- scores, in powers of two
-        f32x4 s[RB];
+        // ---- scores, in powers of two; two sums a row block, where there are few
+        f32x4 s[RB], s2[RB];
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) s[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < RB; ++b) s[b] = s2[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < NX; ++x)
-            if (16 * x < D) {
-                const float k4[4] = {kr[x].x, kr[x].y, kr[x].z, kr[x].w};
+        for (int x = 0; x < NX; ++x) {
+            const float k4[4] = {kr[x].x, kr[x].y, kr[x].z, kr[x].w};
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) {
-                        const float4 &q = qr[rb][x];
-                        const float q1 = j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w;
-                        s[rb] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[j], q1, s[rb], 0, 0, 0);
-                    }
-            }
-        if (t + step < end) load_k(t + step);
-        // ---- the rows' references
-        bool moved = false;
-        float was[RB];
-        const int left = rows(t).len - place(t) - 4 * g;
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[rb][r] = r < left ? s[rb][r] * f : -INFINITY;
-            const float top =
-                max_over_groups(fmaxf(fmaxf(s[rb][0], s[rb][1]), fmaxf(s[rb][2], s[rb][3])));
-            was[rb] = st.m[rb];
-            if (top > st.m[rb]) st.m[rb] = top + kLead;
-            moved |= st.m[rb] != was[rb];
+                for (int b = 0; b < RB; ++b) {
+                    const float4 &q = qr[b][x];
+                    f32x4 &d = RB <= 2 && j & 1 ? s2[b] : s[b];
+                    d = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                        k4[j], j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w, d, 0, 0, 0);
+                }
         }
-        if (__any(moved)) {
+        if (t + step < end) load_k(t + step);
+        const int left = rows(t).len - place(t);
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                const float alpha =
-                    was[rb] == st.m[rb] ? 1.f : __builtin_amdgcn_exp2f(was[rb] - st.m[rb]);
-                st.l[rb] *= alpha;
+        for (int b = 0; b < RB; ++b) s[b] = (RB <= 2 ? s[b] + s2[b] : s[b]) * f;
+        if (left < kTile) {   // the last tile of a cache: weight 0, which must meet no infinity or NaN
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool in = 4 * g + r < left;
+#pragma unroll
+                for (int b = 0; b < RB; ++b) s[b][r] = in ? s[b][r] : -INFINITY;
+#pragma unroll
+                for (int q = 0; q < NB; ++q) vr[r][q] = in ? vr[r][q] : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+        // ---- the rows' references
+        float top[RB];
+        bool moves = false;
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            top[b] = max_over_groups(fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])));
+            moves |= top[b] > m[b];
+        }
+        if (__any(moves)) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                const float was = m[b];
+                if (top[b] > m[b]) m[b] = top[b] + kLead;
+                const float alpha = was == m[b] ? 1.f : __builtin_amdgcn_exp2f(was - m[b]);
+                l[b] *= alpha;
 #pragma unroll
                 for (int q = 0; q < NB; ++q)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) st.o[rb][q][i] *= alpha;
+                    for (int i = 0; i < 4; ++i) o[b][q][i] *= alpha;
             }
         }
         // ---- weights and outputs
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            const float base = st.m[rb] == -INFINITY ? 0.f : st.m[rb];
+        for (int b = 0; b < RB; ++b) {
+            const float base = m[b] == -INFINITY ? 0.f : m[b];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[rb][r] = __builtin_amdgcn_exp2f(s[rb][r] - base);
-                st.l[rb] += s[rb][r];
+                s[b][r] = __builtin_amdgcn_exp2f(s[b][r] - base);
+                l[b] += s[b][r];
             }
         }
 #pragma unroll
@@ -292,51 +300,50 @@ __device__ __forceinline__ void stream(const PrefixAttn &a, const Job &job, int 
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int rb = 0; rb < RB; ++rb)
-                        st.o[rb][q][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                            v4[i], s[rb][j], st.o[rb][q][i], 0, 0, 0);
+                    for (int b = 0; b < RB; ++b)
+                        o[b][q][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v4[i], s[b][j], o[b][q][i],
+                                                                          0, 0, 0);
             }
         if (t + step < end) load_v(t + step);
     }
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        st.l[rb] = sum_over_groups(st.l[rb]);
+    for (int b = 0; b < RB; ++b) {
+        st.l[b] = sum_over_groups(l[b]);
         // NaN and nothing else: the reference of a row that is NaN
-        if (st.l[rb] != st.l[rb] && st.m[rb] == -INFINITY) st.m[rb] = INFINITY;
+        st.m[b] = st.l[b] != st.l[b] && m[b] == -INFINITY ? INFINITY : m[b];
     }
 }
 
 // LDS of a block of NW waves that meet: their outputs, references, sums and shares.
-template <int DP, int RB, int NW>
+template <int D, int RB, int NW>
 struct Meeting {
-    float o[NW][16 * RB][DP + 4];
+    float o[NW][16 * RB][(D + 63) / 64 * 64 + 4];
     float m[NW][16 * RB], l[NW][16 * RB], share[NW][16 * RB], top[16 * RB], sum[16 * RB];
 };
 
 // A block's NW waves take tiles of 16 positions in turn, each with the block's rows and a
 // state of its own, and meet in LDS once at the end.
-template <int DP, int RB, int NW>
+template <int D, int RB, int NW>
 __device__ __forceinline__ void stream_block(const PrefixAttn &a, const Plan &plan, const Job &job,
-                                             Meeting<DP, RB, NW> &lds, float *part, float *pml) {
-    constexpr int NB = DP / 64;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, g = lane >> 4;
-    const int D = a.hd;
-    State<DP, RB> st;
-    stream<DP, RB>(a, job, job.i0, job.i1, wave, NW, st);
+                                             Meeting<D, RB, NW> &lds, float *part, float *pml) {
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    State<D, RB> st;
+    stream<D, RB>(a, job, job.i0, job.i1, wave, NW, st);
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const int r = 16 * rb + c;
+    for (int b = 0; b < RB; ++b) {
+        const int r = 16 * b + c;
         if (g == 0) {
-            lds.m[wave][r] = st.m[rb];
-            lds.l[wave][r] = st.l[rb];
+            lds.m[wave][r] = st.m[b];
+            lds.l[wave][r] = st.l[b];
         }
 #pragma unroll
-        for (int q = 0; q < NB; ++q)
+        for (int q = 0; q < (D + 63) / 64; ++q)
 #pragma unroll
             for (int i = 0; i < 4; ++i)   // dimensions 64 q + 16 g + 4 i .. + 3
                 *reinterpret_cast<float4 *>(&lds.o[wave][r][64 * q + 16 * g + 4 * i]) =
-                    make_float4(st.o[rb][q][0][i], st.o[rb][q][1][i], st.o[rb][q][2][i],
-                                st.o[rb][q][3][i]);
+                    make_float4(st.o[b][q][0][i], st.o[b][q][1][i], st.o[b][q][2][i],
+                                st.o[b][q][3][i]);
     }
     __syncthreads();
     // ---- each row's reference, sum and the waves' factors: e^(m - top) over the sum
@@ -357,9 +364,10 @@ __device__ __forceinline__ void stream_block(const PrefixAttn &a, const Plan &pl
         lds.sum[t] = sum;
     }
     __syncthreads();
-    const int cols = D / 4, n = job.i1 - job.i0, R = a.rows * (a.hq / a.hkv);
+    constexpr int cols = D / 4;
+    const int n = job.i1 - job.i0, R = a.rows * (a.hq / a.hkv);
     for (int x = t; x < n * cols; x += 64 * NW) {
-        const int r = x / cols, d = x - r * cols;
+        const int r = x / cols, d = x % cols;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
@@ -386,13 +394,19 @@ __device__ __forceinline__ void stream_block(const PrefixAttn &a, const Plan &pl
     }
 }
 
-template <int DP, int RB, int NW>
-__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_prefix_stream(
+template <int D, int RB, int NW>
+__global__ __launch_bounds__(64 * NW, D <= 192 ? 2 : 1) void k_prefix_stream(
     PrefixAttn a, Plan plan, float *__restrict__ part, float *__restrict__ pml) {
-    __shared__ __attribute__((aligned(16))) Meeting<DP, RB, NW> lds;
+    __shared__ __attribute__((aligned(16))) union {
+        Meeting<D, RB, NW> prefix;
+        Meeting<D, 1, NW> own;
+    } lds;
     const Job job = job_of(a, plan, blockIdx.x, part != nullptr);
     if (job.none) return;
-    stream_block<DP, RB, NW>(a, plan, job, lds, part, pml);
+    if (RB > 1 && (int)blockIdx.x < plan.pblocks)
+        stream_block<D, RB, NW>(a, plan, job, lds.prefix, part, pml);
+    else
+        stream_block<D, 1, NW>(a, plan, job, lds.own, part, pml);
 }
 
 // ---- many rows: bf16 MFMA -------------------------------------------------------
@@ -415,6 +429,14 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 &hi, bf16x8 &
 }
 
 // d += a b of two factors of three limbs: all products but those below 2^-25 of it.
+__device__ __forceinline__ f32x4 mfma6(const bf16x8 (&a)[3], const bf16x8 (&b)[3], f32x4 d) {
+    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[2], b[0], d, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[2], d, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[1], d, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], b[0], d, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[1], d, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], b[0], d, 0, 0, 0);
+}
 __device__ __forceinline__ f32x16 mfma6(const bf16x8 (&a)[3], const bf16x8 (&b)[3], f32x16 d) {
     d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[2], b[0], d, 0, 0, 0);
     d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[2], d, 0, 0, 0);
@@ -424,96 +446,118 @@ __device__ __forceinline__ f32x16 mfma6(const bf16x8 (&a)[3], const bf16x8 (&b)[
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], d, 0, 0, 0);
 }
 
-// The largest of the two lanes that share a row.
-__device__ __forceinline__ float max_of_halves(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_of_halves(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+// Over the lanes that share a row, two of 32 rows or four of 16.
+template <int W, class F>
+__device__ __forceinline__ float over_row(float v, F f) {
+    if constexpr (W == 16) {
+        return over_groups(v, f);
+    } else {
+        const auto r =
+            __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
 }
 
-// LDS of a dense block: a tile's limbs of 32 positions in operand order.
-template <int DP>
+// LDS of a dense block: a tile's limbs of 32 positions in operand order, [limb][lane].
+template <int D>
 struct Limbs {
-    bf16x8 k[DP / 16][3][64];      // [16 dimensions][limb][lane]
-    bf16x8 v[2][DP / 32][3][64];   // [16 positions][32 dimensions][limb][lane]
+    bf16x8 k[D / 16][3][64], v[D / 16][3][64];
 };
 
-// A block of four waves takes 128 rows of a group, 32 a wave, and a split of the prefix in
-// tiles of 32 positions.  Per tile its waves build the limbs of K and V, a quarter each, in
-// LDS, and then every wave multiplies all of them with its rows, so that each f32 of the
-// prefix is read and split once for 128 rows; the next tile is requested before.
-// Products are of depth 16 (v_mfma_f32_32x32x16_bf16): lane (h, c) = (lane / 32, lane % 32)
-// has A[c][8h ..] and B[8h ..][c] and gets D[8 (r / 4) + 4h + r % 4][c] in register r:
-//   S^T = K Q^T: A = position c's dimensions 16 x + 8h .., B = row c's, in registers;
-//   O^T = V^T P^T: A = dimension 32 y + c's positions 16 t + 4h + (0 .. 3, 8 .. 11), which
-//     are those whose scores the lane holds for row c.
+// A block of four waves takes 4 W rows of a group, W = 32 or 16 a wave, and a split of the
+// prefix in tiles of 32 positions.  Per tile its waves build the limbs of K and V, a
+// quarter each, in LDS, and then every wave multiplies all of them with its rows, so that
+// each f32 of the prefix is read and split once a block; the next tile is requested before.
+// Products are of depth P = 512 / W (v_mfma_f32_32x32x16_bf16, v_mfma_f32_16x16x32_bf16): lane
+// (h, c) = (lane / W, lane % W) has A[c][8h ..] and B[8h ..][c], and gets D[4h + r % 4 +
+// 8 (r / 4)][c] in register r (W = 16: r < 4):
+//   S^T = K Q^T: A = W positions, position c's dimensions P x + 8h .., B = row c's, in registers;
+//   O^T = V^T P^T: A = W dimensions, dimension c's eight positions whose scores the lane
+//     holds for row c: 16 u + 4h + (0 .. 3, 8 .. 11), or 4h + (0 .. 3, 16 .. 19).
 // Every product of f32 factors is six of limbs (mfma6): 22 bits and more of it, at a sixth
 // of the bf16 rate, where the f32 MFMA has a sixteenth.  An infinity or NaN among K, V or
 // the queries makes NaN of the limbs' products: a wave that has one in its results
 // works its rows out anew in f32 (stream()).
-template <int DP>
+template <int D, int W>
 __device__ __forceinline__ void dense_block(const PrefixAttn &a, const Plan &plan, const Job &job,
-                                            Limbs<DP> &lds, float *part, float *pml) {
-    constexpr int NX = DP / 16, NY = DP / 32, KD = DP / 8, U = DP / 64;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 31, h = lane >> 5;
-    const int D = a.hd, G = a.hq / a.hkv, R = a.rows * G;
+                                            Limbs<D> &lds, float *part, float *pml) {
+    constexpr int P = 512 / W, H = 64 / W;          // depth of a product; lanes that share a row
+    constexpr int NX = D / P, NY = D / W;           // products of a score, blocks of dimensions
+    constexpr int NS = 32 / W, SR = W * W / 64;     // blocks of positions, their registers
+    constexpr int KD = D / 8, KU = (KD + 7) / 8, VU = (D + 63) / 64;
+    constexpr int kSwap = KD > 8 ? 1 : 16 / KD;
+    typedef float acc __attribute__((ext_vector_type(SR)));
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int c = lane & (W - 1), h = lane / W;
+    const int G = a.hq / a.hkv, R = a.rows * G;
     const int t0 = job.t0 / 2, t1 = (job.t1 + 1) / 2, len = job.x.len;
 
-    // ---- this thread's parts of a tile: 8 dimensions kd .. of position kp, and 8 positions
-    // of dimension vd
-    float kr[U][8], vr[U][8];
+    // ---- this thread's parts of a tile: 8 dimensions of position kunit / KD, and of dimension
+    // lane + 64 u the positions vpos(0) .. vpos(7)
+    float kr[KU][8], vr[VU][8];
+    auto kunit = [&](int u) { return min(t + 256 * u, 32 * KD - 1); };
+    auto vpos = [&](int i) {
+        return W == 32 ? 16 * (wave >> 1) + 4 * (wave & 1) + 8 * (i >> 2) + (i & 3)
+                       : 4 * wave + 16 * (i >> 2) + (i & 3);
+    };
     auto load = [&](int tile) {
+        const bool whole = 32 * tile + 32 <= len;
+        const float *kt = job.x.k + (int64_t)32 * tile * job.x.ks;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int kd = t % KD, kp = (t + 256 * u) / KD;
-            const float *k = job.x.k + min(32 * tile + kp, len - 1) * job.x.ks + min(8 * kd, D - 8);
+        for (int u = 0; u < KU; ++u) {
+            const int kp = kunit(u) / KD;
+            const float *k = kt + (kp * job.x.ks + 8 * (kunit(u) % KD));
+            if (!whole)   // the last tile repeats the last position
+                k -= max(32 * tile + kp - (len - 1), 0) * job.x.ks;
             const float4 x = reinterpret_cast<const float4 *>(k)[0];
             const float4 y = reinterpret_cast<const float4 *>(k)[1];
             kr[u][0] = x.x; kr[u][1] = x.y; kr[u][2] = x.z; kr[u][3] = x.w;
             kr[u][4] = y.x; kr[u][5] = y.y; kr[u][6] = y.z; kr[u][7] = y.w;
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int vd = t % DP, th = (t + 256 * u) / DP;   // positions 16 (th / 2) + 4 (th % 2) ..
-            const int p0 = 32 * tile + 16 * (th >> 1) + 4 * (th & 1);
-            const float *v = job.x.v + min(vd, D - 1);
+        for (int i = 0; i < 8; ++i) {
+            const float *v = job.x.v + min(32 * tile + vpos(i), len - 1) * job.x.vs;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = p0 + 8 * (i >> 2) + (i & 3);
-                vr[u][i] = v[min(at, len - 1) * job.x.vs];
-                if (at >= len) vr[u][i] = 0.f;   // weight 0 must meet no infinity or NaN
-            }
+            for (int u = 0; u < VU; ++u) vr[u][i] = v[(uint32_t)min(lane + 64 * u, D - 1)];
         }
     };
-    auto store = [&]() {
+    // Lanes are swapped within 16 by the dimensions, or a wave's stores of K would meet in a
+    // part of the banks.
+    auto klane = [](int p, int kd) { return (p + W * (kd % H)) ^ (kd * kSwap); };
+    auto store = [&](int tile) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            // lanes are swapped within 16 by the dimensions, or a wave's stores would meet in
-            // a quarter of the banks
-            const int kd = t % KD, kp = (t + 256 * u) / KD;
-            const int at = (kp + 32 * (kd & 1)) ^ (kd * (16 / KD));
+        for (int u = 0; u < KU; ++u) {
+            const int kp = kunit(u) / KD, kd = kunit(u) % KD;
             bf16x8 x[3];
             split8(kr[u], x[0], x[1], x[2]);
+            if (32 * KD % 256 == 0 || t + 256 * u < 32 * KD)
 #pragma unroll
-            for (int i = 0; i < 3; ++i) lds.k[kd >> 1][i][at] = x[i];
+                for (int i = 0; i < 3; ++i)
+                    lds.k[kd / H * NS + kp / W][i][klane(kp & (W - 1), kd)] = x[i];
+        }
+        if (32 * tile + 32 > len) {   // weight 0 must meet no infinity or NaN
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (32 * tile + vpos(i) >= len)
+#pragma unroll
+                    for (int u = 0; u < VU; ++u) vr[u][i] = 0.f;
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int vd = t % DP, th = (t + 256 * u) / DP;
+        for (int u = 0; u < VU; ++u) {
+            const int vd = lane + 64 * u;
             bf16x8 x[3];
             split8(vr[u], x[0], x[1], x[2]);
+            if (D % 64 == 0 || vd < D)
 #pragma unroll
-            for (int i = 0; i < 3; ++i)
-                lds.v[th >> 1][vd >> 5][i][(vd & 31) + 32 * (th & 1)] = x[i];
+                for (int i = 0; i < 3; ++i)
+                    lds.v[W == 32 ? (wave >> 1) * NY + vd / W : vd / W][i]
+                         [vd % W + W * (wave & (H - 1))] = x[i];
         }
     };
     if (t0 < t1) load(t0);
 
     // ---- the wave's query rows, row c in this lane; with the sign of the score's factor
-    const int w0 = job.i0 + 32 * wave;
+    const int w0 = job.i0 + W * wave;
     const bool busy = w0 < job.i1;
     const float f = fabsf(a.scale) * kLog2e;
     bf16x8 q[NX][3];
@@ -521,53 +565,56 @@ __device__ __forceinline__ void dense_block(const PrefixAttn &a, const Plan &pla
         const float *x = a.q + row_of(a, job, min(w0 + c, R - 1)) * D + 8 * h;
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
-            float y[8];
-            const bool in = 16 * i < D;
-            const float4 u = reinterpret_cast<const float4 *>(x + (in ? 16 * i : 0))[0];
-            const float4 v = reinterpret_cast<const float4 *>(x + (in ? 16 * i : 0))[1];
-            y[0] = u.x; y[1] = u.y; y[2] = u.z; y[3] = u.w;
-            y[4] = v.x; y[5] = v.y; y[6] = v.z; y[7] = v.w;
+            const float4 u = reinterpret_cast<const float4 *>(x + P * i)[0];
+            const float4 v = reinterpret_cast<const float4 *>(x + P * i)[1];
+            float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = a.scale < 0.f ? -y[j] : y[j];
             split8(y, q[i][0], q[i][1], q[i][2]);
         }
     }
     float m = -INFINITY, l = 0.f;
-    f32x16 o[NY];
+    acc o[NY];
 #pragma unroll
     for (int y = 0; y < NY; ++y)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[y][r] = 0.f;
+        for (int r = 0; r < SR; ++r) o[y][r] = 0.f;
 
     for (int tile = t0; tile < t1; ++tile) {
         __syncthreads();
-        store();
+        store(tile);
         if (tile + 1 < t1) load(tile + 1);
         __syncthreads();
         if (!busy) continue;
-        // ---- scores
-        f32x16 s;
+        // ---- scores: the lane's positions in its registers' order
+        acc sa[NS];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        for (int y = 0; y < NS; ++y)
+#pragma unroll
+            for (int r = 0; r < SR; ++r) sa[y][r] = 0.f;
 #pragma unroll
         for (int x = 0; x < NX; ++x)
-            if (16 * x < D) {
+#pragma unroll
+            for (int y = 0; y < NS; ++y) {
                 bf16x8 k[3];
 #pragma unroll
-                for (int i = 0; i < 3; ++i) k[i] = lds.k[x][i][lane ^ ((2 * x + h) * (16 / KD))];
-                s = mfma6(k, q[x], s);
+                for (int i = 0; i < 3; ++i) k[i] = lds.k[x * NS + y][i][klane(c, H * x + h)];
+                sa[y] = mfma6(k, q[x], sa[y]);
             }
-        // ---- the rows' references, in powers of two
-        const int left = len - 32 * tile - 4 * h;
-        if (left < 32 - 4 * h) {
+        float s[NS * SR];
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (8 * (r >> 2) + (r & 3) >= left) s[r] = -INFINITY;
+        for (int i = 0; i < NS * SR; ++i) s[i] = sa[i / SR][i % SR];
+        // ---- the rows' references, in powers of two
+        if (32 * tile + 32 > len) {
+            const int left = len - 32 * tile - 4 * h;
+#pragma unroll
+            for (int i = 0; i < NS * SR; ++i)
+                if ((W == 32 ? 8 : 16) * (i >> 2) + (i & 3) >= left) s[i] = -INFINITY;
         }
         float top = s[0];
 #pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-        top = max_of_halves(top) * f;
+        for (int i = 1; i < NS * SR; ++i) top = fmaxf(top, s[i]);
+        top = over_row<W>(top, [](float x, float y) { return fmaxf(x, y); }) * f;
         if (__any(top > m)) {
             const float was = m;
             if (top > m) m = top + kLead;
@@ -576,12 +623,12 @@ __device__ __forceinline__ void dense_block(const PrefixAttn &a, const Plan &pla
 #pragma unroll
             for (int y = 0; y < NY; ++y)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[y][r] *= alpha;
+                for (int r = 0; r < SR; ++r) o[y][r] *= alpha;
         }
         // ---- weights and outputs
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < NS * SR / 8; ++u) {
             float w[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -591,46 +638,45 @@ __device__ __forceinline__ void dense_block(const PrefixAttn &a, const Plan &pla
             bf16x8 p[3];
             split8(w, p[0], p[1], p[2]);
 #pragma unroll
-            for (int y = 0; y < NY; ++y)
-                if (32 * y < D) {
-                    bf16x8 v[3];
+            for (int y = 0; y < NY; ++y) {
+                bf16x8 v[3];
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) v[i] = lds.v[u][y][i][lane];
-                    o[y] = mfma6(v, p, o[y]);
-                }
+                for (int i = 0; i < 3; ++i) v[i] = lds.v[u * NY + y][i][lane];
+                o[y] = mfma6(v, p, o[y]);
+            }
         }
     }
     if (!busy) return;
-    l = sum_of_halves(l);
+    l = over_row<W>(l, [](float x, float y) { return x + y; });
     const bool row = w0 + c < job.i1;
     bool bad = !(l <= 3.4e38f);
 #pragma unroll
     for (int y = 0; y < NY; ++y)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) bad |= 32 * y < D && !(fabsf(o[y][r]) <= 3.4e38f);
+        for (int r = 0; r < SR; ++r) bad |= !(fabsf(o[y][r]) <= 3.4e38f);
     const size_t slot = (((size_t)job.group * a.hkv + job.kvh) * plan.slots + job.slot) * R;
     if (__builtin_expect(__any(bad && row), 0)) {
-        const int c16 = lane & 15, g16 = lane >> 4;
-        State<DP, 2> st;
-        stream<DP, 2>(a, job, w0, min(w0 + 32, job.i1), 0, 1, st);
-#pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-            const int i = w0 + 16 * rb + c16;
-            if (i >= job.i1) continue;
-            const float inv = st.l[rb] == 0.f ? 0.f : 1.0f / st.l[rb];
+        const int c16 = lane & 15, g16 = lane >> 4, i1 = min(w0 + W, job.i1);
+#pragma unroll 1
+        for (int i0 = w0; i0 < i1; i0 += 16) {
+            State<D, 1> st;
+            stream<D, 1>(a, job, i0, i1, 0, 1, st);
+            const int i = i0 + c16;
+            if (i >= i1) continue;
+            const float inv = st.l[0] == 0.f ? 0.f : 1.0f / st.l[0];
             float *to = part ? part + (slot + i) * D : a.out + row_of(a, job, i) * D;
             if (part && g16 == 0) {
-                pml[2 * (slot + i)] = st.m[rb];
-                pml[2 * (slot + i) + 1] = st.l[rb];
+                pml[2 * (slot + i)] = st.m[0];
+                pml[2 * (slot + i) + 1] = st.l[0];
             }
 #pragma unroll
-            for (int y = 0; y < DP / 64; ++y)
+            for (int y = 0; y < (D + 63) / 64; ++y)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (64 * y + 16 * g16 < D)
                         *reinterpret_cast<float4 *>(to + 64 * y + 16 * g16 + 4 * r) =
-                            make_float4(st.o[rb][y][0][r] * inv, st.o[rb][y][1][r] * inv,
-                                        st.o[rb][y][2][r] * inv, st.o[rb][y][3][r] * inv);
+                            make_float4(st.o[0][y][0][r] * inv, st.o[0][y][1][r] * inv,
+                                        st.o[0][y][2][r] * inv, st.o[0][y][3][r] * inv);
         }
         return;
     }
@@ -645,26 +691,25 @@ __device__ __forceinline__ void dense_block(const PrefixAttn &a, const Plan &pla
 #pragma unroll
     for (int y = 0; y < NY; ++y)
 #pragma unroll
-        for (int r = 0; r < 16; r += 4)
-            if (32 * y < D)
-                *reinterpret_cast<float4 *>(to + 32 * y + 2 * r + 4 * h) = make_float4(
-                    o[y][r] * inv, o[y][r + 1] * inv, o[y][r + 2] * inv, o[y][r + 3] * inv);
+        for (int r = 0; r < SR; r += 4)
+            *reinterpret_cast<float4 *>(to + W * y + 2 * r + 4 * h) =
+                make_float4(o[y][r] * inv, o[y][r + 1] * inv, o[y][r + 2] * inv, o[y][r + 3] * inv);
 }
 
-template <int DP, int RB>
-__global__ __launch_bounds__(256, 2) void k_prefix_dense(PrefixAttn a, Plan plan,
-                                                         float *__restrict__ part,
-                                                         float *__restrict__ pml) {
+template <int D, int W>
+__global__ __launch_bounds__(256, W == 32 ? 2 : 3) void k_prefix_dense(PrefixAttn a, Plan plan,
+                                                                       float *__restrict__ part,
+                                                                       float *__restrict__ pml) {
     __shared__ __attribute__((aligned(16))) union {
-        Limbs<DP> limbs;
-        Meeting<DP, RB, 4> meeting;
+        Limbs<D> limbs;
+        Meeting<D, 1, 4> meeting;
     } lds;
     const Job job = job_of(a, plan, blockIdx.x, part != nullptr);
     if (job.none) return;
     if ((int)blockIdx.x < plan.pblocks)
-        dense_block<DP>(a, plan, job, lds.limbs, part, pml);
+        dense_block<D, W>(a, plan, job, lds.limbs, part, pml);
     else
-        stream_block<DP, RB, 4>(a, plan, job, lds.meeting, part, pml);
+        stream_block<D, 1, 4>(a, plan, job, lds.meeting, part, pml);
 }
 
 // A row's partial results, normalised, in the shares of their sums, in the order of the slots, by
@@ -764,12 +809,13 @@ Plan plan_of(int groups, int rows, int hq, int hkv, int hd, int prefix, int own)
     const int64_t seqs = (int64_t)groups * rows;
     // Short caches: a sequence's block reads the prefix for itself, and nothing is merged.
     p.joined = pt + ot <= 32;
-    p.dense = !p.joined && R > 64 && hd <= 128;
-    p.rb = (p.joined || p.dense ? G : R) <= 16 || hd > 128 ? 1 : 2;
+    p.dense = !p.joined && R > 32 && hd <= 128;
+    // One block's rows for all of up to 64: K and V are read once.
+    p.rb = p.joined || p.dense ? 1 : std::min((R + 15) / 16, hd <= 128 ? 2 : 1);
+    p.prows = p.dense ? (R <= 64 ? 64 : 128) : 16 * p.rb;
     p.nw = p.joined && hd <= 128 ? 8 : 4;
-    p.prows = p.dense ? 128 : 16 * p.rb;
     p.ptiles = (R + p.prows - 1) / p.prows;
-    p.gtiles = (G + 16 * p.rb - 1) / (16 * p.rb);
+    p.gtiles = (G + 15) / 16;
     if (p.joined) {
         p.ocap = p.slots = 1;
         p.oblocks = (int)(seqs * hkv * p.gtiles);
@@ -780,7 +826,13 @@ Plan plan_of(int groups, int rows, int hq, int hkv, int hd, int prefix, int own)
         return (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, most));
     };
     const int64_t units = (int64_t)groups * hkv, ob = seqs * hkv * p.gtiles;
-    p.pcap = pt ? cap(p.dense ? 512 : 256, units * p.ptiles, pt) : 0;
+    // Blocks wanted, us with them / with half as many or half as many again: 256 for one pass of
+    // few rows (32 rows on 4096 positions 17.4, 512: 20.2; 16 rows 12.8, 13.9), or 512 past
+    // 128 dimensions, where a CU has one at a time (28 rows of 256, 7 groups of up to 13296:
+    // 169, 256: 186); 768 dense ones of 64 rows, three a CU (64 rows on 4096 positions 20.2,
+    // 512: 25.3), 512 of 128 (32767 positions 119, 256: 148).
+    const int want = p.prows == 64 ? 768 : p.dense || hd > 128 ? 512 : 256;
+    p.pcap = pt ? cap(want, units * p.ptiles, pt) : 0;
     p.ocap = ot ? cap(256, ob, ot) : 0;
     p.pblocks = (int)((units * p.pcap + 7) / 8 * 8 * p.ptiles);
     p.oblocks = (int)(ob * p.ocap);
@@ -814,33 +866,28 @@ int launch_prefix_attention(const PrefixAttn &a, float *scratch, hipStream_t s) 
     const size_t rows = (size_t)a.groups * a.rows * a.hq;
     float *pml = part ? part + rows * p.slots * a.hd : nullptr;
     const dim3 grid(p.pblocks + p.oblocks);
-#define TB_PS(DP, RB, NW)                                                                   \
-    if (p.rb == RB && p.nw == NW)                                                           \
-    hipLaunchKernelGGL((k_prefix_stream<DP, RB, NW>), grid, dim3(64 * NW), 0, s, a, p, part, pml)
-#define TB_PD(DP, RB)                                                                       \
-    if (p.rb == RB)                                                                         \
-    hipLaunchKernelGGL((k_prefix_dense<DP, RB>), grid, dim3(256), 0, s, a, p, part, pml)
-    if (p.dense && a.hd <= 64) {
-        TB_PD(64, 1);
-        TB_PD(64, 2);
-    } else if (p.dense) {
-        TB_PD(128, 1);
-        TB_PD(128, 2);
-    } else if (a.hd <= 64) {
-        TB_PS(64, 1, 4);
-        TB_PS(64, 2, 4);
-        TB_PS(64, 1, 8);
-        TB_PS(64, 2, 8);
-    } else if (a.hd <= 128) {
-        TB_PS(128, 1, 4);
-        TB_PS(128, 2, 4);
-        TB_PS(128, 1, 8);
-        TB_PS(128, 2, 8);
-    } else {
-        TB_PS(256, 1, 4);
+#define TB_PREFIX(D)                                                                          \
+    case D:                                                                                   \
+        if constexpr (D <= 128) {                                                             \
+            if (p.dense) k = p.prows == 64 ? k_prefix_dense<D, 16> : k_prefix_dense<D, 32>;   \
+            else if (p.nw == 8) k = k_prefix_stream<D, 1, 8>;                                 \
+            else if (p.rb == 2) k = k_prefix_stream<D, 2, 4>;                                 \
+        }                                                                                     \
+        if (!k) k = k_prefix_stream<D, 1, 4>;                                                 \
+        break
+    void (*k)(PrefixAttn, Plan, float *, float *) = nullptr;
+    switch (a.hd) {
+        TB_PREFIX(32);
+        TB_PREFIX(64);
+        TB_PREFIX(96);
+        TB_PREFIX(128);
+        TB_PREFIX(160);
+        TB_PREFIX(192);
+        TB_PREFIX(224);
+        TB_PREFIX(256);
     }
-#undef TB_PD
-#undef TB_PS
+#undef TB_PREFIX
+    hipLaunchKernelGGL(k, grid, dim3(64 * p.nw), 0, s, a, p, part, pml);
     TB_LAUNCHED();
     if (part) {
         if (a.hd <= 32) merge<8>(a, p, part, pml, s);
