@@ -55,7 +55,8 @@ struct Piece {
 // head), or 2 W dimensions behind it.  W = 4: 16-byte loads, and both pieces of a pair
 // of the half layout in one lane; W = 1 where sizes, strides or addresses do not allow it.
 //
-// Bound by the heads' bytes, on few tokens by the launch.
+// Bound by the heads' bytes, on few tokens by the launch: 4096 tokens of 32 + 8 heads of 128,
+// 168 MB, take 35.0 us (4.8 TB/s, a large copy 4.9); four tokens 5.1.
 template <int L, int NU, int W, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void k_norm_rope(RopeParams p, int per, int parts) {
     const int lane = threadIdx.x % L;
