@@ -83,8 +83,8 @@ U, V = _lib.TB_ERR_UNSUPPORTED, _lib.TB_ERR_VALUE
     (attention, dict(own=17), V, b"exceed"), (attention, dict(own=2 ** 63 - 1), V, b"exceed"),
     (attention, dict(kp_ss=66), U, b"strides"), (attention, dict(v_sb=-4), U, b"strides"),
     (attention, dict(pl=A + 2), U, b"misaligned"), (attention, dict(ol=A + 1), U, b"misaligned"),
-    (attention, dict(scratch=A, size=8), U, b"scratch"),
-    (attention, dict(scratch=A + 8, size=1 << 40), U, b"scratch"),
+    (attention, dict(scratch=A, size=8, max_prefix=9000, prefix=9000), U, b"scratch"),
+    (attention, dict(scratch=A + 8, size=1 << 40, max_prefix=9000, prefix=9000), U, b"scratch"),
     (select, dict(x=None), U, b"null"), (select, dict(tokens=None), U, b"null"),
     (select, dict(beams=65), U, b"64"), (select, dict(beams=0), U, b"no beams"),
     (select, dict(groups=-1), U, b"groups"), (select, dict(groups=40000), U, b"65535"),
@@ -117,8 +117,9 @@ def test_empty_calls_touch_nothing():
     assert reorder(len=0) == _lib.TB_OK
     L = _lib.lib()
     assert L.tb_prefix_attention_scratch(0, 3, 4, 2, 64, 100, 9) == 0
-    assert L.tb_prefix_attention_scratch(1, 3, 4, 2, 64, 100, 9) > 0
-    assert L.tb_prefix_attention_scratch(1, 3, 5, 2, 64, 100, 9) == 0
+    assert L.tb_prefix_attention_scratch(1, 3, 4, 2, 64, 9000, 9) > 0
+    assert L.tb_prefix_attention_scratch(1, 3, 4, 2, 64, 100, 9) == 0      # one block sees all
+    assert L.tb_prefix_attention_scratch(1, 3, 5, 2, 64, 9000, 9) == 0
     assert L.tb_beam_select_scratch(2, 3, 100, 65) == 0
     assert L.tb_beam_select_scratch(2, 3, 100, 3) >= 2 * 3 * (16 + 24)
 

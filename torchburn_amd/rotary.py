@@ -77,23 +77,28 @@ def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optional[
     return f.to(device), attention
 
 
+def _ready(t: torch.Tensor, dtype: torch.dtype, index: int) -> bool:
+    """Whether the kernels can read t where it is."""
+    return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+
+
 def _heads(op: str, name: str, t: torch.Tensor, lead, hd: int, dev):
     """(tensor, heads, token stride, head stride): the caller's memory where a token's heads
     are a constant number of elements apart and the tokens too, else a copy."""
-    shape = t.shape
-    if len(shape) < 2 or shape[:-2] != lead or shape[-1] != hd:
+    *first, heads, width = t.shape if t.ndim >= 2 else (0, 0, -1)
+    if width != hd or first != lead:
         raise _bad(op, f"{name} must be [{', '.join(map(str, lead))}, heads, {hd}], got "
-                       f"{list(shape)}")
+                       f"{list(t.shape)}")
     st = t.stride()
     if t.dtype is not torch.float32 or t.get_device() != dev.index or (st[-1] != 1 and hd > 1):
         t = _on_gpu(t.detach(), torch.float32, dev)
         st = t.stride()
-    if len(shape) == 3:
-        return t, shape[1], st[0], st[1]
-    if len(shape) == 2:
-        return t, shape[0], 0, st[0]
+    if len(st) == 3:
+        return t, heads, st[0], st[1]
+    if len(st) == 2:
+        return t, heads, 0, st[0]
     flat = _flat(t.detach(), 2)
-    return flat, shape[-2], flat.stride(0), flat.stride(1)
+    return flat, heads, flat.stride(0), flat.stride(1)
 
 
 def _flat(t: torch.Tensor, last: int) -> torch.Tensor:
@@ -106,66 +111,73 @@ def _flat(t: torch.Tensor, last: int) -> torch.Tensor:
 
 def _own_caches(op: str, name: str, c: torch.Tensor, lead, heads: int, hd: int, dev):
     """A cache [.., heads, positions, head_dim] as an f32 device tensor whose sequences are a
-    constant number of elements apart, and those strides: the caller's memory or a copy."""
-    shape = c.shape
-    if len(shape) < 3 or shape[:-3] != lead or shape[-3] != heads or shape[-1] != hd:
+    constant number of elements apart, its positions and those strides: the caller's memory
+    or a copy."""
+    *first, kvh, rows, width = c.shape if c.ndim >= 3 else (0, 0, 0, -1)
+    if width != hd or kvh != heads or first != lead:
         raise _bad(op, f"{name} must be [{', '.join(map(str, lead))}, {heads}, max_seq, {hd}], "
-                       f"got {list(shape)}")
+                       f"got {list(c.shape)}")
     st = c.stride()
     if c.dtype is not torch.float32 or c.get_device() != dev.index or (st[-1] != 1 and hd > 1):
         c = c.detach().to(device=dev, dtype=torch.float32, copy=True).contiguous()
         st = c.stride()
-    if len(shape) == 4:
-        return c, st
-    if len(shape) == 3:
-        return c, (0, *st)
+    if len(st) == 4:
+        return c, rows, st
+    if len(st) == 3:
+        return c, rows, (0, *st)
     flat = _flat(c.detach(), 3)
-    return flat, flat.stride()
+    return flat, rows, flat.stride()
 
 
 def _call(op, q, k, v, positions, inv_freq, q_weight, k_weight, eps, interleaved,
           attention_factor, k_cache, v_cache, at):
     if q.ndim < 2:
         raise _bad(op, f"q must be [.., num_heads, head_dim], got {list(q.shape)}")
-    dev, lead, hd = _target(q), q.shape[:-2], q.shape[-1]
+    dev = _target(q)
+    index = dev.index
+    *lead, hq, hd = q.shape
     x, hq, q_st, q_sh = _heads(op, "q", q, lead, hd, dev)
     y, hkv, k_st, k_sh = _heads(op, "k", k, lead, hd, dev)
-    if not isinstance(positions, torch.Tensor) or positions.shape != lead or \
+    if not isinstance(positions, torch.Tensor) or [*positions.shape] != lead or \
             positions.dtype.is_floating_point:
-        raise _bad(op, f"positions must be integers {list(lead)}, one a token")
-    pairs = inv_freq.shape[0] if inv_freq.ndim == 1 else hd
-    if 2 * pairs > hd:
+        raise _bad(op, f"positions must be integers {lead}, one a token")
+    pairs = inv_freq.numel()
+    if 2 * pairs > hd or inv_freq.ndim != 1:
         raise _bad(op, f"inv_freq must hold at most head_dim / 2 = {hd // 2} frequencies, got "
                        f"{list(inv_freq.shape)}")
-    pos = _on_gpu(positions, torch.int64, dev)
-    freq = _on_gpu(inv_freq, torch.float64, dev)
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.ndim != 1 or w.shape[0] != hd):
-            raise _bad(op, f"{name} must be [{hd}], got {list(w.shape)}")
-    qw, kw = _on_gpu(q_weight, torch.float32, dev), _on_gpu(k_weight, torch.float32, dev)
+    pos = positions if _ready(positions, torch.int64, index) else \
+        _on_gpu(positions, torch.int64, dev)
+    freq = inv_freq if _ready(inv_freq, torch.float64, index) else \
+        _on_gpu(inv_freq, torch.float64, dev)
+    weights = []
+    for w in (q_weight, k_weight):
+        if w is not None:
+            if w.numel() != hd or w.ndim != 1:
+                raise _bad(op, f"the heads' weights must be [{hd}], got {list(w.shape)}")
+            if not _ready(w, torch.float32, index):
+                w = _on_gpu(w, torch.float32, dev)
+        weights.append(w)
+    qw, kw = weights
     out = x.new_empty((*lead, hq, hd))
+    z = kc = vc = lens = k_out = None
+    v_st = v_sh = where = rows = 0
+    ks = vs = (0, 0, 0)
     if v is None:
         k_out = x.new_empty((*lead, hkv, hd))
-        z = kc = vc = lens = None
-        v_st = v_sh = where = rows = 0
-        ks = vs = (0, 0, 0, 0)
     else:
-        k_out = None
         z, v_heads, v_st, v_sh = _heads(op, "v", v, lead, hd, dev)
         if v_heads != hkv:
             raise _bad(op, f"k has {hkv} heads, v {v_heads}")
-        kc, ks = _own_caches(op, "k_cache", k_cache, lead, hkv, hd, dev)
-        vc, vs = _own_caches(op, "v_cache", v_cache, lead, hkv, hd, dev)
-        rows = kc.shape[-2]
-        if vc.shape[-2] != rows:
-            raise _bad(op, f"k_cache has {rows} positions, v_cache {vc.shape[-2]}")
+        kc, rows, ks = _own_caches(op, "k_cache", k_cache, lead, hkv, hd, dev)
+        vc, v_rows, vs = _own_caches(op, "v_cache", v_cache, lead, hkv, hd, dev)
+        if v_rows != rows:
+            raise _bad(op, f"k_cache has {rows} positions, v_cache {v_rows}")
         if isinstance(at, torch.Tensor):
-            if at.shape != lead or at.dtype.is_floating_point:
-                raise _bad(op, f"kv_len must be integers {list(lead)}, got {at.dtype} "
-                               f"{list(at.shape)}")
-            lens, where = _int32_on_gpu(at, dev), 0
+            if [*at.shape] != lead or at.dtype.is_floating_point:
+                raise _bad(op, f"kv_len must be integers {lead}, got {at.dtype} {list(at.shape)}")
+            lens = at if _ready(at, torch.int32, index) else _int32_on_gpu(at, dev)
         else:
-            lens, where = None, _lib.int64(at)
+            where = _lib.int64(at)
     _lib.call_on(dev, "tb_norm_rope", x.data_ptr(), y.data_ptr(), _ptr(z), pos.data_ptr(),
                  freq.data_ptr(), _ptr(qw), _ptr(kw), out.data_ptr(), _ptr(k_out), _ptr(kc),
                  _ptr(vc), _ptr(lens), pos.numel(), hq, hkv, hd, 2 * pairs, q_st, q_sh, k_st, k_sh,
