@@ -697,7 +697,7 @@ __device__ __forceinline__ void dense_block(const PrefixAttn &a, const Plan &pla
 }
 
 template <int D, int W>
-__global__ __launch_bounds__(256, W == 32 ? 2 : 3) void k_prefix_dense(PrefixAttn a, Plan plan,
+__global__ __launch_bounds__(256, D > 128 ? 1 : W == 32 ? 2 : 3) void k_prefix_dense(PrefixAttn a, Plan plan,
                                                                        float *__restrict__ part,
                                                                        float *__restrict__ pml) {
     __shared__ __attribute__((aligned(16))) union {
@@ -809,8 +809,9 @@ Plan plan_of(int groups, int rows, int hq, int hkv, int hd, int prefix, int own)
     const int64_t seqs = (int64_t)groups * rows;
     // Short caches: a sequence's block reads the prefix for itself, and nothing is merged.
     p.joined = pt + ot <= 32;
-    p.dense = !p.joined && R > 32 && hd <= 128;
-    // One block's rows for all of up to 64: K and V are read once.
+    // f32 MFMA, which takes 16 or 32 rows as they are, or limbs for 64 or 128 of them: us of 32
+    // rows of 128 on 32767 positions 57 / 62, of 64 rows 104 / 76.
+    p.dense = !p.joined && R > 32;
     p.rb = p.joined || p.dense ? 1 : std::min((R + 15) / 16, hd <= 128 ? 2 : 1);
     p.prows = p.dense ? (R <= 64 ? 64 : 128) : 16 * p.rb;
     p.nw = p.joined && hd <= 128 ? 8 : 4;
@@ -827,11 +828,12 @@ Plan plan_of(int groups, int rows, int hq, int hkv, int hd, int prefix, int own)
     };
     const int64_t units = (int64_t)groups * hkv, ob = seqs * hkv * p.gtiles;
     // Blocks wanted, us with them / with half as many or half as many again: 256 for one pass of
-    // few rows (32 rows on 4096 positions 17.4, 512: 20.2; 16 rows 12.8, 13.9), or 512 past
-    // 128 dimensions, where a CU has one at a time (28 rows of 256, 7 groups of up to 13296:
-    // 169, 256: 186); 768 dense ones of 64 rows, three a CU (64 rows on 4096 positions 20.2,
-    // 512: 25.3), 512 of 128 (32767 positions 119, 256: 148).
-    const int want = p.prows == 64 ? 768 : p.dense || hd > 128 ? 512 : 256;
+    // few rows (32 rows on 4096 positions 17.4, 512: 20.2; 16 rows 12.8, 13.9), but 512 past
+    // 128 dimensions (28 rows of 256, 7 groups of up to 13296: 169, 256: 186); 768 dense ones of
+    // 64 rows, three a CU (64 rows on 4096 positions 20.2, 512: 25.3), 512 of 128 (32767
+    // positions 119, 256: 148), and 256 past 128 dimensions, one a CU (256 rows of 256 on 8192
+    // positions 199, 512: 219, on f32 MFMA 257; of 160 dimensions 95, on f32 MFMA 160).
+    const int want = hd > 128 ? (p.dense ? 256 : 512) : !p.dense ? 256 : p.prows == 64 ? 768 : 512;
     p.pcap = pt ? cap(want, units * p.ptiles, pt) : 0;
     p.ocap = ot ? cap(256, ob, ot) : 0;
     p.pblocks = (int)((units * p.pcap + 7) / 8 * 8 * p.ptiles);
@@ -868,10 +870,10 @@ int launch_prefix_attention(const PrefixAttn &a, float *scratch, hipStream_t s) 
     const dim3 grid(p.pblocks + p.oblocks);
 #define TB_PREFIX(D)                                                                          \
     case D:                                                                                   \
+        if (p.dense) k = p.prows == 64 ? k_prefix_dense<D, 16> : k_prefix_dense<D, 32>;       \
         if constexpr (D <= 128) {                                                             \
-            if (p.dense) k = p.prows == 64 ? k_prefix_dense<D, 16> : k_prefix_dense<D, 32>;   \
-            else if (p.nw == 8) k = k_prefix_stream<D, 1, 8>;                                 \
-            else if (p.rb == 2) k = k_prefix_stream<D, 2, 4>;                                 \
+            if (!k && p.nw == 8) k = k_prefix_stream<D, 1, 8>;                                \
+            if (!k && p.rb == 2) k = k_prefix_stream<D, 2, 4>;                                \
         }                                                                                     \
         if (!k) k = k_prefix_stream<D, 1, 4>;                                                 \
         break
