@@ -190,11 +190,48 @@ def test_ranges(cuda, rows, kind):
           want, bound)
 
 
-@pytest.mark.parametrize("rows", [2, 48])
-def test_infinities_and_nan(cuda, rows):
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("rows", [5, 25, 50, 100])
+def test_every_width(cuda, d, rows):
+    """Each head_dim on every route: few rows, two tiles of them, 64 and 128 a block; the prefix
+    split and ending inside of a tile, ragged groups, a negative scale."""
+    print(f"case prefix_attention d={d} rows={rows}", flush=True)
+    arrays = inputs(d + rows, 2, rows, 2, 2, d, 703, 21)
+    q, kp, vp, k, v = (torch.from_numpy(a).to(cuda) for a in arrays)
+    plen = [703, 518 + rows]
+    olen = np.random.default_rng(rows).integers(0, 22, (2, rows)).tolist()
+    kp[1, :, plen[1]:], vp[1, :, plen[1]:] = float("inf"), float("nan")
+    want, bound = reference(*arrays[:3], plen, *arrays[3:], olen, -0.05)
+    got = tb.prefix_attention(q, kp, vp, torch.tensor(plen, device=cuda), k, v,
+                              torch.tensor(olen, device=cuda), scale=-0.05)
+    check(got, want, bound)
+
+
+@pytest.mark.parametrize("rows", [5, 25, 50, 100])
+@pytest.mark.parametrize("d", [64, 128, 192])
+def test_errors_are_those_of_f32(cuda, d, rows):
+    """The bound above takes every rounding at its largest.  The errors' root mean square is
+    held to twice that of the same formula in f32 products and sums, whose order is another:
+    a limb or product of limbs that is lost makes it a hundred times as large."""
+    arrays = inputs(d + rows, 1, rows, 2, 2, d, 3000, 9)
+    want, _ = reference(*arrays[:3], [3000], *arrays[3:], [[0] * rows], d ** -0.5)
+    q, kp, vp = (torch.from_numpy(a).to(cuda) for a in arrays[:3])
+    x = q[0].transpose(0, 1)
+    a = (x @ kp[0].transpose(-1, -2)) * d ** -0.5
+    e = torch.exp(a - a.amax(-1, keepdim=True))
+    plain = ((e @ vp[0]) / e.sum(-1, keepdim=True)).transpose(0, 1).cpu().numpy()
+    got = tb.prefix_attention(q, kp, vp, 3000)[0].cpu().numpy()
+    rms = [float(np.sqrt(((g - want[0]) ** 2).mean())) for g in (got, plain)]
+    print(f"root mean square error {rms[0]:.3g}, in f32 {rms[1]:.3g}", flush=True)
+    assert rms[0] <= 2 * rms[1]
+
+
+@pytest.mark.parametrize("rows", [2, 20, 48, 100])
+@pytest.mark.parametrize("P", [100, 700])
+def test_infinities_and_nan(cuda, rows, P):
     """What a row sees counts as the formula has it: a K of -inf or +inf against factors of one
     sign, infinities and NaN in V, NaN in a query."""
-    H, KVH, D, P, L = 2, 2, 32, 100, 9
+    H, KVH, D, L = 2, 2, 32, 9
     q, kp, vp, k, v = inputs(4, 1, rows, H, KVH, D, P, L)
     q[0, 0] = np.abs(q[0, 0])
     q[0, 1] = -np.abs(q[0, 1])

@@ -97,6 +97,7 @@ struct Range {
 };
 __device__ __forceinline__ Range split_range(int len, int cap, int split) {
     const int tiles = (len + kTile - 1) / kTile;
+    cap = max(cap, 1);   // 0 for a cache without positions
     const int each = max(((tiles + cap - 1) / cap + 3) & ~3, kMinTiles);   // the waves' alike
     return {min(split * each, tiles), min((split + 1) * each, tiles), (tiles + each - 1) / each};
 }
