@@ -18,6 +18,7 @@ namespace tb {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kThreads = 256;
 constexpr double kLog2e = 1.44269504088896340736, kLn2 = 0.69314718055994530942;
@@ -83,48 +84,38 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// A chunk's exponentials, at most 2 each and 2^13 of them, are multiples of 2^-kGrid: their
-// sum takes 53 bits.  (e + kRound) - kRound is e so rounded.
-constexpr int kGrid = 39;
-constexpr double kRound = 1.5 * (double)(1ull << (52 - kGrid));
-
 // A chunk's sum of exponentials: that of e^(x - top).
 struct Part {
     double sum, top;
 };
 
-// 2^(t - n) of n an integer, n in the low word of y = t - n + kMagic as rounded.  A fit of
-// degree 8 to 2^f on +-1/2, 1.1e-12 off at most.
-constexpr double kMagic = 1.5 * (double)(1ull << 52);
+// A fit of degree 7 to 2^f on +-1/2, 5.5e-11 of it off at most.
+constexpr double kMagic = 1.5 * (double)(1ull << 52);   // y + kMagic has rint(y) in its low word
 __device__ __forceinline__ double exp2_fit(double f) {
-    constexpr double c[9] = {1.0, 0.6931471805459335, 0.2402265069581299, 0.05550410941205933,
-                             0.009618129159402558, 0.0013333450568000645, 0.00015403455852453838,
-                             1.5310079402249296e-05, 1.3255224878668817e-06};
-    double p = c[8];
+    constexpr double c[8] = {0.9999999999595618, 0.6931471805568324, 0.24022651213498092, 0.055504109063258665, 0.009618025613318034, 0.0013333478473685416, 0.00015469729214118296, 1.5303700711365693e-05};
+    double p = c[7];
 #pragma unroll
-    for (int i = 7; i >= 0; --i) p = fma(p, f, c[i]);
+    for (int i = 6; i >= 0; --i) p = fma(p, f, c[i]);
     return p;
 }
 
 // One block per row and chunk of 1024 U tokens, whose logits stay in registers: the
 // largest, the sum of exponentials from it, and the k largest logits in order.  The k-th
 // largest of the threads' own largest bounds the k-th largest of all from below, so that
-// few logits are collected in LDS, at most the 4 U + 1 of each of k threads; they are
-// ranked there.  Where logits that are equal at this border make them more, the border is
-// found anew with the tokens, which differ.  Exponentials are rounded to multiples of
-// 2^-kGrid, whose sums are exact, so that rows that are alike have sums that are alike,
-// however they lie in memory: vectors start where the row's address is a multiple of 16
-// bytes, `lead` tokens ahead of the chunk's first, and its last `lead` tokens are left to a
-// thread each.
+// few logits are collected in LDS, at most the 4 U of each of k threads; they are ranked
+// there.  Where logits that are equal at this border make them more, the border is found
+// anew with the tokens, which differ.  Threads take tokens by their number, not by their
+// address (rows of an odd vocabulary are read in vectors that are not aligned), so that rows
+// that are alike have sums that are alike to the last bit.
 //
-// Bound by the logits' bytes, 28 us of 131 MB, and the exponentials, 20 instructions in 64 bits
-// each, 11 more: 256 rows of 128256 take 38.8 us, 56.8 with a Taylor sum and the border by
-// every wave from logits and tokens; blocks that ask for their next chunk ahead, and so have
-// fewer waves side by side, 59.6.
+// Bound by the logits' bytes, 28 us of 131 MB, and the exponentials, 14 instructions in 64
+// bits each: 256 rows of 128256 take 32.7 us with seven blocks a CU, 37.8 with five (which its
+// registers would have), 59.6 where blocks ask for their next chunk ahead and three fit, 56.8
+// with a Taylor sum of degree 10 and the border by every wave from logits and tokens.
 template <int U>
-__global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamSelect p, Part *__restrict__ parts,
+__global__ __launch_bounds__(kThreads, 7) void k_beam_chunk(BeamSelect p, Part *__restrict__ parts,
                                                          uint64_t *__restrict__ best) {
-    extern __shared__ uint64_t items[];   // [(4 U + 1) k]
+    extern __shared__ uint64_t items[];   // [4 U k]
     __shared__ uint64_t top_of[kThreads];
     __shared__ uint32_t keys[kThreads];
     __shared__ double sums[kThreads / 64];
@@ -133,36 +124,23 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamSelect p, Part *__r
     const int tid = threadIdx.x, row = blockIdx.y, V = p.vocab;
     if (p.finished && p.finished[row]) return;
     const float *x = p.logits + (size_t)row * V;
-    const int lead = (int)(reinterpret_cast<uintptr_t>(x) % 16 / 4);
-    const int c0 = blockIdx.x * 1024 * U, c1 = min(V, c0 + 1024 * U);
-    const int t0 = c0 - lead + 4 * tid;   // of vector 0
+    const int c0 = blockIdx.x * 1024 * U, t0 = c0 + 4 * tid;
     float v[U][4];
-    if (c0 + 1024 * U <= V && !lead) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float4 y = *reinterpret_cast<const float4 *>(x + t0 + 1024 * u);
+    for (int u = 0; u < U; ++u) {
+        const int t = t0 + 1024 * u;
+        if (t + 3 < V) {
+            const f32x4_any y = *reinterpret_cast<const f32x4_any *>(x + t);
             v[u][0] = y.x; v[u][1] = y.y; v[u][2] = y.z; v[u][3] = y.w;
-        }
-    } else {
+        } else {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int t = t0 + 1024 * u;
-            if (t >= c0 && t + 3 < c1) {
-                const float4 y = *reinterpret_cast<const float4 *>(x + t);
-                v[u][0] = y.x; v[u][1] = y.y; v[u][2] = y.z; v[u][3] = y.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    v[u][i] = t + i >= c0 && t + i < c1 ? x[t + i] : -INFINITY;
-            }
+            for (int i = 0; i < 4; ++i) v[u][i] = t + i < V ? x[t + i] : -INFINITY;
         }
     }
-    const int t_rest = c0 + 1024 * U - lead + tid;
-    const float rest = tid < lead && t_rest < c1 ? x[t_rest] : -INFINITY;
     if (tid == 0) found = bad = 0;
     // ---- the largest
-    float mine = rest;
-    bool nan = rest != rest;
+    float mine = -INFINITY;
+    bool nan = false;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -198,27 +176,25 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamSelect p, Part *__r
     double sum = 0.0, ref = 0.0;
     if (fabsf(top) < 524288.f) {
         const double n = rint((double)top * kLog2e), low = n - kMagic;
-        const float least = top - 40.f;   // rounds to 0, as -inf does
+        const float least = top - 80.f;   // e^-80 for -inf, which is no part of the sum
         ref = n * kLn2;
         auto add = [&](float y) {
-            const double t = (double)fmaxf(y, least) * kLog2e, r = t - low;
+            const double t = (double)fmaxf(y, least) * kLog2e, r = t - low;   // rint(t) - n
             const double e = exp2_fit(t - (r + low));
             const int up = (int)__double2loint(r);
-            sum += (__hiloint2double(__double2hiint(e) + (up << 20), __double2loint(e)) + kRound) - kRound;
+            sum += __hiloint2double(__double2hiint(e) + (up << 20), __double2loint(e));
         };
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) add(v[u][i]);
-        if (lead) add(rest);
     } else if (top > -INFINITY) {   // far out, or infinite, which makes it NaN
         ref = top;
-        auto add = [&](float y) { sum += (exp64((double)y - ref) + kRound) - kRound; };
+        auto add = [&](float y) { sum += exp64((double)y - ref); };
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) add(v[u][i]);
-        add(rest);
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
@@ -230,7 +206,7 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamSelect p, Part *__r
         parts[at] = {bad ? (double)NAN : sum, ref};
     }
     // ---- what is not below the border
-    const int cap = (4 * U + 1) * p.k;
+    const int cap = 4 * U * p.k;
     const float least = border;
     auto item = [](float y, int t) { return ((uint64_t)order_key(y) << 32) | (uint32_t)~t; };
     auto collect = [&](float y, int t) {
@@ -243,7 +219,6 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamSelect p, Part *__r
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) collect(v[u][i], t0 + 1024 * u + i);
-    if (lead) collect(rest, t_rest);
     __syncthreads();
     int n = found;
     if (n > cap) {   // many equal ones: the border among the threads' best tokens of them
@@ -256,7 +231,6 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamSelect p, Part *__r
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) larger(v[u][i], t0 + 1024 * u + i);
-        larger(rest, t_rest);
         top_of[tid] = most;
         __syncthreads();
         if (tid == 0) found = 0;
@@ -273,7 +247,6 @@ __global__ __launch_bounds__(kThreads) void k_beam_chunk(BeamSelect p, Part *__r
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) again(v[u][i], t0 + 1024 * u + i);
-        again(rest, t_rest);
         __syncthreads();
         n = found;
     }
@@ -500,7 +473,7 @@ int launch_beam_select(const BeamSelect &p, void *scratch, hipStream_t s) {
     const int rows = p.groups * p.beams, u = vectors(rows, p.vocab), chunks = chunks_of(p.vocab, u);
     Part *parts = static_cast<Part *>(scratch);
     uint64_t *best = reinterpret_cast<uint64_t *>(parts + (size_t)rows * chunks);
-    const size_t lds = (size_t)(4 * u + 1) * p.k * sizeof(uint64_t);
+    const size_t lds = (size_t)4 * u * p.k * sizeof(uint64_t);
     auto *k = u == 1 ? k_beam_chunk<1> : u == 2 ? k_beam_chunk<2> : u == 4 ? k_beam_chunk<4> : k_beam_chunk<8>;
     hipLaunchKernelGGL(k, dim3(chunks, rows), dim3(kThreads), lds, s, p, parts, best);
     TB_LAUNCHED();

@@ -214,7 +214,7 @@ void launch(const RopeParams &p, hipStream_t s) {
     // Heads a group: all that share the angles, but groups for every CU first.
     const int64_t groups = (int64_t)p.n * heads;
     int per = 1;
-    while (per < 8 && groups / (2 * per) * L >= 256 * 512) per *= 2;
+    while (per < 4 && groups / (2 * per) * L >= 256 * 512) per *= 2;
     const int parts = (heads + per - 1) / per;
     const int64_t blocks = ((int64_t)p.n * parts + 256 / L - 1) / (256 / L);
     if (p.interleaved)
