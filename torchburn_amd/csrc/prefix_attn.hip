@@ -808,8 +808,10 @@ Plan plan_of(int groups, int rows, int hq, int hkv, int hd, int prefix, int own)
     const int G = hq / hkv, R = rows * G;
     const int pt = (prefix + kTile - 1) / kTile, ot = (own + kTile - 1) / kTile;
     const int64_t seqs = (int64_t)groups * rows;
-    // Short caches: a sequence's block reads the prefix for itself, and nothing is merged.
-    p.joined = pt + ot <= 32;
+    // Short caches: a sequence's block reads the prefix for itself, and nothing is merged.  us so
+    // / in two launches: 17 tiles, 4 sequences in groups of 7 heads of 64 8.3 / 7.1 + 3.7; 20
+    // tiles, 64 in groups of 4 of 128 26 / 20 + 4; 29 tiles, 4 sequences 17.2 / 7.4 + 3.8.
+    p.joined = pt + ot <= 20;
     // f32 MFMA, which takes 16 or 32 rows as they are, or limbs for 64 or 128 of them: us of 32
     // rows of 128 on 32767 positions 57 / 62, of 64 rows 104 / 76.
     p.dense = !p.joined && R > 32;
