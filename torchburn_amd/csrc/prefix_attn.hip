@@ -6,7 +6,9 @@
 //
 // over the prefix's positions and the row's own ones.  One pass over K and V with a
 // running reference m and sum; the positions are split over blocks, whose
-// results are merged in the order of the splits.
+// results are merged in the order of the splits.  Few rows go through f32 MFMA,
+// whose factors are as they are in memory (k_prefix_stream), many through bf16 MFMA with
+// three limbs a factor (k_prefix_dense); the sequences' own caches always through the first.
 #include <math.h>
 
 #include <algorithm>
@@ -178,6 +180,11 @@ struct State {
 //     register j for row c, and A's row c of block (q, i) is dimension 64 q + 4 c + i.
 // The next tile's K is requested when this one's scores are on their way, its V when
 // this one's outputs are.
+//
+// Bound by memory, on short prefixes by the launch and the blocks' first and last
+// steps (6.4 us of the second): 8 KV heads of 128, 16 rows on 32767 positions 50 us (5.4 TB/s
+// of K and V), 32 rows on 4096 17.4.  The f32 MFMA (154 TFLOP/s in a large product) would
+// bound 64 rows: 104 us on 32767 positions, k_prefix_dense 76.
 template <int D, int RB>
 __device__ __forceinline__ void stream(const PrefixAttn &a, const Job &job, int i0, int i1, int first,
                                        int step, State<D, RB> &st) {
@@ -479,6 +486,12 @@ struct Limbs {
 // of the bf16 rate, where the f32 MFMA has a sixteenth.  An infinity or NaN among K, V or
 // the queries makes NaN of the limbs' products: a wave that has one in its results
 // works its rows out anew in f32 (stream()).
+//
+// Bound by the matrix unit at the clock it leaves itself, and by what shares the SIMDs
+// with it: 256 rows of 128 on 32767 positions of 8 KV heads 205 us (168 TFLOP/s of f32
+// products, six bf16 ones each; a large bf16 product reaches 1219), of which the MFMAs
+// alone take 131, with their operands' reads 160, with the limbs 182.  Operands read an
+// MFMA group ahead by force spill and gain nothing (218).
 template <int D, int W>
 __device__ __forceinline__ void dense_block(const PrefixAttn &a, const Plan &plan, const Job &job,
                                             Limbs<D> &lds, float *part, float *pml) {
@@ -716,7 +729,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : W == 32 ? 2 : 3) void k_prefix_d
 // A row's partial results, normalised, in the shares of their sums, in the order of the slots, by
 // WR waves: groups of LC lanes of four dimensions each take every 64 WR / LC-th slot, the
 // first of them requested before the shares are known (every slot's place in the scratch
-// can be read, and what was not written has a share of 0).
+// can be read, and what was not written has a share of 0).  Bound by the launch and the way
+// of those reads: 4.0 us for 256 rows of 33 slots, 9.5 for 2048 (34.6 MB).
 template <int LC, int WR>
 __global__ __launch_bounds__(256) void k_prefix_merge(PrefixAttn a, Plan plan,
                                                       const float *__restrict__ part,
@@ -812,8 +826,8 @@ Plan plan_of(int groups, int rows, int hq, int hkv, int hd, int prefix, int own)
     // / in two launches: 17 tiles, 4 sequences in groups of 7 heads of 64 8.3 / 7.1 + 3.7; 20
     // tiles, 64 in groups of 4 of 128 26 / 20 + 4; 29 tiles, 4 sequences 17.2 / 7.4 + 3.8.
     p.joined = pt + ot <= 20;
-    // f32 MFMA, which takes 16 or 32 rows as they are, or limbs for 64 or 128 of them: us of 32
-    // rows of 128 on 32767 positions 57 / 62, of 64 rows 104 / 76.
+    // f32 MFMA for up to 32 rows, or limbs for 64 or 128 of them: us of 32 rows of 128 on 32767
+    // positions 57 / 62, of 64 rows 104 / 76.
     p.dense = !p.joined && R > 32;
     p.rb = p.joined || p.dense ? 1 : std::min((R + 15) / 16, hd <= 128 ? 2 : 1);
     p.prows = p.dense ? (R <= 64 ? 64 : 128) : 16 * p.rb;

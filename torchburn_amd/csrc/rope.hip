@@ -52,11 +52,11 @@ struct Piece {
 // A group of L lanes takes a token's heads h0 .. h0 + per - 1 (queries, then keys, then
 // values), a lane NU units of 2 W dimensions of each: W pairs of the rotation, whose
 // angles it works out once for all of them (180 instructions in 64 bits, against 60 a
-// head), or 2 W dimensions behind it.  W = 4: 16-byte loads, and both pieces of a pair
+// head: 4096 tokens take 68, 45, 36 and 42 us with 1, 2, 4 and 8 heads), or 2 W dimensions behind it.  W = 4: 16-byte loads, and both pieces of a pair
 // of the half layout in one lane; W = 1 where sizes, strides or addresses do not allow it.
 //
 // Bound by the heads' bytes, on few tokens by the launch: 4096 tokens of 32 + 8 heads of 128,
-// 168 MB, take 35.0 us (4.8 TB/s, a large copy 4.9); four tokens 5.1.
+// 168 MB, take 36 us (4.6 TB/s, a large copy 4.9); four tokens 5.2.
 template <int L, int NU, int W, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void k_norm_rope(RopeParams p, int per, int parts) {
     const int lane = threadIdx.x % L;
@@ -211,7 +211,7 @@ bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 template <int L, int NU, int W>
 void launch(const RopeParams &p, hipStream_t s) {
     const int heads = p.hq + (p.append ? 2 : 1) * p.hkv;
-    // Heads a group: all that share the angles, but groups for every CU first.
+    // Heads a group: up to four share the angles, but groups for every CU first.
     const int64_t groups = (int64_t)p.n * heads;
     int per = 1;
     while (per < 4 && groups / (2 * per) * L >= 256 * 512) per *= 2;
