@@ -209,3 +209,26 @@ def test_captured_and_two_streams(cuda):
         for i in range(2):
             assert torch.equal(k[:, i, :, :, :5], was[:, i, out[2][i], :, :5])
             assert torch.equal(k[:, i, :, :, 5:], was[:, i, :, :, 5:])
+
+
+def test_captured_widest(cuda):
+    """64 beams and 64 results, whose selection needs more LDS than a launch has by itself."""
+    x, scores = torch.randn((64, 3001), device=cuda), torch.randn(64, device=cuda)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = tb.beam_select(x, scores, k=64)
+    for _ in range(3):
+        x.normal_()
+        graph.replay()
+        want = tb.beam_select(x, scores, k=64)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+def test_a_cache_given_twice(cuda):
+    k = torch.randn((2, 1, 3, 32), device=cuda)
+    par = torch.tensor([1, 0], device=cuda)
+    for c in (k, k.cpu()):
+        with pytest.raises(tb.UnsupportedOpError, match="twice"):
+            tb.beam_reorder(par, [c], [c], 2)

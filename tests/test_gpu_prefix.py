@@ -14,6 +14,7 @@ import pytest
 import torch
 
 import torchburn_amd as tb
+from torchburn_amd import _lib
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -305,6 +306,35 @@ def test_captured_two_graphs(cuda):
         torch.cuda.synchronize()
         for _, out in graphs:
             assert torch.equal(out, want)
+
+
+def test_the_streams_workspace(cuda):
+    """Without scratch of the caller's the C entries take the stream's, and refuse a capture."""
+    arrays = inputs(6, 1, 6, 8, 2, 64, 900, 32)
+    q, kp, vp, k, v = (torch.from_numpy(a[0]).to(cuda) for a in arrays)
+    want = tb.prefix_attention(q, kp, vp, 900, k, v, 32)
+    got = torch.empty_like(want)
+    x, scores = torch.randn((3, 4001), device=cuda), torch.zeros(3, device=cuda)
+    s, t, b = (torch.empty(3, dtype=d, device=cuda) for d in (torch.float32, torch.int64, torch.int64))
+    P = lambda a: a.data_ptr()
+
+    def calls():
+        stream = torch.cuda.current_stream().cuda_stream
+        yield _lib.lib().tb_prefix_attention(
+            P(q), P(kp), P(vp), None, P(k), P(v), None, P(got), 1, 6, 8, 2, 64, 900, 32, 900, 32, 0,
+            900 * 64, 64, 0, 900 * 64, 64, 2 * 32 * 64, 32 * 64, 64, 2 * 32 * 64, 32 * 64, 64, 0.125,
+            None, 0, stream)
+        yield _lib.lib().tb_beam_select(P(x), P(scores), None, P(s), P(t), P(b), 1, 3, 4001, 3, 0,
+                                        None, 0, stream)
+    assert list(calls()) == [_lib.TB_OK] * 2
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    for a, c in zip((s, t, b), tb.beam_select(x, scores)):
+        assert torch.equal(a, c)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert list(calls()) == [_lib.TB_ERR_UNSUPPORTED] * 2
+        got.zero_()
 
 
 def test_streams_side_by_side(cuda):

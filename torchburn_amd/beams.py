@@ -92,8 +92,8 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     (rows,) / (groups, rows); numbers past the caches raise ValueError, tensors are clamped
     on the device.  Without k_cache and v_cache there is the prefix only.  Positions past the
     lengths take no part, whatever the caches hold there; a row that sees none gives zeros.
-    ``scale`` defaults to head_dim ** -0.5.  f32, in q's shape.  A number and a tensor of the
-    same length may differ in their last bits, since the work is split by what the call
+    ``scale`` defaults to head_dim ** -0.5; head_dim is a multiple of 32 up to 256.  f32, in
+    q's shape.  A number and a tensor of the same length may differ in their last bits, since the work is split by what the call
     knows.  Does not wait for the device."""
     op = "prefix_attention"
     shape = q.shape
@@ -154,8 +154,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = N
     ``eos`` alone and keeps its score.  Logits of -inf (process_logits() masks) are never
     taken; a beam whose score is infinite or NaN, or that has a logit of NaN or +inf, has no
     continuation (scores of a group's first step: 0 and then -inf).  Where fewer than k are
-    left, tokens and beams are -1 and scores -inf.  Up to 64 beams, k up to 64.  Does not wait
-    for the device."""
+    left, tokens and beams are -1 and scores -inf.  Up to 64 beams, k up to 64, a vocabulary
+    up to 2 ** 20.  Does not wait for the device."""
     op = "beam_select"
     shape = logits.shape
     if len(shape) not in (2, 3) or scores.shape != shape[:-1]:
@@ -230,6 +230,8 @@ def beam_reorder(beams: torch.Tensor, k_caches: Sequence[torch.Tensor],
     if not alike:
         if any(c.shape != k0.shape for c in given):
             raise _bad(op, "the layers' caches differ in shape")
+        if len(set(ptrs)) != len(given) and k0.numel():
+            raise _bad(op, "a cache is given twice")
         caches = [_copied(c, dev) for c in given]
         k0, v0 = caches[0], caches[layers]
         ptrs = (C.c_void_p * len(given))(*map(T.data_ptr, caches))

@@ -419,8 +419,9 @@ __global__ __launch_bounds__(64 * NW, D <= 192 ? 2 : 1) void k_prefix_stream(
 
 // ---- many rows: bf16 MFMA -------------------------------------------------------
 
-// 8 values as three bf16 limbs, x = hi + mid + lo but for 2^-27 of x: each is the
-// rounded rest of those before.  bf16 has f32's exponents, so that nothing is scaled.
+// 8 values as three bf16 limbs, x = hi + mid + lo but for 2^-27 of x (and 2^-134, the half of
+// bf16's smallest step): each is the rounded rest of those before.  bf16 has f32's
+// exponents, so that nothing is scaled.
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 &hi, bf16x8 &mid, bf16x8 &lo) {
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {

@@ -51,9 +51,10 @@ struct Piece {
 
 // A group of L lanes takes a token's heads h0 .. h0 + per - 1 (queries, then keys, then
 // values), a lane NU units of 2 W dimensions of each: W pairs of the rotation, whose
-// angles it works out once for all of them (180 instructions in 64 bits, against 60 a
-// head: 4096 tokens take 68, 45, 36 and 42 us with 1, 2, 4 and 8 heads), or 2 W dimensions behind it.  W = 4: 16-byte loads, and both pieces of a pair
-// of the half layout in one lane; W = 1 where sizes, strides or addresses do not allow it.
+// angles it works out once for all of them (180 instructions in 64 bits, against 60 a head:
+// 4096 tokens of 40 heads take 68, 45, 36 and 42 us with 1, 2, 4 and 8 heads a group), or 2 W
+// dimensions behind it.  W = 4: 16-byte loads, and both pieces of a pair of the half layout in
+// one lane; W = 1 where sizes, strides or addresses do not allow it.
 //
 // Bound by the heads' bytes, on few tokens by the launch: 4096 tokens of 32 + 8 heads of 128,
 // 168 MB, take 36 us (4.6 TB/s, a large copy 4.9); four tokens 5.2.

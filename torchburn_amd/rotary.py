@@ -222,7 +222,7 @@ def norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
     ``v`` as it is.  Returns the turned queries.
 
     A number outside the caches raises ValueError; a sequence whose kv_len is outside has no
-    row written.  Caches in f32 on q's device with head_dim contiguous and sequences
+    row written; no two rows of the caches may share memory.  Caches in f32 on q's device with head_dim contiguous and sequences
     a constant stride apart are written in place; any others are converted whole at every
     call.  Does not wait for the device."""
     return _call("norm_rope_append", q, k, v, positions, inv_freq, q_weight, k_weight, eps,
