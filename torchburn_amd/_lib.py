@@ -33,6 +33,7 @@ class UnsupportedOpError(RuntimeError):
 
 _lock = threading.Lock()
 _lib = None
+_device = None   # torch.cuda.current_device, once torch is needed
 
 _p = C.c_void_p
 _i64 = C.c_int64
@@ -143,9 +144,13 @@ def int64(x) -> int:
 
 def call_on(dev, name: str, *args) -> None:
     """call() with ``dev`` as the current device, for kernels launched on one of its streams."""
-    import torch
-    if dev.index == torch.cuda.current_device():
+    global _device
+    if _device is None:
+        import torch
+        _device = torch.cuda.current_device
+    if dev.index == _device():
         return call(name, *args)
+    import torch
     with torch.cuda.device(dev):
         return call(name, *args)
 

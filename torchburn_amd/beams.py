@@ -23,6 +23,7 @@ import torch
 from . import _lib
 from ._lib import UnsupportedOpError
 from .quantization import _int32_on_gpu, _on_gpu, _ptr, _stream, _target, _write_back
+from .rotary import _ready
 
 _dtype = attrgetter("dtype")
 _ALIGNED = bytes(range(0, 256, 16))   # the low bytes of 16-byte aligned addresses
@@ -32,15 +33,17 @@ def _bad(op: str, msg: str) -> UnsupportedOpError:
     return UnsupportedOpError(f"{_lib.UNSUPPORTED_MARKER} {op}: {msg}")
 
 
-def _usable(c: torch.Tensor, st, dev: torch.device) -> bool:
+# The checks below are most of a small call's time (0.1 us for each thing asked of a tensor):
+# what the kernels can take as it is passes with as few of them as tell that.
+
+
+def _usable(c: torch.Tensor, st, index) -> bool:
     """Whether the kernels can take a cache of strides st where it is."""
-    if c.dtype is not torch.float32 or c.get_device() != dev.index or c.data_ptr() % 16 or \
-            (st[-1] != 1 and c.shape[-1] != 1):
-        return False
+    odd = 0
     for s in st[:-1]:
-        if s % 4:
-            return False
-    return True
+        odd |= s
+    return c.dtype is torch.float32 and c.get_device() == index and not odd & 3 and \
+        (st[-1] == 1 or c.shape[-1] == 1) and not c.data_ptr() & 15
 
 
 def _copied(c: torch.Tensor, dev: torch.device) -> torch.Tensor:
@@ -52,7 +55,7 @@ def _cache(op: str, name: str, c: torch.Tensor, ndim: int, dev: torch.device):
     st = c.stride()
     if len(st) != ndim:
         raise _bad(op, f"{name} must have {ndim} dimensions, got {list(c.shape)}")
-    if not _usable(c, st, dev):
+    if not _usable(c, st, dev.index):
         c = _copied(c, dev)
         st = c.stride()
     return c, st
@@ -63,7 +66,7 @@ def _sequences(op: str, name: str, c: torch.Tensor, batched: bool, dev: torch.de
     c, st = _cache(op, name, c, 5 if batched else 4, dev)
     if not batched:
         return c, st
-    if st[0] != c.shape[1] * st[1] and c.shape[0] > 1:      # groups apart
+    if c.shape[0] > 1 and st[0] != c.shape[1] * st[1]:      # groups apart
         c = _copied(c, dev)
         st = c.stride()
     return c, st[1:]
@@ -75,7 +78,7 @@ def _lengths(op: str, name: str, t, count: int, dev) -> Tuple[Optional[torch.Ten
     if t.numel() != count or t.dtype.is_floating_point:
         raise _bad(op, f"{name} must be a number or {count} integers, got {t.dtype} "
                        f"{list(t.shape)}")
-    return _int32_on_gpu(t, dev), 0
+    return (t if _ready(t, torch.int32, dev.index) else _int32_on_gpu(t, dev)), 0
 
 
 def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
@@ -97,19 +100,23 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     knows.  Does not wait for the device."""
     op = "prefix_attention"
     shape = q.shape
-    if len(shape) not in (3, 4):
+    if len(shape) == 4:
+        groups, rows, heads, hd = shape
+        batched = True
+    elif len(shape) == 3:
+        rows, heads, hd = shape
+        groups, batched = 1, False
+    else:
         raise _bad(op, f"q must be [rows, num_heads, head_dim] or [groups, rows, num_heads, "
                        f"head_dim], got {list(shape)}")
-    dev, batched = _target(q), len(shape) == 4
-    rows, heads, hd = shape[-3:]
-    groups = shape[0] if batched else 1
-    x = _on_gpu(q, torch.float32, dev)
-    if x.data_ptr() % 16:      # a view that starts inside a 16-byte unit
+    dev = _target(q)
+    x = q if _ready(q, torch.float32, dev.index) else _on_gpu(q.detach(), torch.float32, dev)
+    if x.data_ptr() & 15:      # a view that starts inside a 16-byte unit
         x = x.detach().clone()
     kp, kps = _cache(op, "k_prefix", k_prefix, 4 if batched else 3, dev)
     vp, vps = _cache(op, "v_prefix", v_prefix, 4 if batched else 3, dev)
-    kvh, max_prefix, width = kp.shape[-3:]
-    if kp.shape != vp.shape or width != hd or (batched and kp.shape[0] != groups):
+    *lead, kvh, max_prefix, width = kp.shape
+    if vp.shape != kp.shape or width != hd or (batched and lead[0] != groups):
         raise _bad(op, f"prefixes {list(k_prefix.shape)} / {list(v_prefix.shape)} do not fit q "
                        f"{list(shape)}")
     if not batched:
@@ -120,13 +127,15 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     if k_cache is not None:
         kc, ks = _sequences(op, "k_cache", k_cache, batched, dev)
         vc, vs = _sequences(op, "v_cache", v_cache, batched, dev)
-        max_own = kc.shape[-2]
-        if kc.shape != vc.shape or kc.shape != (*shape[:-2], kvh, max_own, hd):
+        own = kc.shape
+        max_own = own[-2]
+        want = (groups, rows, kvh, max_own, hd) if batched else (rows, kvh, max_own, hd)
+        if own != want or vc.shape != want:
             raise _bad(op, f"caches {list(k_cache.shape)} / {list(v_cache.shape)} do not fit q "
                            f"{list(shape)} and {kvh} KV heads")
     pl, p = _lengths(op, "prefix_len", prefix_len, groups, dev)
     ol, o = _lengths(op, "kv_len", kv_len, groups * rows, dev)
-    out = x.new_empty(shape)
+    out = torch.empty_like(x, requires_grad=False)
     # scratch of this call's own, so that graphs captured on one stream share none
     size = _lib.lib().tb_prefix_attention_scratch(groups, rows, heads, kvh, hd,
                                                   p if pl is None else max_prefix,
@@ -157,24 +166,26 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = N
     left, tokens and beams are -1 and scores -inf.  Up to 64 beams, k up to 64, a vocabulary
     up to 2 ** 20.  Does not wait for the device."""
     op = "beam_select"
-    shape = logits.shape
-    if len(shape) not in (2, 3) or scores.shape != shape[:-1]:
+    *lead, beams, vocab = logits.shape if logits.ndim in (2, 3) else (0, 0, 0, -1)
+    if vocab < 0 or scores.shape != (*lead, beams):
         raise _bad(op, f"logits must be [.., beams, vocab] and scores [.., beams], got "
-                       f"{list(shape)} and {list(scores.shape)}")
+                       f"{list(logits.shape)} and {list(scores.shape)}")
     dev = _target(logits)
-    beams, vocab = shape[-2:]
-    groups = shape[0] if len(shape) == 3 else 1
+    groups = lead[0] if lead else 1
     k = beams if k is None else _lib.int64(k)
-    x, sc = _on_gpu(logits, torch.float32, dev), _on_gpu(scores, torch.float32, dev)
+    x = logits if _ready(logits, torch.float32, dev.index) else \
+        _on_gpu(logits.detach(), torch.float32, dev)
+    sc = scores if _ready(scores, torch.float32, dev.index) else \
+        _on_gpu(scores.detach(), torch.float32, dev)
     done = None
     if finished is not None:
         if finished.shape != scores.shape or eos is None:
             raise _bad(op, f"finished {list(finished.shape)} needs the scores' shape "
                            f"{list(scores.shape)}, and eos")
         done = _on_gpu(finished if finished.dtype is torch.bool else finished != 0, torch.bool, dev)
-    lead = (*shape[:-2], max(k, 0))
-    out = x.new_empty(lead)
-    tokens, parents = x.new_empty((2, *lead), dtype=torch.int64).unbind(0)
+    out = x.new_empty((*lead, max(k, 0)))
+    tokens = torch.empty_like(out, dtype=torch.int64)
+    parents = torch.empty_like(tokens)
     size = _lib.lib().tb_beam_select_scratch(groups, beams, vocab, k)
     scratch = x.new_empty(size // 4) if size > 0 else None
     _lib.call_on(dev, "tb_beam_select", x.data_ptr(), sc.data_ptr(), _ptr(done), out.data_ptr(),
@@ -206,42 +217,53 @@ def beam_reorder(beams: torch.Tensor, k_caches: Sequence[torch.Tensor],
     b = _on_gpu(beams, torch.int64, dev)
     n = beams.shape[-1]
     groups = beams.shape[0] if batched else 1
-    ks_in, vs_in = list(k_caches), list(v_caches)
-    if len(ks_in) != len(vs_in):
-        raise _bad(op, f"{len(ks_in)} k_caches against {len(vs_in)} v_caches")
     lens, ln = _lengths(op, "kv_len", kv_len, groups * n, dev)
-    layers, given = len(ks_in), ks_in + vs_in
+    layers, ndim = len(k_caches), 5 if batched else 4
+    if len(v_caches) != layers:
+        raise _bad(op, f"{layers} k_caches against {len(v_caches)} v_caches")
     if not layers:
         return
-    # Device caches of one layout are used as they are, checked as whole lists.
-    k0, v0, T = given[0], given[layers], torch.Tensor
-    ndim = 5 if batched else 4
-    if k0.ndim != ndim or k0.shape[-4] != n or (batched and k0.shape[0] != groups):
-        raise _bad(op, f"caches {list(k0.shape)} do not fit beams {list(beams.shape)}")
-    ptrs = (C.c_void_p * len(given))(*map(T.data_ptr, given))
-    alike = set(map(T.get_device, given)) == {dev.index} and \
-        set(map(_dtype, given)) == {torch.float32} and \
-        list(map(T.size, given)) == [k0.shape] * len(given) and \
-        list(map(T.stride, ks_in)) == [k0.stride()] * layers and \
-        list(map(T.stride, vs_in)) == [v0.stride()] * layers and \
-        not bytes(ptrs)[::8].translate(None, _ALIGNED) and _usable(k0, k0.stride(), dev) and \
-        _usable(v0, v0.stride(), dev)
-    caches = given
+    given, caches, stacked = (), (), True
+    for c in (k_caches, v_caches):
+        stacked = stacked and isinstance(c, torch.Tensor) and c.ndim == ndim + 1 and \
+            _usable(c, c.stride(), dev.index)
+    if stacked:      # a stack's caches differ by their addresses
+        shape, ks, vs = k_caches.shape[1:], k_caches.stride(), v_caches.stride()
+        alike = v_caches.shape == k_caches.shape
+        ptrs = (C.c_void_p * (2 * layers))(
+            *(c.data_ptr() + 4 * s[0] * i for c, s in ((k_caches, ks), (v_caches, vs))
+              for i in range(layers)))
+        ks, vs = ks[1:], vs[1:]
+    if not stacked or not alike:
+        # Device caches of one layout are used as they are, checked as whole lists.
+        ks_in, vs_in = list(k_caches), list(v_caches)
+        given = ks_in + vs_in
+        k0, v0, T = given[0], given[layers], torch.Tensor
+        shape, ks, vs = k0.shape, k0.stride(), v0.stride()
+        ptrs = (C.c_void_p * len(given))(*map(T.data_ptr, given))
+        alike = set(map(T.get_device, given)) == {dev.index} and \
+            set(map(_dtype, given)) == {torch.float32} and \
+            list(map(T.size, given)) == [shape] * len(given) and \
+            list(map(T.stride, ks_in)) == [ks] * layers and \
+            list(map(T.stride, vs_in)) == [vs] * layers and \
+            not bytes(ptrs)[::8].translate(None, _ALIGNED) and _usable(k0, ks, dev.index) and \
+            _usable(v0, vs, dev.index)
+    if len(shape) != ndim or shape[-4] != n or (batched and shape[0] != groups):
+        raise _bad(op, f"caches {list(shape)} do not fit beams {list(beams.shape)}")
     if not alike:
-        if any(c.shape != k0.shape for c in given):
+        if any(c.shape != shape for c in given):
             raise _bad(op, "the layers' caches differ in shape")
         if len(set(ptrs)) != len(given) and k0.numel():
             raise _bad(op, "a cache is given twice")
         caches = [_copied(c, dev) for c in given]
-        k0, v0 = caches[0], caches[layers]
+        ks, vs = caches[0].stride(), caches[layers].stride()
         ptrs = (C.c_void_p * len(given))(*map(T.data_ptr, caches))
-    ks, vs = k0.stride(), v0.stride()
     if not batched:
         ks, vs = (0, *ks), (0, *vs)
     kp = C.addressof(ptrs)
     _lib.call_on(dev, "tb_beam_reorder", _ptr(b), _ptr(lens), ln, kp,
-                 kp + layers * C.sizeof(C.c_void_p), layers, groups, n, k0.shape[-3], k0.shape[-1],
-                 k0.shape[-2], ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3], _stream(dev))
+                 kp + layers * C.sizeof(C.c_void_p), layers, groups, n, shape[-3], shape[-1],
+                 shape[-2], ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3], _stream(dev))
     if not alike:
         for c, g in zip(given, caches):
             _write_back(c, g)
