@@ -232,3 +232,46 @@ def test_a_cache_given_twice(cuda):
     for c in (k, k.cpu()):
         with pytest.raises(tb.UnsupportedOpError, match="twice"):
             tb.beam_reorder(par, [c], [c], 2)
+
+
+def test_reorder_converted_rows_stay(cuda):
+    """Of caches in 64 bits only what is taken over is rounded."""
+    par = torch.tensor([1, 1, 0], device=cuda)
+    k, v = (torch.randn((3, 2, 5, 32), device=cuda, dtype=torch.float64) for _ in range(2))
+    want = []
+    for c in (k, v):
+        w = c.clone()
+        w[:, :, :3] = c[par, :, :3].float().double()
+        w[1] = c[1]      # goes on from itself
+        want.append(w)
+    tb.beam_reorder(par, [k], [v], 3)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+def test_reorder_stacked(cuda):
+    """Stacks with spare layers, positions and unlike strides, as the lists of their layers."""
+    par = torch.tensor([[2, 0, 1], [1, 1, 1]], device=cuda)
+    kb = torch.randn((4, 2, 3, 2, 9, 64), device=cuda)
+    vb = torch.randn((3, 2, 5, 2, 3, 2, 64), device=cuda)
+    kb2, vb2 = kb.clone(), vb.clone()
+
+    def stacks(kb, vb):
+        k = kb[1:, :, :, :, 2:7]                            # [3, 2, 3, 2, 5, 64]
+        return k, vb.permute(0, 1, 4, 3, 2, 5, 6)[..., 1, :]  # [3, 2, 3, 2, 5, 64]
+    k, v = stacks(kb, vb)
+    assert k.shape == v.shape
+    tb.beam_reorder(par, k, v, 4)
+    k2, v2 = stacks(kb2, vb2)
+    for c in (k2, v2):
+        for g in range(2):
+            c[:, g, :, :, :4] = c[:, g, par[g], :, :4].clone()
+    assert torch.equal(kb, kb2) and torch.equal(vb, vb2)
+    tb.beam_reorder(par, list(k), v, 4)
+    for c in (k2, v2):
+        for g in range(2):
+            c[:, g, :, :, :4] = c[:, g, par[g], :, :4].clone()
+    assert torch.equal(kb, kb2) and torch.equal(vb, vb2)
+    with pytest.raises(tb.UnsupportedOpError, match="twice"):
+        tb.beam_reorder(par, k, k, 4)
+    with pytest.raises(tb.UnsupportedOpError, match="twice"):
+        tb.beam_reorder(par, k[:1].expand(3, -1, -1, -1, -1, -1), v, 4)

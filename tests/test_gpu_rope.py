@@ -212,3 +212,29 @@ def test_frequencies_turn_as_documented(cuda):
         a, _ = tb.norm_rope(q, q, torch.from_numpy(pos).to(cuda), f, attention_factor=c)
         check(a, *reference(q.cpu().numpy(), None, pos, f.cpu().numpy(), 0.0, False, c))
     assert math.isclose(c, 0.1 * math.log(16.0) + 1.0)
+
+
+def test_converted_caches_keep_their_other_rows(cuda):
+    """Of a cache in 64 bits only the row that is written is rounded; no cache is both."""
+    f, _ = tb.rope_frequencies(32, device=cuda)
+    q, k, v = (torch.randn((3, 2, 32), device=cuda) for _ in range(3))
+    pos = torch.tensor([4, 5, 6], device=cuda)
+    kc, vc = (torch.randn((3, 2, 4, 32), device=cuda, dtype=torch.float64) for _ in range(2))
+    was = kc.clone(), vc.clone()
+    tb.norm_rope_append(q, k, v, pos, f, kc, vc, 2)
+    for c, w, row in zip((kc, vc), was, (tb.norm_rope(q, k, pos, f)[1], v)):
+        assert torch.equal(c[:, :, 2], row.double())
+        c[:, :, 2] = w[:, :, 2]
+        assert torch.equal(c, w)
+    for c in (kc, kc.half(), kc.float(), kc.float().cpu()):
+        with pytest.raises(tb.UnsupportedOpError):
+            tb.norm_rope_append(q, k, v, pos, f, c, c, 2)
+
+
+def test_no_heads(cuda):
+    """A batch of two dimensions whose keys have no heads."""
+    f, _ = tb.rope_frequencies(32, device=cuda)
+    q, k = torch.randn((2, 3, 4, 32), device=cuda), torch.randn((2, 3, 0, 32), device=cuda)
+    pos = torch.arange(6, device=cuda).view(2, 3)
+    a, b = tb.norm_rope(q, k, pos, f)
+    assert torch.equal(a, tb.norm_rope(q, q, pos, f)[0]) and b.shape == k.shape

@@ -22,8 +22,8 @@ import torch
 
 from . import _lib
 from ._lib import UnsupportedOpError
-from .quantization import _int32_on_gpu, _on_gpu, _ptr, _stream, _target, _write_back
-from .rotary import _ready
+from .quantization import _int32_on_gpu, _on_gpu, _ptr, _stream, _target
+from .rotary import _give_back, _ready
 
 _dtype = attrgetter("dtype")
 _ALIGNED = bytes(range(0, 256, 16))   # the low bytes of 16-byte aligned addresses
@@ -96,8 +96,8 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     on the device.  Without k_cache and v_cache there is the prefix only.  Positions past the
     lengths take no part, whatever the caches hold there; a row that sees none gives zeros.
     ``scale`` defaults to head_dim ** -0.5; head_dim is a multiple of 32 up to 256.  f32, in
-    q's shape.  A number and a tensor of the same length may differ in their last bits, since the work is split by what the call
-    knows.  Does not wait for the device."""
+    q's shape.  A number and a tensor of the same length may differ in their last bits, since
+    the work is split by what the call knows.  Does not wait for the device."""
     op = "prefix_attention"
     shape = q.shape
     if len(shape) == 4:
@@ -266,4 +266,4 @@ def beam_reorder(beams: torch.Tensor, k_caches: Sequence[torch.Tensor],
                  shape[-2], ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3], _stream(dev))
     if not alike:
         for c, g in zip(given, caches):
-            _write_back(c, g)
+            _give_back(c, g)

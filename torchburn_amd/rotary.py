@@ -103,10 +103,17 @@ def _heads(op: str, name: str, t: torch.Tensor, lead, hd: int, dev):
 
 def _flat(t: torch.Tensor, last: int) -> torch.Tensor:
     """t with one dimension before its last ones: a view, or a copy where there is none."""
-    try:
-        return t.view(-1, *t.shape[-last:])
-    except RuntimeError:
-        return t.reshape(-1, *t.shape[-last:])
+    return t.flatten(0, -1 - last)
+
+
+def _give_back(c: torch.Tensor, new: torch.Tensor) -> None:
+    """A converted cache's rows to the caller's.  What did not change stays as it was there:
+    a type that f32 does not hold is rounded only in rows that are written."""
+    with torch.no_grad():
+        if c.dtype is not torch.float32 and c.dtype.itemsize > 2:
+            same = new.reshape(c.shape) == c.to(new.device, torch.float32)
+            new = torch.where(same, c.to(new.device), new.reshape(c.shape).to(c.dtype))
+        _write_back(c, new)
 
 
 def _own_caches(op: str, name: str, c: torch.Tensor, lead, heads: int, hd: int, dev):
@@ -172,6 +179,9 @@ def _call(op, q, k, v, positions, inv_freq, q_weight, k_weight, eps, interleaved
         vc, v_rows, vs = _own_caches(op, "v_cache", v_cache, lead, hkv, hd, dev)
         if v_rows != rows:
             raise _bad(op, f"k_cache has {rows} positions, v_cache {v_rows}")
+        if (kc is not k_cache or vc is not v_cache) and k_cache.numel() and \
+                k_cache.data_ptr() == v_cache.data_ptr():
+            raise _bad(op, "k_cache and v_cache share memory")
         if isinstance(at, torch.Tensor):
             if [*at.shape] != lead or at.dtype.is_floating_point:
                 raise _bad(op, f"kv_len must be integers {lead}, got {at.dtype} {list(at.shape)}")
@@ -185,9 +195,9 @@ def _call(op, q, k, v, positions, inv_freq, q_weight, k_weight, eps, interleaved
                  1 if interleaved else 0, float(attention_factor), float(eps), _stream(dev))
     if v is not None:
         if kc.data_ptr() != k_cache.data_ptr():
-            _write_back(k_cache, kc)
+            _give_back(k_cache, kc)
         if vc.data_ptr() != v_cache.data_ptr():
-            _write_back(v_cache, vc)
+            _give_back(v_cache, vc)
     if q.is_cuda:
         return out, k_out
     return out.to(q.device), None if k_out is None else k_out.to(q.device)
@@ -222,8 +232,8 @@ def norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, position
     ``v`` as it is.  Returns the turned queries.
 
     A number outside the caches raises ValueError; a sequence whose kv_len is outside has no
-    row written; no two rows of the caches may share memory.  Caches in f32 on q's device with head_dim contiguous and sequences
-    a constant stride apart are written in place; any others are converted whole at every
-    call.  Does not wait for the device."""
+    row written; no two rows of the caches may share memory.  Caches in f32 on q's device with
+    head_dim contiguous and sequences a constant stride apart are written in place; any others
+    are converted whole at every call.  Does not wait for the device."""
     return _call("norm_rope_append", q, k, v, positions, inv_freq, q_weight, k_weight, eps,
                  interleaved, attention_factor, k_cache, v_cache, kv_len)[0]
