@@ -275,3 +275,33 @@ def test_reorder_stacked(cuda):
         tb.beam_reorder(par, k, k, 4)
     with pytest.raises(tb.UnsupportedOpError, match="twice"):
         tb.beam_reorder(par, k[:1].expand(3, -1, -1, -1, -1, -1), v, 4)
+
+
+def test_far_apart(cuda):
+    """Element offsets past 32 bits: between beams, positions and groups, and in the logits."""
+    par = torch.tensor([[1, 0], [1, 1]], device=cuda)
+    far = torch.empty((1 << 32) + (1 << 20), device=cuda)
+    shape = (2, 2, 1, 3, 32)
+    for strides in ((4096, 1 << 32, 32, 128, 1), (4096, 1024, 32, 1 << 31, 1),
+                    (1 << 32, 1024, 32, 128, 1)):
+        k, v = (far[off:].as_strided(shape, strides) for off in (0, 1 << 16))
+        for c in (k, v):
+            c.copy_(torch.randn(shape, device=cuda))
+        want = [c.clone() for c in (k, v)]
+        for c in want:
+            c[0, :, :, :2] = c[0, [1, 0], :, :2]
+            c[1, :, :, :2] = c[1, [1, 1], :, :2]
+        tb.beam_reorder(par, [k], [v], 2)
+        assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+    del far, k, v
+    vocab, beams, groups = 1 << 20, 64, 65      # 4160 rows
+    logits = torch.empty((groups, beams, vocab), device=cuda)
+    logits[:-1] = 0.0
+    last = torch.randn((1, beams, vocab), device=cuda)
+    logits[-1] = last[0]
+    scores = torch.randn((groups, beams), device=cuda)
+    got = tb.beam_select(logits, scores, k=5)
+    for a, b in zip(got, tb.beam_select(last, scores[-1:], k=5)):
+        assert torch.equal(a[-1:], b)
+    assert torch.equal(got[1][0], torch.arange(5, device=cuda))     # ties: the lowest tokens
+    assert torch.equal(got[2][0], scores[0].argmax().expand(5))

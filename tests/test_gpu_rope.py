@@ -238,3 +238,20 @@ def test_no_heads(cuda):
     pos = torch.arange(6, device=cuda).view(2, 3)
     a, b = tb.norm_rope(q, k, pos, f)
     assert torch.equal(a, tb.norm_rope(q, q, pos, f)[0]) and b.shape == k.shape
+
+
+def test_positions_far_apart(cuda):
+    """Element offsets past 32 bits, between a cache's positions and between its sequences."""
+    f, _ = tb.rope_frequencies(32, device=cuda)
+    q, k, v = (torch.randn((2, 3, 32), device=cuda) for _ in range(3))
+    pos = torch.tensor([4, 5], device=cuda)
+    want = tb.norm_rope(q, k, pos, f)[1]
+    far = torch.empty((1 << 32) + (1 << 20), device=cuda)
+    for strides in ((4096, 32, 1 << 31, 1), (1 << 32, 32, 4096, 1)):
+        kc, vc = (far[off:].as_strided((2, 3, 3 if strides[0] == 4096 else 2, 32), strides)
+                  for off in (0, 1 << 16))
+        at = kc.shape[2] - 1
+        kc.zero_(), vc.zero_()
+        tb.norm_rope_append(q, k, v, pos, f, kc, vc, at)
+        assert torch.equal(kc[:, :, at], want) and torch.equal(vc[:, :, at], v)
+        assert not kc[:, :, :at].any() and not vc[:, :, :at].any()
