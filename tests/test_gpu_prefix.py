@@ -436,3 +436,27 @@ def test_a_beam_search(cuda):
                 assert (items[j][1], items[j][2]) == (got[1][s, j], got[2][s, j]), (s, step, j)
             beams = [(float(got[0][s, j]), t, beams[b][2] or t == eos, rows[b])
                      for j, (_, t, b) in enumerate(items[:B])]
+
+
+@pytest.mark.parametrize("rows", [2, 20, 48, 100])
+@pytest.mark.parametrize("P", [100, 700])
+def test_nan_beside_far_larger_scores(cuda, rows, P):
+    """A NaN that a row sees is in its result, however small the weights around it are: another
+    wave's or split's scores are so much larger (200 and more) that all of its are 0 in f32."""
+    H, KVH, D, L = 2, 2, 32, 9
+    q, kp, vp, k, v = inputs(5, 1, rows, H, KVH, D, P, L)
+    q = np.abs(q) + 0.5
+    kp[0, :, 5] = 100
+    kp[0, 0, 40, 3] = np.nan        # head 0: every row's score of position 40
+    vp[0, 1, 40, 7] = np.nan        # head 1: a weight of 0 in f32 meets NaN and infinity
+    vp[0, 1, P - 30, 9] = np.inf
+    v[0, 0, 1, 3, 11] = np.nan      # row 0's own cache
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    got = tb.prefix_attention(T(q), T(kp), T(vp), P, T(k), T(v), L).cpu().numpy()[0]
+    assert np.isnan(got[:, 0]).all()
+    assert np.isnan(got[:, 1, 7]).all() and not np.isfinite(got[:, 1, 9]).any()
+    assert np.isnan(got[0, 1, 11]) and np.isfinite(got[1:, 1, 11]).all()
+    # the one position that counts, whose weight is 1 to f32's last bit
+    rest = np.delete(got[:, 1], [7, 9, 11], 1)
+    want = np.delete(vp[0, 1, 5], [7, 9, 11])
+    assert (np.abs(rest - want) <= 32 * U * np.abs(want)).all()

@@ -362,12 +362,13 @@ __device__ __forceinline__ void stream_block(const PrefixAttn &a, const Plan &pl
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             const float m = lds.m[w][t];
-            e[w] = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-            if (e[w] != 0.f) sum = fmaf(lds.l[w][t], e[w], sum);
+            e[w] = m == -INFINITY ? -1.f : __builtin_amdgcn_exp2f(m - top);
+            if (m != -INFINITY) sum = fmaf(lds.l[w][t], e[w], sum);
         }
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        // A share of 0 counts too: NaN times 0 is NaN.  -1: the wave saw nothing of the row.
 #pragma unroll
-        for (int w = 0; w < NW; ++w) lds.share[w][t] = e[w] * inv;
+        for (int w = 0; w < NW; ++w) lds.share[w][t] = e[w] == -1.f ? -1.f : e[w] * inv;
         lds.top[t] = top;
         lds.sum[t] = sum;
     }
@@ -381,7 +382,7 @@ __device__ __forceinline__ void stream_block(const PrefixAttn &a, const Plan &pl
         for (int w = 0; w < NW; ++w) {
             const float4 z = *reinterpret_cast<const float4 *>(&lds.o[w][r][4 * d]);
             const float k = lds.share[w][r];
-            if (k != 0.f) {   // a wave that saw nothing of the row counts for nothing
+            if (!(k < 0.f)) {
                 y.x = fmaf(z.x, k, y.x);
                 y.y = fmaf(z.y, k, y.y);
                 y.z = fmaf(z.z, k, y.z);
@@ -730,7 +731,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : W == 32 ? 2 : 3) void k_prefix_d
 // A row's partial results, normalised, in the shares of their sums, in the order of the slots, by
 // WR waves: groups of LC lanes of four dimensions each take every 64 WR / LC-th slot, the
 // first of them requested before the shares are known (every slot's place in the scratch
-// can be read, and what was not written has a share of 0).  Bound by the launch and the way
+// can be read, and what was not written is left out).  Bound by the launch and the way
 // of those reads: 4.0 us for 256 rows of 33 slots, 9.5 for 2048 (34.6 MB).
 template <int LC, int WR>
 __global__ __launch_bounds__(256) void k_prefix_merge(PrefixAttn a, Plan plan,
@@ -751,6 +752,7 @@ __global__ __launch_bounds__(256) void k_prefix_merge(PrefixAttn a, Plan plan,
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) z[k] = src[min(grp + NG * k, plan.slots - 1) * step];
     float m[2], l[2], top = -INFINITY, sum = 0.f;
+    bool seen[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const float *p = pml + 2 * (at + (size_t)min(lane + 64 * x, plan.slots - 1) * R);
@@ -772,21 +774,22 @@ __global__ __launch_bounds__(256) void k_prefix_merge(PrefixAttn a, Plan plan,
     for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-        m[x] = m[x] == -INFINITY ? 0.f : l[x] * __builtin_amdgcn_exp2f(m[x] - top);
+        seen[x] = m[x] != -INFINITY;
+        m[x] = seen[x] ? l[x] * __builtin_amdgcn_exp2f(m[x] - top) : 0.f;
         sum += m[x];
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) w[wave][lane + 64 * x] = m[x] * inv;
+    for (int x = 0; x < 2; ++x) w[wave][lane + 64 * x] = seen[x] ? m[x] * inv : -1.f;
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](int s, const float4 &v) {
         const float x = w[wave][s];
-        if (x != 0.f) {   // a split that sees nothing of the row counts for nothing
+        if (!(x < 0.f)) {   // a split that sees nothing of the row counts for nothing
             y.x = fmaf(v.x, x, y.x);
             y.y = fmaf(v.y, x, y.y);
             y.z = fmaf(v.z, x, y.z);
