@@ -255,3 +255,23 @@ def test_positions_far_apart(cuda):
         tb.norm_rope_append(q, k, v, pos, f, kc, vc, at)
         assert torch.equal(kc[:, :, at], want) and torch.equal(vc[:, :, at], v)
         assert not kc[:, :, :at].any() and not vc[:, :, :at].any()
+
+
+@pytest.mark.parametrize("d", [64, 34])
+def test_norms_at_the_ends_of_f32(cuda, d):
+    """Heads whose scale is past f32's largest number or below its smallest normal one: the
+    largest finite numbers, subnormal ones, and a single element that is not 0, without eps."""
+    g = np.random.default_rng(d)
+    f, _ = tb.rope_frequencies(16, device=cuda)
+    x = g.uniform(0.5, 1.0, (1, 6, d)) * g.choice((-1, 1), (1, 6, d))
+    x *= np.array([3.4e38, 1.2e38, 1e-38, 1e-40, 1e-43, 1.0])[:, None]
+    x = x.astype(np.float32)
+    x[0, 5] = 0
+    x[0, 5, 3] = 2.0 ** -149
+    w = g.standard_normal(d).astype(np.float32)
+    T = lambda a: torch.from_numpy(a).to(cuda)
+    for inter in (False, True):
+        a, b = tb.norm_rope(T(x), T(x[:, 1:]), torch.tensor([77], device=cuda), f, T(w), T(w),
+                            eps=0.0, interleaved=inter)
+        assert torch.equal(b, a[:, 1:])
+        check(a, *reference(x, w, np.array([77]), f.cpu().numpy(), 0.0, inter, 1.0))

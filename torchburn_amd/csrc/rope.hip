@@ -148,7 +148,8 @@ __global__ __launch_bounds__(256) void k_norm_rope(RopeParams p, int per, int pa
             const int h = h0 + d + i;
             const bool is_q = h < p.hq, is_v = h >= p.hq + p.hkv;
             const bool norm = is_q ? p.qw != nullptr : p.kw != nullptr && !is_v;
-            float scale = 1.f;
+            float scale = 1.f;   // times 2^up: of a head at f32's ends it is no f32 itself
+            int up = 0;
             if (p.qw || p.kw) {   // squares and their sum in 64 bits: none is out of range
                 double sum = 0.0;
 #pragma unroll
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(256) void k_norm_rope(RopeParams p, int per, int pa
                         sum = fma((double)x[i][n].a[j], (double)x[i][n].a[j], sum);
                         sum = fma((double)x[i][n].b[j], (double)x[i][n].b[j], sum);
                     }
-                if (norm) scale = (float)(1.0 / sqrt(head_sum<L>(sum) / D + p.eps));
+                if (norm) scale = (float)frexp(1.0 / sqrt(head_sum<L>(sum) / D + p.eps), &up);
             }
             if (d + i >= per || h >= h1) continue;
 #pragma unroll
@@ -168,8 +169,8 @@ __global__ __launch_bounds__(256) void k_norm_rope(RopeParams p, int per, int pa
                     const Piece<W> &w = is_q ? qw[n] : kw[n];
 #pragma unroll
                     for (int j = 0; j < W; ++j) {
-                        y.a[j] = y.a[j] * scale * w.a[j];
-                        y.b[j] = y.b[j] * scale * w.b[j];
+                        y.a[j] = ldexpf(y.a[j], up) * scale * w.a[j];
+                        y.b[j] = ldexpf(y.b[j], up) * scale * w.b[j];
                     }
                 }
                 if (!is_v && lane + n * L < turning) {
