@@ -1,6 +1,8 @@
 """beam_select and beam_reorder against their definitions: tokens, beams and moved rows have to
 be equal; a score is rounded once (2^-24 of it) and its sum of exponentials kept in 64
 bits (1e-9 allows for every rounding there)."""
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 import torch
@@ -305,3 +307,28 @@ def test_far_apart(cuda):
         assert torch.equal(a[-1:], b)
     assert torch.equal(got[1][0], torch.arange(5, device=cuda))     # ties: the lowest tokens
     assert torch.equal(got[2][0], scores[0].argmax().expand(5))
+
+
+@pytest.mark.parametrize("case", [(1, 47, 2000, 64), (1, 48, 2000, 64), (1, 49, 2000, 64), (2, 63, 9001, 64),
+                                  (1, 64, 1000, 64)], ids=lambda c: "-".join(map(str, c)))
+def test_select_at_the_border_of_lds(cuda, case):
+    """Selections whose second kernel takes about the 64 KiB that a launch has by itself."""
+    test_select(cuda, case, "plain")
+    test_select(cuda, case, "ties")
+
+
+def test_wide_selections_side_by_side(cuda):
+    """Threads whose selections need LDS of different sizes past what a launch has by itself."""
+    shapes = [(64, 1000), (64, 3001), (64, 70001), (60, 200001)]
+    inputs = [(torch.randn(s, device=cuda), torch.randn(s[0], device=cuda)) for s in shapes]
+    want = [tb.beam_select(x, s, k=64) for x, s in inputs]
+    torch.cuda.synchronize()
+
+    def many(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [tb.beam_select(*inputs[i], k=64) for _ in range(25)]
+            torch.cuda.current_stream().synchronize()
+        return got
+    with ThreadPoolExecutor(len(shapes)) as pool:
+        for got, w in zip(pool.map(many, range(len(shapes))), want):
+            assert all(torch.equal(a, b) for g in got for a, b in zip(g, w))

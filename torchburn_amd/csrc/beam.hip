@@ -261,6 +261,14 @@ __global__ __launch_bounds__(kThreads, 7) void k_beam_chunk(BeamSelect p, Part *
 }
 
 constexpr int kAhead = 8;   // a lane's items of a row that are requested at once
+constexpr int kPickWaves = 16;
+// LDS of k_beam_pick: what every block has, and what the launch adds.  A launch may have 64 KiB in
+// all by itself; for more the kernel's limit is set to the most that any call takes, with 64
+// beams, 64 results and 128 chunks: it is one for all threads of the process, so that a limit of
+// the call's own size could be another's between its set and its launch.
+constexpr size_t kPickStatic = (kPickWaves + kMaxBeams) * sizeof(int);
+constexpr size_t kPickPlain = (64 << 10) - kPickStatic;
+constexpr size_t kPickMost = 128 << 10;
 
 // A row's k largest of a group, ready to be ranked among the other rows'.
 struct Pick {
@@ -273,11 +281,11 @@ struct Pick {
 // Then each of them is ranked among the group's, by a search in every row's list.
 // Bound by the launch and the waits of these steps: 9.1 us for 32 groups of 8 beams, 16 chunks
 // and k = 16, 6.0 for one of 4 beams, 32 chunks and k = 8.
-__global__ __launch_bounds__(1024) void k_beam_pick(BeamSelect p, const Part *__restrict__ parts,
-                                                    const uint64_t *__restrict__ best, int chunks,
-                                                    int cap) {
+__global__ __launch_bounds__(64 * kPickWaves) void k_beam_pick(
+    BeamSelect p, const Part *__restrict__ parts, const uint64_t *__restrict__ best, int chunks,
+    int cap) {
     extern __shared__ uint64_t lds[];   // picks [beams][k], then items [waves][cap]
-    __shared__ int counts[16], lengths[kMaxBeams];
+    __shared__ int counts[kPickWaves], lengths[kMaxBeams];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
     const int k = p.k, group = blockIdx.x;
     Pick *pick = reinterpret_cast<Pick *>(lds);
@@ -480,12 +488,12 @@ int launch_beam_select(const BeamSelect &p, void *scratch, hipStream_t s) {
     // A lane's items are each its largest at most: so many pass the border.
     const int cap = p.k * ((chunks * p.k + 63) / 64);
     const size_t picks = (size_t)p.beams * p.k * sizeof(Pick);
-    int waves = std::min(16, p.beams);
-    while (waves > 1 && picks + (size_t)waves * cap * sizeof(uint64_t) > (64 << 10)) --waves;
+    int waves = std::min(kPickWaves, p.beams);
+    while (waves > 1 && picks + (size_t)waves * cap * sizeof(uint64_t) > kPickPlain) --waves;
     const size_t need = picks + (size_t)waves * cap * sizeof(uint64_t);
-    if (need > (64 << 10))
+    if (need > kPickPlain)
         TB_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(k_beam_pick),
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)need));
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)kPickMost));
     hipLaunchKernelGGL(k_beam_pick, dim3(p.groups), dim3(64 * waves), need, s, p, parts, best,
                        chunks, cap);
     TB_LAUNCHED();
