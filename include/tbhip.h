@@ -511,7 +511,8 @@ TB_API int tb_process_logits(const float *logits, float *out, int64_t *tokens, i
  * positions) at position kv_lens[token] (device i32 [n]; where it is outside of
  * [0, max_seq) nothing is written), or kv_len for all of them with kv_lens NULL
  * (TB_ERR_VALUE outside).  No two cache rows may share memory.  head_dim and
- * rotary_dim even, head_dim up to 512.
+ * rotary_dim even, head_dim up to 512; up to 2^28 heads in all, and what one launch's
+ * 2^32 - 1 threads do: 4 to 64 for each group of up to four heads of a token.
  */
 TB_API int tb_norm_rope(const float *q, const float *k, const float *v, const int64_t *positions,
                         const double *inv_freq, const float *q_weight, const float *k_weight,
@@ -535,7 +536,8 @@ TB_API int tb_norm_rope(const float *q, const float *k, const float *v, const in
  * to [0, max_prefix], or NULL: prefix_len for every group; kv_lens device i32
  * [groups * rows], clamped to [0, max_seq], or NULL: kv_len for every row
  * (TB_ERR_VALUE past the caches).  max_seq 0: no own caches.  head_dim a multiple
- * of 32 up to 256, num_heads up to 1024; q, out and the caches 16-byte aligned.
+ * of 32 up to 256, num_heads up to 1024, 2^23 query heads in all (half as many where
+ * each is a KV head's only one); q, out and the caches 16-byte aligned.
  * scratch: tb_prefix_attention_scratch bytes of device memory, 16-byte aligned
  * (prefix: prefix_len, or max_prefix with prefix_lens; own: kv_len, or max_seq with
  * kv_lens); NULL: the stream's workspace (TB_ERR_UNSUPPORTED while capturing, since

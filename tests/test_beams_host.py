@@ -251,3 +251,27 @@ def test_frequencies():
     assert math.isclose(c, 0.1 * math.log(8.0) + 1)
     assert tb.rope_frequencies(0, device="cpu")[0].shape == (0,)
     assert tb.rope_frequencies(2, scaling="ntk", factor=4.0, device="cpu")[0].tolist() == [1.0]
+
+
+@pytest.mark.parametrize("call,kw", [
+    # a head's 64 lanes for each of 2^26 tokens; two groups of heads a token
+    (rope, dict(n=1 << 26, heads=1, kv_heads=0, hd=34, rotary=34)),
+    (rope, dict(n=1 << 25, heads=5, kv_heads=0, hd=34, rotary=34)),
+    (append, dict(n=1 << 26, heads=0, kv_heads=1, hd=512, rotary=512, kc_sb=1 << 13, vc_sb=1 << 13,
+                  kc_sh=1 << 13, vc_sh=1 << 13, kc_ss=512, vc_ss=512)),
+    # 512 threads for each of 2^23 heads on a short prefix; 256 twice on a long one
+    (attention, dict(rows=8192, heads=1024, kv_heads=1024)),
+    (attention, dict(groups=8192, rows=1, heads=1024, kv_heads=1024, max_prefix=9000, prefix=9000)),
+    (attention, dict(groups=8192, rows=1, heads=1024, kv_heads=1024, max_prefix=9000, pl=A, prefix=0)),
+])
+def test_launches_past_the_threads_of_one(call, kw):
+    """Sizes within the other limits whose launch would have 2^32 threads."""
+    assert call(**kw) == U, kw
+    assert b"2^32" in _lib.lib().tb_last_error()
+
+
+def test_scratch_at_the_threads_of_a_launch():
+    L = _lib.lib()
+    assert L.tb_prefix_attention_scratch(8192, 1, 1024, 1024, 64, 9000, 9) == 0
+    assert L.tb_prefix_attention_scratch(8190, 1, 1024, 1024, 64, 9000, 9) > 0
+    assert L.tb_prefix_attention_scratch(8192, 1, 1024, 128, 64, 9000, 9) > 0

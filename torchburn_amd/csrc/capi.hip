@@ -1517,7 +1517,9 @@ int64_t tb_prefix_attention_scratch(int64_t groups, int64_t rows, int64_t num_he
                                     int64_t num_kv_heads, int64_t head_dim, int64_t prefix,
                                     int64_t own) {
     if (check_prefix(groups, rows, num_heads, num_kv_heads, head_dim, prefix, own) ||
-        groups * rows == 0)
+        groups * rows == 0 ||
+        !prefix_attention_fits((int)groups, (int)rows, (int)num_heads, (int)num_kv_heads,
+                               (int)head_dim, (int)prefix, (int)own))
         return 0;
     return (int64_t)prefix_attention_scratch((int)groups, (int)rows, (int)num_heads,
                                              (int)num_kv_heads, (int)head_dim, (int)prefix, (int)own);
@@ -1566,9 +1568,13 @@ int tb_prefix_attention(const float *q, const float *k_prefix, const float *v_pr
     a.max_prefix = (int)max_prefix; a.max_own = (int)max_seq;
     a.groups = (int)groups; a.rows = (int)rows;
     a.hq = (int)num_heads; a.hkv = (int)num_kv_heads; a.hd = (int)head_dim; a.scale = scale;
-    const size_t need = prefix_attention_scratch(
-        a.groups, a.rows, a.hq, a.hkv, a.hd, prefix_lens ? a.max_prefix : a.prefix_len,
-        kv_lens ? a.max_own : a.own_len);
+    const int prefix = prefix_lens ? a.max_prefix : a.prefix_len;
+    const int own = kv_lens ? a.max_own : a.own_len;
+    TB_REQUIRE(prefix_attention_fits(a.groups, a.rows, a.hq, a.hkv, a.hd, prefix, own),
+               TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: prefix_attention: more threads than one launch has, 2^32 - 1");
+    const size_t need =
+        prefix_attention_scratch(a.groups, a.rows, a.hq, a.hkv, a.hd, prefix, own);
     hipStream_t st = (hipStream_t)stream;
     WsLease lease;
     if (need && !scratch) {

@@ -29,6 +29,8 @@ struct PrefixAttn {
     float scale;
 };
 
+// Whether one launch can have the threads of a call with lengths up to prefix and own.
+bool prefix_attention_fits(int groups, int rows, int hq, int hkv, int hd, int prefix, int own);
 // Scratch for lengths up to prefix and own; 0 where a single block sees a row's all.
 size_t prefix_attention_scratch(int groups, int rows, int hq, int hkv, int hd, int prefix, int own);
 int launch_prefix_attention(const PrefixAttn &a, float *scratch, hipStream_t s);

@@ -876,6 +876,11 @@ void merge(const PrefixAttn &a, const Plan &p, const float *part, const float *p
 
 }  // namespace
 
+bool prefix_attention_fits(int groups, int rows, int hq, int hkv, int hd, int prefix, int own) {
+    const Plan p = plan_of(groups, rows, hq, hkv, hd, prefix, own);
+    return ((int64_t)p.pblocks + p.oblocks) * 64 * p.nw <= kMaxThreads;
+}
+
 size_t prefix_attention_scratch(int groups, int rows, int hq, int hkv, int hd, int prefix, int own) {
     const int slots = plan_of(groups, rows, hq, hkv, hd, prefix, own).slots;
     return slots > 1 ? (size_t)groups * rows * hq * slots * (hd + 2) * sizeof(float) : 0;

@@ -211,7 +211,7 @@ __global__ __launch_bounds__(256) void k_norm_rope(RopeParams p, int per, int pa
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 template <int L, int NU, int W>
-void launch(const RopeParams &p, hipStream_t s) {
+int launch(const RopeParams &p, hipStream_t s) {
     const int heads = p.hq + (p.append ? 2 : 1) * p.hkv;
     // Heads a group: up to four share the angles, but groups for every CU first.
     const int64_t groups = (int64_t)p.n * heads;
@@ -219,12 +219,16 @@ void launch(const RopeParams &p, hipStream_t s) {
     while (per < 4 && groups / (2 * per) * L >= 256 * 512) per *= 2;
     const int parts = (heads + per - 1) / per;
     const int64_t blocks = ((int64_t)p.n * parts + 256 / L - 1) / (256 / L);
+    TB_REQUIRE(blocks * 256 <= kMaxThreads, TB_ERR_UNSUPPORTED,
+               "TB_UNSUPPORTED: norm_rope: more threads than one launch has, 2^32 - 1");
     if (p.interleaved)
         hipLaunchKernelGGL((k_norm_rope<L, NU, W, true>), dim3((uint32_t)blocks), dim3(256), 0, s, p,
                            per, parts);
     else
         hipLaunchKernelGGL((k_norm_rope<L, NU, W, false>), dim3((uint32_t)blocks), dim3(256), 0, s,
                            p, per, parts);
+    TB_LAUNCHED();
+    return TB_OK;
 }
 
 }  // namespace
@@ -239,19 +243,15 @@ int launch_norm_rope(const RopeParams &p, hipStream_t s) {
                       rows4(p.vc.p, p.vc.sb, p.vc.sh, p.vc.ss) && aligned16(p.qw) &&
                       aligned16(p.kw) && aligned16(p.q_out) && aligned16(p.k_out);
     const int units = wide ? p.hd / 8 : p.hd / 2;
-    if (wide) {
-        if (units <= 4) launch<4, 1, 4>(p, s);
-        else if (units <= 8) launch<8, 1, 4>(p, s);
-        else if (units <= 16) launch<16, 1, 4>(p, s);
-        else if (units <= 32) launch<32, 1, 4>(p, s);
-        else launch<64, 1, 4>(p, s);
-    } else {
-        if (units <= 16) launch<16, 1, 1>(p, s);
-        else if (units <= 64) launch<64, 1, 1>(p, s);
-        else launch<64, 4, 1>(p, s);
-    }
-    TB_LAUNCHED();
-    return TB_OK;
+    if (wide)
+        return units <= 4    ? launch<4, 1, 4>(p, s)
+               : units <= 8  ? launch<8, 1, 4>(p, s)
+               : units <= 16 ? launch<16, 1, 4>(p, s)
+               : units <= 32 ? launch<32, 1, 4>(p, s)
+                             : launch<64, 1, 4>(p, s);
+    return units <= 16   ? launch<16, 1, 1>(p, s)
+           : units <= 64 ? launch<64, 1, 1>(p, s)
+                         : launch<64, 4, 1>(p, s);
 }
 
 }  // namespace tb

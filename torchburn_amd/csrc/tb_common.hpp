@@ -14,6 +14,9 @@ namespace tb {
 // Records the message of the last failing call on this thread and returns code.
 int fail(int code, const std::string &msg);
 
+// Threads that one dimension of a launch can have.
+constexpr int64_t kMaxThreads = ((int64_t)1 << 32) - 1;
+
 // A stream's device scratch, held by one op while it enqueues its kernels.
 struct WsLease {
     std::unique_lock<std::mutex> lock;
