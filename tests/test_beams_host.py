@@ -275,3 +275,38 @@ def test_scratch_at_the_threads_of_a_launch():
     assert L.tb_prefix_attention_scratch(8192, 1, 1024, 1024, 64, 9000, 9) == 0
     assert L.tb_prefix_attention_scratch(8190, 1, 1024, 1024, 64, 9000, 9) > 0
     assert L.tb_prefix_attention_scratch(8192, 1, 1024, 128, 64, 9000, 9) > 0
+
+
+Q4, P4, C5 = (2, 3, 4, 64), (2, 2, 9, 64), (2, 3, 2, 5, 64)
+
+
+@pytest.mark.parametrize("call", [
+    # as many numbers as there are sequences, in another order
+    lambda: tb.prefix_attention(f(Q4), f(P4), f(P4), 9, f(C5), f(C5), i(3, 2)),
+    lambda: tb.prefix_attention(f(Q4), f(P4), f(P4), 9, f(C5), f(C5), i(2, 1, 3, 1).transpose(0, 2)),
+    lambda: tb.prefix_attention(f(Q4), f(P4), f(P4), 9, f(C5), f(C5), i(5)),
+    lambda: tb.prefix_attention(f(4, 3, 4, 64), f(4, 2, 9, 64), f(4, 2, 9, 64), i(2, 2)),
+    lambda: tb.beam_reorder(i(2, 3), [f(C5)], [f(C5)], i(3, 2)),
+    lambda: tb.beam_reorder(i(6), [f(6, 2, 5, 64)], [f(6, 2, 5, 64)], i(2, 3)),
+])
+def test_lengths_of_another_shape(host, call):
+    with pytest.raises(tb.UnsupportedOpError, match="must be a number or integers"):
+        call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: tb.prefix_attention(f(Q4), f(P4), f(P4), i(2), f(C5), f(C5), i(2, 3)),
+    lambda: tb.prefix_attention(f(Q4), f(P4), f(P4), i(2, 1), f(C5), f(C5), i(6)),
+    lambda: tb.prefix_attention(f(Q4), f(P4), f(P4), i(1, 2), f(C5), f(C5), i(2, 3, 1)),
+    lambda: tb.prefix_attention(f(3, 4, 64), f(2, 9, 64), f(2, 9, 64), i(), f(3, 2, 5, 64),
+                                f(3, 2, 5, 64), i(3)),
+    lambda: tb.prefix_attention(f(3, 4, 64), f(2, 9, 64), f(2, 9, 64), i(1), f(3, 2, 5, 64),
+                                f(3, 2, 5, 64), i(1, 3)),
+    lambda: tb.beam_reorder(i(2, 3), [f(C5)], [f(C5)], i(6)),
+    lambda: tb.beam_reorder(i(2, 3), [f(C5)], [f(C5)], i(2, 3)),
+    lambda: tb.beam_reorder(i(1, 3), [f(1, 3, 2, 5, 64)], [f(1, 3, 2, 5, 64)], i(3)),
+])
+def test_lengths_in_their_order(host, call):
+    """Shapes that say the same reach the library."""
+    with pytest.raises(AssertionError, match="not refused"):
+        call()

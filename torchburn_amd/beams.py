@@ -15,6 +15,7 @@ beam_reorder): keep them in that form.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from operator import attrgetter
 from typing import Optional, Sequence, Tuple, Union
 
@@ -72,11 +73,14 @@ def _sequences(op: str, name: str, c: torch.Tensor, batched: bool, dev: torch.de
     return c, st[1:]
 
 
-def _lengths(op: str, name: str, t, count: int, dev) -> Tuple[Optional[torch.Tensor], int]:
+def _lengths(op: str, name: str, t, shape, dev) -> Tuple[Optional[torch.Tensor], int]:
     if not isinstance(t, torch.Tensor):
         return None, _lib.int64(t)
-    if t.numel() != count or t.dtype.is_floating_point:
-        raise _bad(op, f"{name} must be a number or {count} integers, got {t.dtype} "
+    # flat or with other dimensions of 1: still in this order
+    if t.dtype.is_floating_point or (t.shape != shape and not (
+            t.numel() == math.prod(shape) and (t.ndim == 1 or [n for n in t.shape if n != 1] ==
+                                    [n for n in shape if n != 1]))):
+        raise _bad(op, f"{name} must be a number or integers {list(shape)}, got {t.dtype} "
                        f"{list(t.shape)}")
     return (t if _ready(t, torch.int32, dev.index) else _int32_on_gpu(t, dev)), 0
 
@@ -133,8 +137,8 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
         if own != want or vc.shape != want:
             raise _bad(op, f"caches {list(k_cache.shape)} / {list(v_cache.shape)} do not fit q "
                            f"{list(shape)} and {kvh} KV heads")
-    pl, p = _lengths(op, "prefix_len", prefix_len, groups, dev)
-    ol, o = _lengths(op, "kv_len", kv_len, groups * rows, dev)
+    pl, p = _lengths(op, "prefix_len", prefix_len, (groups,) if batched else (), dev)
+    ol, o = _lengths(op, "kv_len", kv_len, (groups, rows) if batched else (rows,), dev)
     out = torch.empty_like(x, requires_grad=False)
     # scratch of this call's own, so that graphs captured on one stream share none
     size = _lib.lib().tb_prefix_attention_scratch(groups, rows, heads, kvh, hd,
@@ -217,7 +221,7 @@ def beam_reorder(beams: torch.Tensor, k_caches: Sequence[torch.Tensor],
     b = _on_gpu(beams, torch.int64, dev)
     n = beams.shape[-1]
     groups = beams.shape[0] if batched else 1
-    lens, ln = _lengths(op, "kv_len", kv_len, groups * n, dev)
+    lens, ln = _lengths(op, "kv_len", kv_len, beams.shape, dev)
     layers, ndim = len(k_caches), 5 if batched else 4
     if len(v_caches) != layers:
         raise _bad(op, f"{layers} k_caches against {len(v_caches)} v_caches")
