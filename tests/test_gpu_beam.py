@@ -332,3 +332,48 @@ def test_wide_selections_side_by_side(cuda):
     with ThreadPoolExecutor(len(shapes)) as pool:
         for got, w in zip(pool.map(many, range(len(shapes))), want):
             assert all(torch.equal(a, b) for g in got for a, b in zip(g, w))
+
+
+def test_two_streams_and_graphs(cuda):
+    """Two searches, each eager and captured on a stream of its own, side by side: every result,
+    and both K and V, after every replay."""
+    B, L, S = 4, 2, 9
+    searches = []
+    for i in range(2):
+        stream = torch.cuda.Stream()
+        x, scores = torch.randn((2, B, 30011), device=cuda), torch.randn((2, B), device=cuda)
+        k, v = (torch.randn((L, 2, B, 2, S, 64), device=cuda) for _ in range(2))
+        lens = torch.randint(0, S + 1, (2, B), device=cuda)
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = tb.beam_select(x, scores)
+            tb.beam_reorder(out[2], k, list(v), lens)
+        searches.append((stream, x, scores, k, v, lens, graph, out))
+    for step in range(4):
+        torch.cuda.synchronize()
+        was, eager = [], []
+        for stream, x, scores, k, v, lens, graph, out in searches:
+            with torch.cuda.stream(stream):
+                x.normal_()
+                lens.random_(0, S + 1)
+                was.append((k.clone(), v.clone()))
+        for stream, x, scores, k, v, lens, graph, out in searches:
+            with torch.cuda.stream(stream):
+                if step != 2:
+                    graph.replay()
+                else:      # an eager step between the replays
+                    got = tb.beam_select(x, scores)
+                    tb.beam_reorder(got[2], list(k), list(v), lens)
+                    for a, b in zip(out, got):
+                        a.copy_(b)
+        torch.cuda.synchronize()
+        for (stream, x, scores, k, v, lens, graph, out), before in zip(searches, was):
+            check(out, x.cpu().numpy(), scores.cpu().numpy(), B)
+            par, n = out[2].tolist(), lens.tolist()
+            for now, w in zip((k, v), before):
+                want = w.clone()
+                for g in range(2):
+                    for j, p in enumerate(par[g]):
+                        want[:, g, j, :, :n[g][p]] = w[:, g, p, :, :n[g][p]]
+                assert torch.equal(now, want)

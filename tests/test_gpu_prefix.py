@@ -460,3 +460,101 @@ def test_nan_beside_far_larger_scores(cuda, rows, P):
     rest = np.delete(got[:, 1], [7, 9, 11], 1)
     want = np.delete(vp[0, 1, 5], [7, 9, 11])
     assert (np.abs(rest - want) <= 32 * U * np.abs(want)).all()
+
+
+def split_scratch(S, rows, H, KVH, D, P, L):
+    """The scratch of a call whose prefix is split: past the one launch of short caches."""
+    size = _lib.lib().tb_prefix_attention_scratch(S, rows, H, KVH, D, P, L)
+    assert size > 0
+    return size
+
+
+@pytest.mark.parametrize("d", [64, 160])
+@pytest.mark.parametrize("rows", [4, 12, 30, 70])
+def test_layouts_of_split_prefixes(cuda, rows, d):
+    """The layouts of test_layouts where the prefix is split over blocks, two query heads a KV
+    head: 8, 24, 60 and 140 rows of it are a tile, two tiles and blocks of 64 and 128 rows; own
+    caches of up to three splits (with 4 rows)."""
+    print(f"case prefix_attention layouts rows={rows} d={d}", flush=True)
+    S, H, KVH, P, L = 2, 8, 4, 700, 150
+    split_scratch(S, rows, H, KVH, d, P, L)
+    arrays = inputs(rows + d, 1, S * rows, H, KVH, d, P, L)
+    q, k, v = (a.reshape(S, rows, *a.shape[2:]) for a in (arrays[0], *arrays[3:]))
+    olen = np.arange(S * rows).reshape(S, rows) * 37 % (L + 1)
+    plen = [690, 333]
+    both = [np.broadcast_to(a, (S, *a.shape[1:])) for a in arrays[1:3]]
+    expected, bound = reference(q, *both, plen, k, v, olen.tolist(), d ** -0.5)
+    q, k, v, kp, vp = (torch.from_numpy(a).to(cuda) for a in (q, k, v, *arrays[1:3]))
+    pl, ol = torch.tensor(plen, device=cuda), torch.from_numpy(olen).to(cuda)
+    both = [c.expand(S, -1, -1, -1) for c in (kp, vp)]      # one prompt under both groups
+    want = tb.prefix_attention(q, *(c.contiguous() for c in both), pl, k, v, ol)
+    check(want, expected, bound)
+    assert torch.equal(tb.prefix_attention(q, *both, pl, k, v, ol), want)
+    # positions before heads, wider rows, spare positions, with NaN in the gaps
+    wide = [torch.full((S, P + 3, KVH, d + 4), float("nan"), device=cuda) for _ in range(2)]
+    views = []
+    for w, c in zip(wide, both):
+        w[:, :P, :, :d] = c.transpose(1, 2)
+        views.append(w[:, :P, :, :d].transpose(1, 2))
+    own = [torch.full((S, rows, L + 1, KVH, d + 8), float("nan"), device=cuda) for _ in range(2)]
+    mine = []
+    for w, c in zip(own, (k, v)):
+        w[..., :L, :, :d] = c.transpose(2, 3)
+        mine.append(w[..., :L, :, :d].transpose(2, 3))
+    assert torch.equal(tb.prefix_attention(q, *views, pl, *mine, ol), want)
+    # K laid out one way, V another; own caches whose groups are not a constant stride apart
+    apart = [torch.stack((c[0], c[0], c[1])) for c in (k, v)]
+    assert torch.equal(tb.prefix_attention(q, views[0], both[1], pl, *(c[::2] for c in apart), ol),
+                       want)
+    # one own cache under every sequence of a group
+    alone = [c[:, :1].contiguous() for c in (k, v)]
+    shared = [c.expand(-1, rows, -1, -1, -1) for c in alone]
+    assert torch.equal(tb.prefix_attention(q, *both, pl, *shared, ol),
+                       tb.prefix_attention(q, *both, pl, *(c.contiguous() for c in shared), ol))
+    off = torch.empty(q.numel() + 1, device=cuda)[1:].view(q.shape).copy_(q)
+    assert torch.equal(tb.prefix_attention(off, *both, pl, k, v, ol), want)
+    # lengths outside of the caches
+    low = tb.prefix_attention(q, *both, torch.tensor([-5, 1 << 40], device=cuda), k, v, ol - 20)
+    assert torch.equal(low, tb.prefix_attention(q, *both, torch.tensor([0, P], device=cuda), k, v,
+                                                (ol - 20).clamp(min=0)))
+    high = tb.prefix_attention(q, *both, pl, k, v, ol + (1 << 33))
+    assert torch.equal(high, tb.prefix_attention(q, *both, pl, k, v, torch.full_like(ol, L)))
+
+
+@pytest.mark.parametrize("rows", [2, 12, 24, 50])
+@pytest.mark.parametrize("far", ["positions", "heads", "groups"])
+def test_split_prefixes_far_apart(cuda, rows, far):
+    """Element offsets past 32 bits on the routes that split the prefix: 4, 24, 48 and 100 rows
+    of a KV head, and the own caches beside them."""
+    print(f"case prefix_attention far apart rows={rows} {far}", flush=True)
+    S, H, KVH, D, P, L = 2, 4, 2, 32, 345, 70
+    split_scratch(S, rows, H, KVH, D, P, L)
+    arrays = inputs(rows, S, rows, H, KVH, D, P, L)
+    olen = (np.arange(S * rows).reshape(S, rows) * 29 % (L + 1)).tolist()
+    plen = [P, 340]
+    want, bound = reference(*arrays[:3], plen, *arrays[3:], olen, D ** -0.5)
+    q, kp, vp, k, v = (torch.from_numpy(a).to(cuda) for a in arrays)
+    # strides of group, KV head and position of the prefix, of sequence, KV head and position of
+    # the own caches; where V lies behind K; where the own caches begin; elements in all
+    big, small = 1 << 32, 1 << 15
+    if far == "positions":      # the prefix's at 2^24, the own ones' at 2^26
+        st, own = (1 << 10, 1 << 11, 1 << 24), (1 << 13, 1 << 12, 1 << 26)
+        behind, v_prefix, v_own, room = 1 << 20, 1 << 9, 1 << 11, (P + 1) << 24
+    elif far == "heads":
+        st, own = (small, big, 32), (small, big, 32)
+        behind, v_prefix, v_own, room = 4 * small, 2 * small, 1 << 22, big + (1 << 23)
+    else:                       # the last of 100 sequences at 99 * 2^26
+        st, own = (big, small, 32), (1 << 26, small, 32)
+        behind, v_prefix, v_own = 4 * small, 2 * small, 1 << 22
+        room = max(big, S * rows << 26) + (1 << 23)
+    room = torch.empty(room, device=cuda)      # 17 to 27 GB
+    views = [room[x:].as_strided((S, KVH, P, D), (*st, 1)) for x in (0, v_prefix)]
+    mine = [room[behind + x:].as_strided((S, rows, KVH, L, D), (rows * own[0], *own, 1))
+            for x in (0, v_own)]
+    for w, a in zip((*views, *mine), (kp, vp, k, v)):
+        w.copy_(a)
+    for w, a in zip((*views, *mine), (kp, vp, k, v)):
+        assert torch.equal(w, a)      # no two of them share memory
+    got = tb.prefix_attention(q, *views, torch.tensor(plen, device=cuda), *mine,
+                              torch.tensor(olen, device=cuda))
+    check(got, want, bound)
