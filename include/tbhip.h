@@ -560,8 +560,10 @@ TB_API int tb_prefix_attention(const float *q, const float *k_prefix, const floa
 /*
  * The k best continuations of each group of beams, best first.  Token t after beam
  * b has the value scores[b] + x[b][t] - log sum_u exp x[b][u], x = logits f32
- * [groups, beams, vocab], scores f32 [groups, beams]; worked out in 64 bits.  Of
- * equal values the lowest beam's and then the lowest token is taken.  A beam that
+ * [groups, beams, vocab], scores f32 [groups, beams].  Of equal values the lowest
+ * beam's and then the lowest token is taken; the order is exact among a beam's tokens,
+ * that of values in 64 bits among beams of the same logits, and otherwise that of
+ * values good to 1e-10 (of logits up to 10^5); scores are rounded once.  A beam that
  * is finished (u8 [groups, beams], or NULL) has the one continuation eos, at its
  * score.  Logits of -inf are never taken; a beam whose score is infinite or NaN, or
  * that has a logit of NaN or +inf, has no continuation.  out_scores f32, tokens and

@@ -377,3 +377,22 @@ def test_two_streams_and_graphs(cuda):
                     for j, p in enumerate(par[g]):
                         want[:, g, j, :, :n[g][p]] = w[:, g, p, :, :n[g][p]]
                 assert torch.equal(now, want)
+
+
+@pytest.mark.parametrize("V", [1000, 5003, 128256])
+@pytest.mark.parametrize("step", [1, -1])
+def test_order_between_beams(cuda, V, step):
+    """Beams with the same logits at other places and moved by whole numbers: their values differ
+    by their scores alone, 2e-10 from beam to beam, twice what a log-sum may be off: the fit's
+    5.5e-11 and 3.4e-16 of a logit up to 10^3."""
+    g = np.random.default_rng(V)
+    B = 16
+    base = np.round(3 * g.standard_normal(V) * 1024) / 1024      # moved without a rounding
+    base[7] = np.abs(base).max() + 2
+    x = np.stack([g.permutation(base) + b * 60 for b in range(B)]).astype(np.float32)
+    assert (np.sort(x, -1) == np.sort(base) + 60.0 * np.arange(B)[:, None]).all()
+    scores = (2e-10 * step * np.arange(B)).astype(np.float32)
+    got = tb.beam_select(torch.from_numpy(x).to(cuda), torch.from_numpy(scores).to(cuda))
+    order = np.arange(B)[::-step]
+    assert got[2].tolist() == order.tolist()
+    assert got[1].tolist() == x.argmax(-1)[order].tolist()

@@ -162,8 +162,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = N
     Token t after beam b has the value scores[b] + log_softmax(logits[b])[t], for ``logits``
     (.., beams, vocab) and ``scores`` (.., beams); ``k`` defaults to the number of beams (twice
     as many leave enough when some of them end).  Of equal values the lowest beam's and then
-    the lowest token is taken; values are worked out in 64 bits and their order is exact,
-    scores are rounded once.  A beam that is ``finished`` (.., beams) goes on with the token
+    the lowest token is taken; scores are rounded once.  The order is exact among a beam's
+    tokens, and that of values in 64 bits among beams of the same logits; a beam's log-sum is
+    good to 1e-10 (logits up to 10^5), so that tokens of other beams whose values are within
+    2e-10 may change places.  A beam that is ``finished`` (.., beams) goes on with the token
     ``eos`` alone and keeps its score.  Logits of -inf (process_logits() masks) are never
     taken; a beam whose score is infinite or NaN, or that has a logit of NaN or +inf, has no
     continuation (scores of a group's first step: 0 and then -inf).  Where fewer than k are

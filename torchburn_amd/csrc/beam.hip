@@ -3,8 +3,11 @@
 //
 // Candidate (b, t) of a group has the value  score[b] + x[b][t] - log sum_u exp x[b][u];
 // a finished beam has the single one (eos, score[b]).  The k largest are taken, of equal
-// ones the lowest beam's and then the lowest token.  Values are kept in 64 bits, so that
-// only what is equal ties: sums of exponentials, their logarithm and the values.
+// ones the lowest beam's and then the lowest token.  Sums of exponentials, their logarithm and
+// the values are kept in 64 bits; the exponentials are a fit to 5.5e-11, which with the
+// argument's rounding, 3.4e-16 of the logit, is a row's error.  So the order is exact among a
+// row's tokens, that of 64 bits among rows that are alike, whose errors are equal, and good to
+// 2e-10 between others.
 #include <float.h>
 #include <math.h>
 
