@@ -526,8 +526,9 @@ TB_API int tb_norm_rope(const float *q, const float *k, const float *v, const in
 
 /*
  * GQA attention of one token of each sequence: row r of group s sees the first
- * prefix_lens[s] positions of its group's prefix, whose K and V are read once for
- * all of its rows, and the first kv_lens[s * rows + r] of its own cache.  Positions
+ * prefix_lens[s] positions of its group's prefix, whose K and V are read for many of
+ * its rows at once (up to 320 positions in all for few sequences, by each sequence for
+ * itself), and the first kv_lens[s * rows + r] of its own cache.  Positions
  * past those take no part, whatever the caches hold; a row that sees none gives
  * zeros.  q and out f32 [groups, rows, num_heads, head_dim] (query head h reads KV
  * head h / (num_heads / num_kv_heads)); prefixes f32 with strides for group (sb),

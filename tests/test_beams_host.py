@@ -259,8 +259,8 @@ def test_frequencies():
     (rope, dict(n=1 << 25, heads=5, kv_heads=0, hd=34, rotary=34)),
     (append, dict(n=1 << 26, heads=0, kv_heads=1, hd=512, rotary=512, kc_sb=1 << 13, vc_sb=1 << 13,
                   kc_sh=1 << 13, vc_sh=1 << 13, kc_ss=512, vc_ss=512)),
-    # 512 threads for each of 2^23 heads on a short prefix; 256 twice on a long one
-    (attention, dict(rows=8192, heads=1024, kv_heads=1024)),
+    # 256 threads twice for each of 2^23 heads
+    (attention, dict(groups=8192, rows=1, heads=1024, kv_heads=1024)),
     (attention, dict(groups=8192, rows=1, heads=1024, kv_heads=1024, max_prefix=9000, prefix=9000)),
     (attention, dict(groups=8192, rows=1, heads=1024, kv_heads=1024, max_prefix=9000, pl=A, prefix=0)),
 ])

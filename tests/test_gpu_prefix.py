@@ -558,3 +558,18 @@ def test_split_prefixes_far_apart(cuda, rows, far):
     got = tb.prefix_attention(q, *views, torch.tensor(plen, device=cuda), *mine,
                               torch.tensor(olen, device=cuda))
     check(got, want, bound)
+
+
+@pytest.mark.parametrize("rows,P,joined", [(32, 304, True), (38, 304, True), (39, 304, False),
+                                           (128, 80, True), (129, 80, False), (4, 305, False)])
+def test_one_launch_or_two(cuda, rows, P, joined):
+    """Short caches in one launch for few sequences only: at the borders of 20 tiles in all and of
+    blocks times tiles, of which 6144 are 307 blocks of 20 tiles and 1024 of 6."""
+    H, KVH, D, L = 16, 8, 64, 16
+    size = _lib.lib().tb_prefix_attention_scratch(1, rows, H, KVH, D, P, L)
+    assert (size == 0) == joined
+    arrays = inputs(rows + P, 1, rows, H, KVH, D, P, L)
+    olen = np.random.default_rng(rows).integers(0, L + 1, (1, rows)).tolist()
+    want, bound = reference(*arrays[:3], [P], *arrays[3:], olen, D ** -0.5)
+    q, kp, vp, k, v = (torch.from_numpy(a).to(cuda) for a in arrays)
+    check(tb.prefix_attention(q, kp, vp, P, k, v, torch.tensor(olen, device=cuda)), want, bound)

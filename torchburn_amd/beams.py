@@ -2,8 +2,8 @@
 beams of a beam search.
 
 The sequences of a group share the cache of their prompt (the prefix) and have
-a short cache each for what they added.  A step reads the prefix once for all of
-them; a beam search then takes the best continuations of the group and moves the
+a short cache each for what they added.  A step reads a long prefix for many of
+them at once; a beam search then takes the best continuations of the group and moves the
 short caches after them, while the prefix stays.  No reference counterpart: it
 decodes one sequence over one cache (src/llm/decoder.rs:788-832).
 

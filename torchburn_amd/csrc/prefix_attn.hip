@@ -1,6 +1,7 @@
 // Attention of sequences that share a prefix: each query row over its group's
-// prefix, whose K and V are read once for all of the group's rows, and over its
-// own cache, for GQA and f32 caches.
+// prefix and over its own cache, for GQA and f32 caches.  A prefix's K and V are read
+// once for a block's 16 to 128 of the group's rows; where caches are short and
+// sequences few, by each sequence for itself.
 //
 //   o = sum_p w_p v_p / sum_p w_p,  w_p = exp(scale q.k_p - m)
 //
@@ -826,10 +827,20 @@ Plan plan_of(int groups, int rows, int hq, int hkv, int hd, int prefix, int own)
     const int G = hq / hkv, R = rows * G;
     const int pt = (prefix + kTile - 1) / kTile, ot = (own + kTile - 1) / kTile;
     const int64_t seqs = (int64_t)groups * rows;
-    // Short caches: a sequence's block reads the prefix for itself, and nothing is merged.  us so
-    // / in two launches: 17 tiles, 4 sequences in groups of 7 heads of 64 8.3 / 7.1 + 3.7; 20
-    // tiles, 64 in groups of 4 of 128 26 / 20 + 4; 29 tiles, 4 sequences 17.2 / 7.4 + 3.8.
-    p.joined = pt + ot <= 20;
+    p.gtiles = (G + 15) / 16;
+    const int64_t units = (int64_t)groups * hkv, ob = seqs * hkv * p.gtiles;
+    // Short caches and few sequences: a sequence's block reads the prefix for itself, and nothing
+    // is merged.  That reads the prefix once a sequence, so it pays for a block a CU, or more
+    // blocks of few tiles.  us in one launch / in two, 8 KV heads of 128, 4 query heads each:
+    //   sequences        4        16        32        64       128       256
+    //    6 tiles    9 /  9   10 / 15   10 / 19   16 / 20   28 / 24   50 / 33
+    //   20 tiles   15 / 11   15 / 15   16 / 20   27 / 22   48 / 29   91 / 43
+    // Over 1512 shapes of 1, 4 and 8 query heads of 32 to 256 for each of 2 and 8 KV heads, 1 to
+    // 256 sequences and 3 to 20 tiles this is 3% slower than the faster one each time (always
+    // one: 7%, two: 28%), at worst 1.65 times (one sequence, 20 tiles of 256: 21 / 13), where
+    // one launch for all is 3.3.  29 tiles, 4 sequences in groups of 7 heads of 64: 17 / 11.
+    const int tiles = std::max(pt + ot, 1);
+    p.joined = tiles <= 20 && (ob <= 256 || ob * tiles <= 6144);
     // f32 MFMA for up to 32 rows, or limbs for 64 or 128 of them: us of 32 rows of 128 on 32767
     // positions 57 / 62, of 64 rows 104 / 76.
     p.dense = !p.joined && R > 32;
@@ -837,17 +848,15 @@ Plan plan_of(int groups, int rows, int hq, int hkv, int hd, int prefix, int own)
     p.prows = p.dense ? (R <= 64 ? 64 : 128) : 16 * p.rb;
     p.nw = p.joined && hd <= 128 ? 8 : 4;
     p.ptiles = (R + p.prows - 1) / p.prows;
-    p.gtiles = (G + 15) / 16;
     if (p.joined) {
         p.ocap = p.slots = 1;
-        p.oblocks = (int)(seqs * hkv * p.gtiles);
+        p.oblocks = (int)ob;
         return p;
     }
     auto cap = [](int64_t want, int64_t blocks, int tiles) {
         const int64_t most = std::min<int64_t>((tiles + kMinTiles - 1) / kMinTiles, kMaxSplits);
         return (int)std::max<int64_t>(1, std::min<int64_t>(want / blocks, most));
     };
-    const int64_t units = (int64_t)groups * hkv, ob = seqs * hkv * p.gtiles;
     // Blocks wanted, us with them / with half as many or half as many again: 256 for one pass of
     // few rows (32 rows on 4096 positions 17.4, 512: 20.2; 16 rows 12.8, 13.9), but 512 past
     // 128 dimensions (28 rows of 256, 7 groups of up to 13296: 169, 256: 186); 768 dense ones of
