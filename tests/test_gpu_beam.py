@@ -396,3 +396,59 @@ def test_order_between_beams(cuda, V, step):
     order = np.arange(B)[::-step]
     assert got[2].tolist() == order.tolist()
     assert got[1].tolist() == x.argmax(-1)[order].tolist()
+
+
+def test_a_search_with_few_continuations(cuda):
+    """A loop of selection and reordering whose groups have fewer continuations than beams at
+    first and in one group for good, with own caches of different lengths and beams that end:
+    each beam's cache holds its own history, against a search over lists in 64 bits."""
+    g = np.random.default_rng(3)
+    G, B, V, D, S, steps, eos = 2, 7, 5, 32, 12, 6, 4
+    table = (2 * g.standard_normal((G, V, V))).astype(np.float32)      # logits by the last token
+    table[:, :, 3] = -np.inf
+    table[0, :, eos] += 3          # group 0: beams end
+    table[1, :, 1:] = -np.inf      # group 1: token 0 alone
+    start = np.array([2, 5])
+    T = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda)
+    logits_of, group = T(table), torch.arange(G, device=cuda)[:, None]
+    # ---- on the device: a cache's rows are the tokens taken
+    k, v = (torch.full((1, G, B, 1, S, D), -7.0, device=cuda) for _ in range(2))
+    none_to_turn = torch.zeros(0, dtype=torch.float64, device=cuda)
+    tokens = torch.zeros((G, B), dtype=torch.int64, device=cuda)
+    scores = torch.full((G, B), float("-inf"), device=cuda)
+    scores[:, 0] = 0
+    ended = torch.zeros((G, B), dtype=torch.bool, device=cuda)
+    kv_len = T(start).int()[:, None].repeat(1, B)
+    for _ in range(steps):
+        rows = tokens.float()[..., None, None].expand(G, B, 1, D)
+        tb.norm_rope_append(rows, rows, -rows, kv_len.long(), none_to_turn, k[0], v[0], kv_len)
+        scores, tokens, beams = tb.beam_select(logits_of[group, tokens], scores, finished=ended,
+                                               eos=eos)
+        tb.beam_reorder(beams, k, v, kv_len + 1)
+        source, none = beams.clamp(min=0), beams < 0
+        ended = (ended.gather(-1, source) | (tokens == eos)) & ~none
+        kv_len = (kv_len + 1).gather(-1, source)
+        tokens = tokens.clamp(min=0)
+    assert ended[0].any() and (beams[1, 1:] == -1).all() and (beams[0] >= 0).all()
+    # ---- over lists
+    x = table.astype(np.float64)
+    with np.errstate(divide="ignore"):
+        x = x - np.log(np.exp(x).sum(-1, keepdims=True))
+    for i in range(G):
+        held = [(0.0, [0], False)]
+        for _ in range(steps):
+            items = []
+            for s, hist, done in held:
+                items += [(s, hist + [eos], True)] if done else \
+                    [(np.float32(s + x[i, hist[-1], t]), hist + [t], t == eos)
+                     for t in range(V) if x[i, hist[-1], t] > -np.inf]
+            held = sorted(items, key=lambda c: -c[0])[:B]
+        assert len(held) == int((beams[i] >= 0).sum())
+        for j, (s, hist, done) in enumerate(held):
+            assert abs(float(scores[i, j]) - s) < 1e-5 and bool(ended[i, j]) == done
+            assert int(tokens[i, j]) == hist[-1] and int(kv_len[i, j]) == start[i] + steps
+            n = start[i]
+            row = k[0, i, j, 0, :, 0].tolist()
+            assert row[n:n + steps] == hist[:steps] and row[:n] == [-7.0] * n
+            assert row[n + steps:] == [-7.0] * (S - n - steps)
+            assert torch.equal(v[0, i, j, 0, n:n + steps], -k[0, i, j, 0, n:n + steps])
