@@ -9,8 +9,9 @@ decodes one sequence over one cache (src/llm/decoder.rs:788-832).
 
 A batch has ``groups`` as its leading dimension; without it, one group.  Caches are
 used where they are when they are f32 on the device with 16-byte rows, contiguous or
-not.  Any others are converted whole at every call (and written back by
-beam_reorder): keep them in that form.
+not; prefix_attention's sequences have to be a constant stride apart over all groups.
+Any others are converted whole at every call (and written back by beam_reorder):
+keep them in that form.
 """
 from __future__ import annotations
 
@@ -96,11 +97,13 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     (rows, num_kv_heads, max_seq, head_dim), of which row i sees the first ``kv_len``, its new
     token's among them.  All with a leading ``groups`` dimension for several prompts.
     ``prefix_len`` is a number or integers () / (groups,), ``kv_len`` a number or integers
-    (rows,) / (groups, rows); numbers past the caches raise ValueError, tensors are clamped
-    on the device.  Without k_cache and v_cache there is the prefix only.  Positions past the
+    (rows,) / (groups, rows), or flat in that order; numbers past the caches raise ValueError,
+    tensors are clamped on the device.  Without k_cache and v_cache there is the prefix only.  Positions past the
     lengths take no part, whatever the caches hold there; a row that sees none gives zeros.
     ``scale`` defaults to head_dim ** -0.5; head_dim is a multiple of 32 up to 256.  f32, in
-    q's shape.  A number and a tensor of the same length may differ in their last bits, since
+    q's shape; with more than 32 query rows of a KV head factors are kept to 2 ** -27 of
+    themselves and 2 ** -134.  Infinities and NaN that a row sees count as in f32: a weight
+    that is 0 there makes NaN of them.  A number and a tensor of the same length may differ in their last bits, since
     the work is split by what the call knows.  Does not wait for the device."""
     op = "prefix_attention"
     shape = q.shape
@@ -169,8 +172,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: Optional[int] = N
     ``eos`` alone and keeps its score.  Logits of -inf (process_logits() masks) are never
     taken; a beam whose score is infinite or NaN, or that has a logit of NaN or +inf, has no
     continuation (scores of a group's first step: 0 and then -inf).  Where fewer than k are
-    left, tokens and beams are -1 and scores -inf.  Up to 64 beams, k up to 64, a vocabulary
-    up to 2 ** 20.  Does not wait for the device."""
+    left, scores are -inf and tokens and beams -1, no index of anything.  Up to 64 beams, k up
+    to 64, a vocabulary up to 2 ** 20.  Does not wait for the device."""
     op = "beam_select"
     *lead, beams, vocab = logits.shape if logits.ndim in (2, 3) else (0, 0, 0, -1)
     if vocab < 0 or scores.shape != (*lead, beams):

@@ -95,7 +95,9 @@ struct Part {
 // A fit of degree 7 to 2^f on +-1/2, 5.5e-11 of it off at most.
 constexpr double kMagic = 1.5 * (double)(1ull << 52);   // y + kMagic has rint(y) in its low word
 __device__ __forceinline__ double exp2_fit(double f) {
-    constexpr double c[8] = {0.9999999999595618, 0.6931471805568324, 0.24022651213498092, 0.055504109063258665, 0.009618025613318034, 0.0013333478473685416, 0.00015469729214118296, 1.5303700711365693e-05};
+    constexpr double c[8] = {0.9999999999595618,    0.6931471805568324,   0.24022651213498092,
+                             0.055504109063258665,  0.009618025613318034, 0.0013333478473685416,
+                             0.00015469729214118296, 1.5303700711365693e-05};
     double p = c[7];
 #pragma unroll
     for (int i = 6; i >= 0; --i) p = fma(p, f, c[i]);
@@ -111,10 +113,11 @@ __device__ __forceinline__ double exp2_fit(double f) {
 // address (rows of an odd vocabulary are read in vectors that are not aligned), so that rows
 // that are alike have sums that are alike to the last bit.
 //
-// Bound by the logits' bytes, 28 us of 131 MB, and the exponentials, 14 instructions in 64
-// bits each: 256 rows of 128256 take 32.7 us with seven blocks a CU, 37.8 with five (which its
-// registers would have), 59.6 where blocks ask for their next chunk ahead and three fit, 56.8
-// with a Taylor sum of degree 10 and the border by every wave from logits and tokens.
+// Bound by the logits' bytes, 27 us of 131 MB, and the exponentials, 14 instructions in 64
+// bits each: 256 rows of 128256 take 32.7 us with seven blocks a CU, for which U = 8 spills 8
+// registers, 37.8 with the five that they would have without, 59.6 where blocks ask for their
+// next chunk ahead and three fit, 56.8 with a Taylor sum of degree 10 and the border by every
+// wave from logits and tokens.
 template <int U>
 __global__ __launch_bounds__(kThreads, 7) void k_beam_chunk(BeamSelect p, Part *__restrict__ parts,
                                                          uint64_t *__restrict__ best) {
@@ -426,6 +429,8 @@ struct LayerCaches {
 // from itself, or from none, is neither read nor written.
 // Bound by the bytes moved: 32 layers of four groups of eight beams, 93 positions of 8 heads of
 // 128, 631 MB, 151 us and 4.2 TB/s, where a large copy reaches 4.9; 157 with ordinary stores.
+// Two groups of 16 beams, one of 32 and one of 64 (32, 32 and 16 layers of that) move at 4.4, 5.1
+// and 4.9 TB/s, although 34, 146 and 372 scalar registers spill and the last has a wave a SIMD.
 // Grid (units side by side, 2 * layers, groups).
 template <int NB>
 __global__ __launch_bounds__(256) void k_beam_reorder(BeamReorder p, LayerCaches lc) {
@@ -485,7 +490,10 @@ int launch_beam_select(const BeamSelect &p, void *scratch, hipStream_t s) {
     Part *parts = static_cast<Part *>(scratch);
     uint64_t *best = reinterpret_cast<uint64_t *>(parts + (size_t)rows * chunks);
     const size_t lds = (size_t)4 * u * p.k * sizeof(uint64_t);
-    auto *k = u == 1 ? k_beam_chunk<1> : u == 2 ? k_beam_chunk<2> : u == 4 ? k_beam_chunk<4> : k_beam_chunk<8>;
+    auto *k = u == 1   ? k_beam_chunk<1>
+              : u == 2 ? k_beam_chunk<2>
+              : u == 4 ? k_beam_chunk<4>
+                       : k_beam_chunk<8>;
     hipLaunchKernelGGL(k, dim3(chunks, rows), dim3(kThreads), lds, s, p, parts, best);
     TB_LAUNCHED();
     // A lane's items are each its largest at most: so many pass the border.
@@ -515,7 +523,8 @@ int launch_beam_reorder(const BeamReorder &p, float *const *kc, float *const *vc
         const int64_t units = (int64_t)p.hkv * ((most + each - 1) / each);
         // us at 512 / 1024 / 2048 / 4096 blocks in all: 160 / 155 / 151 / 152 (k_beam_reorder)
         const int64_t want = std::max<int64_t>(1, 2048 / ((int64_t)2 * layers * p.groups));
-        const dim3 grid((uint32_t)std::max<int64_t>(1, std::min(units, want)), 2 * layers, p.groups);
+        const dim3 grid((uint32_t)std::max<int64_t>(1, std::min(units, want)), 2 * layers,
+                        p.groups);
         auto *k = p.beams <= 4    ? k_beam_reorder<4>
                   : p.beams <= 8  ? k_beam_reorder<8>
                   : p.beams <= 16 ? k_beam_reorder<16>

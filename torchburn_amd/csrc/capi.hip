@@ -1212,8 +1212,9 @@ static int check_cache(const char *what, int64_t hkv, int64_t hd, int64_t max_se
     return TB_OK;
 }
 
-// Whether no two elements of a cache of this geometry share memory.
 }  // extern "C"
+
+// Whether no two elements of a cache of this geometry share memory.
 template <size_t N>
 static bool disjoint(const int64_t (&st)[N], const int64_t (&size)[N], int64_t hd) {
     std::pair<int64_t, int64_t> d[N];
@@ -1227,6 +1228,7 @@ static bool disjoint(const int64_t (&st)[N], const int64_t (&size)[N], int64_t h
     }
     return true;
 }
+
 extern "C" {
 
 int tb_tree_masks(const int32_t *parents, int32_t *mask, int32_t *depth, int64_t batch, int64_t n,

@@ -28,7 +28,12 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kMaxSplits = 64;   // of the prefix, and of a row's own cache
+// Splits of the prefix, and of a row's own cache, at most: a wave of the merge has both in two
+// passes over its lanes.  With eight KV heads the blocks wanted are fewer; with one or two, on
+// prefixes past some thousand positions, it leaves CUs without a block: 32768 positions of two KV
+// heads of 64, in cache, are read at 2.1 TB/s for 2 sequences and 1.1 for 5, those of eight heads
+// of 128 at 5.8 for 2.
+constexpr int kMaxSplits = 64;
 // A row's reference is set this far (in powers of two) above a score that passes it, so
 // that the outputs' rescale runs in few tiles; weights stay below 1.
 constexpr float kLead = 8.f;
@@ -83,7 +88,7 @@ struct Job {
 // The plan of a launch; the blocks' order: the prefix's, then the sequences' own.
 struct Plan {
     int nw;               // waves a block
-    int rb, prows;        // 16 * rb rows of a group a block (16 of a sequence), or prows of a dense one
+    int rb, prows;        // 16 * rb rows of a group a block (16 of a sequence), dense ones prows
     int ptiles, gtiles;   // row tiles of a group's rows, of a sequence's
     int pcap, ocap;       // splits at most
     int pblocks, oblocks;
@@ -187,8 +192,8 @@ struct State {
 // of K and V), 32 rows on 4096 17.4.  The f32 MFMA (154 TFLOP/s in a large product) would
 // bound 64 rows: 104 us on 32767 positions, k_prefix_dense 76.
 template <int D, int RB>
-__device__ __forceinline__ void stream(const PrefixAttn &a, const Job &job, int i0, int i1, int first,
-                                       int step, State<D, RB> &st) {
+__device__ __forceinline__ void stream(const PrefixAttn &a, const Job &job, int i0, int i1,
+                                       int first, int step, State<D, RB> &st) {
     constexpr int NX = D / 16, NB = (D + 63) / 64;
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int xt = job.t1 - job.t0, end = xt + (job.y.len + kTile - 1) / kTile;
@@ -260,14 +265,15 @@ __device__ __forceinline__ void stream(const PrefixAttn &a, const Job &job, int 
         const int left = rows(t).len - place(t);
 #pragma unroll
         for (int b = 0; b < RB; ++b) s[b] = (RB <= 2 ? s[b] + s2[b] : s[b]) * f;
-        if (left < kTile) {   // the last tile of a cache: weight 0, which must meet no infinity or NaN
+        if (left < kTile) {   // a cache's last tile: weight 0, which must meet no infinity or NaN
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const bool in = 4 * g + r < left;
 #pragma unroll
                 for (int b = 0; b < RB; ++b) s[b][r] = in ? s[b][r] : -INFINITY;
 #pragma unroll
-                for (int q = 0; q < NB; ++q) vr[r][q] = in ? vr[r][q] : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int q = 0; q < NB; ++q)
+                    vr[r][q] = in ? vr[r][q] : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         }
         // ---- the rows' references
@@ -310,8 +316,8 @@ __device__ __forceinline__ void stream(const PrefixAttn &a, const Job &job, int 
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int b = 0; b < RB; ++b)
-                        o[b][q][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v4[i], s[b][j], o[b][q][i],
-                                                                          0, 0, 0);
+                        o[b][q][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            v4[i], s[b][j], o[b][q][i], 0, 0, 0);
             }
         if (t + step < end) load_v(t + step);
     }
@@ -494,7 +500,9 @@ struct Limbs {
 // with it: 256 rows of 128 on 32767 positions of 8 KV heads 205 us (168 TFLOP/s of f32
 // products, six bf16 ones each; a large bf16 product reaches 1219), of which the MFMAs
 // alone take 131, with their operands' reads 160, with the limbs 182.  Operands read an
-// MFMA group ahead by force spill and gain nothing (218).
+// MFMA group ahead by force spill and gain nothing (218).  Registers spill in this form too, 91
+// and 9 with 16 and 32 rows of 128 a wave, 57 and 104 with 32 of 224 and 256; the first has three
+// blocks a CU for it (64 rows on 4096 positions 20 us, with two 25).
 template <int D, int W>
 __device__ __forceinline__ void dense_block(const PrefixAttn &a, const Plan &plan, const Job &job,
                                             Limbs<D> &lds, float *part, float *pml) {
@@ -714,9 +722,8 @@ __device__ __forceinline__ void dense_block(const PrefixAttn &a, const Plan &pla
 }
 
 template <int D, int W>
-__global__ __launch_bounds__(256, D > 128 ? 1 : W == 32 ? 2 : 3) void k_prefix_dense(PrefixAttn a, Plan plan,
-                                                                       float *__restrict__ part,
-                                                                       float *__restrict__ pml) {
+__global__ __launch_bounds__(256, D > 128 ? 1 : W == 32 ? 2 : 3) void k_prefix_dense(
+    PrefixAttn a, Plan plan, float *__restrict__ part, float *__restrict__ pml) {
     __shared__ __attribute__((aligned(16))) union {
         Limbs<D> limbs;
         Meeting<D, 1, 4> meeting;
@@ -760,11 +767,10 @@ __global__ __launch_bounds__(256) void k_prefix_merge(PrefixAttn a, Plan plan,
         m[x] = p[0];
         l[x] = p[1];
     }
-    const int pu = split_range(length(a.prefix_lens, a.prefix_len, group, a.max_prefix), plan.pcap, 0)
-                       .splits;
-    const int ou = split_range(length(a.own_lens, a.own_len, group * a.rows + i / G, a.max_own),
-                               plan.ocap, 0)
-                       .splits;
+    const int plen = length(a.prefix_lens, a.prefix_len, group, a.max_prefix);
+    const int olen = length(a.own_lens, a.own_len, group * a.rows + i / G, a.max_own);
+    const int pu = split_range(plen, plan.pcap, 0).splits;
+    const int ou = split_range(olen, plan.ocap, 0).splits;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int s = lane + 64 * x;
@@ -879,8 +885,8 @@ void merge(const PrefixAttn &a, const Plan &p, const float *part, const float *p
         hipLaunchKernelGGL((k_prefix_merge<LC, 4>), dim3(R, a.hkv, a.groups), dim3(256), 0, s, a, p,
                            part, pml);
     else
-        hipLaunchKernelGGL((k_prefix_merge<LC, 1>), dim3((R + 3) / 4, a.hkv, a.groups), dim3(256), 0,
-                           s, a, p, part, pml);
+        hipLaunchKernelGGL((k_prefix_merge<LC, 1>), dim3((R + 3) / 4, a.hkv, a.groups), dim3(256),
+                           0, s, a, p, part, pml);
 }
 
 }  // namespace
@@ -890,7 +896,8 @@ bool prefix_attention_fits(int groups, int rows, int hq, int hkv, int hd, int pr
     return ((int64_t)p.pblocks + p.oblocks) * 64 * p.nw <= kMaxThreads;
 }
 
-size_t prefix_attention_scratch(int groups, int rows, int hq, int hkv, int hd, int prefix, int own) {
+size_t prefix_attention_scratch(int groups, int rows, int hq, int hkv, int hd, int prefix,
+                                int own) {
     const int slots = plan_of(groups, rows, hq, hkv, hd, prefix, own).slots;
     return slots > 1 ? (size_t)groups * rows * hq * slots * (hd + 2) * sizeof(float) : 0;
 }

@@ -54,10 +54,12 @@ struct Piece {
 // angles it works out once for all of them (180 instructions in 64 bits, against 60 a head:
 // 4096 tokens of 40 heads take 68, 45, 36 and 42 us with 1, 2, 4 and 8 heads a group), or 2 W
 // dimensions behind it.  W = 4: 16-byte loads, and both pieces of a pair of the half layout in
-// one lane; W = 1 where sizes, strides or addresses do not allow it.
+// one lane; W = 1 where sizes, strides or addresses do not allow it, bound by its 4-byte loads: 40
+// heads of 80 that turn in 20 dimensions, 4096 tokens in cache, 54 us; all 80 turning, W = 4, 27.
 //
 // Bound by the heads' bytes, on few tokens by the launch: 4096 tokens of 32 + 8 heads of 128,
-// 168 MB, take 36 us (4.6 TB/s, a large copy 4.9); four tokens 5.2.
+// 168 MB, take 37 us a call (4.5 TB/s, a large copy 4.9; the kernel 32 where part of its input
+// is in cache); four tokens 5.2.
 template <int L, int NU, int W, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void k_norm_rope(RopeParams p, int per, int parts) {
     const int lane = threadIdx.x % L;
@@ -183,7 +185,8 @@ __global__ __launch_bounds__(256) void k_norm_rope(RopeParams p, int per, int pa
 #pragma unroll
                     for (int j = 0; j < W; ++j) {
                         // pair j: elements j and W + j of the unit, or 2j and 2j + 1
-                        const int ea = INTERLEAVED ? 2 * j : j, eb = INTERLEAVED ? 2 * j + 1 : W + j;
+                        const int ea = INTERLEAVED ? 2 * j : j;
+                        const int eb = INTERLEAVED ? 2 * j + 1 : W + j;
                         const float a = z[ea], b = z[eb];
                         z[ea] = fmaf(a, co[n][j], -(b * si[n][j]));
                         z[eb] = fmaf(b, co[n][j], a * si[n][j]);
@@ -222,8 +225,8 @@ int launch(const RopeParams &p, hipStream_t s) {
     TB_REQUIRE(blocks * 256 <= kMaxThreads, TB_ERR_UNSUPPORTED,
                "TB_UNSUPPORTED: norm_rope: more threads than one launch has, 2^32 - 1");
     if (p.interleaved)
-        hipLaunchKernelGGL((k_norm_rope<L, NU, W, true>), dim3((uint32_t)blocks), dim3(256), 0, s, p,
-                           per, parts);
+        hipLaunchKernelGGL((k_norm_rope<L, NU, W, true>), dim3((uint32_t)blocks), dim3(256), 0, s,
+                           p, per, parts);
     else
         hipLaunchKernelGGL((k_norm_rope<L, NU, W, false>), dim3((uint32_t)blocks), dim3(256), 0, s,
                            p, per, parts);
